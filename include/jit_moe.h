@@ -502,6 +502,77 @@ int jit_threefry_uniform(const uint32_t *keys, int B, float *u, void *stream);
 int jit_kv_copy_pages(uint16_t *pool, int num_pages, int Hkv, const int32_t *src, const int32_t *dst, int n,
                       void *stream);
 
+/* ------------------------------------------------------------ 8-bit KV cache --
+ * A KV pool held in 8 bits with a scale for each token and kv head, at 0.516 of the bf16 pool's bytes.  No
+ * counterpart in the reference, whose caches are bf16 (Q36/kvcache/kv_cache.py:27-85).  A layer's pool is
+ * [num_pages, Hkv] records of JIT_KV8_RECORD_BYTES bytes (a page's 16 tokens of one kv head, 128-byte lines):
+ *   [0, 2048)     K codes [2][4][16][16]: index (i, g, slot, x) is dim 64 i + 16 g + x;
+ *   [2048, 4096)  V codes [2][4][16][4][4]: index (q, g, r, c, j) is dim 16 (4 q + c) + r of slot 4 g + j;
+ *   [4096, 4224)  32 fp32 scales: K of slots 0 .. 15, then V of slots 0 .. 15.
+ * Codes are OCP e4m3 (no infinity, largest 448).  A block is the 128 values of one token's K (or V) of one kv head;
+ * its scale is 2^e, e = E - 8 (E - 7 where m > 0.75) for a largest finite magnitude of (1 + m) 2^E, e in
+ * [-100, 118], and 1 for a block of zeros; code = the e4m3 nearest to x 2^-e (ties to even; within +-448, past
+ * which a value gets only where e was cut to 118), and the NaN code 255 for an x that is not finite.  A token's slot is
+ * 16 page + position % 16.  The pool's base is 16-byte aligned; zeros are an empty pool. */
+#define JIT_KV8_RECORD_BYTES 4224
+
+/* The tables of one step from its sequences' lengths, in one launch: sequence b (< S) has ctx[b] tokens in the
+ * cache and brings new_rows[b] more (negative values count as 0); the step's rows are the sequences' new tokens in
+ * order.  page_table [S, max_pages].  Outputs:
+ *   row_start [S + 1]  first row of each sequence (and the row count);
+ *   row_seq, pos, slots [rows]  each row's sequence, position and slot; -1, 0, -1 past the last row;
+ *   lens [S]           ctx + new_rows, what attention reads;
+ *   status [4]         rows, where the free list goes on, sequences refused, 0.
+ * n_free >= 0: the tables grow -- every page past the ceil(ctx / 16) that a sequence holds is taken from
+ * free_pages[n_free], in sequence order from index *free_at (NULL: 0), and written into page_table.  n_free < 0:
+ * the tables hold the step's pages already.  A sequence is refused -- its slots are -1, its lens stays ctx, no page is taken --
+ * where its pages pass max_pages, its rows pass `rows`, or the free list ends before its pages (counted over the
+ * sequences so far).  A page id outside [0, 2^27) gives slot -1; a sum past 2^31 - 1 stays there.
+ * Contract: S >= 0, max_pages > 0, rows >= 0 (JIT_EINVAL); S <= JIT_STEP_TABLES_MAX_SEQS (JIT_EUNSUPPORTED). */
+#define JIT_STEP_TABLES_MAX_SEQS 8192
+int jit_step_tables(const int32_t *ctx, const int32_t *new_rows, int S, int32_t *page_table, int max_pages,
+                    int rows, const int32_t *free_pages, int n_free, const int32_t *free_at,
+                    int32_t *row_start, int32_t *row_seq, int32_t *pos, int32_t *slots, int32_t *lens,
+                    int32_t *status, void *stream);
+
+/* jit_kv_append_paged into an 8-bit pool: k, v [B, Hkv, 128] bf16 of row b at slot slots[b].  A slot outside the
+ * pool (-1) is not written; the others are distinct.  B <= 65535 (JIT_EUNSUPPORTED). */
+int jit_kv8_append_paged(const uint16_t *k, const uint16_t *v, int B, int Hkv, const int32_t *slots, void *pool,
+                         int num_pages, void *stream);
+
+/* jit_qk_norm_rope_append into an 8-bit pool: the same formulas evaluated in fp32 with the angle pos[b] *
+ * inv_freq[i] in fp64, and rounded once -- q to bf16, k and v to their codes.  Rows whose slot is outside the pool
+ * still give their q. */
+int jit_qk_norm_rope_append_kv8(const uint16_t *qkv, int B, int H, int Hkv, const uint16_t *q_norm_w,
+                                const uint16_t *k_norm_w, float eps, const float *inv_freq, const int32_t *pos,
+                                const int32_t *slots, void *pool, int num_pages, uint16_t *q_out, void *stream);
+
+/* jit_kv_copy_pages of an 8-bit pool. */
+int jit_kv8_copy_pages(void *pool, int num_pages, int Hkv, const int32_t *src, const int32_t *dst, int n, void *stream);
+
+/* Keys of a chunk of the split of a sequence of `len` keys: a function of the length alone, so a row's bits do not
+ * depend on the batch. */
+int jit_kv8_chunk_tokens(int len);
+/* Workspace bytes of jit_paged_decode_attn_kv8 for B rows of at most max_len keys. */
+int64_t jit_kv8_decode_workspace_bytes(int B, int H, int max_len);
+
+/* Paged GQA decode attention over an 8-bit pool, one query per row: out[b, h] = softmax(scale * q[b, h] . K_b^T) .
+ * V_b over the first lens[b] tokens (device values; at most max_len and 16 max_pages count) of the values the cache
+ * holds.  No keys: zeros.  Keys of page ids outside the pool are left out; what the other slots of a page hold does
+ * not matter.  q, out [B, H, 128] bf16; page_table [B, max_pages].
+ * Contract: H % Hkv == 0 (JIT_EINVAL), H / Hkv <= 16 (JIT_EUNSUPPORTED). */
+int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, int num_pages, const int32_t *page_table,
+                              int max_pages, const int32_t *lens, int B, int H, int Hkv, int max_len, float scale,
+                              void *workspace, int64_t workspace_bytes, uint16_t *out, void *stream);
+
+/* jit_paged_prefill_attn over an 8-bit pool: the same chunks, work items, parts and workspace.  Keys of page ids
+ * outside the pool are left out. */
+int jit_paged_prefill_attn_kv8(const uint16_t *q, const void *pool, int num_pages, const int32_t *page_table,
+                               int max_pages, const int32_t *chunk_seq, const int32_t *chunk_ctx,
+                               const int32_t *chunk_len, const int32_t *chunk_row, int C, const int32_t *blk_chunk,
+                               const int32_t *blk_q0, const int32_t *blk_part, int nblk, int pmax, int max_len, int H,
+                               int Hkv, float scale, void *workspace, uint16_t *out, void *stream);
+
 /* ------------------------------------------------------------ whole layers --
  * One decoder layer per call (Q36/model/model.py:65-80): the launches above, in their order, issued from
  * native code.  All weights are packed matrices and stacks (jit_q4_prepack). */

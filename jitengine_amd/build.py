@@ -42,6 +42,8 @@ SOURCES = {
     "block.hip": [],
     "head.hip": [],
     "sampler.hip": ["-ffp-contract=off"],
+    "kv8.hip": [],
+    "kv8_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 _COMMON = [

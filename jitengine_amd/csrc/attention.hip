@@ -120,26 +120,6 @@ struct AttnArgs {
   float eps;
 };
 
-// xor-16 / xor-32 lane exchanges, one VALU op each (gfx950 permlane swaps): with both
-// operands the same value, the two results are the even and the odd row (of each
-// row pair, resp. half) -- so any symmetric combination of them is the reduction.
-__device__ __forceinline__ float max_xor16(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float max_xor32(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_xor16(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float sum_xor32(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // The K part of kv head kvh in page pg (its V part follows).
 __device__ __forceinline__ const uint16_t *head_part(const uint16_t *pool, int pg, int Hkv, int kvh) {
   return pool + ((long long)pg * Hkv + kvh) * 2 * kPageHead;

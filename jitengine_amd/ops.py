@@ -819,6 +819,218 @@ def paged_decode_attention_noalloc(q: torch.Tensor, pool: torch.Tensor, page_tab
     return out
 
 
+# ----------------------------------------------------------------------------- 8-bit KV cache
+KV8_RECORD = 4224  # bytes of one page's 16 tokens of one kv head: K codes, V codes, 32 fp32 scales
+
+
+def _one_device(**tensors) -> torch.device:
+    """The device that all of a call's tensors share (ValueError otherwise): the call runs there, on that device's
+    current stream."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a device tensor")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {dev}")
+        dev = t.device
+    return dev
+
+
+def _stream_of(dev: torch.device) -> ctypes.c_void_p:
+    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _kv8_heads(pool: torch.Tensor) -> int:
+    """kv heads of a layer's 8-bit pool [num_pages, Hkv, KV8_RECORD] (ValueError otherwise)."""
+    _need(pool, torch.uint8, "pool")
+    if pool.dim() != 3 or pool.shape[2] != KV8_RECORD or pool.shape[0] < 1 or pool.shape[1] < 1:
+        raise ValueError(f"an 8-bit KV pool is a contiguous [pages, Hkv, {KV8_RECORD}] tensor, got {tuple(pool.shape)}")
+    if pool.data_ptr() % 16:
+        raise ValueError("an 8-bit KV pool starts on 16 bytes")
+    return int(pool.shape[1])
+
+
+def is_kv8(pool: torch.Tensor) -> bool:
+    """Whether a layer's pool is an 8-bit one."""
+    return pool.dtype == torch.uint8
+
+
+def kv8_pool(num_pages: int, n_kv_heads: int, device) -> torch.Tensor:
+    """An empty 8-bit KV pool of one layer: [num_pages, Hkv, KV8_RECORD] uint8 (include/jit_moe.h describes a record)."""
+    if num_pages <= 0 or n_kv_heads <= 0:
+        raise ValueError("an 8-bit KV pool needs positive pages and heads")
+    return torch.zeros((int(num_pages), int(n_kv_heads), KV8_RECORD), dtype=torch.uint8, device=device)
+
+
+@dataclass
+class StepTables:
+    """The tables of one step (jit_step_tables), int32 on the device: the rows are the sequences' new tokens in order."""
+
+    row_start: torch.Tensor  # [S + 1]
+    row_seq: torch.Tensor    # [rows]; -1 past the last row
+    pos: torch.Tensor        # [rows]; 0 past the last row
+    slots: torch.Tensor      # [rows]: 16 page + position % 16; -1 where nothing is written
+    lens: torch.Tensor       # [S]: the keys attention reads
+    status: torch.Tensor     # [4]: rows, where the free list goes on, sequences refused, 0
+
+
+def step_tables(ctx: torch.Tensor, new: torch.Tensor, page_table: torch.Tensor, rows: int,
+                free: torch.Tensor | None = None, free_at: torch.Tensor | None = None) -> StepTables:
+    """The positions, slots and lengths of a step whose sequence b has ctx[b] tokens in the cache and brings new[b]
+    more, built on the device in one launch (jit_step_tables).  With `free` (int32 page ids) page_table grows in
+    place: each sequence's new pages come from the list in sequence order, from index free_at[0] on (0 without).  A
+    sequence that does not fit its table, the `rows` or the list is refused (slots -1, lens = ctx; status counts them)."""
+    dev = _one_device(ctx=ctx, new=new, page_table=page_table, free=free, free_at=free_at)
+    for t, name in ((ctx, "ctx"), (new, "new"), (page_table, "page_table"), (free, "free"), (free_at, "free_at")):
+        if t is not None:
+            _need(t, torch.int32, name)
+    S = ctx.numel()
+    if ctx.dim() != 1 or new.shape != ctx.shape or page_table.dim() != 2 or page_table.shape[0] != S:
+        raise ValueError(f"step_tables takes ctx, new [S] and page_table [S, W], got {tuple(ctx.shape)}, "
+                         f"{tuple(new.shape)}, {tuple(page_table.shape)}")
+    if free is not None and free.dim() != 1:
+        raise ValueError("free must be a list of page ids")
+    if free_at is not None and (free is None or free_at.numel() != 1):
+        raise ValueError("free_at is one index into free")
+    rows = int(rows)
+    if rows < 0 or rows > 0x7fffffff // 4:
+        raise ValueError(f"rows must lie in [0, 2^29), got {rows}")
+    buf = torch.empty(2 * S + 5 + 3 * rows, dtype=torch.int32, device=dev)
+    rs, sq, ps, sl, ln, st = torch.split(buf, [S + 1, rows, rows, rows, S, 4])
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().jit_step_tables(_p(ctx), _p(new), S, _p(page_table), page_table.shape[1], rows, _p(free),
+                                              -1 if free is None else free.numel(), _p(free_at), _p(rs), _p(sq), _p(ps),
+                                              _p(sl), _p(ln), _p(st), _stream_of(dev)), "step_tables")
+    return StepTables(rs, sq, ps, sl, ln, st)
+
+
+def kv8_append_paged(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Write k, v [B, Hkv, 128] bf16 into an 8-bit pool at slots [B] int32 (jit_kv8_append_paged; a slot outside the
+    pool is not written)."""
+    dev = _one_device(pool=pool, k=k, v=v, slots=slots)
+    Hkv = _kv8_heads(pool)
+    _need(k, torch.bfloat16, "k")
+    _need(v, torch.bfloat16, "v")
+    _need(slots, torch.int32, "slots")
+    if k.dim() != 3 or k.shape[1:] != (Hkv, HEAD_DIM) or v.shape != k.shape or slots.shape != (k.shape[0],):
+        raise ValueError(f"kv8_append_paged takes k, v [B, {Hkv}, 128] and slots [B], got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}, {tuple(slots.shape)}")
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().jit_kv8_append_paged(_p(k), _p(v), k.shape[0], Hkv, _p(slots), _p(pool), pool.shape[0],
+                                                   _stream_of(dev)), "kv8_append_paged")
+
+
+def qk_norm_rope_append_kv8(qkv: torch.Tensor, H: int, Hkv: int, q_norm: torch.Tensor, k_norm: torch.Tensor, eps: float,
+                            inv_freq: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor,
+                            pool: torch.Tensor) -> torch.Tensor:
+    """qkv [B, (H + 2 Hkv) * 128] -> q [B, H, 128] (normed, rotated by pos); k, v written into the 8-bit pool at slots
+    (jit_qk_norm_rope_append_kv8: one rounding, angles in fp64)."""
+    dev = _one_device(qkv=qkv, q_norm=q_norm, k_norm=k_norm, inv_freq=inv_freq, pos=pos, slots=slots, pool=pool)
+    _need(qkv, torch.bfloat16, "qkv")
+    _need(q_norm, torch.bfloat16, "q_norm")
+    _need(k_norm, torch.bfloat16, "k_norm")
+    _need(inv_freq, torch.float32, "inv_freq")
+    _need(pos, torch.int32, "pos")
+    _need(slots, torch.int32, "slots")
+    if _kv8_heads(pool) != Hkv or qkv.dim() != 2 or qkv.shape[1] != (H + 2 * Hkv) * HEAD_DIM or \
+            inv_freq.numel() != HEAD_DIM // 2 or q_norm.numel() != HEAD_DIM or k_norm.numel() != HEAD_DIM:
+        raise ValueError("qkv / pool / norms / inv_freq do not match the head geometry")
+    B = qkv.shape[0]
+    if pos.shape != (B,) or slots.shape != (B,):
+        raise ValueError(f"pos and slots must be [{B}], got {tuple(pos.shape)} and {tuple(slots.shape)}")
+    q = torch.empty((B, H, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().jit_qk_norm_rope_append_kv8(
+            _p(qkv), B, H, Hkv, _p(q_norm), _p(k_norm), float(eps), _p(inv_freq), _p(pos), _p(slots), _p(pool),
+            pool.shape[0], _p(q), _stream_of(dev)), "qk_norm_rope_append_kv8")
+    return q
+
+
+def kv8_decode_workspace_bytes(B: int, H: int, max_len: int) -> int:
+    return int(_lib.lib().jit_kv8_decode_workspace_bytes(int(B), int(H), int(max_len)))
+
+
+def _kv8_workspace(workspace, need: int, dev) -> torch.Tensor | None:
+    """The caller's workspace if `need` bytes fit it, else a new one (None for no bytes)."""
+    if need <= 0:
+        return None
+    if workspace is not None and workspace.device == dev and workspace.is_contiguous() and workspace.nbytes >= need \
+            and workspace.data_ptr() % 16 == 0:
+        return workspace
+    return torch.empty(need, dtype=torch.uint8, device=dev)
+
+
+def paged_decode_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+                               max_len: int, scale: float, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """q [B, H, 128] bf16 -> out [B, H, 128] bf16 over each sequence's first lens[b] keys of an 8-bit pool
+    (jit_paged_decode_attn_kv8).  lens [B] int32 stays on the device; max_len is any bound of it that the host knows
+    (it sizes the launch and the workspace of kv8_decode_workspace_bytes; the bits do not depend on it).  A row without keys gives zeros."""
+    dev = _one_device(q=q, pool=pool, page_table=page_table, lens=lens)
+    _need(q, torch.bfloat16, "q")
+    _need(page_table, torch.int32, "page_table")
+    _need(lens, torch.int32, "lens")
+    Hkv = _kv8_heads(pool)
+    if q.dim() != 3 or page_table.dim() != 2:
+        raise ValueError("q must be [B, H, 128] and page_table [B, W]")
+    B, H, Dh = q.shape
+    if Dh != HEAD_DIM:
+        raise _lib.UnsupportedShape(f"paged_decode_attention_kv8 covers head_dim 128, got {Dh}")
+    if page_table.shape[0] != B or lens.shape != (B,):
+        raise ValueError("the rows, page_table and lens disagree on the number of sequences")
+    max_len = int(max_len)
+    if max_len < 0 or max_len > page_table.shape[1] * PAGE:
+        raise ValueError(f"max_len must lie in [0, {page_table.shape[1] * PAGE}] (page_table's width), got {max_len}")
+    ws = _kv8_workspace(workspace, kv8_decode_workspace_bytes(B, H, max_len), dev)
+    out = torch.empty_like(q)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().jit_paged_decode_attn_kv8(
+            _p(q), _p(pool), pool.shape[0], _p(page_table), page_table.shape[1], _p(lens), B, H, Hkv, max_len,
+            float(scale), _p(ws), 0 if ws is None else ws.nbytes, _p(out), _stream_of(dev)), "paged_decode_attn_kv8")
+    return out
+
+
+def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, plan: PrefillPlan,
+                                scale: float, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """q [T, H, 128] bf16 (the plan's chunk rows) -> out [T, H, 128]: paged_prefill_attention over an 8-bit pool
+    (jit_paged_prefill_attn_kv8; the same plans and workspace)."""
+    dev = _one_device(q=q, pool=pool, page_table=page_table, plan=plan.tables)
+    _need(q, torch.bfloat16, "q")
+    _need(page_table, torch.int32, "page_table")
+    Hkv = _kv8_heads(pool)
+    if q.dim() != 3 or page_table.dim() != 2:
+        raise ValueError("q must be [T, H, 128] and page_table [S, W]")
+    T, H, Dh = q.shape
+    if Dh != HEAD_DIM:
+        raise _lib.UnsupportedShape(f"paged_prefill_attention_kv8 covers head_dim 128, got {Dh}")
+    if T != plan.rows:
+        raise ValueError(f"q has {T} rows, the plan's chunks {plan.rows}")
+    prefill_contract(plan, page_table)
+    ws = _kv8_workspace(workspace, prefill_workspace_bytes(plan, H), dev)
+    out = torch.empty_like(q)
+    tb, bl = plan.tables, plan.blocks
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().jit_paged_prefill_attn_kv8(
+            _p(q), _p(pool), pool.shape[0], _p(page_table), page_table.shape[1], _p(tb[0]), _p(tb[1]), _p(tb[2]),
+            _p(tb[3]), tb.shape[1], _p(bl[0]), _p(bl[1]), _p(bl[2]), bl.shape[1], plan.pmax, plan.max_len, H, Hkv,
+            float(scale), _p(ws), _p(out), _stream_of(dev)), "paged_prefill_attn_kv8")
+    return out
+
+
+def kv8_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copy pages src[i] -> dst[i] (int32 device tensors) inside one layer's 8-bit pool."""
+    dev = _one_device(pool=pool, src=src, dst=dst)
+    Hkv = _kv8_heads(pool)
+    _need(src, torch.int32, "src")
+    _need(dst, torch.int32, "dst")
+    if src.shape != dst.shape or src.dim() != 1:
+        raise ValueError("src and dst must be equal-length 1-D page lists")
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().jit_kv8_copy_pages(_p(pool), pool.shape[0], Hkv, _p(src), _p(dst), src.shape[0],
+                                                 _stream_of(dev)), "kv8_copy_pages")
+
+
 # ----------------------------------------------------------------------------- step ends, KV pages
 def embed_q4(ids: torch.Tensor, table: QLinear) -> torch.Tensor:
     """Embedding rows [B, D] bf16 of token ids [B] int32 from an MLX 4-bit table [V, D]
