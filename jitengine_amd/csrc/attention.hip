@@ -971,7 +971,8 @@ __global__ __launch_bounds__(64 * WAVES) void prefill_attn_kernel(const PrefillA
     if (!store[j]) continue;
     const int parts = (ctx + tok[j]) / kPfPartKeys + 1;  // the token's key parts
     const long long hrow = (long long)(row0 + tok[j]) * a.H + kvh * G + lr % G;
-    if (parts == 1) {  // (then part == 0): the token's whole result
+    if (part >= parts) continue;  // (a token before this part's keys, in a block whose last token reaches them)
+    if (parts == 1) {  // the token's whole result
       const float inv = 1.0f / l_tot;
       uint16_t *op = a.out + hrow * kD + 4 * lg;
 #pragma unroll
@@ -981,7 +982,7 @@ __global__ __launch_bounds__(64 * WAVES) void prefill_attn_kernel(const PrefillA
         w.y = pack_bf16x2(o[j][cc][2] * inv, o[j][cc][3] * inv);
         *(uint2 *)(op + 16 * cc) = w;
       }
-    } else if (part < parts) {  // this part's (max, sum, unnormalised o) of the token
+    } else {  // this part's (max, sum, unnormalised o) of the token
       float *ps = a.part + (((long long)(row0 + tok[j]) * a.pmax + part) * a.H + kvh * G + lr % G) * kPfSlot;
 #pragma unroll
       for (int cc = 0; cc < 8; cc++)
