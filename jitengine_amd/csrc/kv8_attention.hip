@@ -59,7 +59,11 @@ constexpr int kStateFloats = 32 + 2;  // o[8][4], max, sum per lane
 
 __global__ __launch_bounds__(64 * kSplits) void kv8_decode_kernel(const DecodeArgs a) {
   __shared__ float xstate[kSplits - 1][kStateFloats][64];
-  const int b = blockIdx.x % a.B, c = blockIdx.x / a.B, kvh = blockIdx.y;
+  // Workgroups go to the 8 XCDs in turn, so chunk c of sequence b runs on XCD (c odd + b) % 8: a long sequence's chunks
+  // spread over all of them.  (With B itself in odd's place, B = 32 kept each sequence on one XCD: 32 sequences of 128
+  // to 32,768 keys 105 us, now 32.)
+  const int odd = a.B | 1, b = blockIdx.x % odd, c = blockIdx.x / odd, kvh = blockIdx.y;
+  if (b >= a.B) return;
   const int split = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
   const int lr = l & 15, lg = l >> 4, G = a.G;
   const int L = seq_len(a, b), ck = chunk_tokens(L), n = chunks_of(L);
@@ -530,7 +534,7 @@ extern "C" int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, in
   const int most = (long long)max_pages * kPage < max_len ? max_pages * kPage : max_len;
   const int ncap = max_chunks(most) > 1 ? max_chunks(most) : 1;
   const int64_t need = decode_bytes(B, H, most);
-  if ((int64_t)B * ncap > 0x7fffffff)
+  if (((int64_t)B | 1) * ncap > 0x7fffffff)
     return jit::fail(JIT_EUNSUPPORTED, "paged_decode_attn_kv8: %d sequences of up to %d chunks", B, ncap);
   if (workspace_bytes < need)
     return jit::fail(JIT_EINVAL, "paged_decode_attn_kv8: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
@@ -542,7 +546,7 @@ extern "C" int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, in
   float *part_o = (float *)workspace;
   const DecodeArgs a{q, (const uint8_t *)pool, page_table, lens, part_o, need ? part_o + (int64_t)B * ncap * H * kD : nullptr,
                      out, num_pages, max_pages, B, H, Hkv, H / Hkv, most, ncap, scale * 1.44269504088896341f};
-  kv8_decode_kernel<<<dim3((unsigned)B * ncap, Hkv), 64 * kSplits, 0, (hipStream_t)stream>>>(a);
+  kv8_decode_kernel<<<dim3((unsigned)(B | 1) * ncap, Hkv), 64 * kSplits, 0, (hipStream_t)stream>>>(a);
   const int rc = jit::check_launch("jit_paged_decode_attn_kv8");
   if (rc || ncap == 1) return rc;
   kv8_merge_kernel<<<dim3(B, H), 32 * kMergeLanes, 0, (hipStream_t)stream>>>(a);
