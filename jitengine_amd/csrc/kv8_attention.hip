@@ -260,17 +260,31 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
 }
 
 // ---------------------------------------------------------------- causal prompt chunks
-// A workgroup owns WAVES x TILES q tiles of 16 rows (16 / G tokens x the G q heads of a kv head) and walks the keys up
-// to its last token 128 a step.  A step's codes become bf16 keys (times their scales) and fp16 values in LDS once,
-// for all of the workgroup's rows.
-constexpr int kPfWaves = 8, kPfTiles = 2;  // a row block (jit_prefill_block_tokens)
+// A workgroup owns WAVES x 32 rows (32 / G tokens x the G q heads of a kv head a wave) and walks the keys up to its
+// last token 128 a step.  A step's codes become bf16 keys (times their scales) and fp16 values in LDS once, for all
+// of the workgroup's rows, while the step before is computed: the codes are requested two steps ahead into
+// registers, converted one step ahead into the other half of LDS, and a step has one barrier.
+//   S^T[32 keys x 32 rows] = K . Q^T        (8 MFMA 32x32x16 bf16)
+//   O^T[128 dims x 32 rows] += V^T . P^T    (4 MFMA 32x32x16 fp16 a page)
+// A lane owns one row throughout: its scores of a page are its P operand as they are, since the 16 keys of V's
+// operand are kept in the order in which the score tile holds them.
+constexpr int kRowsWave = 32, kBlockRows = 256;  // a row block (jit_prefill_block_tokens): 256 / G tokens
 constexpr int kStepKeys = 128, kStepPages = kStepKeys / kPage;
-constexpr int kPartKeys = 6144;            // key parts (jit_prefill_part_keys)
+constexpr int kPartKeys = 6144;                  // key parts (jit_prefill_part_keys)
 constexpr int kPartSteps = kPartKeys / kStepKeys;
-constexpr int kPfSlot = kD + 4;            // floats of a (token, part, head) partial: o, max, sum, 2 pad
+constexpr int kPfSlot = kD + 4;                  // floats of a (token, part, head) partial: o, max, sum, 2 pad
 // Values are held in LDS relative to the loudest scale so far, 2^E, times 2^7 (448 x 2^7 < 65,504): a value of a token
 // 2^22 times quieter than that still has all its bits.
 constexpr int kVShift = 7;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32x32x16(const Frag8 &a, const Frag8 &b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32x32x16_f16(const FragH &a, const FragH &b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.v, b.v, c, 0, 0, 0);
+}
 
 struct PrefillArgs {
   const uint16_t *q;
@@ -284,195 +298,243 @@ struct PrefillArgs {
   float qk_scale;
 };
 
-template <int WAVES, int TILES>
-__global__ __launch_bounds__(64 * WAVES) void kv8_prefill_kernel(const PrefillArgs a) {
-  constexpr int kSub = kPfWaves * kPfTiles / (WAVES * TILES);  // workgroups a row block
-  __shared__ __attribute__((aligned(16))) uint4 s_k[kStepPages * 4 * 64];  // [page][fragment][lane] 8 bf16
-  __shared__ __attribute__((aligned(16))) uint4 s_v[kStepPages / 2 * 8 * 64];  // [page pair][16 dims][lane] 8 fp16
+// What a wave requests of a step: its pages' codes and scales, and the step's V scales (2 keys a lane).
+template <int PAGES>
+struct Staged {
+  uint4 k[PAGES][2], v[PAGES][2];
+  float ks[PAGES];
+  float4 vs[PAGES][2];
+  float2 all_vs;
+  uint32_t bad;  // the step's pages outside the pool
+};
+
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4 < 1 ? 1 : WAVES / 4, 2)))
+void kv8_prefill_kernel(const PrefillArgs a) {
+  constexpr int kSub = kBlockRows / (WAVES * kRowsWave);  // workgroups a row block
+  constexpr int kPages = kStepPages / WAVES;              // pages a wave stages a step
+  __shared__ __attribute__((aligned(16))) uint4 s_k[2][kStepPages / 2][8][64];  // [page pair][16 dims][lane] 8 bf16
+  __shared__ __attribute__((aligned(16))) uint4 s_v[2][kStepPages][4][64];      // [page][32 dims][lane] 8 fp16
   const int item = blockIdx.x / (kSub * a.Hkv), kvh = blockIdx.x % a.Hkv;
   const int ch = a.blk_chunk[item], part = a.blk_part[item];
   const int seq = a.chunk_seq[ch], ctx = a.chunk_ctx[ch], len = a.chunk_len[ch], row0 = a.chunk_row[ch];
-  const int G = a.G, TR = 16 / G, tpw = TILES * TR;
+  const int G = a.G, tpw = kRowsWave / G;  // tokens a wave
   int q0 = a.blk_q0[item];
   if constexpr (kSub > 1) q0 += blockIdx.x / a.Hkv % kSub * WAVES * tpw;
   if (q0 >= len) return;  // (uniform)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
-  const int lr = l & 15, lg = l >> 4;
+  const int lr = l & 31, lh = l >> 5;
   const int kend = ctx + min(q0 + WAVES * tpw, len);  // the workgroup's keys: [0, kend)
   const int nst = (kend + kStepKeys - 1) / kStepKeys, npages = min((kend + kPage - 1) / kPage, a.max_pages);
   const int st0 = part * kPartSteps, st1 = min(nst, st0 + kPartSteps);
   if (st0 >= st1) return;  // (uniform: a piece of a block whose last token alone reaches the part)
   const int32_t *prow = a.page_table + (long long)seq * a.max_pages;
 
-  int tok[TILES];
-  bool store[TILES];
-  Frag8 qf[TILES][4];
-  float m_run[TILES], l_run[TILES];
-  f32x4 o[TILES][8];
+  const int t = q0 + wave * tpw + lr / G, tok = min(t, len - 1), pos = ctx + tok;  // the lane's row
+  const int first_pos = ctx + min(q0 + wave * tpw, len - 1);                       // the wave's first
+  Frag8 qf[8];
+  {
+    const uint16_t *qp = a.q + ((long long)(row0 + tok) * a.H + kvh * G + lr % G) * kD + 8 * lh;
 #pragma unroll
-  for (int j = 0; j < TILES; j++) {
-    const int t = q0 + wave * tpw + j * TR + lr / G;
-    store[j] = t < len;
-    tok[j] = min(t, len - 1);
-    const uint16_t *qp = a.q + ((long long)(row0 + tok[j]) * a.H + kvh * G + lr % G) * kD + 16 * lg;
-#pragma unroll
-    for (int f = 0; f < 4; f++) qf[j][f].q = *(const uint4 *)(qp + 64 * (f >> 1) + 8 * (f & 1));
-    m_run[j] = kLowest;
-    l_run[j] = 0.0f;
-#pragma unroll
-    for (int cc = 0; cc < 8; cc++) o[j][cc] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < 8; s++) qf[s].q = *(const uint4 *)(qp + 16 * s);
   }
-  int e_run = kMinExp;  // the exponent of the loudest value so far
-  for (int st = st0; st < st1; st++) {
-    const int k0 = kStepKeys * st;
-    // the step's page ids (lane i: page i % 8) and which of them lie outside the pool
-    int my_page = prow[min(kStepPages * st + (l & (kStepPages - 1)), npages - 1)];
-    const bool bad = my_page < 0 || my_page >= a.num_pages;
-    const uint32_t bad_pages = (uint32_t)__ballot(bad) & 0xffu;
-    if (bad) my_page = 0;
-    // the loudest live value of the step: lane i's keys 2 i, 2 i + 1
-    int e_step = kMinExp;
-    {
-      const int p = l >> 3;
-      const uint8_t *rec = record(a.pool, __shfl(my_page, p, 64), a.Hkv, kvh);
-      const float2 s2 = *(const float2 *)(rec + kScaleOff + 4 * kPage + 8 * (l & 7));
-      if (!((bad_pages >> p) & 1)) {
-        if (k0 + 2 * l < kend) e_step = max(e_step, (int)(__float_as_uint(s2.x) >> 23) - 127);
-        if (k0 + 2 * l + 1 < kend) e_step = max(e_step, (int)(__float_as_uint(s2.y) >> 23) - 127);
-      }
+  float m_run = kLowest, l_run = 0.0f;
+  f32x16 o[4];
 #pragma unroll
-      for (int x = 1; x < 64; x <<= 1) e_step = max(e_step, __shfl_xor(e_step, x, 64));
-    }
-    const int e_new = max(e_run, min(e_step, kMaxExp));
-    const float e_alpha = e_new - e_run > 126 ? 0.0f : exp_bits(e_run - e_new);
-    e_run = e_new;
-    __syncthreads();  // (the previous step's reads are done)
-    for (int u = wave; u < kStepPages; u += WAVES) {  // keys: page u
-      const uint8_t *rec = record(a.pool, __builtin_amdgcn_readlane(my_page, u), a.Hkv, kvh);
-      const float s = *(const float *)(rec + kScaleOff + 4 * lr);
+  for (int c = 0; c < 4; c++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[c][i] = 0.0f;
+
+  // a step's page ids, lane i page i % 8 (past the keys: the last page again, its keys masked)
+  auto page_ids = [&](int st) { return prow[min(kStepPages * st + (l & (kStepPages - 1)), npages - 1)]; };
+  auto request = [&](Staged<kPages> &r, int pages) {
+    const bool bad = pages < 0 || pages >= a.num_pages;
+    r.bad = (uint32_t)__ballot(bad) & 0xffu;
+    const int ids = bad ? 0 : pages;
+#pragma unroll
+    for (int p = 0; p < kPages; p++) {
+      const uint8_t *rec = record(a.pool, __builtin_amdgcn_readlane(ids, kPages * wave + p), a.Hkv, kvh);
+      const float *sc = (const float *)(rec + kScaleOff);
+      r.ks[p] = sc[l & 15];
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        const uint4 w = *(const uint4 *)(rec + 1024 * i + 16 * l);
-        uint4 f0, f1;
-        to_bf16(w.x, s, f0.x, f0.y);
-        to_bf16(w.y, s, f0.z, f0.w);
-        to_bf16(w.z, s, f1.x, f1.y);
-        to_bf16(w.w, s, f1.z, f1.w);
-        s_k[(u * 4 + 2 * i) * 64 + l] = f0;
-        s_k[(u * 4 + 2 * i + 1) * 64 + l] = f1;
+        r.k[p][i] = *(const uint4 *)(rec + 1024 * i + 16 * l);
+        // lane (q = l / 32, h = l / 16 % 2, r = l % 16): slots 4 h .. and 8 + 4 h .. of dims 64 q + 16 c + r
+        r.v[p][i] = *(const uint4 *)(rec + kVOff + 1024 * (l >> 5) + 512 * i + 16 * (l & 31));
+        r.vs[p][i] = *(const float4 *)(sc + kPage + 8 * i + 4 * ((l >> 4) & 1));
       }
     }
-    for (int u = wave; u < kStepPages; u += WAVES) {  // values: page pair u / 2, dims 64 (u % 2) ..
-      const int h = u >> 1, qd = u & 1;
-      uint32_t w[2][4];
+    const uint8_t *rec = record(a.pool, __shfl(ids, l >> 3, 64), a.Hkv, kvh);
+    r.all_vs = *(const float2 *)(rec + kScaleOff + 4 * kPage + 8 * (l & 7));
+  };
+  // the step's loudest live value; E over the part so far grows with it, and O's unit with E
+  int e_run = kMinExp;
+  auto grow_unit = [&](const Staged<kPages> &r, int k0) {
+    int e = kMinExp;
+    if (!((r.bad >> (l >> 3)) & 1)) {
+      if (k0 + 2 * l < kend) e = max(e, (int)(__float_as_uint(r.all_vs.x) >> 23) - 127);
+      if (k0 + 2 * l + 1 < kend) e = max(e, (int)(__float_as_uint(r.all_vs.y) >> 23) - 127);
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) e = max(e, __shfl_xor(e, x, 64));
+    const int e_new = max(e_run, min(__builtin_amdgcn_readfirstlane(e), kMaxExp));
+    const float f = e_new - e_run > 126 ? 0.0f : exp_bits(e_run - e_new);
+    e_run = e_new;
+    return f;
+  };
+  auto convert = [&](const Staged<kPages> &r, int st) {
+    const int buf = st & 1, k0 = kStepKeys * st;
+#pragma unroll
+    for (int p = 0; p < kPages; p++) {
+      const int pg = kPages * wave + p;
+#pragma unroll
+      for (int i = 0; i < 2; i++) {  // lane (g = l / 16, slot = l % 16): dims 64 i + 16 g ..
+        uint4 f0, f1;
+        to_bf16(r.k[p][i].x, r.ks[p], f0.x, f0.y);
+        to_bf16(r.k[p][i].y, r.ks[p], f0.z, f0.w);
+        to_bf16(r.k[p][i].z, r.ks[p], f1.x, f1.y);
+        to_bf16(r.k[p][i].w, r.ks[p], f1.z, f1.w);
+        uint4 *dst = &s_k[buf][pg >> 1][4 * i + (l >> 4)][16 * (pg & 1) + (l & 15)];
+        dst[0] = f0;
+        dst[32] = f1;
+      }
       f16x2_t fac[2][2];
+      uint32_t w[2][4];
 #pragma unroll
-      for (int p = 0; p < 2; p++) {
-        const uint8_t *rec = record(a.pool, __builtin_amdgcn_readlane(my_page, 2 * h + p), a.Hkv, kvh);
-        const uint4 v = *(const uint4 *)(rec + kVOff + 1024 * qd + 16 * l);
-        const float4 s = *(const float4 *)(rec + kScaleOff + 4 * kPage + 16 * lg);
-        const int keep = (bad_pages >> (2 * h + p)) & 1 ? 0 : kend - (k0 + 32 * h + 16 * p + 4 * lg);
-        const uint32_t km = keep_bytes(keep);
-        w[p][0] = v.x & km, w[p][1] = v.y & km, w[p][2] = v.z & km, w[p][3] = v.w & km;
-        const float *sp = (const float *)&s;
+      for (int i = 0; i < 2; i++) {
+        const int keep = (r.bad >> pg) & 1 ? 0 : kend - (k0 + kPage * pg + 8 * i + 4 * ((l >> 4) & 1));
+        const uint32_t km = keep_bytes(keep);  // (what lies past the keys may be anything: no NaN code gets in)
+        w[i][0] = r.v[p][i].x & km, w[i][1] = r.v[p][i].y & km, w[i][2] = r.v[p][i].z & km, w[i][3] = r.v[p][i].w & km;
+        const float *sp = (const float *)&r.vs[p][i];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {  // 2^(e - E + 7) (below fp16's range: 0)
-          const int e = i < keep ? (int)(__float_as_uint(sp[i]) >> 23) - 127 - e_run + kVShift : -100;
-          fac[p][i >> 1][i & 1] = (_Float16)exp_bits(max(min(e, kVShift), -100));
+        for (int j = 0; j < 4; j++) {  // 2^(e - E + 7); below fp16's range 0
+          const int e = (int)(__float_as_uint(sp[j]) >> 23) - 127 - e_run + kVShift;
+          fac[i][j >> 1][j & 1] = (_Float16)exp_bits(max(min(e, kVShift), -100));
         }
       }
 #pragma unroll
       for (int c = 0; c < 4; c++) {
-        uint32_t r[4];
+        uint32_t u[4];
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
-          to_f16(w[p][c], r[2 * p], r[2 * p + 1]);
+        for (int i = 0; i < 2; i++) {
+          to_f16(w[i][c], u[2 * i], u[2 * i + 1]);
 #pragma unroll
-          for (int i = 0; i < 2; i++)
-            r[2 * p + i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, r[2 * p + i]) * fac[p][i]);
+          for (int j = 0; j < 2; j++)
+            u[2 * i + j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, u[2 * i + j]) * fac[i][j]);
         }
-        s_v[(h * 8 + 4 * qd + c) * 64 + l] = make_uint4(r[0], r[1], r[2], r[3]);
+        s_v[buf][pg][2 * (l >> 5) + (c >> 1)][32 * ((l >> 4) & 1) + 16 * (c & 1) + (l & 15)] =
+            make_uint4(u[0], u[1], u[2], u[3]);
       }
     }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < TILES; j++) {
-      f32x4 sc[kStepPages];
-      const int pos = ctx + tok[j];
-      float tmax = -INFINITY;
-#pragma unroll
-      for (int p = 0; p < kStepPages; p++) {
-        sc[p] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int f = 0; f < 4; f++) {
-          Frag8 kf;
-          kf.q = s_k[(p * 4 + f) * 64 + l];
-          sc[p] = mfma16x16x32(kf, qf[j][f], sc[p]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int key = k0 + 16 * p + 4 * lg + i;
-          if (key > pos || ((bad_pages >> p) & 1)) sc[p][i] = -INFINITY;
-          tmax = fmaxf(tmax, sc[p][i]);
-        }
-      }
-      tmax = max_xor32(max_xor16(tmax)) * a.qk_scale;
-      const float m_new = fmaxf(m_run[j], tmax), alpha = __builtin_amdgcn_exp2f(m_run[j] - m_new);
-      float psum = 0.0f;
-#pragma unroll
-      for (int cc = 0; cc < 8; cc++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[j][cc][i] *= alpha * e_alpha;
-#pragma unroll
-      for (int h = 0; h < kStepPages / 2; h++) {
-        FragH pf;
-#pragma unroll
-        for (int p = 0; p < 2; p++) {
-          float t[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            t[i] = __builtin_amdgcn_exp2f(fmaf(sc[2 * h + p][i], a.qk_scale, kPShift - m_new));
-            psum += t[i];
-          }
-          pf.u[2 * p] = pack_f16x2(t[0], t[1]);
-          pf.u[2 * p + 1] = pack_f16x2(t[2], t[3]);
-        }
-#pragma unroll
-        for (int cc = 0; cc < 8; cc++) {
-          FragH vf;
-          vf.q = s_v[(h * 8 + cc) * 64 + l];
-          o[j][cc] = mfma16x16x32_f16(vf, pf, o[j][cc]);
-        }
-      }
-      l_run[j] = fmaf(l_run[j], alpha, psum);
-      m_run[j] = m_new;
+  };
+
+  Staged<kPages> r;
+  request(r, page_ids(st0));
+  int ids = page_ids(st0 + 1);
+  float e_next = grow_unit(r, kStepKeys * st0);
+  uint32_t bad = r.bad;
+  convert(r, st0);
+  request(r, ids);
+  ids = page_ids(st0 + 2);
+  for (int st = st0; st < st1; st++) {
+    const int k0 = kStepKeys * st, buf = st & 1;
+    // every wave has written its share of this step and read the step before (a bare barrier: __syncthreads would
+    // also wait for the codes in flight)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const float e_alpha = e_next;
+    const uint32_t bad_pages = bad;
+    if (st + 1 < st1) {
+      e_next = grow_unit(r, k0 + kStepKeys);
+      bad = r.bad;
+      convert(r, st + 1);
+      request(r, ids);
+      ids = page_ids(st + 3);
     }
+    f32x16 sc[kStepPages / 2];
+#pragma unroll
+    for (int g = 0; g < kStepPages / 2; g++) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) sc[g][i] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 8; s++) {
+        Frag8 kf;
+        kf.q = s_k[buf][g][s][l];
+        sc[g] = mfma32x32x16(kf, qf[s], sc[g]);
+      }
+    }
+    // score i of a lane in key group g: key 32 g + 8 (i / 4) + 4 lh + i % 4
+    if (k0 + kStepKeys - 1 > first_pos || bad_pages) {
+#pragma unroll
+      for (int g = 0; g < kStepPages / 2; g++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int key = k0 + 32 * g + 8 * (i >> 2) + 4 * lh + (i & 3);
+          if (key > pos || ((bad_pages >> (2 * g + (i >> 3))) & 1)) sc[g][i] = -INFINITY;
+        }
+    }
+    float tmax = sc[0][0];
+#pragma unroll
+    for (int g = 0; g < kStepPages / 2; g++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) tmax = fmaxf(tmax, sc[g][i]);
+    tmax = max_xor32(tmax) * a.qk_scale;
+    const float m_new = fmaxf(m_run, tmax), alpha = __builtin_amdgcn_exp2f(m_run - m_new), scale_o = alpha * e_alpha;
+    if (__any(scale_o != 1.0f)) {
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[c][i] *= scale_o;
+    }
+    float psum = 0.0f;
+    const float off = kPShift - m_new;
+#pragma unroll
+    for (int p = 0; p < kStepPages; p++) {
+      FragH pf;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(sc[p >> 1][8 * (p & 1) + 2 * j], a.qk_scale, off));
+        const float y = __builtin_amdgcn_exp2f(fmaf(sc[p >> 1][8 * (p & 1) + 2 * j + 1], a.qk_scale, off));
+        psum += x + y;
+        pf.u[j] = pack_f16x2(x, y);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        FragH vf;
+        vf.q = s_v[buf][p][c][l];
+        o[c] = mfma32x32x16_f16(vf, pf, o[c]);
+      }
+    }
+    l_run = fmaf(l_run, alpha, psum);
+    m_run = m_new;
   }
   const float unit = exp_bits(e_run - kVShift);
+  const float l_tot = sum_xor32(l_run);
+  const int parts = pos / kPartKeys + 1;
+  if (t >= len || part >= parts) return;  // (a token before this part's keys: finished by its own last part)
+  const long long hrow = (long long)(row0 + tok) * a.H + kvh * G + lr % G;
+  if (parts == 1) {
+    const float inv = l_tot == 0.0f ? 0.0f : unit / l_tot;
 #pragma unroll
-  for (int j = 0; j < TILES; j++) {
-    const float l_tot = sum_xor32(sum_xor16(l_run[j]));
-    if (!store[j]) continue;
-    const int parts = (ctx + tok[j]) / kPartKeys + 1;
-    if (part >= parts) continue;  // (a token before this part's keys: finished by its own last part)
-    const long long hrow = (long long)(row0 + tok[j]) * a.H + kvh * G + lr % G;
-    if (parts == 1) {
-      const float inv = l_tot == 0.0f ? 0.0f : unit / l_tot;
+    for (int c = 0; c < 4; c++)
 #pragma unroll
-      for (int cc = 0; cc < 8; cc++) {
+      for (int i = 0; i < 4; i++) {
         uint2 w;
-        w.x = pack_bf16x2(o[j][cc][0] * inv, o[j][cc][1] * inv);
-        w.y = pack_bf16x2(o[j][cc][2] * inv, o[j][cc][3] * inv);
-        *(uint2 *)(a.out + hrow * kD + 16 * cc + 4 * lg) = w;
+        w.x = pack_bf16x2(o[c][4 * i] * inv, o[c][4 * i + 1] * inv);
+        w.y = pack_bf16x2(o[c][4 * i + 2] * inv, o[c][4 * i + 3] * inv);
+        *(uint2 *)(a.out + hrow * kD + 32 * c + 8 * i + 4 * lh) = w;
       }
-    } else {
-      float *ps = a.part + (((long long)(row0 + tok[j]) * a.pmax + part) * a.H + kvh * G + lr % G) * kPfSlot;
+  } else {
+    float *ps = a.part + (((long long)(row0 + tok) * a.pmax + part) * a.H + kvh * G + lr % G) * kPfSlot;
 #pragma unroll
-      for (int cc = 0; cc < 8; cc++)
-        *(float4 *)(ps + 16 * cc + 4 * lg) =
-            make_float4(o[j][cc][0] * unit, o[j][cc][1] * unit, o[j][cc][2] * unit, o[j][cc][3] * unit);
-      if (lg == 0) *(float2 *)(ps + kD) = make_float2(m_run[j], l_tot);
-    }
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        *(float4 *)(ps + 32 * c + 8 * i + 4 * lh) = make_float4(o[c][4 * i] * unit, o[c][4 * i + 1] * unit,
+                                                                o[c][4 * i + 2] * unit, o[c][4 * i + 3] * unit);
+    if (lh == 0) *(float2 *)(ps + kD) = make_float2(m_run, l_tot);
   }
 }
 
@@ -578,7 +640,7 @@ extern "C" int jit_paged_prefill_attn_kv8(const uint16_t *q, const void *pool, i
                       chunk_row, out, (float *)workspace, num_pages, max_pages, H, Hkv, H / Hkv, pmax,
                       scale * 1.44269504088896341f};
   const hipStream_t st = (hipStream_t)stream;
-  kv8_prefill_kernel<kPfWaves, kPfTiles><<<dim3(nblk * Hkv), 64 * kPfWaves, 0, st>>>(a);
+  kv8_prefill_kernel<8><<<dim3(nblk * Hkv), 64 * 8, 0, st>>>(a);
   const int rc = jit::check_launch("jit_paged_prefill_attn_kv8");
   if (rc || pmax == 1 || max_len == 0) return rc;
   kv8_prefill_merge_kernel<<<dim3(max_len, C), 8 * H, 0, st>>>(a);
