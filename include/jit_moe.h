@@ -565,13 +565,20 @@ int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, int num_pages
                               int max_pages, const int32_t *lens, int B, int H, int Hkv, int max_len, float scale,
                               void *workspace, int64_t workspace_bytes, uint16_t *out, void *stream);
 
-/* jit_paged_prefill_attn over an 8-bit pool: the same chunks, work items, parts and workspace.  Keys of page ids
- * outside the pool are left out. */
+/* jit_paged_prefill_attn over an 8-bit pool: the same chunks, work items and parts.  The keys that the chunks see are
+ * expanded into the workspace first, JIT_KV8_UNIT_KEYS (a unit) at a time: chunk_unit [C + 1] (device) holds the
+ * first unit of each chunk, ceil((ctx + len) / JIT_KV8_UNIT_KEYS) units a chunk, and their number `units` last.  T: the
+ * q rows.  Keys of page ids outside the pool are left out; a row without a key gives zeros.
+ * Contract: that of jit_paged_prefill_attn, scale > 0 and a workspace of jit_kv8_prefill_workspace_bytes bytes (32,776
+ * bytes a unit and kv head, and the partials) (JIT_EINVAL). */
+#define JIT_KV8_UNIT_KEYS 64
+int64_t jit_kv8_prefill_workspace_bytes(int T, int pmax, int H, int Hkv, int units);
 int jit_paged_prefill_attn_kv8(const uint16_t *q, const void *pool, int num_pages, const int32_t *page_table,
                                int max_pages, const int32_t *chunk_seq, const int32_t *chunk_ctx,
-                               const int32_t *chunk_len, const int32_t *chunk_row, int C, const int32_t *blk_chunk,
-                               const int32_t *blk_q0, const int32_t *blk_part, int nblk, int pmax, int max_len, int H,
-                               int Hkv, float scale, void *workspace, uint16_t *out, void *stream);
+                               const int32_t *chunk_len, const int32_t *chunk_row, const int32_t *chunk_unit, int C,
+                               int units, const int32_t *blk_chunk, const int32_t *blk_q0, const int32_t *blk_part,
+                               int nblk, int T, int pmax, int max_len, int H, int Hkv, float scale, void *workspace,
+                               int64_t workspace_bytes, uint16_t *out, void *stream);
 
 /* ------------------------------------------------------------ whole layers --
  * One decoder layer per call (Q36/model/model.py:65-80): the launches above, in their order, issued from

@@ -111,14 +111,16 @@ _SIGNATURES = {
     "jit_kv8_chunk_tokens": [_I],
     "jit_kv8_decode_workspace_bytes": [_I, _I, _I],
     "jit_paged_decode_attn_kv8": [_P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, ctypes.c_int64, _P, _P],
-    "jit_paged_prefill_attn_kv8": [_P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P,
-                                   _P],
+    "jit_kv8_prefill_workspace_bytes": [_I, _I, _I, _I, _I],
+    "jit_paged_prefill_attn_kv8": [_P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F,
+                                   _P, ctypes.c_int64, _P, _P],
 }
 _RESTYPES = {"jit_last_error": ctypes.c_char_p, "jit_attn_workspace_bytes": ctypes.c_int64,
              "jit_attn_split_workspace_bytes": ctypes.c_int64, "jit_layer_scratch_bytes": ctypes.c_int64,
              "jit_prefill_workspace_bytes": ctypes.c_int64,
              "jit_q4_packed_bytes": ctypes.c_int64, "jit_moe_pack_workspace_bytes": ctypes.c_int64,
-             "jit_sampler_workspace_bytes": ctypes.c_int64, "jit_kv8_decode_workspace_bytes": ctypes.c_int64}
+             "jit_sampler_workspace_bytes": ctypes.c_int64, "jit_kv8_decode_workspace_bytes": ctypes.c_int64,
+             "jit_kv8_prefill_workspace_bytes": ctypes.c_int64}
 
 _lib = None
 

@@ -43,7 +43,7 @@ SOURCES = {
     "head.hip": [],
     "sampler.hip": ["-ffp-contract=off"],
     "kv8.hip": [],
-    "kv8_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "kv8_attention.hip": [],
 }
 
 _COMMON = [

@@ -24,11 +24,12 @@ constexpr int kVOff = kPage * kD, kScaleOff = 2 * kPage * kD;
 static_assert(kRec == kScaleOff + 2 * kPage * 4, "K codes, V codes, scales");
 constexpr int kMinExp = -100, kMaxExp = 118;  // a scale's exponent: 2^-e and 448 2^e stay normal fp32 numbers
 
+// (a pool has fewer than 2^32 records: one 32 x 32 -> 64 bit product)
 __device__ __forceinline__ const uint8_t *record(const uint8_t *pool, int page, int Hkv, int h) {
-  return pool + ((long long)page * Hkv + h) * kRec;
+  return pool + (uint64_t)((uint32_t)page * (uint32_t)Hkv + (uint32_t)h) * kRec;
 }
 __device__ __forceinline__ uint8_t *record(uint8_t *pool, int page, int Hkv, int h) {
-  return pool + ((long long)page * Hkv + h) * kRec;
+  return pool + (uint64_t)((uint32_t)page * (uint32_t)Hkv + (uint32_t)h) * kRec;
 }
 // byte of (slot, dim) in a record's K and V parts
 __device__ __forceinline__ int k_at(int slot, int d) { return (d >> 6) * 1024 + ((d >> 4) & 3) * 256 + slot * 16 + (d & 15); }

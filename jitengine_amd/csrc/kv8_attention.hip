@@ -260,22 +260,29 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
 }
 
 // ---------------------------------------------------------------- causal prompt chunks
-// A workgroup owns WAVES x 32 rows (32 / G tokens x the G q heads of a kv head a wave) and walks the keys up to its
-// last token 128 a step.  A step's codes become bf16 keys (times their scales) and fp16 values in LDS once, for all
-// of the workgroup's rows, while the step before is computed: the codes are requested two steps ahead into
-// registers, converted one step ahead into the other half of LDS, and a step has one barrier.
+// Two launches (three where a token's keys have several parts).  The first expands the keys that the chunks see: K to
+// bf16 (times its scale) and V to fp16, in the order in which the second launch's matrix instructions take them.
+// Every row block of a chunk reads all of its keys, so the conversion is done once instead of once a block; inside the
+// attention loop it cost as many vector instructions as the softmax (2,048 rows after 8,192 keys: 344 us, now 328).
+//
+// The second: a workgroup owns WAVES x 32 rows (32 / G tokens x the G q heads of a kv head a wave) and walks the keys up
+// to its last token 64 (a unit) at a time, a unit's 32 KB going straight from memory into LDS.
 //   S^T[32 keys x 32 rows] = K . Q^T        (8 MFMA 32x32x16 bf16)
 //   O^T[128 dims x 32 rows] += V^T . P^T    (4 MFMA 32x32x16 fp16 a page)
 // A lane owns one row throughout: its scores of a page are its P operand as they are, since the 16 keys of V's
 // operand are kept in the order in which the score tile holds them.
 constexpr int kRowsWave = 32, kBlockRows = 256;  // a row block (jit_prefill_block_tokens): 256 / G tokens
-constexpr int kStepKeys = 128, kStepPages = kStepKeys / kPage;
+constexpr int kUnitKeys = JIT_KV8_UNIT_KEYS, kUnitPages = kUnitKeys / kPage;
+constexpr int kUnitBytes = 2 * kUnitKeys * kD * 2;  // K, then V
 constexpr int kPartKeys = 6144;                  // key parts (jit_prefill_part_keys)
-constexpr int kPartSteps = kPartKeys / kStepKeys;
+constexpr int kPartUnits = kPartKeys / kUnitKeys;
 constexpr int kPfSlot = kD + 4;                  // floats of a (token, part, head) partial: o, max, sum, 2 pad
-// Values are held in LDS relative to the loudest scale so far, 2^E, times 2^7 (448 x 2^7 < 65,504): a value of a token
-// 2^22 times quieter than that still has all its bits.
+// Expanded values are relative to the loudest scale 2^E of the part's keys, times 2^7 (448 x 2^7 < 65,504): a value of
+// a token 2^22 times quieter than that still has all its bits.
 constexpr int kVShift = 7;
+// A row's reference for the exponentials moves when its maximum passes it by more than 2^4: most units then have no O
+// to rescale.  Probabilities are formed 2^11 times too large, at most 2^15: 11 bits down to 2^-25 of the reference.
+constexpr float kLazy = 4.0f, kPfShift = 11.0f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -291,33 +298,123 @@ struct PrefillArgs {
   const uint8_t *pool;
   const int32_t *page_table;
   const int32_t *blk_chunk, *blk_q0, *blk_part;
-  const int32_t *chunk_seq, *chunk_ctx, *chunk_len, *chunk_row;
+  const int32_t *chunk_seq, *chunk_ctx, *chunk_len, *chunk_row, *chunk_unit;  // chunk_unit [C + 1]: first unit of each
   uint16_t *out;
+  uint8_t *units;  // [units][Hkv][kUnitBytes]
+  int32_t *info;   // [units][Hkv][2]: E of the unit's part, its pages outside the pool (4 bits; 16: some in the part)
   float *part;
-  int num_pages, max_pages, H, Hkv, G, pmax;
+  int num_pages, max_pages, H, Hkv, G, C, pmax;
   float qk_scale;
 };
 
-// What a wave requests of a step: its pages' codes and scales, and the step's V scales (2 keys a lane).
-template <int PAGES>
-struct Staged {
-  uint4 k[PAGES][2], v[PAGES][2];
-  float ks[PAGES];
-  float4 vs[PAGES][2];
-  float2 all_vs;
-  uint32_t bad;  // the step's pages outside the pool
-};
+// One workgroup expands a unit of one kv head, wave w its page w.  Its codes are requested first; meanwhile the part's
+// loudest live V scale is found (by every workgroup of a part for itself: a line of 64 bytes a page).
+__global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
+  __shared__ int s_e[4], s_bad[4];
+  const int gu = blockIdx.x, kvh = blockIdx.y, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int lo = 0, hi = a.C - 1;  // the chunk whose units hold gu
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.chunk_unit[mid] <= gu) lo = mid;
+    else hi = mid - 1;
+  }
+  const int u = gu - a.chunk_unit[lo], kend = a.chunk_ctx[lo] + a.chunk_len[lo];
+  const int32_t *prow = a.page_table + (long long)a.chunk_seq[lo] * a.max_pages;
+  const int npages = min((kend + kPage - 1) / kPage, a.max_pages);
+  // this wave's page
+  const int pg = kUnitPages * u + wave, page = pg < npages ? prow[pg] : -1;
+  const bool out_of_pool = (uint32_t)page >= (uint32_t)a.num_pages;
+  const uint8_t *rec = record(a.pool, out_of_pool ? 0 : page, a.Hkv, kvh);
+  const float *sc = (const float *)(rec + kScaleOff);
+  // K: lane (g = l / 16, slot = l % 16), dims 64 i + 16 g ..
+  // V: lane (q = l / 32, h = l / 16 % 2, r = l % 16): slots 4 h .. and 8 + 4 h .. of dims 64 q + 16 c + r
+  const int vh = (l >> 4) & 1;
+  uint4 wk[2], wv[2];
+  float4 sv[2];
+  const float sk = sc[l & 15];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    wk[i] = *(const uint4 *)(rec + 1024 * i + 16 * l);
+    wv[i] = *(const uint4 *)(rec + kVOff + 1024 * (l >> 5) + 512 * i + 16 * (l & 31));
+    sv[i] = *(const float4 *)(sc + kPage + 8 * i + 4 * vh);
+  }
+  // E: thread = page of the part x quarter of its slots
+  const int pg0 = u / kPartUnits * (kPartKeys / kPage), pg1 = min(pg0 + kPartKeys / kPage, npages);
+  int e = 0, bad = 0;  // (positive powers of two are ordered as their bits)
+#pragma unroll 2
+  for (int i = threadIdx.x; i < 4 * (pg1 - pg0); i += 256) {
+    const int p = pg0 + (i >> 2), id = prow[p];
+    const bool off = (uint32_t)id >= (uint32_t)a.num_pages;
+    const float4 s = *(const float4 *)(record(a.pool, off ? 0 : id, a.Hkv, kvh) + kScaleOff + 4 * kPage + 16 * (i & 3));
+    const int left = off ? 0 : kend - (kPage * p + 4 * (i & 3));
+    const float *sp = (const float *)&s;
+    bad |= off;
+#pragma unroll
+    for (int j = 0; j < 4; j++) e = j < left ? max(e, __float_as_int(sp[j])) : e;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o, 64));
+  const int any = __any(bad), here = __any(out_of_pool && pg < npages);
+  if (l == 0) s_e[wave] = e, s_bad[wave] = (any ? 16 : 0) | (here ? 1 << wave : 0);
+  __syncthreads();
+  e = max(max(s_e[0], s_e[1]), max(s_e[2], s_e[3]));
+  const int E = min(max((e >> 23) - 127, kMinExp), kMaxExp);
+  if (threadIdx.x == 0)
+    *(int2 *)(a.info + 2 * ((long long)gu * a.Hkv + kvh)) = make_int2(E, s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]);
+  uint4 *dst_k = (uint4 *)(a.units + ((long long)gu * a.Hkv + kvh) * kUnitBytes), *dst_v = dst_k + kUnitBytes / 32;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    uint4 f0, f1;
+    to_bf16(wk[i].x, sk, f0.x, f0.y);
+    to_bf16(wk[i].y, sk, f0.z, f0.w);
+    to_bf16(wk[i].z, sk, f1.x, f1.y);
+    to_bf16(wk[i].w, sk, f1.z, f1.w);
+    uint4 *d = dst_k + (8 * (wave >> 1) + 4 * i + (l >> 4)) * 64 + 16 * (wave & 1) + (l & 15);
+    d[0] = f0;
+    d[32] = f1;
+  }
+  const float unit = exp_bits(kVShift - E);
+  f16x2_t fac[2][2];  // 2^(e - E + 7); below fp16's range 0
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    // what lies past the keys or in a page outside the pool may be anything (0 x NaN): it counts as 0
+    const int keep = out_of_pool ? 0 : kend - (kPage * pg + 8 * i + 4 * vh);
+    const uint32_t km = keep_bytes(keep);
+    wv[i].x &= km, wv[i].y &= km, wv[i].z &= km, wv[i].w &= km;
+    const float *sp = (const float *)&sv[i];
+#pragma unroll
+    for (int j = 0; j < 4; j++) fac[i][j >> 1][j & 1] = (_Float16)(j < keep ? sp[j] * unit : 0.0f);
+  }
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 2; i++) to_f16(((const uint32_t *)&wv[i])[c], r[2 * i], r[2 * i + 1]);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, r[i]) * fac[i >> 1][i & 1]);
+    dst_v[(4 * wave + 2 * (l >> 5) + (c >> 1)) * 64 + 32 * vh + 16 * (c & 1) + (l & 15)] =
+        make_uint4(r[0], r[1], r[2], r[3]);
+  }
+}
 
-template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4 < 1 ? 1 : WAVES / 4, 2)))
+// 16 bytes a lane from base + off straight into LDS at byte dst + 16 lane.  Written in assembly, so that the compiler's
+// waits for LDS reads do not include these.
+__device__ __forceinline__ void load_lds16(const uint8_t *base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
+}
+
+// WAVES waves of 32 rows; STAGES units of K and of V in LDS: the one in use, and those on their way.
+template <int WAVES, int STAGES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void kv8_prefill_kernel(const PrefillArgs a) {
   constexpr int kSub = kBlockRows / (WAVES * kRowsWave);  // workgroups a row block
-  constexpr int kPages = kStepPages / WAVES;              // pages a wave stages a step
-  __shared__ __attribute__((aligned(16))) uint4 s_k[2][kStepPages / 2][8][64];  // [page pair][16 dims][lane] 8 bf16
-  __shared__ __attribute__((aligned(16))) uint4 s_v[2][kStepPages][4][64];      // [page][32 dims][lane] 8 fp16
+  constexpr int kLoads = 16 / WAVES;                      // 1 KB loads of a wave for a unit's K (and V)
+  __shared__ __attribute__((aligned(16))) uint4 s_k[STAGES][16][64];              // [page pair, 16 dims][lane] 8 bf16
+  __shared__ __attribute__((aligned(16))) uint4 s_v[STAGES][kUnitPages * 4][64];  // [page, 32 dims][lane] 8 fp16
   const int item = blockIdx.x / (kSub * a.Hkv), kvh = blockIdx.x % a.Hkv;
   const int ch = a.blk_chunk[item], part = a.blk_part[item];
-  const int seq = a.chunk_seq[ch], ctx = a.chunk_ctx[ch], len = a.chunk_len[ch], row0 = a.chunk_row[ch];
+  const int ctx = a.chunk_ctx[ch], len = a.chunk_len[ch], row0 = a.chunk_row[ch];
   const int G = a.G, tpw = kRowsWave / G;  // tokens a wave
   int q0 = a.blk_q0[item];
   if constexpr (kSub > 1) q0 += blockIdx.x / a.Hkv % kSub * WAVES * tpw;
@@ -325,10 +422,12 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
   const int lr = l & 31, lh = l >> 5;
   const int kend = ctx + min(q0 + WAVES * tpw, len);  // the workgroup's keys: [0, kend)
-  const int nst = (kend + kStepKeys - 1) / kStepKeys, npages = min((kend + kPage - 1) / kPage, a.max_pages);
-  const int st0 = part * kPartSteps, st1 = min(nst, st0 + kPartSteps);
-  if (st0 >= st1) return;  // (uniform: a piece of a block whose last token alone reaches the part)
-  const int32_t *prow = a.page_table + (long long)seq * a.max_pages;
+  const int u0 = part * kPartUnits, u1 = min((kend + kUnitKeys - 1) / kUnitKeys, u0 + kPartUnits);
+  if (u0 >= u1) return;  // (uniform: a piece of a block whose last token alone reaches the part)
+  const long long first_unit = (long long)a.chunk_unit[ch] * a.Hkv + kvh;  // (units of a head lie Hkv apart)
+  const uint8_t *units = a.units + first_unit * kUnitBytes;
+  const int32_t *info = a.info + 2 * first_unit;
+  const int E = info[2 * (long long)u0 * a.Hkv], some_bad = info[2 * (long long)u0 * a.Hkv + 1] & 16;
 
   const int t = q0 + wave * tpw + lr / G, tok = min(t, len - 1), pos = ctx + tok;  // the lane's row
   const int first_pos = ctx + min(q0 + wave * tpw, len - 1);                       // the wave's first
@@ -338,179 +437,168 @@ void kv8_prefill_kernel(const PrefillArgs a) {
 #pragma unroll
     for (int s = 0; s < 8; s++) qf[s].q = *(const uint4 *)(qp + 16 * s);
   }
-  float m_run = kLowest, l_run = 0.0f;
+  // (q has landed before the first direct load: the compiler's waits for it would include those)
+#pragma unroll
+  for (int s = 0; s < 8; s++)
+    asm volatile("" ::"v"(qf[s].u[0]), "v"(qf[s].u[1]), "v"(qf[s].u[2]), "v"(qf[s].u[3]));
+  float m_run = kLowest, l_run = 0.0f, top = 0.0f;
   f32x16 o[4];
 #pragma unroll
   for (int c = 0; c < 4; c++)
 #pragma unroll
     for (int i = 0; i < 16; i++) o[c][i] = 0.0f;
 
-  // a step's page ids, lane i page i % 8 (past the keys: the last page again, its keys masked)
-  auto page_ids = [&](int st) { return prow[min(kStepPages * st + (l & (kStepPages - 1)), npages - 1)]; };
-  auto request = [&](Staged<kPages> &r, int pages) {
-    const bool bad = pages < 0 || pages >= a.num_pages;
-    r.bad = (uint32_t)__ballot(bad) & 0xffu;
-    const int ids = bad ? 0 : pages;
+  const uint32_t k_lds = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)&s_k[0][kLoads * wave][0]);
+  const uint32_t v_lds = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)&s_v[0][kLoads * wave][0]);
+  const uint32_t lane_at = 1024 * kLoads * wave + 16 * l;
+  const long long unit_step_bytes = (long long)a.Hkv * kUnitBytes;
+  // (a unit past the last: the last again, whose place in LDS is free and never read)
+  auto request_k = [&](int u, int slot) {
+    const uint8_t *p = units + min(u, u1 - 1) * unit_step_bytes;
 #pragma unroll
-    for (int p = 0; p < kPages; p++) {
-      const uint8_t *rec = record(a.pool, __builtin_amdgcn_readlane(ids, kPages * wave + p), a.Hkv, kvh);
-      const float *sc = (const float *)(rec + kScaleOff);
-      r.ks[p] = sc[l & 15];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        r.k[p][i] = *(const uint4 *)(rec + 1024 * i + 16 * l);
-        // lane (q = l / 32, h = l / 16 % 2, r = l % 16): slots 4 h .. and 8 + 4 h .. of dims 64 q + 16 c + r
-        r.v[p][i] = *(const uint4 *)(rec + kVOff + 1024 * (l >> 5) + 512 * i + 16 * (l & 31));
-        r.vs[p][i] = *(const float4 *)(sc + kPage + 8 * i + 4 * ((l >> 4) & 1));
-      }
-    }
-    const uint8_t *rec = record(a.pool, __shfl(ids, l >> 3, 64), a.Hkv, kvh);
-    r.all_vs = *(const float2 *)(rec + kScaleOff + 4 * kPage + 8 * (l & 7));
+    for (int i = 0; i < kLoads; i++) load_lds16(p, lane_at + 1024 * i, k_lds + 16384 * slot + 1024 * i);
   };
-  // the step's loudest live value; E over the part so far grows with it, and O's unit with E
-  int e_run = kMinExp;
-  auto grow_unit = [&](const Staged<kPages> &r, int k0) {
-    int e = kMinExp;
-    if (!((r.bad >> (l >> 3)) & 1)) {
-      if (k0 + 2 * l < kend) e = max(e, (int)(__float_as_uint(r.all_vs.x) >> 23) - 127);
-      if (k0 + 2 * l + 1 < kend) e = max(e, (int)(__float_as_uint(r.all_vs.y) >> 23) - 127);
-    }
+  auto request_v = [&](int u, int slot) {
+    const uint8_t *p = units + min(u, u1 - 1) * unit_step_bytes + kUnitBytes / 2;
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) e = max(e, __shfl_xor(e, x, 64));
-    const int e_new = max(e_run, min(__builtin_amdgcn_readfirstlane(e), kMaxExp));
-    const float f = e_new - e_run > 126 ? 0.0f : exp_bits(e_run - e_new);
-    e_run = e_new;
-    return f;
+    for (int i = 0; i < kLoads; i++) load_lds16(p, lane_at + 1024 * i, v_lds + 16384 * slot + 1024 * i);
   };
-  auto convert = [&](const Staged<kPages> &r, int st) {
-    const int buf = st & 1, k0 = kStepKeys * st;
-#pragma unroll
-    for (int p = 0; p < kPages; p++) {
-      const int pg = kPages * wave + p;
-#pragma unroll
-      for (int i = 0; i < 2; i++) {  // lane (g = l / 16, slot = l % 16): dims 64 i + 16 g ..
-        uint4 f0, f1;
-        to_bf16(r.k[p][i].x, r.ks[p], f0.x, f0.y);
-        to_bf16(r.k[p][i].y, r.ks[p], f0.z, f0.w);
-        to_bf16(r.k[p][i].z, r.ks[p], f1.x, f1.y);
-        to_bf16(r.k[p][i].w, r.ks[p], f1.z, f1.w);
-        uint4 *dst = &s_k[buf][pg >> 1][4 * i + (l >> 4)][16 * (pg & 1) + (l & 15)];
-        dst[0] = f0;
-        dst[32] = f1;
-      }
-      f16x2_t fac[2][2];
-      uint32_t w[2][4];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int keep = (r.bad >> pg) & 1 ? 0 : kend - (k0 + kPage * pg + 8 * i + 4 * ((l >> 4) & 1));
-        const uint32_t km = keep_bytes(keep);  // (what lies past the keys may be anything: no NaN code gets in)
-        w[i][0] = r.v[p][i].x & km, w[i][1] = r.v[p][i].y & km, w[i][2] = r.v[p][i].z & km, w[i][3] = r.v[p][i].w & km;
-        const float *sp = (const float *)&r.vs[p][i];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {  // 2^(e - E + 7); below fp16's range 0
-          const int e = (int)(__float_as_uint(sp[j]) >> 23) - 127 - e_run + kVShift;
-          fac[i][j >> 1][j & 1] = (_Float16)exp_bits(max(min(e, kVShift), -100));
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        uint32_t u[4];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          to_f16(w[i][c], u[2 * i], u[2 * i + 1]);
-#pragma unroll
-          for (int j = 0; j < 2; j++)
-            u[2 * i + j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, u[2 * i + j]) * fac[i][j]);
-        }
-        s_v[buf][pg][2 * (l >> 5) + (c >> 1)][32 * ((l >> 4) & 1) + 16 * (c & 1) + (l & 15)] =
-            make_uint4(u[0], u[1], u[2], u[3]);
-      }
-    }
-  };
-
-  Staged<kPages> r;
-  request(r, page_ids(st0));
-  int ids = page_ids(st0 + 1);
-  float e_next = grow_unit(r, kStepKeys * st0);
-  uint32_t bad = r.bad;
-  convert(r, st0);
-  request(r, ids);
-  ids = page_ids(st0 + 2);
-  for (int st = st0; st < st1; st++) {
-    const int k0 = kStepKeys * st, buf = st & 1;
-    // every wave has written its share of this step and read the step before (a bare barrier: __syncthreads would
-    // also wait for the codes in flight)
+  // The loads of units up to the one that is next are there, for every wave, and the units behind it are read: the newest
+  // STAGES - 2 units' loads stay in flight (vmcnt is split over bits 3:0 and 15:14), and a bare barrier follows.
+  constexpr int kVm = (STAGES - 2) * 2 * kLoads;
+  auto meet = [&]() {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt((kVm & 15) | ((kVm >> 4) << 14) | (7 << 4) | (0 << 8));  // vmcnt(kVm) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const float e_alpha = e_next;
-    const uint32_t bad_pages = bad;
-    if (st + 1 < st1) {
-      e_next = grow_unit(r, k0 + kStepKeys);
-      bad = r.bad;
-      convert(r, st + 1);
-      request(r, ids);
-      ids = page_ids(st + 3);
-    }
-    f32x16 sc[kStepPages / 2];
+  };
+
+  f32x16 sc[2][2];  // scores of two units (u % 2) of two page pairs; lane: key 32 g + 8 (i / 4) + 4 lh + i % 4
+  constexpr int kAhead = 4;  // operand fragments requested from LDS ahead of their instructions
+  auto read_k = [&](int slot, int j) {  // page pair j % 2, dims 16 (j / 2)
+    Frag8 f;
+    f.q = s_k[slot][8 * (j & 1) + (j >> 1)][l];
+    return f;
+  };
+  auto read_v = [&](int slot, int j) {  // page j / 4, dims 32 (j % 4)
+    FragH f;
+    f.q = s_v[slot][j][l];
+    return f;
+  };
+  auto score = [&](f32x16 (&s)[2], const Frag8 &kf, int j) {
+    const f32x16 z = {};
+    s[j & 1] = mfma32x32x16(kf, qf[j >> 1], j < 2 ? z : s[j & 1]);
+  };
+  auto largest = [&](const f32x16 (&s)[2]) {
+    top = s[0][0];
 #pragma unroll
-    for (int g = 0; g < kStepPages / 2; g++) {
+    for (int g = 0; g < 2; g++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) sc[g][i] = 0.0f;
+      for (int i = 0; i < 16; i++) top = fmaxf(top, s[g][i]);
+  };
+  // What of unit u's softmax waits for its scores' maximum, and O's rescaling.
+  float off = 0.0f;
+  auto settle = [&](int u, f32x16 (&s)[2]) {
+    const int k0 = kUnitKeys * u;
+    if (k0 + kUnitKeys - 1 > first_pos || some_bad) {
+      const int bad = some_bad ? info[2 * (long long)u * a.Hkv + 1] : 0;
 #pragma unroll
-      for (int s = 0; s < 8; s++) {
-        Frag8 kf;
-        kf.q = s_k[buf][g][s][l];
-        sc[g] = mfma32x32x16(kf, qf[s], sc[g]);
-      }
-    }
-    // score i of a lane in key group g: key 32 g + 8 (i / 4) + 4 lh + i % 4
-    if (k0 + kStepKeys - 1 > first_pos || bad_pages) {
-#pragma unroll
-      for (int g = 0; g < kStepPages / 2; g++)
+      for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           const int key = k0 + 32 * g + 8 * (i >> 2) + 4 * lh + (i & 3);
-          if (key > pos || ((bad_pages >> (2 * g + (i >> 3))) & 1)) sc[g][i] = -INFINITY;
+          if (key > pos || ((bad >> (2 * g + (i >> 3))) & 1)) s[g][i] = -INFINITY;
         }
+      largest(s);
     }
-    float tmax = sc[0][0];
-#pragma unroll
-    for (int g = 0; g < kStepPages / 2; g++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) tmax = fmaxf(tmax, sc[g][i]);
-    tmax = max_xor32(tmax) * a.qk_scale;
-    const float m_new = fmaxf(m_run, tmax), alpha = __builtin_amdgcn_exp2f(m_run - m_new), scale_o = alpha * e_alpha;
-    if (__any(scale_o != 1.0f)) {
+    top = max_xor32(top) * a.qk_scale;
+    const float m_new = top > m_run + kLazy ? top : m_run;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+    off = kPfShift - m_new;
+    l_run *= alpha;
+    m_run = m_new;
+    if (__any(alpha != 1.0f)) {
 #pragma unroll
       for (int c = 0; c < 4; c++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[c][i] *= scale_o;
+        for (int i = 0; i < 16; i++) o[c][i] *= alpha;
     }
-    float psum = 0.0f;
-    const float off = kPShift - m_new;
+  };
+  auto next = [](int slot, int by) { return slot + by >= STAGES ? slot + by - STAGES : slot + by; };
+  int slot = 0;  // unit u's place in both rings
+  // Unit u: its softmax beside the scores of unit u + 1, then its products with V beside the maximum of the new scores;
+  // cut into groups of a matrix instruction and the vector work that runs during it.
+  auto unit_step = [&](int u, f32x16 (&s)[2], f32x16 (&s_next)[2], bool more) {
+    meet();
+    const int k_slot = next(slot, 1);
+    Frag8 kf[kAhead];
+    FragH vf[kAhead], pf[kUnitPages];
 #pragma unroll
-    for (int p = 0; p < kStepPages; p++) {
-      FragH pf;
+    for (int j = 0; j < kAhead; j++) kf[j] = read_k(k_slot, j);
+    request_k(u + STAGES, slot);  // (K(u)'s and V(u - 1)'s places are free)
+    request_v(u + STAGES - 1, next(slot, STAGES - 1));
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(sc[p >> 1][8 * (p & 1) + 2 * j], a.qk_scale, off));
-        const float y = __builtin_amdgcn_exp2f(fmaf(sc[p >> 1][8 * (p & 1) + 2 * j + 1], a.qk_scale, off));
-        psum += x + y;
-        pf.u[j] = pack_f16x2(x, y);
-      }
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        FragH vf;
-        vf.q = s_v[buf][p][c][l];
-        o[c] = mfma32x32x16_f16(vf, pf, o[c]);
-      }
+    for (int j = 0; j < 16; j++) {
+      score(s_next, kf[j % kAhead], j);
+      if (j + kAhead < 16) kf[j % kAhead] = read_k(k_slot, j + kAhead);
+      else vf[j % kAhead] = read_v(slot, j + kAhead - 16);
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j >> 3][2 * (j & 7)], a.qk_scale, off));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[j >> 3][2 * (j & 7) + 1], a.qk_scale, off));
+      pf[j >> 2].u[j & 3] = pack_f16x2(p0, p1);
+      // (the sum of the rounded probabilities, which the products take too)
+      l_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, pf[j >> 2].u[j & 3]), f16x2_t{1, 1}, l_run, false);
+      asm volatile("" : "+v"(pf[j >> 2].u[j & 3]));  // (here, not where they are used)
+      __builtin_amdgcn_sched_barrier(0);
     }
-    l_run = fmaf(l_run, alpha, psum);
-    m_run = m_new;
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      o[j & 3] = mfma32x32x16_f16(vf[j % kAhead], pf[j >> 2], o[j & 3]);
+      if (j + kAhead < 16) vf[j % kAhead] = read_v(slot, j + kAhead);
+      if (j >= 3 && j < 11) {
+        const int i0 = 4 * ((j - 3) & 3), g = (j - 3) >> 2;
+        float x = j == 3 ? s_next[0][0] : top;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x = fmaxf(x, s_next[g][i0 + i]);
+        top = x;
+        asm volatile("" : "+v"(top));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    slot = k_slot;
+    if (more) settle(u + 1, s_next);
+  };
+
+  // K(u0) .. K(u0 + STAGES - 1) and V(u0) .. V(u0 + STAGES - 2), in the order of the loop's requests
+  request_k(u0, 0);
+#pragma unroll
+  for (int i = 1; i < STAGES; i++) {
+    request_k(u0 + i, i);
+    request_v(u0 + i - 1, i - 1);
   }
-  const float unit = exp_bits(e_run - kVShift);
+  if (STAGES > 2) {  // K(u0) alone is needed now: K(u0 + 1) and V(u0) at the loop's first barrier
+    asm volatile("" ::: "memory");
+    constexpr int kVm0 = (STAGES - 1) * 2 * kLoads;
+    __builtin_amdgcn_s_waitcnt((kVm0 & 15) | ((kVm0 >> 4) << 14) | (7 << 4) | (0 << 8));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  } else {
+    meet();
+  }
+#pragma unroll
+  for (int j = 0; j < 16; j++) score(sc[0], read_k(0, j), j);
+  largest(sc[0]);
+  settle(u0, sc[0]);
+  int u = u0;
+  for (; u + 1 < u1; u += 2) {
+    unit_step(u, sc[0], sc[1], true);
+    unit_step(u + 1, sc[1], sc[0], u + 2 < u1);
+  }
+  if (u < u1) unit_step(u, sc[0], sc[1], false);
+  __builtin_amdgcn_s_waitcnt(0);  // no load may still write the LDS when the workgroup ends
+  const float unit = exp_bits(E - kVShift);
   const float l_tot = sum_xor32(l_run);
   const int parts = pos / kPartKeys + 1;
   if (t >= len || part >= parts) return;  // (a token before this part's keys: finished by its own last part)
@@ -615,33 +703,59 @@ extern "C" int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, in
   return jit::check_launch("jit_paged_decode_attn_kv8");
 }
 
+namespace {
+int64_t units_bytes(int units, int Hkv) { return (int64_t)units * Hkv * (kUnitBytes + 8); }
+}  // namespace
+
+extern "C" int64_t jit_kv8_prefill_workspace_bytes(int T, int pmax, int H, int Hkv, int units) {
+  if (T < 0 || pmax < 1 || H <= 0 || Hkv <= 0 || units < 0) return -1;
+  return units_bytes(units, Hkv) + jit_prefill_workspace_bytes(T, pmax, H);
+}
+
 extern "C" int jit_paged_prefill_attn_kv8(const uint16_t *q, const void *pool, int num_pages, const int32_t *page_table,
                                           int max_pages, const int32_t *chunk_seq, const int32_t *chunk_ctx,
-                                          const int32_t *chunk_len, const int32_t *chunk_row, int C,
-                                          const int32_t *blk_chunk, const int32_t *blk_q0, const int32_t *blk_part,
-                                          int nblk, int pmax, int max_len, int H, int Hkv, float scale, void *workspace,
-                                          uint16_t *out, void *stream) {
-  if (C < 0 || nblk < 0 || H <= 0 || Hkv <= 0 || max_pages <= 0 || num_pages <= 0 || pmax < 1 || max_len < 0)
-    return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: bad dims C=%d nblk=%d H=%d Hkv=%d pmax=%d max_len=%d", C, nblk, H,
-                     Hkv, pmax, max_len);
+                                          const int32_t *chunk_len, const int32_t *chunk_row, const int32_t *chunk_unit,
+                                          int C, int units, const int32_t *blk_chunk, const int32_t *blk_q0,
+                                          const int32_t *blk_part, int nblk, int T, int pmax, int max_len, int H, int Hkv,
+                                          float scale, void *workspace, int64_t workspace_bytes, uint16_t *out,
+                                          void *stream) {
+  if (C < 0 || nblk < 0 || T < 0 || units < 0 || H <= 0 || Hkv <= 0 || max_pages <= 0 || num_pages <= 0 || pmax < 1 ||
+      max_len < 0)
+    return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: bad dims C=%d nblk=%d T=%d H=%d Hkv=%d pmax=%d max_len=%d units=%d", C,
+                     nblk, T, H, Hkv, pmax, max_len, units);
   if (H % Hkv != 0) return jit::fail(JIT_EINVAL, "%d query heads do not share %d KV heads evenly", H, Hkv);
+  if (!(scale > 0.0f)) return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: the scale must be positive");
   if (16 % (H / Hkv) != 0)
     return jit::fail(JIT_EUNSUPPORTED, "paged_prefill_attn_kv8 covers H / Hkv in {1, 2, 4, 8, 16}, got %d", H / Hkv);
   if (pmax > 1 && H > 64)
     return jit::fail(JIT_EUNSUPPORTED, "paged_prefill_attn_kv8 merges key parts of up to 64 query heads, got %d", H);
-  if (C > 65535) return jit::fail(JIT_EUNSUPPORTED, "paged_prefill_attn_kv8 covers up to 65535 chunks, got %d", C);
+  if (C > 65535 || Hkv > 65535)
+    return jit::fail(JIT_EUNSUPPORTED, "paged_prefill_attn_kv8 covers up to 65535 chunks and heads, got %d and %d", C, Hkv);
   if (C == 0 || nblk == 0) return JIT_OK;
-  if (!q || !pool || !page_table || !chunk_seq || !chunk_ctx || !chunk_len || !chunk_row || !blk_chunk || !blk_q0 ||
-      !blk_part || !out || (pmax > 1 && !workspace))
+  const int64_t need = jit_kv8_prefill_workspace_bytes(T, pmax, H, Hkv, units);
+  if (units == 0 || workspace_bytes < need)
+    return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: workspace of %lld bytes for %d units, %lld needed",
+                     (long long)workspace_bytes, units, (long long)need);
+  if (!q || !pool || !page_table || !chunk_seq || !chunk_ctx || !chunk_len || !chunk_row || !chunk_unit || !blk_chunk ||
+      !blk_q0 || !blk_part || !out || !workspace)
     return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: null pointer");
   if (((uintptr_t)q | (uintptr_t)pool | (uintptr_t)out | (uintptr_t)workspace) & 15)
     return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: q, the pool, the workspace and out must be 16-byte aligned");
+  uint8_t *ws = (uint8_t *)workspace;
+  int32_t *info = (int32_t *)(ws + (int64_t)units * Hkv * kUnitBytes);
   const PrefillArgs a{q, (const uint8_t *)pool, page_table, blk_chunk, blk_q0, blk_part, chunk_seq, chunk_ctx, chunk_len,
-                      chunk_row, out, (float *)workspace, num_pages, max_pages, H, Hkv, H / Hkv, pmax,
-                      scale * 1.44269504088896341f};
+                      chunk_row, chunk_unit, out, ws, info, (float *)(ws + units_bytes(units, Hkv)), num_pages, max_pages,
+                      H, Hkv, H / Hkv, C, pmax, scale * 1.44269504088896341f};
   const hipStream_t st = (hipStream_t)stream;
-  kv8_prefill_kernel<8><<<dim3(nblk * Hkv), 64 * 8, 0, st>>>(a);
-  const int rc = jit::check_launch("jit_paged_prefill_attn_kv8");
+  kv8_expand_kernel<<<dim3(units, Hkv), 256, 0, st>>>(a);
+  int rc = jit::check_launch("jit_paged_prefill_attn_kv8");
+  if (rc) return rc;
+  // few work items leave CUs idle: their row blocks are cut in two
+  if (2ll * nblk * Hkv <= jit::cu_count())
+    kv8_prefill_kernel<4, 2><<<dim3(2 * nblk * Hkv), 64 * 4, 0, st>>>(a);
+  else
+    kv8_prefill_kernel<8, 3><<<dim3(nblk * Hkv), 64 * 8, 0, st>>>(a);
+  rc = jit::check_launch("jit_paged_prefill_attn_kv8");
   if (rc || pmax == 1 || max_len == 0) return rc;
   kv8_prefill_merge_kernel<<<dim3(max_len, C), 8 * H, 0, st>>>(a);
   return jit::check_launch("jit_paged_prefill_attn_kv8");

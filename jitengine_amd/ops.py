@@ -656,6 +656,12 @@ class PrefillPlan:
     rows: int
     pmax: int = 1  # most key parts of a token (jit_prefill_part_keys keys a part)
     max_len: int = 0  # the longest chunk
+    units: torch.Tensor | None = None  # [C + 1]: first unit of KV8_UNIT keys of each chunk, and their number
+    total_units: int = 0
+
+
+def _chunk_units(chunks) -> np.ndarray:
+    return np.cumsum([0] + [-(-(ctx + n) // KV8_UNIT) for _, ctx, n in chunks], dtype=np.int64).astype(np.int32)
 
 
 def prefill_plan(chunks, H: int, Hkv: int, device) -> PrefillPlan:
@@ -683,10 +689,12 @@ def prefill_plan(chunks, H: int, Hkv: int, device) -> PrefillPlan:
             for p in range((nst - 1) // part_steps + 1):
                 items.append((min(nst, (p + 1) * part_steps) - p * part_steps, keys, c, q0, p))
     items.sort(key=lambda it: (-it[0], -it[1]))
-    tables = upload(np.array(tab, np.int32).T.copy() if tab else np.zeros((4, 0), np.int32), device)
+    C, units = len(tab), _chunk_units(chunks)
+    tables = upload(np.concatenate([np.array(tab, np.int32).T.reshape(-1), units]) if tab else units, device)
     blocks = upload(np.array([it[2:] for it in items], np.int32).T.copy() if items
                     else np.zeros((3, 0), np.int32), device)
-    return PrefillPlan(list(chunks), tables.contiguous(), blocks.contiguous(), rows, pmax, max_len)
+    return PrefillPlan(list(chunks), tables[:4 * C].view(4, C), blocks.contiguous(), rows, pmax, max_len, tables[4 * C:],
+                       int(units[-1]))
 
 
 def prefill_workspace_bytes(plan: PrefillPlan, H: int) -> int:
@@ -820,6 +828,7 @@ def paged_decode_attention_noalloc(q: torch.Tensor, pool: torch.Tensor, page_tab
 
 
 # ----------------------------------------------------------------------------- 8-bit KV cache
+KV8_UNIT = 64  # keys of a unit of prompt attention's expanded cache
 KV8_RECORD = 4224  # bytes of one page's 16 tokens of one kv head: K codes, V codes, 32 fp32 scales
 
 
@@ -991,10 +1000,16 @@ def paged_decode_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: 
     return out
 
 
+def kv8_prefill_workspace_bytes(plan: PrefillPlan, H: int, Hkv: int) -> int:
+    total = plan.total_units if plan.units is not None else int(_chunk_units(plan.chunks)[-1])
+    return int(_lib.lib().jit_kv8_prefill_workspace_bytes(plan.rows, plan.pmax, int(H), int(Hkv), total))
+
+
 def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, plan: PrefillPlan,
                                 scale: float, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """q [T, H, 128] bf16 (the plan's chunk rows) -> out [T, H, 128]: paged_prefill_attention over an 8-bit pool
-    (jit_paged_prefill_attn_kv8; the same plans and workspace)."""
+    (jit_paged_prefill_attn_kv8; the same plans), through a workspace of kv8_prefill_workspace_bytes (allocated when not
+    given) that the chunks' keys are expanded into."""
     dev = _one_device(q=q, pool=pool, page_table=page_table, plan=plan.tables)
     _need(q, torch.bfloat16, "q")
     _need(page_table, torch.int32, "page_table")
@@ -1007,14 +1022,19 @@ def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table:
     if T != plan.rows:
         raise ValueError(f"q has {T} rows, the plan's chunks {plan.rows}")
     prefill_contract(plan, page_table)
-    ws = _kv8_workspace(workspace, prefill_workspace_bytes(plan, H), dev)
+    units, total = plan.units, plan.total_units
+    if units is None:  # (a plan put together from its tables)
+        host = _chunk_units(plan.chunks)
+        units, total = upload(host, dev), int(host[-1])
+    ws = _kv8_workspace(workspace, kv8_prefill_workspace_bytes(plan, H, Hkv), dev)
     out = torch.empty_like(q)
     tb, bl = plan.tables, plan.blocks
     with torch.cuda.device(dev):
         _lib.check(_lib.lib().jit_paged_prefill_attn_kv8(
             _p(q), _p(pool), pool.shape[0], _p(page_table), page_table.shape[1], _p(tb[0]), _p(tb[1]), _p(tb[2]),
-            _p(tb[3]), tb.shape[1], _p(bl[0]), _p(bl[1]), _p(bl[2]), bl.shape[1], plan.pmax, plan.max_len, H, Hkv,
-            float(scale), _p(ws), _p(out), _stream_of(dev)), "paged_prefill_attn_kv8")
+            _p(tb[3]), _p(units), tb.shape[1], total, _p(bl[0]), _p(bl[1]), _p(bl[2]), bl.shape[1], T, plan.pmax,
+            plan.max_len, H, Hkv, float(scale), _p(ws), 0 if ws is None else ws.nbytes, _p(out), _stream_of(dev)),
+            "paged_prefill_attn_kv8")
     return out
 
 

@@ -56,9 +56,10 @@ def _decode(q=X, pool=X, pages=8, W=4, B=2, H=32, Hkv=4, max_len=64, ws=None, nb
     return _lib.lib().jit_paged_decode_attn_kv8(q, pool, pages, X, W, lens, B, H, Hkv, max_len, 0.1, ws, nb, out, None)
 
 
-def _prefill(q=X, pool=X, pages=8, W=4, C=1, nblk=1, pmax=1, max_len=4, H=32, Hkv=4, ws=None, out=X):
-    return _lib.lib().jit_paged_prefill_attn_kv8(q, pool, pages, X, W, X, X, X, X, C, X, X, X, nblk, pmax, max_len, H, Hkv,
-                                                 0.1, ws, out, None)
+def _prefill(q=X, pool=X, pages=8, W=4, C=1, nblk=1, T=4, pmax=1, max_len=4, units=1, H=32, Hkv=4, scale=0.1, ws=X, nb=1 << 40,
+             out=X, unit=X):
+    return _lib.lib().jit_paged_prefill_attn_kv8(q, pool, pages, X, W, X, X, X, X, unit, C, units, X, X, X, nblk, T, pmax,
+                                                 max_len, H, Hkv, scale, ws, nb, out, None)
 
 
 def _tables(S=2, W=4, rows=2, free=None, n_free=-1, ctx=X, row_start=X, pos=X, status=X):
@@ -77,7 +78,10 @@ def _tables(S=2, W=4, rows=2, free=None, n_free=-1, ctx=X, row_start=X, pos=X, s
     (lambda: _decode(W=4096, max_len=65536, ws=X, nb=16), EINVAL),  # a workspace too small for the chunks
     (lambda: _decode(q=ODD), EINVAL), (lambda: _decode(out=ODD), EINVAL), (lambda: _decode(pool=ODD), EINVAL),
     (lambda: _prefill(H=30), EINVAL), (lambda: _prefill(H=24, Hkv=8), EUNS), (lambda: _prefill(H=12, Hkv=4), EUNS),
-    (lambda: _prefill(pmax=0), EINVAL), (lambda: _prefill(pmax=2), EINVAL), (lambda: _prefill(pmax=2, H=128, Hkv=16, ws=X), EUNS),
+    (lambda: _prefill(pmax=0), EINVAL), (lambda: _prefill(ws=None), EINVAL), (lambda: _prefill(pmax=2, H=128, Hkv=16), EUNS),
+    (lambda: _prefill(nb=32776 * 4 - 1), EINVAL), (lambda: _prefill(nb=32776 * 4, pmax=2), EINVAL), (lambda: _prefill(units=0), EINVAL),
+    (lambda: _prefill(scale=0.0), EINVAL), (lambda: _prefill(scale=-1.0), EINVAL), (lambda: _prefill(scale=float("nan")), EINVAL),
+    (lambda: _prefill(unit=None), EINVAL), (lambda: _prefill(T=-1), EINVAL),
     (lambda: _prefill(C=0, q=None), OK), (lambda: _prefill(out=None), EINVAL), (lambda: _prefill(C=65536), EUNS),
     (lambda: _prefill(q=ODD), EINVAL), (lambda: _prefill(pool=ODD), EINVAL),
     (lambda: _tables(S=-1), EINVAL), (lambda: _tables(W=0), EINVAL), (lambda: _tables(rows=-1), EINVAL),
