@@ -832,33 +832,49 @@ KV8_UNIT = 64  # keys of a unit of prompt attention's expanded cache
 KV8_RECORD = 4224  # bytes of one page's 16 tokens of one kv head: K codes, V codes, 32 fp32 scales
 
 
-def _one_device(**tensors) -> torch.device:
-    """The device that all of a call's tensors share (ValueError otherwise): the call runs there, on that device's
-    current stream."""
-    dev = None
-    for name, t in tensors.items():
+def _take(*tensors) -> int:
+    """Check the dtype and layout of a call's (tensor or None, dtype, name) arguments and that they share one device;
+    returns its index (ValueError otherwise)."""
+    dev = -1
+    for t, dtype, name in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        if t.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+        d = t.get_device()
+        if d < 0:
             raise ValueError(f"{name} must be a device tensor")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {dev}")
-        dev = t.device
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if d != dev:
+            if dev >= 0:
+                raise ValueError(f"{name} is on device {d}, the call's other tensors on {dev}")
+            dev = d
     return dev
 
 
-def _stream_of(dev: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+def _launch(dev: int, fn, what: str, *args) -> None:
+    """fn(*args, stream) on device `dev` and its current stream, whichever device is current (pointers as integers: the
+    calls below are a few microseconds of GPU time, and so is their host side)."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc < 0:
+        _lib.check(rc, what)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _kv8_heads(pool: torch.Tensor) -> int:
     """kv heads of a layer's 8-bit pool [num_pages, Hkv, KV8_RECORD] (ValueError otherwise)."""
-    _need(pool, torch.uint8, "pool")
-    if pool.dim() != 3 or pool.shape[2] != KV8_RECORD or pool.shape[0] < 1 or pool.shape[1] < 1:
-        raise ValueError(f"an 8-bit KV pool is a contiguous [pages, Hkv, {KV8_RECORD}] tensor, got {tuple(pool.shape)}")
-    if pool.data_ptr() % 16:
-        raise ValueError("an 8-bit KV pool starts on 16 bytes")
-    return int(pool.shape[1])
+    shape = pool.shape
+    if len(shape) != 3 or shape[2] != KV8_RECORD or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"an 8-bit KV pool is a contiguous [pages, Hkv, {KV8_RECORD}] tensor, got {tuple(shape)}")
+    return shape[1]
 
 
 def is_kv8(pool: torch.Tensor) -> bool:
@@ -891,11 +907,10 @@ def step_tables(ctx: torch.Tensor, new: torch.Tensor, page_table: torch.Tensor, 
     more, built on the device in one launch (jit_step_tables).  With `free` (int32 page ids) page_table grows in
     place: each sequence's new pages come from the list in sequence order, from index free_at[0] on (0 without).  A
     sequence that does not fit its table, the `rows` or the list is refused (slots -1, lens = ctx; status counts them)."""
-    dev = _one_device(ctx=ctx, new=new, page_table=page_table, free=free, free_at=free_at)
-    for t, name in ((ctx, "ctx"), (new, "new"), (page_table, "page_table"), (free, "free"), (free_at, "free_at")):
-        if t is not None:
-            _need(t, torch.int32, name)
-    S = ctx.numel()
+    i32 = torch.int32
+    dev = _take((ctx, i32, "ctx"), (new, i32, "new"), (page_table, i32, "page_table"), (free, i32, "free"),
+                (free_at, i32, "free_at"))
+    S, rows = ctx.numel(), int(rows)
     if ctx.dim() != 1 or new.shape != ctx.shape or page_table.dim() != 2 or page_table.shape[0] != S:
         raise ValueError(f"step_tables takes ctx, new [S] and page_table [S, W], got {tuple(ctx.shape)}, "
                          f"{tuple(new.shape)}, {tuple(page_table.shape)}")
@@ -903,32 +918,29 @@ def step_tables(ctx: torch.Tensor, new: torch.Tensor, page_table: torch.Tensor, 
         raise ValueError("free must be a list of page ids")
     if free_at is not None and (free is None or free_at.numel() != 1):
         raise ValueError("free_at is one index into free")
-    rows = int(rows)
-    if rows < 0 or rows > 0x7fffffff // 4:
+    if rows < 0 or rows >= 1 << 29:
         raise ValueError(f"rows must lie in [0, 2^29), got {rows}")
-    buf = torch.empty(2 * S + 5 + 3 * rows, dtype=torch.int32, device=dev)
-    rs, sq, ps, sl, ln, st = torch.split(buf, [S + 1, rows, rows, rows, S, 4])
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().jit_step_tables(_p(ctx), _p(new), S, _p(page_table), page_table.shape[1], rows, _p(free),
-                                              -1 if free is None else free.numel(), _p(free_at), _p(rs), _p(sq), _p(ps),
-                                              _p(sl), _p(ln), _p(st), _stream_of(dev)), "step_tables")
-    return StepTables(rs, sq, ps, sl, ln, st)
+    buf = torch.empty(2 * S + 5 + 3 * rows, dtype=i32, device=ctx.device)
+    at = buf.data_ptr()
+    p_seq = at + 4 * (S + 1)
+    p_len = p_seq + 12 * rows
+    _launch(dev, _lib.lib().jit_step_tables, "step_tables", ctx.data_ptr(), new.data_ptr(), S, page_table.data_ptr(),
+            page_table.shape[1], rows, _ptr(free), -1 if free is None else free.numel(), _ptr(free_at), at, p_seq,
+            p_seq + 4 * rows, p_seq + 8 * rows, p_len, p_len + 4 * S)
+    return StepTables(*buf.split_with_sizes([S + 1, rows, rows, rows, S, 4]))
 
 
 def kv8_append_paged(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Write k, v [B, Hkv, 128] bf16 into an 8-bit pool at slots [B] int32 (jit_kv8_append_paged; a slot outside the
     pool is not written)."""
-    dev = _one_device(pool=pool, k=k, v=v, slots=slots)
-    Hkv = _kv8_heads(pool)
-    _need(k, torch.bfloat16, "k")
-    _need(v, torch.bfloat16, "v")
-    _need(slots, torch.int32, "slots")
-    if k.dim() != 3 or k.shape[1:] != (Hkv, HEAD_DIM) or v.shape != k.shape or slots.shape != (k.shape[0],):
+    dev = _take((pool, torch.uint8, "pool"), (k, torch.bfloat16, "k"), (v, torch.bfloat16, "v"),
+                (slots, torch.int32, "slots"))
+    Hkv, B = _kv8_heads(pool), slots.numel()
+    if k.shape != (B, Hkv, HEAD_DIM) or v.shape != k.shape or slots.dim() != 1:
         raise ValueError(f"kv8_append_paged takes k, v [B, {Hkv}, 128] and slots [B], got {tuple(k.shape)}, "
                          f"{tuple(v.shape)}, {tuple(slots.shape)}")
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().jit_kv8_append_paged(_p(k), _p(v), k.shape[0], Hkv, _p(slots), _p(pool), pool.shape[0],
-                                                   _stream_of(dev)), "kv8_append_paged")
+    _launch(dev, _lib.lib().jit_kv8_append_paged, "kv8_append_paged", k.data_ptr(), v.data_ptr(), B, Hkv,
+            slots.data_ptr(), pool.data_ptr(), pool.shape[0])
 
 
 def qk_norm_rope_append_kv8(qkv: torch.Tensor, H: int, Hkv: int, q_norm: torch.Tensor, k_norm: torch.Tensor, eps: float,
@@ -936,24 +948,19 @@ def qk_norm_rope_append_kv8(qkv: torch.Tensor, H: int, Hkv: int, q_norm: torch.T
                             pool: torch.Tensor) -> torch.Tensor:
     """qkv [B, (H + 2 Hkv) * 128] -> q [B, H, 128] (normed, rotated by pos); k, v written into the 8-bit pool at slots
     (jit_qk_norm_rope_append_kv8: one rounding, angles in fp64)."""
-    dev = _one_device(qkv=qkv, q_norm=q_norm, k_norm=k_norm, inv_freq=inv_freq, pos=pos, slots=slots, pool=pool)
-    _need(qkv, torch.bfloat16, "qkv")
-    _need(q_norm, torch.bfloat16, "q_norm")
-    _need(k_norm, torch.bfloat16, "k_norm")
-    _need(inv_freq, torch.float32, "inv_freq")
-    _need(pos, torch.int32, "pos")
-    _need(slots, torch.int32, "slots")
-    if _kv8_heads(pool) != Hkv or qkv.dim() != 2 or qkv.shape[1] != (H + 2 * Hkv) * HEAD_DIM or \
-            inv_freq.numel() != HEAD_DIM // 2 or q_norm.numel() != HEAD_DIM or k_norm.numel() != HEAD_DIM:
-        raise ValueError("qkv / pool / norms / inv_freq do not match the head geometry")
+    bf, i32 = torch.bfloat16, torch.int32
+    dev = _take((qkv, bf, "qkv"), (q_norm, bf, "q_norm"), (k_norm, bf, "k_norm"), (inv_freq, torch.float32, "inv_freq"),
+                (pos, i32, "pos"), (slots, i32, "slots"), (pool, torch.uint8, "pool"))
     B = qkv.shape[0]
+    if _kv8_heads(pool) != Hkv or qkv.shape != (B, (H + 2 * Hkv) * HEAD_DIM) or inv_freq.numel() != HEAD_DIM // 2 or \
+            q_norm.numel() != HEAD_DIM or k_norm.numel() != HEAD_DIM:
+        raise ValueError("qkv / pool / norms / inv_freq do not match the head geometry")
     if pos.shape != (B,) or slots.shape != (B,):
         raise ValueError(f"pos and slots must be [{B}], got {tuple(pos.shape)} and {tuple(slots.shape)}")
-    q = torch.empty((B, H, HEAD_DIM), dtype=torch.bfloat16, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().jit_qk_norm_rope_append_kv8(
-            _p(qkv), B, H, Hkv, _p(q_norm), _p(k_norm), float(eps), _p(inv_freq), _p(pos), _p(slots), _p(pool),
-            pool.shape[0], _p(q), _stream_of(dev)), "qk_norm_rope_append_kv8")
+    q = torch.empty((B, H, HEAD_DIM), dtype=bf, device=qkv.device)
+    _launch(dev, _lib.lib().jit_qk_norm_rope_append_kv8, "qk_norm_rope_append_kv8", qkv.data_ptr(), B, H, Hkv,
+            q_norm.data_ptr(), k_norm.data_ptr(), float(eps), inv_freq.data_ptr(), pos.data_ptr(), slots.data_ptr(),
+            pool.data_ptr(), pool.shape[0], q.data_ptr())
     return q
 
 
@@ -976,27 +983,25 @@ def paged_decode_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: 
     """q [B, H, 128] bf16 -> out [B, H, 128] bf16 over each sequence's first lens[b] keys of an 8-bit pool
     (jit_paged_decode_attn_kv8).  lens [B] int32 stays on the device; max_len is any bound of it that the host knows
     (it sizes the launch and the workspace of kv8_decode_workspace_bytes; the bits do not depend on it).  A row without keys gives zeros."""
-    dev = _one_device(q=q, pool=pool, page_table=page_table, lens=lens)
-    _need(q, torch.bfloat16, "q")
-    _need(page_table, torch.int32, "page_table")
-    _need(lens, torch.int32, "lens")
+    dev = _take((q, torch.bfloat16, "q"), (pool, torch.uint8, "pool"), (page_table, torch.int32, "page_table"),
+                (lens, torch.int32, "lens"))
     Hkv = _kv8_heads(pool)
     if q.dim() != 3 or page_table.dim() != 2:
         raise ValueError("q must be [B, H, 128] and page_table [B, W]")
-    B, H, Dh = q.shape
+    (B, H, Dh), (Bt, W) = q.shape, page_table.shape
     if Dh != HEAD_DIM:
         raise _lib.UnsupportedShape(f"paged_decode_attention_kv8 covers head_dim 128, got {Dh}")
-    if page_table.shape[0] != B or lens.shape != (B,):
+    if Bt != B or lens.shape != (B,):
         raise ValueError("the rows, page_table and lens disagree on the number of sequences")
     max_len = int(max_len)
-    if max_len < 0 or max_len > page_table.shape[1] * PAGE:
-        raise ValueError(f"max_len must lie in [0, {page_table.shape[1] * PAGE}] (page_table's width), got {max_len}")
-    ws = _kv8_workspace(workspace, kv8_decode_workspace_bytes(B, H, max_len), dev)
+    if max_len < 0 or max_len > W * PAGE:
+        raise ValueError(f"max_len must lie in [0, {W * PAGE}] (page_table's width), got {max_len}")
+    lib = _lib.lib()
+    ws = _kv8_workspace(workspace, lib.jit_kv8_decode_workspace_bytes(B, H, max_len), q.device)
     out = torch.empty_like(q)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().jit_paged_decode_attn_kv8(
-            _p(q), _p(pool), pool.shape[0], _p(page_table), page_table.shape[1], _p(lens), B, H, Hkv, max_len,
-            float(scale), _p(ws), 0 if ws is None else ws.nbytes, _p(out), _stream_of(dev)), "paged_decode_attn_kv8")
+    _launch(dev, lib.jit_paged_decode_attn_kv8, "paged_decode_attn_kv8", q.data_ptr(), pool.data_ptr(), pool.shape[0],
+            page_table.data_ptr(), W, lens.data_ptr(), B, H, Hkv, max_len, float(scale), _ptr(ws),
+            0 if ws is None else ws.nbytes, out.data_ptr())
     return out
 
 
@@ -1010,9 +1015,9 @@ def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table:
     """q [T, H, 128] bf16 (the plan's chunk rows) -> out [T, H, 128]: paged_prefill_attention over an 8-bit pool
     (jit_paged_prefill_attn_kv8; the same plans), through a workspace of kv8_prefill_workspace_bytes (allocated when not
     given) that the chunks' keys are expanded into."""
-    dev = _one_device(q=q, pool=pool, page_table=page_table, plan=plan.tables)
-    _need(q, torch.bfloat16, "q")
-    _need(page_table, torch.int32, "page_table")
+    tb, bl = plan.tables, plan.blocks
+    dev = _take((q, torch.bfloat16, "q"), (pool, torch.uint8, "pool"), (page_table, torch.int32, "page_table"),
+                (tb, torch.int32, "plan"), (bl, torch.int32, "plan"))
     Hkv = _kv8_heads(pool)
     if q.dim() != 3 or page_table.dim() != 2:
         raise ValueError("q must be [T, H, 128] and page_table [S, W]")
@@ -1025,30 +1030,26 @@ def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table:
     units, total = plan.units, plan.total_units
     if units is None:  # (a plan put together from its tables)
         host = _chunk_units(plan.chunks)
-        units, total = upload(host, dev), int(host[-1])
-    ws = _kv8_workspace(workspace, kv8_prefill_workspace_bytes(plan, H, Hkv), dev)
+        units, total = upload(host, q.device), int(host[-1])
+    lib = _lib.lib()
+    ws = _kv8_workspace(workspace, lib.jit_kv8_prefill_workspace_bytes(T, plan.pmax, H, Hkv, total), q.device)
     out = torch.empty_like(q)
-    tb, bl = plan.tables, plan.blocks
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().jit_paged_prefill_attn_kv8(
-            _p(q), _p(pool), pool.shape[0], _p(page_table), page_table.shape[1], _p(tb[0]), _p(tb[1]), _p(tb[2]),
-            _p(tb[3]), _p(units), tb.shape[1], total, _p(bl[0]), _p(bl[1]), _p(bl[2]), bl.shape[1], T, plan.pmax,
-            plan.max_len, H, Hkv, float(scale), _p(ws), 0 if ws is None else ws.nbytes, _p(out), _stream_of(dev)),
-            "paged_prefill_attn_kv8")
+    C, nblk, t, b = tb.shape[1], bl.shape[1], tb.data_ptr(), bl.data_ptr()
+    _launch(dev, lib.jit_paged_prefill_attn_kv8, "paged_prefill_attn_kv8", q.data_ptr(), pool.data_ptr(), pool.shape[0],
+            page_table.data_ptr(), page_table.shape[1], t, t + 4 * C, t + 8 * C, t + 12 * C, units.data_ptr(), C, total, b,
+            b + 4 * nblk, b + 8 * nblk, nblk, T, plan.pmax, plan.max_len, H, Hkv, float(scale), _ptr(ws),
+            0 if ws is None else ws.nbytes, out.data_ptr())
     return out
 
 
 def kv8_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     """Copy pages src[i] -> dst[i] (int32 device tensors) inside one layer's 8-bit pool."""
-    dev = _one_device(pool=pool, src=src, dst=dst)
+    dev = _take((pool, torch.uint8, "pool"), (src, torch.int32, "src"), (dst, torch.int32, "dst"))
     Hkv = _kv8_heads(pool)
-    _need(src, torch.int32, "src")
-    _need(dst, torch.int32, "dst")
     if src.shape != dst.shape or src.dim() != 1:
         raise ValueError("src and dst must be equal-length 1-D page lists")
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().jit_kv8_copy_pages(_p(pool), pool.shape[0], Hkv, _p(src), _p(dst), src.shape[0],
-                                                 _stream_of(dev)), "kv8_copy_pages")
+    _launch(dev, _lib.lib().jit_kv8_copy_pages, "kv8_copy_pages", pool.data_ptr(), pool.shape[0], Hkv, src.data_ptr(),
+            dst.data_ptr(), src.shape[0])
 
 
 # ----------------------------------------------------------------------------- step ends, KV pages
