@@ -6,6 +6,8 @@
 // probability keeps 11 bits, 8 times what bf16 would, at half the instructions of a bf16 high and low part).
 #include "kv8.hpp"
 
+#include <type_traits>
+
 namespace {
 
 using namespace kv8;
@@ -44,172 +46,300 @@ struct DecodeArgs {
   float *part_o;   // [B][ncap][H][128]
   float *part_ml;  // [B][ncap][H][2]
   uint16_t *out;
-  int num_pages, max_pages, B, H, Hkv, G, max_len, ncap;
-  float qk_scale;  // scale * log2(e)
+  int num_pages, max_pages, B, H, Hkv, G, max_len, ncap;  // max_len: at most the page table's width
+  float qk_scale;                                         // scale * log2(e)
 };
 
-__device__ __forceinline__ int seq_len(const DecodeArgs &a, int b) {
-  const long long most = (long long)a.max_pages * kPage;
-  int L = max(a.lens[b], 0);
-  L = min(L, a.max_len);
-  return L > most ? (int)most : L;
-}
+__device__ __forceinline__ int seq_len(const DecodeArgs &a, int b) { return min(max(a.lens[b], 0), a.max_len); }
 
 constexpr int kStateFloats = 32 + 2;  // o[8][4], max, sum per lane
+constexpr int kDecodeWgs = 3;         // workgroups a CU holds (160 registers a lane)
+constexpr int kDecodeSeqs = 4096;     // sequences a launch covers (8 bytes of LDS each)
 
-__global__ __launch_bounds__(64 * kSplits) void kv8_decode_kernel(const DecodeArgs a) {
-  __shared__ float xstate[kSplits - 1][kStateFloats][64];
-  // Workgroups go to the 8 XCDs in turn, so chunk c of sequence b runs on XCD (c odd + b) % 8: a long sequence's chunks
-  // spread over all of them.  (With B itself in odd's place, B = 32 kept each sequence on one XCD: 32 sequences of 128
-  // to 32,768 keys 105 us, now 32.)
-  const int odd = a.B | 1, b = blockIdx.x % odd, c = blockIdx.x / odd, kvh = blockIdx.y;
-  if (b >= a.B) return;
+// A bare barrier behind LDS accesses: __syncthreads would also wait for the loads in flight.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Lane J's value of each quad of lanes.
+template <int J>
+__device__ __forceinline__ float quad(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x55 * J, 0xF, 0xF, true));
+}
+
+// What a wave needs of its run of a chunk.
+struct Run {
+  int b, c, n;         // sequence, chunk, the sequence's chunks
+  int k0, k1, pages;   // keys [k0, k1), their pages
+  int id;              // lane i: page i's id (a page outside the pool: 0, and its bit in bad)
+  unsigned long long bad;
+};
+
+// The chunks of all sequences are one list (a sequence without keys has one empty chunk); a workgroup takes every
+// gridDim.x-th of them for one kv head, each wave a quarter.  The grid is what the GPU holds at once, whatever the
+// lengths: sized by the host's bound (32 sequences of 128 to 32,768 keys: 8,448 workgroups for 1,003 chunks) most
+// workgroups only took a CU's place for the microsecond in which they found that they had nothing to do.  A
+// wave never runs dry: the first loads of its next chunk are in flight while it ends one.
+__global__ __launch_bounds__(64 * kSplits) __attribute__((amdgpu_waves_per_eu(kDecodeWgs, kDecodeWgs)))
+void kv8_decode_kernel(const DecodeArgs a) {
+  __shared__ float xstate[kSplits][kStateFloats][64];
+  __shared__ int s_sum[kSplits];
+  extern __shared__ int s_seq[];  // [B]: chunks up to and with b; [B]: length
+  const int kvh = blockIdx.y;
   const int split = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
   const int lr = l & 15, lg = l >> 4, G = a.G;
-  const int L = seq_len(a, b), ck = chunk_tokens(L), n = chunks_of(L);
-  const long long row = (long long)b * a.H + kvh * G + lr;  // this lane's q head
-  if (c >= n) {
-    if (c == 0 && split == 0 && lr < G) {  // no keys: zeros
+  int total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64 * kSplits) {
+    const int b = b0 + threadIdx.x, L = b < a.B ? seq_len(a, b) : 0;
+    int v = b < a.B ? max(chunks_of(L), 1) : 0;
 #pragma unroll
-      for (int cc = 0; cc < 8; cc++) *(uint2 *)(a.out + row * kD + 16 * cc + 4 * lg) = make_uint2(0u, 0u);
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(v, o, 64);
+      if (l >= o) v += u;
     }
-    return;
+    if (l == 63) s_sum[split] = v;
+    __syncthreads();
+    for (int w = 0; w < kSplits; w++) {
+      if (w < split) v += s_sum[w];
+    }
+    if (b < a.B) s_seq[b] = total + v, s_seq[a.B + b] = L;
+    for (int w = 0; w < kSplits; w++) total += s_sum[w];
+    __syncthreads();
   }
-  const int run = ck / kSplits, k_begin = c * ck + split * run, k_end = min(k_begin + run, L);
-  const int npg = k_end > k_begin ? (k_end - k_begin + kPage - 1) / kPage : 0;
-  // the run's page ids, one per lane; a page outside the pool has its keys left out
-  int my_page = l < npg ? a.page_table[(long long)b * a.max_pages + k_begin / kPage + l] : 0;
-  const bool bad = my_page < 0 || my_page >= a.num_pages;
-  const unsigned long long bad_pages = __ballot(bad);
-  if (bad) my_page = 0;
-
-  FragH qf[4];  // (bf16) Q^T: q head lr, dims 64 (f / 2) + 16 lg + 8 (f % 2) ..
-#pragma unroll
-  for (int f = 0; f < 4; f++)
-    qf[f].q = lr < G ? *(const uint4 *)(a.q + row * kD + 64 * (f >> 1) + 16 * lg + 8 * (f & 1)) : make_uint4(0, 0, 0, 0);
-
-  float m_run = kLowest, l_run = 0.0f;
-  f32x4 o[8];
-#pragma unroll
-  for (int cc = 0; cc < 8; cc++) o[cc] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int st = 0; 2 * st < npg; st++) {
-    const int k0 = k_begin + 32 * st;
-    uint4 kc[2][2], vc[2][2];
-    float4 ks[2], vs[2];
-#pragma unroll
-    for (int p = 0; p < 2; p++) {
-      const int i = min(2 * st + p, npg - 1);  // (a page past the run: the last one again, its keys masked)
-      const uint8_t *rec = record(a.pool, __builtin_amdgcn_readlane(my_page, i), a.Hkv, kvh);
-#pragma unroll
-      for (int i2 = 0; i2 < 2; i2++) {
-        kc[p][i2] = ld_stream16(rec + 1024 * i2 + 16 * l);
-        vc[p][i2] = ld_stream16(rec + kVOff + 1024 * i2 + 16 * l);
-      }
-      ks[p] = *(const float4 *)(rec + kScaleOff + 16 * lg);
-      vs[p] = *(const float4 *)(rec + kScaleOff + 4 * kPage + 16 * lg);
+  auto locate = [&](int item, Run &r) {
+    int lo = 0, hi = a.B - 1;  // the first sequence whose chunks end past the item
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (__builtin_amdgcn_readfirstlane(s_seq[mid]) > item) hi = mid;
+      else lo = mid + 1;
     }
-    // keys of this step that count: below k_end, of pages in the pool (lane: 4 of each page)
-    int keep[2];
+    const int L = __builtin_amdgcn_readfirstlane(s_seq[a.B + lo]), ck = chunk_tokens(L), run = ck / kSplits;
+    r.b = lo;
+    r.c = item - (lo ? __builtin_amdgcn_readfirstlane(s_seq[lo - 1]) : 0);
+    r.n = chunks_of(L);
+    r.k0 = r.c * ck + split * run;
+    r.k1 = min(r.k0 + run, L);
+    r.pages = r.k1 > r.k0 ? (r.k1 - r.k0 + kPage - 1) / kPage : 0;
+    r.id = l < r.pages ? a.page_table[(long long)lo * a.max_pages + r.k0 / kPage + l] : 0;
+  };
+  auto check_pages = [&](Run &r) {  // (waits for the ids)
+    const bool bad = (uint32_t)r.id >= (uint32_t)a.num_pages;
+    r.bad = __ballot(bad);
+    if (bad) r.id = 0;
+  };
+  // Q^T (bf16): q head lr, dims 64 (f / 2) + 16 lg + 8 (f % 2) ..
+  Frag8 qf[4];
+  auto request_q = [&](const Run &r) {
+    const uint16_t *qp = a.q + ((long long)r.b * a.H + kvh * G + lr) * kD + 16 * lg;
 #pragma unroll
-    for (int p = 0; p < 2; p++)
-      keep[p] = (bad_pages >> min(2 * st + p, 63)) & 1 ? 0 : k_end - (k0 + 16 * p + 4 * lg);
-    float t[2][4], iv[2][4];
+    for (int f = 0; f < 4; f++) qf[f].q = lr < G ? *(const uint4 *)(qp + 64 * (f >> 1) + 8 * (f & 1)) : make_uint4(0, 0, 0, 0);
+  };
+  // A step's registers are requested again for the next step as soon as they are used: K and the scales once its
+  // scores are formed, V once its products are issued.
+  uint4 kc[2][2], vc[2][2];
+  float ks[2], vs[2];  // lane (lr, lg): of key 4 lg + lr % 4; a lane's four keys are its quad's
+  const uint32_t lane16 = 16 * l, lane_s = 16 * lg + 4 * (l & 3);
+  auto rec_of = [&](const Run &r, int st, int p) {  // (a page past the run: the last one again, its keys masked)
+    return record(a.pool, __builtin_amdgcn_readlane(r.id, min(2 * st + p, r.pages - 1)), a.Hkv, kvh);
+  };
+  auto request_k = [&](const Run &r, int st) {
 #pragma unroll
     for (int p = 0; p < 2; p++) {
-      f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+      const uint8_t *rec = rec_of(r, st, p);
+      kc[p][0] = ld_stream16(rec + lane16);
+      kc[p][1] = ld_stream16(rec + 1024 + lane16);
+      ks[p] = *(const float *)(rec + kScaleOff + lane_s);
+      vs[p] = *(const float *)(rec + kScaleOff + 4 * kPage + lane_s);
+    }
+  };
+  auto request_v = [&](const Run &r, int st) {
 #pragma unroll
-      for (int f = 0; f < 4; f++) {
-        Frag8 kf, qq;
-        const uint32_t w0 = (f & 1) ? kc[p][f >> 1].z : kc[p][f >> 1].x, w1 = (f & 1) ? kc[p][f >> 1].w : kc[p][f >> 1].y;
-        to_bf16(w0, 1.0f, kf.u[0], kf.u[1]);
-        to_bf16(w1, 1.0f, kf.u[2], kf.u[3]);
-        qq.q = qf[f].q;
-        s = mfma16x16x32(kf, qq, s);
+    for (int p = 0; p < 2; p++) {
+      const uint8_t *rec = rec_of(r, st, p) + kVOff;
+      vc[p][0] = ld_stream16(rec + lane16);
+      vc[p][1] = ld_stream16(rec + 1024 + lane16);
+    }
+  };
+
+  int item = blockIdx.x;
+  if (item >= total) return;  // (uniform)
+  Run cur, nxt;
+  nxt.pages = 0;
+  locate(item, cur);
+  request_q(cur);
+  check_pages(cur);
+  if (cur.pages) {
+    request_k(cur, 0);
+    asm volatile("" ::: "memory");
+    request_v(cur, 0);
+  }
+  for (;;) {
+    const bool more_items = item + (int)gridDim.x < total;
+    if (more_items) locate(item + gridDim.x, nxt);
+    float m_run = kLowest, l_run = 0.0f;
+    f32x4 o[8];
+#pragma unroll
+    for (int cc = 0; cc < 8; cc++) o[cc] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int nst = (cur.pages + 1) >> 1;
+    // LAST: the run's last step, which requests the next run's first
+    auto step = [&](const int st, auto last) {
+      constexpr bool LAST = decltype(last)::value;
+      const int k0 = cur.k0 + 32 * st;
+      const bool cut = LAST || cur.bad;  // (keys past the run: in its last step only)
+      // keys of this step that count: below k1, of pages in the pool (lane: 4 of each page)
+      int keep[2];
+#pragma unroll
+      for (int p = 0; p < 2; p++)
+        keep[p] = !cut ? 4 : (cur.bad >> min(2 * st + p, 63)) & 1 ? 0 : cur.k1 - (k0 + 16 * p + 4 * lg);
+      f32x4 s[2];
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        s[p] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+          Frag8 kf;
+          const uint32_t w0 = (f & 1) ? kc[p][f >> 1].z : kc[p][f >> 1].x, w1 = (f & 1) ? kc[p][f >> 1].w : kc[p][f >> 1].y;
+          to_bf16(w0, 1.0f, kf.u[0], kf.u[1]);
+          to_bf16(w1, 1.0f, kf.u[2], kf.u[3]);
+          s[p] = mfma16x16x32(kf, qf[f], s[p]);
+        }
       }
-      const float *ksp = (const float *)&ks[p], *vsp = (const float *)&vs[p];
+      float t[2][4], iv[2][4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int p = 0; p < 2; p++) {
         // V's scale 2^e is part of the exponent, so a row's maximum is that of its contributions; the sum of the
         // probabilities themselves takes 2^-e back out (a scale of 0, a slot never written, as 2^-100)
-        const uint32_t vb = i < keep[p] ? max(__float_as_uint(vsp[i]), (uint32_t)(kMinExp + 127) << 23) : 127u << 23;
-        const float ev = (float)((int)(vb >> 23) - 127);
-        iv[p][i] = __uint_as_float((254u << 23) - vb);
-        t[p][i] = i < keep[p] ? fmaf(s[i], ksp[i] * a.qk_scale, ev) : -INFINITY;
+        uint32_t vb = max(__float_as_uint(vs[p]), (uint32_t)(kMinExp + 127) << 23);
+        if (cut) vb = (l & 3) < keep[p] ? vb : 127u << 23;
+        const float kq = ks[p] * a.qk_scale, ev = (float)((int)(vb >> 23) - 127), inv = __uint_as_float((254u << 23) - vb);
+        const float kqs[4] = {quad<0>(kq), quad<1>(kq), quad<2>(kq), quad<3>(kq)};
+        const float evs[4] = {quad<0>(ev), quad<1>(ev), quad<2>(ev), quad<3>(ev)};
+        iv[p][0] = quad<0>(inv), iv[p][1] = quad<1>(inv), iv[p][2] = quad<2>(inv), iv[p][3] = quad<3>(inv);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          t[p][i] = fmaf(s[p][i], kqs[i], evs[i]);
+          if (cut) t[p][i] = i < keep[p] ? t[p][i] : -INFINITY;
+        }
       }
-    }
-    float tmax = fmaxf(t[0][0], t[1][0]);
-#pragma unroll
-    for (int i = 1; i < 4; i++) tmax = fmaxf(tmax, fmaxf(t[0][i], t[1][i]));
-    tmax = max_xor32(max_xor16(tmax));
-    const float m_new = fmaxf(m_run, tmax), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-    float psum = 0.0f;
-#pragma unroll
-    for (int p = 0; p < 2; p++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        t[p][i] = __builtin_amdgcn_exp2f(t[p][i] - (m_new - kPShift));
-        psum = fmaf(t[p][i], iv[p][i], psum);
+      asm volatile("" ::: "memory");
+      if constexpr (!LAST) {
+        request_k(cur, st + 1);
+      } else if (more_items) {
+        check_pages(nxt);
+        if (nxt.pages) request_k(nxt, 0);
+        if (nxt.b != cur.b) request_q(nxt);
       }
-    l_run = fmaf(l_run, alpha, psum);
-    m_run = m_new;
-    FragH pf;
-    pf.u[0] = pack_f16x2(t[0][0], t[0][1]);
-    pf.u[1] = pack_f16x2(t[0][2], t[0][3]);
-    pf.u[2] = pack_f16x2(t[1][0], t[1][1]);
-    pf.u[3] = pack_f16x2(t[1][2], t[1][3]);
-    const uint32_t km[2] = {keep_bytes(keep[0]), keep_bytes(keep[1])};  // (a p of 0 does not cancel a NaN code)
+      asm volatile("" ::: "memory");
+      float tmax = fmaxf(t[0][0], t[1][0]);
 #pragma unroll
-    for (int cc = 0; cc < 8; cc++) {
-      FragH vf;
+      for (int i = 1; i < 4; i++) tmax = fmaxf(tmax, fmaxf(t[0][i], t[1][i]));
+      tmax = max_xor32(max_xor16(tmax));
+      const float m_new = fmaxf(m_run, tmax), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      float psum = 0.0f;
 #pragma unroll
-      for (int p = 0; p < 2; p++) to_f16(((const uint32_t *)&vc[p][cc >> 2])[cc & 3] & km[p], vf.u[2 * p], vf.u[2 * p + 1]);
+      for (int p = 0; p < 2; p++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) o[cc][i] *= alpha;
-      o[cc] = mfma16x16x32_f16(vf, pf, o[cc]);
+        for (int i = 0; i < 4; i++) {
+          t[p][i] = __builtin_amdgcn_exp2f(t[p][i] - (m_new - kPShift));
+          psum = fmaf(t[p][i], iv[p][i], psum);
+        }
+      l_run = fmaf(l_run, alpha, psum);
+      m_run = m_new;
+      FragH pf;
+      pf.u[0] = pack_f16x2(t[0][0], t[0][1]);
+      pf.u[1] = pack_f16x2(t[0][2], t[0][3]);
+      pf.u[2] = pack_f16x2(t[1][0], t[1][1]);
+      pf.u[3] = pack_f16x2(t[1][2], t[1][3]);
+      if (cut) {  // (a p of 0 does not cancel a NaN code)
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+          const uint32_t km = keep_bytes(keep[p]);
+#pragma unroll
+          for (int i = 0; i < 2; i++) vc[p][i].x &= km, vc[p][i].y &= km, vc[p][i].z &= km, vc[p][i].w &= km;
+        }
+      }
+      if (__any(alpha != 1.0f)) {
+#pragma unroll
+        for (int cc = 0; cc < 8; cc++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) o[cc][i] *= alpha;
+      }
+#pragma unroll
+      for (int cc = 0; cc < 8; cc++) {
+        FragH vf;
+#pragma unroll
+        for (int p = 0; p < 2; p++) to_f16(((const uint32_t *)&vc[p][cc >> 2])[cc & 3], vf.u[2 * p], vf.u[2 * p + 1]);
+        o[cc] = mfma16x16x32_f16(vf, pf, o[cc]);
+      }
+      asm volatile("" ::: "memory");
+      if constexpr (!LAST) request_v(cur, st + 1);
+      else if (more_items && nxt.pages) request_v(nxt, 0);
+      asm volatile("" ::: "memory");
+    };
+    for (int st = 0; st + 1 < nst; st++) step(st, std::false_type());
+    if (nst > 0) {
+      step(nst - 1, std::true_type());
+    } else if (more_items) {  // (a run without keys)
+      check_pages(nxt);
+      if (nxt.pages) {
+        request_k(nxt, 0);
+        asm volatile("" ::: "memory");
+        request_v(nxt, 0);
+      }
+      if (nxt.b != cur.b) request_q(nxt);
     }
-  }
-  // the runs' states meet in run order
-  if (split > 0) {
-    float(*st)[64] = xstate[split - 1];
+    // the runs' states meet, in run order: each wave merges a quarter of the dims
+    const long long row = (long long)cur.b * a.H + kvh * G + lr;  // this lane's q head
+    lds_barrier();                                               // (the chunk before has been read)
+    {
+      float(*st)[64] = xstate[split];
 #pragma unroll
-    for (int cc = 0; cc < 8; cc++)
+      for (int cc = 0; cc < 8; cc++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) st[4 * cc + i][l] = o[cc][i];
-    st[32][l] = m_run;
-    st[33][l] = l_run;
-  }
-  __syncthreads();
-  if (split > 0) return;
-#pragma unroll
-  for (int sp = 1; sp < kSplits; sp++) {
-    float(*st)[64] = xstate[sp - 1];
-    const float m2 = st[32][l], M = fmaxf(m_run, m2);
-    const float f0 = exp2f(m_run - M), f1 = exp2f(m2 - M);
-#pragma unroll
-    for (int cc = 0; cc < 8; cc++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) o[cc][i] = fmaf(o[cc][i], f0, st[4 * cc + i][l] * f1);
-    l_run = fmaf(l_run, f0, st[33][l] * f1);
-    m_run = M;
-  }
-  const float l_tot = sum_xor32(sum_xor16(l_run));
-  if (lr >= G) return;
-  if (n == 1) {
-    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
-#pragma unroll
-    for (int cc = 0; cc < 8; cc++) {
-      uint2 w;
-      w.x = pack_bf16x2(o[cc][0] * inv, o[cc][1] * inv);
-      w.y = pack_bf16x2(o[cc][2] * inv, o[cc][3] * inv);
-      *(uint2 *)(a.out + row * kD + 16 * cc + 4 * lg) = w;
+        for (int i = 0; i < 4; i++) st[4 * cc + i][l] = o[cc][i];
+      st[32][l] = m_run;
+      st[33][l] = l_run;
     }
-    return;
-  }
-  const long long r = ((long long)b * a.ncap + c) * a.H + kvh * G + lr;
+    lds_barrier();
+    {
+      float f[kSplits], M = xstate[0][32][l], l_tot = 0.0f;
 #pragma unroll
-  for (int cc = 0; cc < 8; cc++)
-    *(float4 *)(a.part_o + r * kD + 16 * cc + 4 * lg) = make_float4(o[cc][0], o[cc][1], o[cc][2], o[cc][3]);
-  if (lg == 0) *(float2 *)(a.part_ml + 2 * r) = make_float2(m_run, l_tot);
+      for (int sp = 0; sp < kSplits; sp++) f[sp] = xstate[sp][32][l];
+#pragma unroll
+      for (int sp = 1; sp < kSplits; sp++) M = fmaxf(M, f[sp]);
+#pragma unroll
+      for (int sp = 0; sp < kSplits; sp++) {
+        f[sp] = __builtin_amdgcn_exp2f(f[sp] - M);
+        l_tot = fmaf(xstate[sp][33][l], f[sp], l_tot);
+      }
+      l_tot = sum_xor32(sum_xor16(l_tot));
+      const float inv = cur.n > 1 ? 1.0f : l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+      const long long r = ((long long)cur.b * a.ncap + cur.c) * a.H + kvh * G + lr;
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        const int cc = 2 * split + x;
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          y[i] = 0.0f;
+#pragma unroll
+          for (int sp = 0; sp < kSplits; sp++) y[i] = fmaf(xstate[sp][4 * cc + i][l], f[sp], y[i]);
+        }
+        if (lr < G && cur.n <= 1)
+          *(uint2 *)(a.out + row * kD + 16 * cc + 4 * lg) =
+              make_uint2(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv));
+        else if (lr < G)
+          *(float4 *)(a.part_o + r * kD + 16 * cc + 4 * lg) = make_float4(y[0], y[1], y[2], y[3]);
+      }
+      if (cur.n > 1 && split == 0 && lg == 0 && lr < G) *(float2 *)(a.part_ml + 2 * r) = make_float2(M, l_tot);
+    }
+    if (!more_items) return;  // (uniform)
+    item += gridDim.x;
+    cur = nxt;
+  }
 }
 
 // The chunks of a (sequence, q head), in order: thread = chunk lane (16) x 4 dims; lane j takes chunks j, j + 16, ..
@@ -684,8 +814,6 @@ extern "C" int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, in
   const int most = (long long)max_pages * kPage < max_len ? max_pages * kPage : max_len;
   const int ncap = max_chunks(most) > 1 ? max_chunks(most) : 1;
   const int64_t need = decode_bytes(B, H, most);
-  if (((int64_t)B | 1) * ncap > 0x7fffffff)
-    return jit::fail(JIT_EUNSUPPORTED, "paged_decode_attn_kv8: %d sequences of up to %d chunks", B, ncap);
   if (workspace_bytes < need)
     return jit::fail(JIT_EINVAL, "paged_decode_attn_kv8: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                      (long long)need);
@@ -693,14 +821,25 @@ extern "C" int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, in
     return jit::fail(JIT_EINVAL, "paged_decode_attn_kv8: null pointer");
   if (((uintptr_t)q | (uintptr_t)pool | (uintptr_t)out | (uintptr_t)workspace) & 15)
     return jit::fail(JIT_EINVAL, "paged_decode_attn_kv8: q, the pool, the workspace and out must be 16-byte aligned");
-  float *part_o = (float *)workspace;
-  const DecodeArgs a{q, (const uint8_t *)pool, page_table, lens, part_o, need ? part_o + (int64_t)B * ncap * H * kD : nullptr,
-                     out, num_pages, max_pages, B, H, Hkv, H / Hkv, most, ncap, scale * 1.44269504088896341f};
-  kv8_decode_kernel<<<dim3((unsigned)(B | 1) * ncap, Hkv), 64 * kSplits, 0, (hipStream_t)stream>>>(a);
-  const int rc = jit::check_launch("jit_paged_decode_attn_kv8");
-  if (rc || ncap == 1) return rc;
-  kv8_merge_kernel<<<dim3(B, H), 32 * kMergeLanes, 0, (hipStream_t)stream>>>(a);
-  return jit::check_launch("jit_paged_decode_attn_kv8");
+  const int slots = kDecodeWgs * jit::cu_count();
+  for (int b0 = 0; b0 < B; b0 += kDecodeSeqs) {
+    const int nb = B - b0 < kDecodeSeqs ? B - b0 : kDecodeSeqs;
+    const int64_t rows = (int64_t)b0 * H, parts = (int64_t)nb * ncap * H;
+    float *part_o = (float *)workspace + rows * ncap * (kD + 2);
+    const DecodeArgs a{q + rows * kD, (const uint8_t *)pool, page_table + (int64_t)b0 * max_pages, lens + b0, part_o,
+                       need ? part_o + parts * kD : nullptr, out + rows * kD, num_pages, max_pages, nb, H, Hkv, H / Hkv,
+                       most, ncap, scale * 1.44269504088896341f};
+    const int64_t chunks = (int64_t)nb * ncap, at_once = slots / Hkv > 1 ? slots / Hkv : 1;
+    kv8_decode_kernel<<<dim3((unsigned)(chunks < at_once ? chunks : at_once), Hkv), 64 * kSplits, 8 * nb,
+                        (hipStream_t)stream>>>(a);
+    int rc = jit::check_launch("jit_paged_decode_attn_kv8");
+    if (rc) return rc;
+    if (ncap == 1) continue;
+    kv8_merge_kernel<<<dim3(nb, H), 32 * kMergeLanes, 0, (hipStream_t)stream>>>(a);
+    rc = jit::check_launch("jit_paged_decode_attn_kv8");
+    if (rc) return rc;
+  }
+  return JIT_OK;
 }
 
 namespace {
