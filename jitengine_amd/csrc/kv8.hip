@@ -5,76 +5,213 @@ namespace {
 
 using namespace kv8;
 
-// One token's block of one head on a wave (lane l: dims l, l + 64): its codes and scale into the record.
-__device__ __forceinline__ void store_block(uint8_t *rec, int slot, bool is_v, int l, float x1, float x2) {
-  const float amax = wave_butterfly<true>(fmaxf(mag(x1), mag(x2)));
+// A wave writes one head of 4 consecutive rows (tokens), 16 lanes a row: lane x of a row has dims 4 x .. + 3 and 64 + 4 x ..
+// + 3, so RoPE's pairs (i, i + 64) are its own, and a norm or a largest magnitude is four lane exchanges.  Bound by
+// latency up to some hundred rows (32 rows of 32 + 2 x 8 heads: 3.3 us, an empty launch 2.5), past that by memory: 2,108
+// such rows read 25.9 MB and write 17.3 MB of q and 4.5 MB of codes in 12.2 us (3.9 TB/s; a copy reaches 4.8).  A wave a
+// row, two dims a lane, took 20.7 us: its V codes went out two bytes a lane, and every wave formed 64 sines.
+
+// Sum or maximum over the 16 lanes of a row (lanes l ^ 1, l ^ 2, then mirrored in 8 and in 16).
+template <bool MAX>
+__device__ __forceinline__ float row16(float v) {
+  auto op = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+  v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, true)));
+  v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, true)));
+  v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true)));
+  return op(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true)));
+}
+
+struct Raw8 {
+  uint2 w[2];
+};
+__device__ __forceinline__ Raw8 load8(const uint16_t *src, int x) {
+  return {{*(const uint2 *)(src + 4 * x), *(const uint2 *)(src + 64 + 4 * x)}};
+}
+__device__ __forceinline__ void widen8(const Raw8 &r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    v[4 * i] = bf2f(r.w[i].x & 0xffffu), v[4 * i + 1] = bf2f_hi(r.w[i].x);
+    v[4 * i + 2] = bf2f(r.w[i].y & 0xffffu), v[4 * i + 3] = bf2f_hi(r.w[i].y);
+  }
+}
+
+// cos and sin of a row's position times the lane's four inverse frequencies.  The angle is formed in fp64 and brought
+// there into [-pi/4, pi/4] about a quarter turn k (at position 262,143 an fp32 product is off by up to 0.016 rad);
+// sine and cosine of the rest are their Taylor series to r^9 and r^10 (2e-9 off at most, 9e-8 with fp32's roundings).
+__device__ __forceinline__ void rotation(int pos, const float *inv_freq, int x, float (&cs)[4], float (&sn)[4]) {
+  const float4 f = *(const float4 *)(inv_freq + 4 * x);
+  const float *fp = (const float *)&f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const double ang = (double)pos * (double)fp[i], k = __builtin_rint(ang * 0.6366197723675814);
+    const float r = (float)__builtin_fma(-k, 6.123233995736766e-17, __builtin_fma(-k, 1.5707963267948966, ang));
+    const int quarter = (int)(long long)k;
+    const float z = r * r;
+    const float s = fmaf(r * z, fmaf(z, fmaf(z, fmaf(z, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), r);
+    const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+    const float a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;  // sine and cosine but for their signs
+    sn[i] = quarter & 2 ? -a : a;
+    cs[i] = (quarter + 1) & 2 ? -b : b;
+  }
+}
+
+// RMSNorm with weights w and the rotation, in fp32 with no rounding in between (q is rounded to bf16, k to its codes,
+// once).
+__device__ __forceinline__ void norm_rope(float (&v)[8], const float (&w)[8], float eps, const float (&cs)[4],
+                                          const float (&sn)[4]) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) ss = fmaf(v[i], v[i], ss);
+  const float r = rsqrtf(row16<false>(ss) * (1.0f / 128.0f) + eps);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float a = v[i] * r * w[i], b = v[i + 4] * r * w[i + 4];
+    v[i] = a * cs[i] - b * sn[i];
+    v[i + 4] = a * sn[i] + b * cs[i];
+  }
+}
+
+// Byte k of four words, in order.
+__device__ __forceinline__ uint32_t byte_of(uint32_t t0, uint32_t t1, uint32_t t2, uint32_t t3, int k) {
+  const uint32_t lo = __builtin_amdgcn_perm(t1, t0, 0x0c0c0400u + 0x0101u * k);  // (0x0c: a zero byte)
+  const uint32_t hi = __builtin_amdgcn_perm(t3, t2, 0x0c0c0400u + 0x0101u * k);
+  return lo | (hi << 16);
+}
+
+template <int J>
+__device__ __forceinline__ uint32_t lane_of_quad(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x55 * J, 0xF, 0xF, true);
+}
+
+// The wave's blocks into their records: rec and slot of the lane's row (on: whether it is written); quad: the rows are
+// the 4 slots of one of V's words (uniform), which then go as words of 4 slots, else V's codes go byte by byte.
+__device__ __forceinline__ void store_blocks(uint8_t *rec, int slot, bool on, bool is_v, bool quad, int l, const float (&v)[8]) {
+  const int x = l & 15, k = l >> 4;
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) amax = fmaxf(amax, mag(v[i]));
+  amax = row16<true>(amax);
   const int e = scale_exp(amax);
   const float inv = exp_bits(-e);
-  const uint32_t c = codes2(to_code_range(x1, inv), to_code_range(x2, inv));
-  const int at = is_v ? v_at(slot, l) : k_at(slot, l);  // (dim l + 64 lies 1,024 bytes on in either part)
-  rec[at] = (uint8_t)c;
-  rec[at + 1024] = (uint8_t)(c >> 8);
-  if (l == 0) ((float *)(rec + kScaleOff))[(is_v ? kPage : 0) + slot] = exp_bits(e);
-}
-
-// One head of one token: RMSNorm with weights w1, w2 (dims l, l + 64) and the rotation by pos * f, in fp32 with no
-// rounding in between (q is rounded to bf16, k to its codes, once).  The angle is formed and brought into one turn
-// in fp64: at position 262,143 an fp32 product is off by up to 0.016 rad.
-__device__ __forceinline__ void norm_rope(float &x1, float &x2, float w1, float w2, float eps, int pos, float f) {
-  float ss = __builtin_fmaf(x1, x1, x2 * x2);
-  ss = wave_butterfly<false>(ss);
-  const float r = rsqrtf(ss * (1.0f / 128.0f) + eps);
-  const float y1 = x1 * r * w1, y2 = x2 * r * w2;
-  const double ang = (double)pos * (double)f;
-  const double turns = __builtin_rint(ang * 0.15915494309189535);
-  double red = __builtin_fma(-turns, 6.283185307179586, ang);
-  red = __builtin_fma(-turns, 2.4492935982947064e-16, red);
-  float sn, cs;
-  sincosf((float)red, &sn, &cs);
-  x1 = y1 * cs - y2 * sn;
-  x2 = y1 * sn + y2 * cs;
-}
-
-// One wave per (token, kv head, K or V).
-__global__ __launch_bounds__(256) void kv8_append_kernel(const uint16_t *__restrict__ k, const uint16_t *__restrict__ v,
-                                                         int Hkv, const int32_t *__restrict__ slots,
-                                                         uint8_t *__restrict__ pool, int num_pages) {
-  const int b = blockIdx.y, l = lane_id();
-  const int head = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int s = slots[b];
-  if (head >= 2 * Hkv || s < 0 || s / kPage >= num_pages) return;
-  const bool is_v = head >= Hkv;
-  const int h = is_v ? head - Hkv : head;
-  const uint16_t *src = (is_v ? v : k) + ((long long)b * Hkv + h) * kD;
-  store_block(record(pool, s / kPage, Hkv, h), s % kPage, is_v, l, bf2f(src[l]), bf2f(src[l + 64]));
-}
-
-// One wave per (token, head) of the fused row [q: H * 128 | k: Hkv * 128 | v: Hkv * 128].
-__global__ __launch_bounds__(256) void qk_norm_rope_append_kv8_kernel(
-    const uint16_t *__restrict__ qkv, int H, int Hkv, const uint16_t *__restrict__ qn_w,
-    const uint16_t *__restrict__ kn_w, float eps, const float *__restrict__ inv_freq, const int32_t *__restrict__ pos,
-    const int32_t *__restrict__ slots, uint8_t *__restrict__ pool, int num_pages, uint16_t *__restrict__ q_out) {
-  const int b = blockIdx.y, l = lane_id();
-  const int head = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int nh = H + 2 * Hkv;
-  if (head >= nh) return;
-  const uint16_t *src = qkv + ((long long)b * nh + head) * kD;
-  float x1 = bf2f(src[l]), x2 = bf2f(src[l + 64]);
-  const bool is_v = head >= H + Hkv;
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) y[i] = to_code_range(v[i], inv);
+  uint32_t c[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) c[i] = codes2(y[4 * i], y[4 * i + 1]) | (codes2(y[4 * i + 2], y[4 * i + 3]) << 16);
+  if (on && x == 0) ((float *)(rec + kScaleOff))[(is_v ? kPage : 0) + slot] = exp_bits(e);
   if (!is_v) {
-    const uint16_t *nw = head < H ? qn_w : kn_w;
-    norm_rope(x1, x2, bf2f(nw[l]), bf2f(nw[l + 64]), eps, pos[b], inv_freq[l]);
-    if (head < H) {
-      uint16_t *qo = q_out + ((long long)b * H + head) * kD;
-      qo[l] = (uint16_t)f2bf(x1);
-      qo[l + 64] = (uint16_t)f2bf(x2);
-      return;
+    if (on) {
+      uint8_t *p = rec + (x >> 2) * 256 + slot * 16 + 4 * (x & 3);
+      *(uint32_t *)p = c[0];
+      *(uint32_t *)(p + 1024) = c[1];
+    }
+  } else if (quad) {
+    // every lane gets the four rows' words of its dims; row k stores dim 4 x + k (of each 64)
+    uint8_t *p = rec + kVOff + (slot >> 2) * 256 + (4 * (x & 3) + k) * 16 + (x >> 2) * 4;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const auto a = __builtin_amdgcn_permlane16_swap(c[i], c[i], false, false);  // rows 0 (2) and 1 (3)
+      const auto b = __builtin_amdgcn_permlane32_swap(a[0], a[0], false, false);  // rows 0 and 2
+      const auto d = __builtin_amdgcn_permlane32_swap(a[1], a[1], false, false);  // rows 1 and 3
+      *(uint32_t *)(p + 1024 * i) = byte_of(b[0], d[0], b[1], d[1], k);
+    }
+  } else {
+    // Byte stores: a lane first gets byte x % 4 of its four lanes' words, so that a store instruction writes 16 bytes of
+    // one 64-byte segment a row and not 4 of each of four.
+    uint8_t *p = rec + kVOff + (slot >> 2) * 256 + (x & 3) * 16 + (x >> 2) * 4 + (slot & 3);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const uint32_t t = byte_of(lane_of_quad<0>(c[i]), lane_of_quad<1>(c[i]), lane_of_quad<2>(c[i]), lane_of_quad<3>(c[i]), x & 3);
+      if (on) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) p[1024 * i + 64 * j] = (uint8_t)(t >> (8 * j));
+      }
     }
   }
-  const int s = slots[b];
-  if (s < 0 || s / kPage >= num_pages) return;
-  const int h = head - H - (is_v ? Hkv : 0);
-  store_block(record(pool, s / kPage, Hkv, h), s % kPage, is_v, l, x1, x2);
+}
+
+// A lane's row of 4 rows from row0: its place in the pool.
+struct Place {
+  int b, slot, page;
+  bool in, on, quad;  // a row of the call; written; the four are a word's slots
+};
+__device__ __forceinline__ Place place_of(int row0, int B, const int32_t *slots, int num_pages, int l) {
+  Place p;
+  p.b = min(row0 + (l >> 4), B - 1);
+  p.in = row0 + (l >> 4) < B;
+  const int s = slots[p.b];
+  p.page = s / kPage;
+  p.slot = s % kPage;
+  p.on = p.in && s >= 0 && p.page < num_pages;
+  const int s0 = __builtin_amdgcn_readfirstlane(s);
+  p.quad = __all(p.on && s == s0 + (l >> 4) && s0 % 4 == 0);
+  if (!p.on) p.page = p.slot = 0;
+  return p;
+}
+
+__global__ __launch_bounds__(256) void kv8_append_kernel(const uint16_t *__restrict__ k, const uint16_t *__restrict__ v,
+                                                         int B, int Hkv, const int32_t *__restrict__ slots,
+                                                         uint8_t *__restrict__ pool, int num_pages) {
+  const int l = lane_id(), unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (unit >= 2 * Hkv) return;
+  const Place p = place_of(4 * blockIdx.y, B, slots, num_pages, l);
+  auto src = [&](int head) {
+    return (head >= Hkv ? v : k) + ((long long)p.b * Hkv + (head >= Hkv ? head - Hkv : head)) * kD;
+  };
+  const int step = 4 * gridDim.x;
+  Raw8 next = load8(src(unit), l & 15);
+  for (int head = unit; head < 2 * Hkv; head += step) {
+    float x[8];
+    widen8(next, x);
+    if (head + step < 2 * Hkv) next = load8(src(head + step), l & 15);
+    const bool is_v = head >= Hkv;
+    store_blocks(record(pool, p.page, Hkv, is_v ? head - Hkv : head), p.slot, p.on, is_v, p.quad, l, x);
+  }
+}
+
+// The fused rows [q: H * 128 | k: Hkv * 128 | v: Hkv * 128].
+__global__ __launch_bounds__(256) void qk_norm_rope_append_kv8_kernel(
+    const uint16_t *__restrict__ qkv, int B, int H, int Hkv, const uint16_t *__restrict__ qn_w,
+    const uint16_t *__restrict__ kn_w, float eps, const float *__restrict__ inv_freq, const int32_t *__restrict__ pos,
+    const int32_t *__restrict__ slots, uint8_t *__restrict__ pool, int num_pages, uint16_t *__restrict__ q_out) {
+  const int l = lane_id(), unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nh = H + 2 * Hkv;
+  if (unit >= nh) return;
+  const Place p = place_of(4 * blockIdx.y, B, slots, num_pages, l);
+  const int step = 4 * gridDim.x;
+  const uint16_t *row = qkv + (long long)p.b * nh * kD;
+  Raw8 next = load8(row + unit * kD, l & 15);
+  float w[8], cs[4], sn[4];
+  widen8(load8(unit < H ? qn_w : kn_w, l & 15), w);
+  if (unit < H + Hkv) rotation(pos[p.b], inv_freq, l & 15, cs, sn);
+  for (int head = unit; head < nh; head += step) {
+    float x[8];
+    widen8(next, x);
+    if (head + step < nh) next = load8(row + (head + step) * kD, l & 15);  // (in flight beside this head's work)
+    if (head < H + Hkv) {
+      if (head >= H && head - step < H && head > unit) widen8(load8(kn_w, l & 15), w);
+      norm_rope(x, w, eps, cs, sn);
+    }
+    if (head < H) {
+      if (!p.in) continue;
+      uint16_t *qo = q_out + ((long long)p.b * H + head) * kD + 4 * (l & 15);
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        *(uint2 *)(qo + 64 * i) =
+            make_uint2(pack_bf16x2(x[4 * i], x[4 * i + 1]), pack_bf16x2(x[4 * i + 2], x[4 * i + 3]));
+    } else {
+      const bool is_v = head >= H + Hkv;
+      store_blocks(record(pool, p.page, Hkv, head - H - (is_v ? Hkv : 0)), p.slot, p.on, is_v, p.quad, l, x);
+    }
+  }
+}
+
+// Blocks of 4 waves a group of rows: one head a wave up to 1,024 blocks (what 256 CUs hold of them at once), else that
+// many, whose waves loop over the heads and form their rows' rotations once.  2,108 rows of 32 + 2 x 8 heads with 512,
+// 1,024, 2,048 and 4,096 blocks: 14.1, 12.2, 15.3 and 19.5 us; 300 rows: 5.2, 4.6, 4.6 and 4.5.
+int head_blocks(int rows, int heads) {
+  const int groups = (rows + 3) / 4, all = (heads + 3) / 4, want = (1024 + groups - 1) / groups;
+  return want < all ? want : all;
 }
 
 // Workgroup i copies page src[i] to page dst[i]; a page id outside the pool copies nothing.
@@ -201,9 +338,10 @@ extern "C" int jit_kv8_append_paged(const uint16_t *k, const uint16_t *v, int B,
   if (B > 65535) return jit::fail(JIT_EUNSUPPORTED, "kv8_append_paged covers up to 65535 rows, got %d", B);
   if (B == 0) return JIT_OK;
   if (!k || !v || !slots || !pool) return jit::fail(JIT_EINVAL, "kv8_append_paged: null pointer");
-  if ((uintptr_t)pool & 15) return jit::fail(JIT_EINVAL, "kv8_append_paged: the pool must be 16-byte aligned");
-  kv8_append_kernel<<<dim3((2 * Hkv + 3) / 4, B), 256, 0, (hipStream_t)stream>>>(k, v, Hkv, slots, (uint8_t *)pool,
-                                                                                 num_pages);
+  if (((uintptr_t)pool & 15) || (((uintptr_t)k | (uintptr_t)v) & 7))
+    return jit::fail(JIT_EINVAL, "kv8_append_paged: the pool must be 16-byte, k and v 8-byte aligned");
+  kv8_append_kernel<<<dim3(head_blocks(B, 2 * Hkv), (B + 3) / 4), 256, 0, (hipStream_t)stream>>>(
+      k, v, B, Hkv, slots, (uint8_t *)pool, num_pages);
   return jit::check_launch("jit_kv8_append_paged");
 }
 
@@ -218,9 +356,12 @@ extern "C" int jit_qk_norm_rope_append_kv8(const uint16_t *qkv, int B, int H, in
   if (B == 0) return JIT_OK;
   if (!qkv || !q_norm_w || !k_norm_w || !inv_freq || !pos || !slots || !pool || !q_out)
     return jit::fail(JIT_EINVAL, "qk_norm_rope_append_kv8: null pointer");
-  if ((uintptr_t)pool & 15) return jit::fail(JIT_EINVAL, "qk_norm_rope_append_kv8: the pool must be 16-byte aligned");
-  qk_norm_rope_append_kv8_kernel<<<dim3((H + 2 * Hkv + 3) / 4, B), 256, 0, (hipStream_t)stream>>>(
-      qkv, H, Hkv, q_norm_w, k_norm_w, eps, inv_freq, pos, slots, (uint8_t *)pool, num_pages, q_out);
+  if ((((uintptr_t)pool | (uintptr_t)inv_freq) & 15) ||
+      (((uintptr_t)qkv | (uintptr_t)q_norm_w | (uintptr_t)k_norm_w | (uintptr_t)q_out) & 7))
+    return jit::fail(JIT_EINVAL, "qk_norm_rope_append_kv8: the pool and inv_freq must be 16-byte, the rows and norms "
+                                 "8-byte aligned");
+  qk_norm_rope_append_kv8_kernel<<<dim3(head_blocks(B, H + 2 * Hkv), (B + 3) / 4), 256, 0, (hipStream_t)stream>>>(
+      qkv, B, H, Hkv, q_norm_w, k_norm_w, eps, inv_freq, pos, slots, (uint8_t *)pool, num_pages, q_out);
   return jit::check_launch("jit_qk_norm_rope_append_kv8");
 }
 

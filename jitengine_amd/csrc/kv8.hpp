@@ -31,11 +31,6 @@ __device__ __forceinline__ const uint8_t *record(const uint8_t *pool, int page, 
 __device__ __forceinline__ uint8_t *record(uint8_t *pool, int page, int Hkv, int h) {
   return pool + (uint64_t)((uint32_t)page * (uint32_t)Hkv + (uint32_t)h) * kRec;
 }
-// byte of (slot, dim) in a record's K and V parts
-__device__ __forceinline__ int k_at(int slot, int d) { return (d >> 6) * 1024 + ((d >> 4) & 3) * 256 + slot * 16 + (d & 15); }
-__device__ __forceinline__ int v_at(int slot, int d) {
-  return kVOff + (d >> 6) * 1024 + (slot >> 2) * 256 + (d & 15) * 16 + ((d >> 4) & 3) * 4 + (slot & 3);
-}
 
 // The scale's exponent of a block whose largest finite magnitude is amax: amax 2^-e lies in (224, 448] (1.75 2^8 is
 // the largest e4m3), clamped; 0 for a block of zeros.
