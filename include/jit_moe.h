@@ -624,6 +624,25 @@ int jit_decode_layer(const jit_layer *layer, const jit_decode_rows *d, uint16_t 
 int jit_mixed_layer(const jit_layer *layer, const jit_prompt_rows *p, const jit_decode_rows *d, uint16_t *pool,
                     const uint16_t *x, void *scratch, uint16_t *y, void *stream);
 
+/* The rows of a step over 8-bit pools: prompt_rows rows with the arguments of jit_paged_prefill_attn_kv8, then B decode
+ * rows with those of jit_paged_decode_attn_kv8; pos, slots [prompt_rows + B] of jit_step_tables.  Both page tables are
+ * max_pages wide. */
+typedef struct {
+  int prompt_rows, B, C, nblk, units, pmax, prompt_max_len, max_pages, max_len;
+  const int32_t *pos, *slots, *prompt_table, *chunk_seq, *chunk_ctx, *chunk_len, *chunk_row, *chunk_unit;
+  const int32_t *blk_chunk, *blk_q0, *blk_part, *page_table, *lens;
+  void *prompt_workspace, *workspace;
+  int64_t prompt_workspace_bytes, workspace_bytes;
+} jit_kv8_step;
+
+/* jit_decode_layer and jit_mixed_layer over an 8-bit pool of num_pages pages.  Their scratch is that of a mixed call
+ * (jit_layer_scratch_bytes with mixed = 1) in both. */
+int jit_decode_layer_kv8(const jit_layer *layer, const jit_kv8_step *step, void *pool, int num_pages, const uint16_t *x,
+                         const uint16_t *xn, const jit_layer *prev_layer, const void *prev, int defer,
+                         const uint16_t *next_norm, void *scratch, uint16_t *y, uint16_t *xn_next, void *stream);
+int jit_mixed_layer_kv8(const jit_layer *layer, const jit_kv8_step *step, void *pool, int num_pages, const uint16_t *x,
+                        void *scratch, uint16_t *y, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -44,7 +44,17 @@ class PromptRows(ctypes.Structure):
                           "blk_chunk", "blk_q0", "blk_part", "workspace")]
 
 
+class Kv8Step(ctypes.Structure):
+    """jit_kv8_step"""
+    _fields_ = [(n, _I) for n in ("prompt_rows", "B", "C", "nblk", "units", "pmax", "prompt_max_len", "max_pages",
+                                  "max_len")] + [
+        (n, _P) for n in ("pos", "slots", "prompt_table", "chunk_seq", "chunk_ctx", "chunk_len", "chunk_row",
+                          "chunk_unit", "blk_chunk", "blk_q0", "blk_part", "page_table", "lens", "prompt_workspace",
+                          "workspace")] + [("prompt_workspace_bytes", _L), ("workspace_bytes", _L)]
+
+
 _PL, _PD, _PP = ctypes.POINTER(Layer), ctypes.POINTER(DecodeRows), ctypes.POINTER(PromptRows)
+_PK = ctypes.POINTER(Kv8Step)
 
 # name -> argtypes (restype int unless listed in _RESTYPES)
 _SIGNATURES = {
@@ -84,6 +94,8 @@ _SIGNATURES = {
     "jit_layer_scratch_bytes": [_PL, _I, _I],
     "jit_decode_layer": [_PL, _PD, _P, _P, _P, _PL, _P, _I, _P, _P, _P, _P, _P],
     "jit_mixed_layer": [_PL, _PP, _PD, _P, _P, _P, _P, _P],
+    "jit_decode_layer_kv8": [_PL, _PK, _P, _I, _P, _P, _PL, _P, _I, _P, _P, _P, _P, _P],
+    "jit_mixed_layer_kv8": [_PL, _PK, _P, _I, _P, _P, _P, _P],
     "jit_paged_decode_attn_ws": [_P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _F, _I, _P, ctypes.c_int64, _P, _P],
     "jit_paged_decode_attn_qkv_ws": [_P, _P, _P, _F, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _F, _I, _P, ctypes.c_int64,
                                      _P, _P],

@@ -129,29 +129,23 @@ int layer_check(const jit_layer *L, int rows, const char *what) {
   return JIT_OK;
 }
 
-}  // namespace
-
-extern "C" int64_t jit_layer_scratch_bytes(const jit_layer *layer, int rows, int mixed) {
-  if (layer_check(layer, rows, "layer_scratch_bytes")) return -1;
-  return Scratch(*layer, rows, mixed != 0, nullptr).bytes;
-}
-
-extern "C" int jit_decode_layer(const jit_layer *layer, const jit_decode_rows *d, uint16_t *pool, const uint16_t *x,
-                                const uint16_t *xn, const jit_layer *prev_layer, const void *prev, int defer,
-                                const uint16_t *next_norm, void *scratch, uint16_t *y, uint16_t *xn_next, void *stream) {
-  if (!d) return jit::fail(JIT_EINVAL, "decode_layer: null step");
-  JIT_TRY(layer_check(layer, d->B, "decode_layer"));
+// A decode step's layer with its attention as a call: attend(L, scratch) turns s.qkv into s.attn.
+template <class Attend>
+int decode_layer(const char *what, const jit_layer *layer, int B, const uint16_t *x, const uint16_t *xn,
+                 const jit_layer *prev_layer, const void *prev, int defer, const uint16_t *next_norm, void *scratch,
+                 bool with_q, uint16_t *y, uint16_t *xn_next, void *stream, Attend attend) {
+  JIT_TRY(layer_check(layer, B, what));
   const jit_layer &L = *layer;
-  const int B = d->B, D = L.D, nqkv = (L.H + 2 * L.Hkv) * JIT_HEAD_DIM;
-  if ((prev || defer) && B != 1) return jit::fail(JIT_EINVAL, "decode_layer: a deferred combine takes one row");
+  const int D = L.D, nqkv = (L.H + 2 * L.Hkv) * JIT_HEAD_DIM;
+  if ((prev || defer) && B != 1) return jit::fail(JIT_EINVAL, "%s: a deferred combine takes one row", what);
   if (!scratch || (!prev && !x) || (!defer && !y) || (next_norm && !defer && !xn_next))
-    return jit::fail(JIT_EINVAL, "decode_layer: null pointer");
+    return jit::fail(JIT_EINVAL, "%s: null pointer", what);
   if (prev) {
-    JIT_TRY(layer_check(prev_layer, 1, "decode_layer: previous layer"));
+    if (int rc = layer_check(prev_layer, 1, "decode_layer: previous layer")) return rc;
     if (prev_layer->D != D)
-      return jit::fail(JIT_EINVAL, "decode_layer: a deferred row of %d for a layer of %d", prev_layer->D, D);
+      return jit::fail(JIT_EINVAL, "%s: a deferred row of %d for a layer of %d", what, prev_layer->D, D);
   }
-  const Scratch s(L, B, false, scratch);
+  const Scratch s(L, B, with_q, scratch);
   if (prev) {
     // (the row's combine is the previous layer's: its tables, top-k and places in its scratch)
     const Scratch p(*prev_layer, 1, false, (void *)prev);
@@ -165,36 +159,105 @@ extern "C" int jit_decode_layer(const jit_layer *layer, const jit_decode_rows *d
     }
     JIT_TRY(jit_qmm_packed(xn, B, D, L.qkv, nqkv, s.qkv, stream));
   }
-  JIT_TRY(jit_paged_decode_attn_qkv_ws(s.qkv, L.q_norm, L.k_norm, L.eps, L.inv_freq, pool, d->page_table,
-                                       d->max_pages, d->lens, d->chunk_start, d->chunk_seq, B, L.H, L.Hkv, L.scale,
-                                       d->total_chunks, d->workspace, d->workspace_bytes, s.attn, stream));
+  JIT_TRY(attend(L, s));
   return layer_tail(L, B, false, x, s, defer, next_norm, y, xn_next, stream);
 }
 
-extern "C" int jit_mixed_layer(const jit_layer *layer, const jit_prompt_rows *p, const jit_decode_rows *d,
-                               uint16_t *pool, const uint16_t *x, void *scratch, uint16_t *y, void *stream) {
-  if (!p || !d) return jit::fail(JIT_EINVAL, "mixed_layer: null step");
-  const int T = p->rows + d->B;
-  if (p->rows < 0 || d->B < 0) return jit::fail(JIT_EINVAL, "mixed_layer: %d prompt and %d decode rows", p->rows, d->B);
-  JIT_TRY(layer_check(layer, T, "mixed_layer"));
-  if (!x || !scratch || !y) return jit::fail(JIT_EINVAL, "mixed_layer: null pointer");
+// A mixed step's layer with its attention as a call.
+template <class Attend>
+int mixed_layer(const char *what, const jit_layer *layer, int prompt_rows, int B, const uint16_t *x, void *scratch,
+                uint16_t *y, void *stream, Attend attend) {
+  if (prompt_rows < 0 || B < 0)
+    return jit::fail(JIT_EINVAL, "%s: %d prompt and %d decode rows", what, prompt_rows, B);
+  const int T = prompt_rows + B;
+  JIT_TRY(layer_check(layer, T, what));
+  if (!x || !scratch || !y) return jit::fail(JIT_EINVAL, "%s: null pointer", what);
   const jit_layer &L = *layer;
   const int D = L.D, nqkv = (L.H + 2 * L.Hkv) * JIT_HEAD_DIM;
   const Scratch s(L, T, true, scratch);
   JIT_TRY(jit_rmsnorm(x, nullptr, T, D, L.input_norm, L.eps, nullptr, s.xn, stream));
   JIT_TRY(project(s.xn, T, D, L.qkv, nqkv, s.qkv, true, stream));
-  JIT_TRY(jit_qk_norm_rope_append(s.qkv, T, L.H, L.Hkv, L.q_norm, L.k_norm, L.eps, L.inv_freq, p->pos, p->table_rows,
-                                  p->table_rows_pages, pool, s.q, stream));
-  // (both halves write their rows of one buffer: no concatenation)
-  if (p->rows)
-    JIT_TRY(jit_paged_prefill_attn(s.q, pool, p->seq_table, p->seq_pages, p->chunk_seq, p->chunk_ctx, p->chunk_len,
-                                   p->chunk_row, p->C, p->blk_chunk, p->blk_q0, p->blk_part, p->nblk, p->pmax,
-                                   p->max_len, L.H, L.Hkv, L.scale, p->workspace, s.attn, stream));
-  if (d->B) {
-    const int64_t at = (int64_t)p->rows * L.H * JIT_HEAD_DIM;
-    JIT_TRY(jit_paged_decode_attn_ws(s.q + at, pool, d->page_table, d->max_pages, d->lens, d->chunk_start,
-                                     d->chunk_seq, d->B, L.H, L.Hkv, L.scale, d->total_chunks, d->workspace,
-                                     d->workspace_bytes, s.attn + at, stream));
-  }
+  JIT_TRY(attend(L, s));
   return layer_tail(L, T, true, x, s, 0, nullptr, y, nullptr, stream);
+}
+
+}  // namespace
+
+extern "C" int64_t jit_layer_scratch_bytes(const jit_layer *layer, int rows, int mixed) {
+  if (layer_check(layer, rows, "layer_scratch_bytes")) return -1;
+  return Scratch(*layer, rows, mixed != 0, nullptr).bytes;
+}
+
+extern "C" int jit_decode_layer(const jit_layer *layer, const jit_decode_rows *d, uint16_t *pool, const uint16_t *x,
+                                const uint16_t *xn, const jit_layer *prev_layer, const void *prev, int defer,
+                                const uint16_t *next_norm, void *scratch, uint16_t *y, uint16_t *xn_next, void *stream) {
+  if (!d) return jit::fail(JIT_EINVAL, "decode_layer: null step");
+  return decode_layer("decode_layer", layer, d->B, x, xn, prev_layer, prev, defer, next_norm, scratch, false, y, xn_next,
+                      stream, [&](const jit_layer &L, const Scratch &s) {
+    return jit_paged_decode_attn_qkv_ws(s.qkv, L.q_norm, L.k_norm, L.eps, L.inv_freq, pool, d->page_table,
+                                        d->max_pages, d->lens, d->chunk_start, d->chunk_seq, d->B, L.H, L.Hkv, L.scale,
+                                        d->total_chunks, d->workspace, d->workspace_bytes, s.attn, stream);
+  });
+}
+
+extern "C" int jit_mixed_layer(const jit_layer *layer, const jit_prompt_rows *p, const jit_decode_rows *d,
+                               uint16_t *pool, const uint16_t *x, void *scratch, uint16_t *y, void *stream) {
+  if (!p || !d) return jit::fail(JIT_EINVAL, "mixed_layer: null step");
+  return mixed_layer("mixed_layer", layer, p->rows, d->B, x, scratch, y, stream, [&](const jit_layer &L, const Scratch &s) {
+    JIT_TRY(jit_qk_norm_rope_append(s.qkv, p->rows + d->B, L.H, L.Hkv, L.q_norm, L.k_norm, L.eps, L.inv_freq, p->pos,
+                                    p->table_rows, p->table_rows_pages, pool, s.q, stream));
+    // (both halves write their rows of one buffer: no concatenation)
+    if (p->rows)
+      JIT_TRY(jit_paged_prefill_attn(s.q, pool, p->seq_table, p->seq_pages, p->chunk_seq, p->chunk_ctx, p->chunk_len,
+                                     p->chunk_row, p->C, p->blk_chunk, p->blk_q0, p->blk_part, p->nblk, p->pmax,
+                                     p->max_len, L.H, L.Hkv, L.scale, p->workspace, s.attn, stream));
+    if (d->B) {
+      const int64_t at = (int64_t)p->rows * L.H * JIT_HEAD_DIM;
+      JIT_TRY(jit_paged_decode_attn_ws(s.q + at, pool, d->page_table, d->max_pages, d->lens, d->chunk_start,
+                                       d->chunk_seq, d->B, L.H, L.Hkv, L.scale, d->total_chunks, d->workspace,
+                                       d->workspace_bytes, s.attn + at, stream));
+    }
+    return (int)JIT_OK;
+  });
+}
+
+namespace {
+
+// The attention of a step's rows over an 8-bit pool: q/k norms, RoPE and the cache's codes, then each half.
+int attend_kv8(const jit_kv8_step &t, const jit_layer &L, const Scratch &s, void *pool, int num_pages, void *stream) {
+  JIT_TRY(jit_qk_norm_rope_append_kv8(s.qkv, t.prompt_rows + t.B, L.H, L.Hkv, L.q_norm, L.k_norm, L.eps, L.inv_freq,
+                                      t.pos, t.slots, pool, num_pages, s.q, stream));
+  if (t.prompt_rows)
+    JIT_TRY(jit_paged_prefill_attn_kv8(s.q, pool, num_pages, t.prompt_table, t.max_pages, t.chunk_seq, t.chunk_ctx,
+                                       t.chunk_len, t.chunk_row, t.chunk_unit, t.C, t.units, t.blk_chunk, t.blk_q0,
+                                       t.blk_part, t.nblk, t.prompt_rows, t.pmax, t.prompt_max_len, L.H, L.Hkv, L.scale,
+                                       t.prompt_workspace, t.prompt_workspace_bytes, s.attn, stream));
+  if (t.B) {
+    const int64_t at = (int64_t)t.prompt_rows * L.H * JIT_HEAD_DIM;
+    JIT_TRY(jit_paged_decode_attn_kv8(s.q + at, pool, num_pages, t.page_table, t.max_pages, t.lens, t.B, L.H, L.Hkv,
+                                      t.max_len, L.scale, t.workspace, t.workspace_bytes, s.attn + at, stream));
+  }
+  return JIT_OK;
+}
+
+}  // namespace
+
+extern "C" int jit_decode_layer_kv8(const jit_layer *layer, const jit_kv8_step *t, void *pool, int num_pages,
+                                    const uint16_t *x, const uint16_t *xn, const jit_layer *prev_layer, const void *prev,
+                                    int defer, const uint16_t *next_norm, void *scratch, uint16_t *y, uint16_t *xn_next,
+                                    void *stream) {
+  if (!t || t->prompt_rows) return jit::fail(JIT_EINVAL, "decode_layer_kv8: null step or prompt rows");
+  return decode_layer("decode_layer_kv8", layer, t->B, x, xn, prev_layer, prev, defer, next_norm, scratch, true, y,
+                      xn_next, stream, [&](const jit_layer &L, const Scratch &s) {
+    return attend_kv8(*t, L, s, pool, num_pages, stream);
+  });
+}
+
+extern "C" int jit_mixed_layer_kv8(const jit_layer *layer, const jit_kv8_step *t, void *pool, int num_pages,
+                                   const uint16_t *x, void *scratch, uint16_t *y, void *stream) {
+  if (!t) return jit::fail(JIT_EINVAL, "mixed_layer_kv8: null step");
+  return mixed_layer("mixed_layer_kv8", layer, t->prompt_rows, t->B, x, scratch, y, stream,
+                     [&](const jit_layer &L, const Scratch &s) {
+    return attend_kv8(*t, L, s, pool, num_pages, stream);
+  });
 }

@@ -66,11 +66,12 @@ class Request:
 
 
 class Engine:
-    """Requests in, tokens out, many sequences per step over one KV pool."""
+    """Requests in, tokens out, many sequences per step over one KV pool.  kv8=True keeps the cache in 8 bits (about
+    twice the tokens a pool of the same bytes holds; ops.kv8_pool)."""
 
     def __init__(self, lm: CausalLM, num_pages: int, prefill_chunk: int = 512, max_step_tokens: int = 2048,
                  prefix_store: bool = True, page_seed: int | None = None, device=None, allocate: bool = True,
-                 pipeline: bool = True, selfcheck: bool = False):
+                 pipeline: bool = True, selfcheck: bool = False, kv8: bool = False):
         if prefill_chunk <= 0 or max_step_tokens <= 0:
             raise ValueError("prefill_chunk and max_step_tokens must be positive")
         if prefill_chunk > max_step_tokens:
@@ -81,7 +82,8 @@ class Engine:
         self.device = torch.device(dev)
         if selfcheck or _selfcheck.enabled_by_env():  # the kernels against torch, once per device
             _selfcheck.run(self.device)
-        self.pool = KVPool(len(lm.layers), num_pages, cfg.kv_heads, self.device, seed=page_seed, allocate=allocate)
+        self.pool = KVPool(len(lm.layers), num_pages, cfg.kv_heads, self.device, seed=page_seed, allocate=allocate,
+                           kv8=kv8)
         self.store = PrefixStore(self.pool) if prefix_store else None
         self.prefill_chunk = int(prefill_chunk)
         self.max_step_tokens = int(max_step_tokens)
@@ -193,7 +195,7 @@ class Engine:
         tokens are each row's token len(tokens) + ahead; returns them, int32 [B] on the device (not
         read)."""
         lm = self.lm
-        st = make_step_state(lm.cfg, pos, self.pool.page_table([r.rid for r in rows]))
+        st = make_step_state(lm.cfg, pos, self.pool.page_table([r.rid for r in rows]), self.pool.kv8)
         ids_t = ids if torch.is_tensor(ids) else ops.upload(ids, self.device, torch.int32)
         h = lm.model.decode_step(lm.embed_tokens(ids_t), self.pool.pools, st)
         return self._draw(rows, h, [len(r.tokens) + ahead for r in rows])
@@ -305,7 +307,7 @@ class Engine:
         lm, dev = self.lm, self.device
         seq_table = self.pool.page_table_host([r.rid])
         ms = make_mixed_state(lm.cfg, [(0, c, n)], seq_table, np.zeros(0, np.int32),
-                              np.zeros((0, seq_table.shape[1]), np.int32), dev)
+                              np.zeros((0, seq_table.shape[1]), np.int32), dev, self.pool.kv8)
         x = lm.embed_tokens(ops.upload(np.asarray(r.prompt[c:c + n], np.int32), dev))
         for layer, pool in zip(lm.layers, self.pool.pools):
             x = layer.mixed(x, pool, ms)

@@ -7,10 +7,11 @@ request's KV that a later request copies back (RequestState.snapshot / restore,
 Q36/kvcache/state.py:58-149; PrefixStore, Q36/kvcache/prefix_cache.py).  Here the KV lives in a
 pool of 16-token pages per layer, [num_pages, Hkv, 2, 16 * 128] bf16 (for each kv head, part 0
 holds K chunk-major ([d / 32][slot][d % 32]) and part 1 holds V dim-major ([d][slot]) -- the
-operand layouts the attention kernels read).  A sequence owns a list of pages, the same page ids
+operand layouts the attention kernels read), or, with kv8=True, [num_pages, Hkv, 4224] uint8 (8-bit codes and a
+scale a token, 0.516 of the bytes; ops.kv8_pool).  A sequence owns a list of pages, the same page ids
 in every layer; token t sits in page pages[t // 16], slot t % 16.  Sharing a prefix is sharing its
 pages: each page carries a reference count, and a sequence about to write into a page that someone
-else also holds first copies it (jit_kv_copy_pages), so a shared page is never written.  The pool
+else also holds first copies it (jit_kv_copy_pages, jit_kv8_copy_pages), so a shared page is never written.  The pool
 is zero-initialised, so every slot of an allocated page always holds finite values.
 """
 
@@ -38,14 +39,15 @@ class KVPool:
 
     `seed` given: free pages are handed out in a seeded random permutation (the configs' page
     tables are "a random permutation of free pages"); otherwise in ascending order.  With
-    allocate=False no device memory is made (bookkeeping only)."""
+    allocate=False no device memory is made (bookkeeping only).  kv8: the 8-bit pools."""
 
     def __init__(self, n_layers: int, num_pages: int, n_kv_heads: int, device, seed: int | None = None,
-                 allocate: bool = True):
+                 allocate: bool = True, kv8: bool = False):
         if num_pages <= 0 or n_layers <= 0 or n_kv_heads <= 0:
             raise ValueError("KVPool needs positive layers, pages and heads")
         self.n_layers, self.num_pages, self.n_kv_heads = int(n_layers), int(num_pages), int(n_kv_heads)
         self.device = torch.device(device)
+        self.kv8 = bool(kv8)
         order = np.arange(num_pages) if seed is None else np.random.default_rng(seed).permutation(num_pages)
         self._free = [int(p) for p in order[::-1]]  # pop() hands out order[0] first
         self.refs = np.zeros(num_pages, np.int32)
@@ -53,7 +55,8 @@ class KVPool:
         self.lengths: dict = {}
         self.copies = 0  # pages copied on write so far
         self.pools = (
-            [torch.zeros((num_pages, n_kv_heads, 2, PAGE * HEAD_DIM), dtype=torch.bfloat16, device=self.device)
+            [ops.kv8_pool(num_pages, n_kv_heads, self.device) if self.kv8 else
+             torch.zeros((num_pages, n_kv_heads, 2, PAGE * HEAD_DIM), dtype=torch.bfloat16, device=self.device)
              for _ in range(n_layers)]
             if allocate else []
         )
@@ -62,7 +65,7 @@ class KVPool:
     @property
     def page_bytes(self) -> int:
         """Bytes of one page in one layer (K and V of every kv head)."""
-        return 2 * self.n_kv_heads * PAGE * HEAD_DIM * 2
+        return self.n_kv_heads * (ops.KV8_RECORD if self.kv8 else 2 * PAGE * HEAD_DIM * 2)
 
     @property
     def free_pages(self) -> int:
@@ -97,7 +100,7 @@ class KVPool:
         s = ops.upload(np.asarray(src, np.int32), self.device)
         d = ops.upload(np.asarray(dst, np.int32), self.device)
         for pool in self.pools:
-            ops.kv_copy_pages(pool, s, d)
+            (ops.kv8_copy_pages if self.kv8 else ops.kv_copy_pages)(pool, s, d)
 
     # -------------------------------------------------------------- sequences
     def open(self, seq_id, pages=(), length: int = 0) -> None:

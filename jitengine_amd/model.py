@@ -81,15 +81,24 @@ class StepState:
 
     pos: torch.Tensor          # int32 [B]: the position each row writes (its length so far)
     page_table: torch.Tensor   # int32 [B, max_pages]
-    plan: ops.AttnPlan         # over lens = pos + 1
+    plan: ops.AttnPlan | None  # over lens = pos + 1 (bf16 pools)
     workspace: torch.Tensor    # attention partials
+    kv8: ops.StepTables | None = None  # 8-bit pools: the step's positions, slots and lengths
+    max_len: int = 0                   # and the longest row's keys
 
 
-def make_step_state(cfg: MoEConfig, pos_host, page_table: torch.Tensor) -> StepState:
+def make_step_state(cfg: MoEConfig, pos_host, page_table: torch.Tensor, kv8: bool = False) -> StepState:
     """Plan one decode step: row b writes position pos_host[b] and attends to pos + 1 keys (the
-    plan and its workspace serve every layer of the step)."""
+    plan and its workspace serve every layer of the step).  kv8: over 8-bit pools."""
     pos_host = np.asarray(pos_host, np.int32)
     dev = page_table.device
+    if kv8:
+        B = pos_host.shape[0]
+        max_len = _kv8_keys(pos_host + 1, page_table.shape[1])
+        up = ops.upload(np.stack([pos_host, np.ones_like(pos_host)]), dev)
+        t = ops.step_tables(up[0], up[1], page_table, B)
+        ws = torch.empty(ops.kv8_decode_workspace_bytes(B, cfg.heads, max_len), dtype=torch.uint8, device=dev)
+        return StepState(t.pos, page_table, None, ws, t, max_len)
     plan = ops.attn_plan(pos_host + 1, dev)
     ws = torch.empty(max(ops.attn_split_workspace_bytes(plan.total, cfg.heads, cfg.kv_heads), 4), dtype=torch.uint8,
                      device=dev)
@@ -105,20 +114,53 @@ class MixedState:
 
     P: int                       # prefill rows (the first P rows)
     pos_rows: torch.Tensor       # int32 [T]
-    table_rows: torch.Tensor     # int32 [T, max_pages]: row r's sequence's pages
-    seq_table: torch.Tensor      # int32 [S, max_pages]: the prefill sequences' pages
+    table_rows: torch.Tensor | None  # int32 [T, max_pages]: row r's sequence's pages (bf16 pools)
+    seq_table: torch.Tensor      # int32 [S, max_pages]: the prefill sequences' pages (8-bit pools: the chunks')
     prefill: ops.PrefillPlan     # chunks (seq index into seq_table, ctx, length)
     dec_table: torch.Tensor      # int32 [D, max_pages]: the decode sequences' pages
-    decode: ops.AttnPlan         # decode lens = pos + 1
+    decode: ops.AttnPlan | None  # decode lens = pos + 1 (bf16 pools)
     workspace: torch.Tensor
+    kv8: ops.StepTables | None = None  # 8-bit pools: positions, slots and lengths of the chunks, then the decode rows
+    max_len: int = 0                   # and the longest decode row's keys
 
 
-def make_mixed_state(cfg: MoEConfig, chunks, seq_table_host, dec_pos_host, dec_table_host, device) -> MixedState:
+def _kv8_keys(lens, width: int) -> int:
+    """The most keys of a step's rows (ValueError where they do not fit page tables `width` pages wide)."""
+    top = int(lens.max()) if lens.size else 0
+    if top > width * ops.PAGE or (lens.size and int(lens.min()) < 1):
+        raise ValueError(f"positions outside [0, {width * ops.PAGE}) (the page table's width)")
+    return top
+
+
+def make_mixed_state(cfg: MoEConfig, chunks, seq_table_host, dec_pos_host, dec_table_host, device,
+                     kv8: bool = False) -> MixedState:
     """chunks [(seq, ctx, length)] over the rows of seq_table_host [S, max_pages]; decode sequence d
-    writes position dec_pos_host[d] through dec_table_host[d] (both tables of equal width)."""
+    writes position dec_pos_host[d] through dec_table_host[d] (both tables of equal width).  kv8: over 8-bit pools."""
     seq_table_host = np.asarray(seq_table_host, np.int32)
     dec_table_host = np.asarray(dec_table_host, np.int32)
     dec_pos = np.asarray(dec_pos_host, np.int32)
+    if kv8:
+        # every chunk and every decode row is a sequence of the step's tables: rows of one page table, no table a row
+        C, D = len(chunks), dec_pos.shape[0]
+        seqs = np.array([c[0] for c in chunks], np.int64)
+        if dec_table_host.shape[0] != D or (C and (seqs.min() < 0 or seqs.max() >= seq_table_host.shape[0])):
+            raise ValueError(f"the step's {C} chunks and {D} decode rows do not match its tables")
+        if C and D and seq_table_host.shape[1] != dec_table_host.shape[1]:
+            raise ValueError("the step's two page tables differ in width")
+        W = seq_table_host.shape[1] if C else dec_table_host.shape[1]
+        tab = np.concatenate([seq_table_host.reshape(-1, W)[seqs] if C else np.zeros((0, W), np.int32),
+                              dec_table_host.reshape(-1, W)])
+        ctx = np.concatenate([np.array([c[1] for c in chunks], np.int32), dec_pos]).astype(np.int32)
+        new = np.concatenate([np.array([c[2] for c in chunks], np.int32), np.ones(D, np.int32)]).astype(np.int32)
+        _kv8_keys(ctx + new, W)
+        max_len = _kv8_keys(dec_pos + 1, W)
+        up = ops.upload(np.concatenate([tab.reshape(-1), ctx, new]), device)
+        table, n = up[:tab.size].view(C + D, W), tab.size
+        P = int(new[:C].sum())
+        t = ops.step_tables(up[n:n + C + D], up[n + C + D:], table, P + D)
+        ws = torch.empty(ops.kv8_decode_workspace_bytes(D, cfg.heads, max_len), dtype=torch.uint8, device=device)
+        plan = ops.prefill_plan([(i, c[1], c[2]) for i, c in enumerate(chunks)], cfg.heads, cfg.kv_heads, device)
+        return MixedState(P, t.pos, None, table[:C], plan, table[C:], None, ws, t, max_len)
     pos, rows = [], []
     for seq, ctx, length in chunks:
         pos += range(ctx, ctx + length)
@@ -206,7 +248,11 @@ class DecoderLayer:
         if defer and B != 1:
             raise ValueError("defer takes a one-token step")
         scale = cfg.head_dim ** -0.5
-        if debug is None:  # q/k norm + RoPE + append inside the attention launch (the same bits)
+        if _over_kv8(pool, st):
+            q = ops.qk_norm_rope_append_kv8(qkv, cfg.heads, cfg.kv_heads, self.q_norm, self.k_norm, cfg.eps,
+                                            self.inv_freq, st.kv8.pos, st.kv8.slots, pool)
+            attn = ops.paged_decode_attention_kv8(q, pool, st.page_table, st.kv8.lens, st.max_len, scale, st.workspace)
+        elif debug is None:  # q/k norm + RoPE + append inside the attention launch (the same bits)
             q = None
             attn = ops.paged_decode_attention_qkv(qkv, cfg.heads, cfg.kv_heads, self.q_norm, self.k_norm, cfg.eps,
                                                   self.inv_freq, pool, st.page_table, st.plan, scale, st.workspace)
@@ -256,16 +302,26 @@ class DecoderLayer:
         if debug is None and T:
             lay = self.native()
             if lay is not None:
-                return self._mixed_native(lay, x, pool, ms)
+                return (self._mixed_native_kv8 if _over_kv8(pool, ms) else self._mixed_native)(lay, x, pool, ms)
         xn = ops.rmsnorm(x, self.input_norm, cfg.eps)
         qkv = ops.qmm(xn, self.qkv)
-        q = ops.qk_norm_rope_append(qkv, cfg.heads, cfg.kv_heads, self.q_norm, self.k_norm, cfg.eps,
-                                    self.inv_freq, ms.pos_rows, ms.table_rows, pool)
         scale = cfg.head_dim ** -0.5
         parts = []
-        if ms.P:
+        if _over_kv8(pool, ms):
+            q = ops.qk_norm_rope_append_kv8(qkv, cfg.heads, cfg.kv_heads, self.q_norm, self.k_norm, cfg.eps,
+                                            self.inv_freq, ms.kv8.pos, ms.kv8.slots, pool)
+            if ms.P:
+                parts.append(ops.paged_prefill_attention_kv8(q[:ms.P], pool, ms.seq_table, ms.prefill, scale))
+            if T > ms.P:
+                parts.append(ops.paged_decode_attention_kv8(q[ms.P:], pool, ms.dec_table,
+                                                            ms.kv8.lens[ms.seq_table.shape[0]:], ms.max_len, scale,
+                                                            ms.workspace))
+        else:
+            q = ops.qk_norm_rope_append(qkv, cfg.heads, cfg.kv_heads, self.q_norm, self.k_norm, cfg.eps,
+                                        self.inv_freq, ms.pos_rows, ms.table_rows, pool)
+        if ms.kv8 is None and ms.P:
             parts.append(ops.paged_prefill_attention(q[:ms.P], pool, ms.seq_table, ms.prefill, scale))
-        if T > ms.P:
+        if ms.kv8 is None and T > ms.P:
             parts.append(ops.paged_decode_attention(q[ms.P:], pool, ms.dec_table, ms.decode, scale, ms.workspace))
         attn = torch.cat(parts) if len(parts) > 1 else parts[0]
         o = ops.qmm(attn.view(T, -1), self.o)
@@ -312,6 +368,32 @@ class DecoderLayer:
                                        x.data_ptr(), scratch.data_ptr(), y.data_ptr(), ops._stream()), "mixed_layer")
         return y
 
+    def _mixed_native_kv8(self, lay, x: torch.Tensor, pool: torch.Tensor, ms: MixedState) -> torch.Tensor:
+        """_mixed_native over an 8-bit pool."""
+        T, D, dev, pf, cfg = x.shape[0], self.cfg.hidden, x.device, ms.prefill, self.cfg
+        _kv8_rows_contract(x, D, pool, cfg.kv_heads, ms.kv8)
+        C, nd = ms.seq_table.shape[0], T - ms.P
+        if nd < 0 or pf.rows != ms.P or ms.kv8.lens.numel() != C + nd or ms.seq_table.shape[1] != ms.dec_table.shape[1]:
+            raise ValueError(f"x has {T} rows, which the step's tables and its {ms.P} prompt rows do not match")
+        p = _lib.Kv8Step(prompt_rows=ms.P, pos=ms.kv8.pos.data_ptr(), slots=ms.kv8.slots.data_ptr())
+        _kv8_decode_rows(p, cfg, ms.dec_table, ms.kv8.lens[C:], ms.max_len, ms.workspace)
+        if ms.P:
+            ops.prefill_contract(pf, ms.seq_table)
+            pws = torch.empty(ops.kv8_prefill_workspace_bytes(pf, cfg.heads, cfg.kv_heads), dtype=torch.uint8, device=dev)
+            tb, bl = pf.tables.data_ptr(), pf.blocks.data_ptr()
+            nblk = pf.blocks.shape[1]
+            p.C, p.nblk, p.units, p.pmax, p.prompt_max_len = C, nblk, pf.total_units, pf.pmax, pf.max_len
+            p.prompt_table, p.max_pages = ms.seq_table.data_ptr(), ms.seq_table.shape[1]
+            p.chunk_seq, p.chunk_ctx, p.chunk_len, p.chunk_row = tb, tb + 4 * C, tb + 8 * C, tb + 12 * C
+            p.chunk_unit, p.blk_chunk, p.blk_q0, p.blk_part = pf.units.data_ptr(), bl, bl + 4 * nblk, bl + 8 * nblk
+            p.prompt_workspace, p.prompt_workspace_bytes = pws.data_ptr(), pws.nbytes
+        lib = _lib.lib()
+        scratch = _layer_scratch(lib, lay, T, 1, dev)
+        y = torch.empty_like(x)
+        ops._launch(x.get_device(), lib.jit_mixed_layer_kv8, "mixed_layer_kv8", ctypes.byref(lay), ctypes.byref(p),
+                    pool.data_ptr(), pool.shape[0], x.data_ptr(), scratch.data_ptr(), y.data_ptr())
+        return y
+
 
 # What a layer's native calls do in place of: replaced in a subclass, an instance or the class itself, these are
 # called (the op-by-op path).
@@ -340,6 +422,37 @@ def _rows_contract(x: torch.Tensor | None, D: int, pool: torch.Tensor, Hkv: int)
         raise ValueError(f"the pool has {pool.shape[1]} kv heads, the layer {Hkv}")
 
 
+def _over_kv8(pool: torch.Tensor, st) -> bool:
+    """Whether a step runs over an 8-bit pool (ValueError where its state was made for the other kind)."""
+    kv8 = ops.is_kv8(pool)
+    if kv8 != (st.kv8 is not None):
+        raise ValueError(f"the pool is {'an 8-bit' if kv8 else 'a bf16'} one, the step's state is for the other kind "
+                         "(make_step_state and make_mixed_state take kv8=)")
+    return kv8
+
+
+def _kv8_rows_contract(x: torch.Tensor, D: int, pool: torch.Tensor, Hkv: int, t: ops.StepTables) -> None:
+    """_rows_contract of an 8-bit pool, with the step's tables."""
+    if x.dim() != 2 or x.shape[1] != D:
+        raise ValueError(f"x {tuple(x.shape)} must be [rows, {D}]")
+    if t.pos.shape != x.shape[:1] or t.slots.shape != x.shape[:1]:
+        raise ValueError(f"x has {x.shape[0]} rows, the step's tables {t.pos.numel()}")
+    ops._take((x, torch.bfloat16, "x"), (pool, torch.uint8, "pool"), (t.pos, torch.int32, "pos"),
+              (t.slots, torch.int32, "slots"), (t.lens, torch.int32, "lens"))
+    if ops._kv8_heads(pool) != Hkv:
+        raise ValueError(f"the pool has {pool.shape[1]} kv heads, the layer {Hkv}")
+
+
+def _kv8_decode_rows(p, cfg: MoEConfig, table: torch.Tensor, lens: torch.Tensor, max_len: int, ws: torch.Tensor) -> None:
+    """The decode rows' fields of a jit_kv8_step."""
+    B = lens.numel()
+    ops._take((lens, torch.int32, "lens"), (table, torch.int32, "page_table"))
+    if table.dim() != 2 or table.shape[0] != B or max_len > table.shape[1] * ops.PAGE:
+        raise ValueError(f"page_table {tuple(table.shape)} does not hold {B} rows of up to {max_len} keys")
+    p.B, p.max_pages, p.max_len = B, table.shape[1], max_len
+    p.page_table, p.lens, p.workspace, p.workspace_bytes = table.data_ptr(), lens.data_ptr(), ws.data_ptr(), ws.nbytes
+
+
 def _decode_rows(cfg: MoEConfig, table: torch.Tensor, plan: ops.AttnPlan, workspace, device):
     """(jit_decode_rows, the workspace it points to) of a step's decode rows."""
     B = plan.lens.shape[0]
@@ -357,8 +470,8 @@ class Model:
         self.cfg = cfg
         self.layers = [DecoderLayer(cfg, w, prepack) for w in layer_weights]
 
-    def make_state(self, pos_host, page_table: torch.Tensor) -> StepState:
-        return make_step_state(self.cfg, pos_host, page_table)
+    def make_state(self, pos_host, page_table: torch.Tensor, kv8: bool = False) -> StepState:
+        return make_step_state(self.cfg, pos_host, page_table, kv8)
 
     def decode_step(self, x: torch.Tensor, pools: list, st: StepState) -> torch.Tensor:
         """x [B, D] bf16 hidden rows -> the last layer's output rows; pools[l] is layer l's KV pool."""
@@ -391,27 +504,38 @@ class Model:
 
     def _decode_native(self, lays: list, x: torch.Tensor, pools: list, st: StepState) -> torch.Tensor:
         """decode_step with a native call a layer (the same launches and bits)."""
-        cfg, lib, stream, dev = self.cfg, _lib.lib(), ops._stream(), x.device
+        cfg, lib, dev = self.cfg, _lib.lib(), x.device
         B, D = x.shape[0], cfg.hidden
-        d, ws = _decode_rows(cfg, st.page_table, st.plan, st.workspace, dev)
+        kv8 = bool(pools) and _over_kv8(pools[0], st)
+        if kv8:
+            d = _lib.Kv8Step(pos=st.kv8.pos.data_ptr(), slots=st.kv8.slots.data_ptr())
+            _kv8_decode_rows(d, cfg, st.page_table, st.kv8.lens, st.max_len, st.workspace)
+        else:
+            d, ws = _decode_rows(cfg, st.page_table, st.plan, st.workspace, dev)
         if B != d.B:
             raise ValueError(f"x has {B} rows, the step {d.B}")
+        stream = ops._stream()
         dp, xn, prev = ctypes.byref(d), None, None
         n = min(len(lays), len(pools))
         for i, (lay, pool) in enumerate(zip(lays, pools)):
             # (x is the step's input, or the rows the previous call wrote; a deferred combine keeps its scratch)
-            _rows_contract(x if i == 0 else None, D, pool, cfg.kv_heads)
+            if kv8:
+                _kv8_rows_contract(x, D, pool, cfg.kv_heads, st.kv8)
+            else:
+                _rows_contract(x if i == 0 else None, D, pool, cfg.kv_heads)
             last = i + 1 == n
             defer = B == 1 and not last and ops.row_prologue_fits(self.layers[i + 1].qkv, D)
             lp = ctypes.byref(lay)
-            scratch = _layer_scratch(lib, lay, B, 0, dev)
+            scratch = _layer_scratch(lib, lay, B, int(kv8), dev)
             out = None if defer else torch.empty((1 if last else 2, B, D), dtype=torch.bfloat16, device=dev)
-            _lib.check(lib.jit_decode_layer(
-                lp, dp, pool.data_ptr(), x.data_ptr(), ops._p(xn), None if prev is None else ctypes.byref(lays[i - 1]),
-                ops._p(prev), int(defer),
-                None if last else self.layers[i + 1].input_norm.data_ptr(), scratch.data_ptr(),
-                None if defer else out[0].data_ptr(), None if defer or last else out[1].data_ptr(), stream),
-                "decode_layer")
+            args = (x.data_ptr(), ops._p(xn), None if prev is None else ctypes.byref(lays[i - 1]), ops._p(prev),
+                    int(defer), None if last else self.layers[i + 1].input_norm.data_ptr(), scratch.data_ptr(),
+                    None if defer else out[0].data_ptr(), None if defer or last else out[1].data_ptr())
+            if kv8:
+                ops._launch(dev.index, lib.jit_decode_layer_kv8, "decode_layer_kv8", lp, dp, pool.data_ptr(),
+                            pool.shape[0], *args)
+            else:
+                _lib.check(lib.jit_decode_layer(lp, dp, pool.data_ptr(), *args, stream), "decode_layer")
             if defer:
                 xn, prev = None, scratch
             else:

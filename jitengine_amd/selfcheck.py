@@ -160,6 +160,40 @@ def _prefill(dev) -> None:
     _close("paged prefill attention", out, want)
 
 
+def _kv8(dev) -> None:
+    """The 8-bit cache: tables, writes, decode and prompt attention over small integers, which its codes hold exactly."""
+    g = torch.Generator(device=dev).manual_seed(11)
+    H, Hkv, D, scale = 8, 2, ops.HEAD_DIM, ops.HEAD_DIM ** -0.5
+    lens = [5, 600]
+    n = sum(lens)
+    W = -(-max(lens) // ops.PAGE)
+    pool = ops.kv8_pool(2 * W, Hkv, dev)
+    table = torch.randperm(2 * W, device=dev).to(torch.int32).view(2, W)
+    # (an integer up to 8 has at most 4 significant bits: exact under any power-of-two scale)
+    k, v = (torch.randint(-8, 9, (n, Hkv, D), generator=g, device=dev).to(torch.bfloat16) for _ in range(2))
+    zero = torch.zeros(2, dtype=torch.int32, device=dev)
+    t = ops.step_tables(zero, torch.tensor(lens, dtype=torch.int32, device=dev), table, n)
+    _equal("step_tables lens", t.lens, torch.tensor(lens, device=dev))
+    _equal("step_tables pos", t.pos, torch.cat([torch.arange(m, device=dev) for m in lens]))
+    ops.kv8_append_paged(pool, k, v, t.slots)
+    q = torch.randn((n, H, D), generator=g, device=dev).to(torch.bfloat16)
+    got = ops.paged_prefill_attention_kv8(q, pool, table, ops.prefill_plan([(0, 0, lens[0]), (1, 0, lens[1])], H, Hkv,
+                                                                          dev), scale)
+    want, row, last = torch.empty((n, H, D), device=dev), 0, []
+    for m in lens:
+        qb = q[row:row + m].float().reshape(m, Hkv, H // Hkv, D).permute(1, 0, 2, 3).reshape(Hkv, -1, D)
+        kb, vb = (x[row:row + m].float().permute(1, 0, 2).contiguous() for x in (k, v))
+        s = (qb @ kb.transpose(1, 2).contiguous() * scale).view(Hkv, m, H // Hkv, m)
+        causal = torch.arange(m, device=dev)[None, :] > torch.arange(m, device=dev)[:, None]
+        p = torch.softmax(s.masked_fill(causal[None, :, None, :], -torch.inf), dim=-1).reshape(Hkv, -1, m)
+        want[row:row + m] = (p @ vb).view(Hkv, m, H // Hkv, D).permute(1, 0, 2, 3).reshape(m, H, D)
+        row += m
+        last.append(row - 1)
+    _close("8-bit prompt attention", got, want)
+    got = ops.paged_decode_attention_kv8(q[last].contiguous(), pool, table, t.lens, max(lens), scale)
+    _close("8-bit decode attention", got, want[last])
+
+
 def _segment(dev) -> None:
     """The segment GEMMs of long expert segments (bf16 weights, bf16(s q + b)) with SwiGLU."""
     g = torch.Generator(device=dev).manual_seed(8)
@@ -186,7 +220,7 @@ def _sampler(dev) -> None:
 
 CASES = (("router + packing", _router_and_pack), ("projections + experts", _projections),
          ("rmsnorm + attention", _norm_and_attention), ("prefill attention", _prefill),
-         ("segment GEMMs", _segment), ("sampler", _sampler))
+         ("8-bit cache", _kv8), ("segment GEMMs", _segment), ("sampler", _sampler))
 
 
 def run(device=None, force: bool = False) -> list:

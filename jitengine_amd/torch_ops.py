@@ -10,7 +10,8 @@ Host-side structures of jitengine_amd.ops are passed as their tensors and sizes:
   * a decode attention plan (ops.AttnPlan) as its three int32 tensors, its chunk count and the
     longest sequence (plan_args);
   * a prefill plan (ops.PrefillPlan) as its two int32 tables, its chunks flattened into (seq, ctx,
-    length) triples, its most key parts of a token and its longest chunk (prefill_plan_args).
+    length) triples, its most key parts of a token and its longest chunk (prefill_plan_args);
+  * a step's tables (ops.StepTables) as the tuple of their six int32 tensors.
 Importing this module registers the operators; it needs the HIP library only when one runs.
 """
 
@@ -325,6 +326,96 @@ def plan_args(plan: ops.AttnPlan) -> tuple:
     return plan.lens, plan.chunk_start, plan.chunk_seq, plan.total, mx
 
 
+# ----------------------------------------------------------------------------- 8-bit KV
+@torch.library.custom_op(f"{_NS}::step_tables", mutates_args=("page_table",))
+def step_tables(ctx: torch.Tensor, new: torch.Tensor, page_table: torch.Tensor, rows: int, free: torch.Tensor | None,
+                free_at: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                                                       torch.Tensor, torch.Tensor]:
+    """(row_start, row_seq, pos, slots, lens, status) of a step (jit_step_tables; page_table grows with `free`)."""
+    t = ops.step_tables(ctx, new, page_table, rows, free, free_at)
+    # (six tensors of their own: an operator's outputs share no storage)
+    return tuple(x.clone() for x in (t.row_start, t.row_seq, t.pos, t.slots, t.lens, t.status))
+
+
+@step_tables.register_fake
+def _(ctx, new, page_table, rows, free, free_at):
+    S = ctx.shape[0]
+    return tuple(ctx.new_empty((n,)) for n in (S + 1, rows, rows, rows, S, 4))
+
+
+@torch.library.custom_op(f"{_NS}::kv8_append_paged", mutates_args=("pool",))
+def kv8_append_paged(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """k, v [B, Hkv, 128] written at slots [B] of the 8-bit pool (jit_kv8_append_paged)."""
+    ops.kv8_append_paged(pool, k, v, slots)
+
+
+@kv8_append_paged.register_fake
+def _(pool, k, v, slots):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rope_append_kv8", mutates_args=("pool",))
+def qk_norm_rope_append_kv8(qkv: torch.Tensor, H: int, Hkv: int, q_norm: torch.Tensor, k_norm: torch.Tensor,
+                            eps: float, inv_freq: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor,
+                            pool: torch.Tensor) -> torch.Tensor:
+    """q bf16 [B, H, 128] (normed, rotated); k and v of every row written into the 8-bit pool
+    (jit_qk_norm_rope_append_kv8)."""
+    return ops.qk_norm_rope_append_kv8(qkv, H, Hkv, q_norm, k_norm, eps, inv_freq, pos, slots, pool)
+
+
+@qk_norm_rope_append_kv8.register_fake
+def _(qkv, H, Hkv, q_norm, k_norm, eps, inv_freq, pos, slots, pool):
+    return qkv.new_empty((qkv.shape[0], H, ops.HEAD_DIM), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op(f"{_NS}::paged_decode_attention_kv8", mutates_args=("workspace",))
+def paged_decode_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+                               max_len: int, scale: float, workspace: torch.Tensor) -> torch.Tensor:
+    """out bf16 [B, H, 128] of paged decode attention over an 8-bit pool (jit_paged_decode_attn_kv8; workspace of
+    kv8_decode_workspace_bytes bytes)."""
+    return ops.paged_decode_attention_kv8(q, pool, page_table, lens, max_len, scale, workspace)
+
+
+@paged_decode_attention_kv8.register_fake
+def _(q, pool, page_table, lens, max_len, scale, workspace):
+    return torch.empty_like(q)
+
+
+@torch.library.custom_op(f"{_NS}::paged_prefill_attention_kv8", mutates_args=("workspace",))
+def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, tables: torch.Tensor,
+                                blocks: torch.Tensor, units: torch.Tensor, chunks: list[int], pmax: int, max_len: int,
+                                scale: float, workspace: torch.Tensor) -> torch.Tensor:
+    """out bf16 [T, H, 128]: paged_prefill_attention over an 8-bit pool (jit_paged_prefill_attn_kv8; the plan by
+    kv8_prefill_plan_args, workspace of kv8_prefill_workspace_bytes bytes)."""
+    trip = [tuple(chunks[i:i + 3]) for i in range(0, len(chunks), 3)]
+    total = int(ops._chunk_units(trip)[-1])
+    plan = ops.PrefillPlan(trip, tables, blocks, sum(c[2] for c in trip), int(pmax), int(max_len), units, total)
+    return ops.paged_prefill_attention_kv8(q, pool, page_table, plan, scale, workspace)
+
+
+@paged_prefill_attention_kv8.register_fake
+def _(q, pool, page_table, tables, blocks, units, chunks, pmax, max_len, scale, workspace):
+    return torch.empty_like(q)
+
+
+def kv8_prefill_plan_args(plan: ops.PrefillPlan) -> tuple:
+    """(tables, blocks, units, chunks, pmax, max_len) of a prefill plan, for
+    torch.ops.jitengine.paged_prefill_attention_kv8."""
+    t, b, *rest = prefill_plan_args(plan)
+    return t, b, plan.units, *rest
+
+
+@torch.library.custom_op(f"{_NS}::kv8_copy_pages", mutates_args=("pool",))
+def kv8_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Pages src[i] copied to dst[i] inside one layer's 8-bit pool (jit_kv8_copy_pages)."""
+    ops.kv8_copy_pages(pool, src, dst)
+
+
+@kv8_copy_pages.register_fake
+def _(pool, src, dst):
+    return None
+
+
 # ----------------------------------------------------------------------------- sampler
 @torch.library.custom_op(f"{_NS}::logprobs_rows", mutates_args=())
 def logprobs_rows(logits: torch.Tensor) -> torch.Tensor:
@@ -374,3 +465,5 @@ OPS = ("router_topk", "moe_pack", "route_pack", "expert_gate_up", "route_gate_up
        "moe_combine_rmsnorm", "qmm", "rmsnorm", "rmsnorm_add", "qmm_add_rmsnorm", "qmm_combine_rmsnorm",
        "qk_norm_rope_append", "paged_decode_attention", "paged_decode_attention_qkv", "paged_prefill_attention",
        "kv_append_paged", "kv_copy_pages", "logprobs_rows", "argmax_rows", "sample_rows", "threefry_uniform")
+OPS_KV8 = ("step_tables", "kv8_append_paged", "qk_norm_rope_append_kv8", "paged_decode_attention_kv8",
+           "paged_prefill_attention_kv8", "kv8_copy_pages")
