@@ -565,20 +565,33 @@ int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, int num_pages
                               int max_pages, const int32_t *lens, int B, int H, int Hkv, int max_len, float scale,
                               void *workspace, int64_t workspace_bytes, uint16_t *out, void *stream);
 
-/* jit_paged_prefill_attn over an 8-bit pool: the same chunks, work items and parts.  The keys that the chunks see are
- * expanded into the workspace first, JIT_KV8_UNIT_KEYS (a unit) at a time: chunk_unit [C + 1] (device) holds the
- * first unit of each chunk, ceil((ctx + len) / JIT_KV8_UNIT_KEYS) units a chunk, and their number `units` last.  T: the
- * q rows.  Keys of page ids outside the pool are left out; a row without a key gives zeros.
- * Contract: that of jit_paged_prefill_attn, scale > 0 and a workspace of jit_kv8_prefill_workspace_bytes bytes (32,776
- * bytes a unit and kv head, and the partials) (JIT_EINVAL). */
+/* jit_paged_prefill_attn over an 8-bit pool: causal attention of prompt chunks in row blocks and key parts of their own.
+ * The keys that the chunks see are expanded into the workspace first, JIT_KV8_UNIT_KEYS (a unit) at a time.  On top of
+ * that call's chunk tables, [C + 1] each (device):
+ *   chunk_unit  first unit of each chunk, ceil((ctx + len) / JIT_KV8_UNIT_KEYS) units a chunk; their number `units` last;
+ *   chunk_part  the units of each chunk's key parts, jit_kv8_prefill_part_units of its ctx and len;
+ *   chunk_slot  first partial slot of each chunk, len x its parts in a chunk of more than one; their number `slots` last.
+ * Work items: (blk_chunk, blk_q0, blk_part) for every jit_kv8_prefill_block_tokens tokens of a chunk and every part that
+ * holds keys of theirs, in any order.  max_len: the longest chunk.  Keys of page ids outside the pool are left out; a row
+ * without a key gives zeros.  A row's bits depend on its sequence and its chunk's ctx and len alone.
+ * Contract: H / Hkv in {1, 2, 4, 8, 16} (JIT_EUNSUPPORTED), scale > 0, a workspace of jit_kv8_prefill_workspace_bytes
+ * bytes (32,776 bytes a unit and kv head, and the partials) (JIT_EINVAL). */
 #define JIT_KV8_UNIT_KEYS 64
-int64_t jit_kv8_prefill_workspace_bytes(int T, int pmax, int H, int Hkv, int units);
+int jit_kv8_prefill_block_tokens(int H, int Hkv);
+int jit_kv8_prefill_part_units(int ctx, int len, int H, int Hkv);
+/* The tables and work items of C chunks (host arrays): tables [3][C + 1] chunk_unit, chunk_part, chunk_slot; blocks [3][n]
+ * blk_chunk, blk_q0, blk_part, the items with the most keys first.  Returns the number of items (blocks NULL: that alone
+ * and the tables) or an error. */
+int jit_kv8_prefill_plan(const int32_t *ctx, const int32_t *len, int C, int H, int Hkv, int32_t *tables, int32_t *blocks,
+                         int n);
+int64_t jit_kv8_prefill_workspace_bytes(int H, int Hkv, int units, int slots);
 int jit_paged_prefill_attn_kv8(const uint16_t *q, const void *pool, int num_pages, const int32_t *page_table,
                                int max_pages, const int32_t *chunk_seq, const int32_t *chunk_ctx,
-                               const int32_t *chunk_len, const int32_t *chunk_row, const int32_t *chunk_unit, int C,
-                               int units, const int32_t *blk_chunk, const int32_t *blk_q0, const int32_t *blk_part,
-                               int nblk, int T, int pmax, int max_len, int H, int Hkv, float scale, void *workspace,
-                               int64_t workspace_bytes, uint16_t *out, void *stream);
+                               const int32_t *chunk_len, const int32_t *chunk_row, const int32_t *chunk_unit,
+                               const int32_t *chunk_part, const int32_t *chunk_slot, int C, int units, int slots,
+                               const int32_t *blk_chunk, const int32_t *blk_q0, const int32_t *blk_part, int nblk,
+                               int max_len, int H, int Hkv, float scale, void *workspace, int64_t workspace_bytes,
+                               uint16_t *out, void *stream);
 
 /* ------------------------------------------------------------ whole layers --
  * One decoder layer per call (Q36/model/model.py:65-80): the launches above, in their order, issued from
@@ -628,8 +641,9 @@ int jit_mixed_layer(const jit_layer *layer, const jit_prompt_rows *p, const jit_
  * rows with those of jit_paged_decode_attn_kv8; pos, slots [prompt_rows + B] of jit_step_tables.  Both page tables are
  * max_pages wide. */
 typedef struct {
-  int prompt_rows, B, C, nblk, units, pmax, prompt_max_len, max_pages, max_len;
-  const int32_t *pos, *slots, *prompt_table, *chunk_seq, *chunk_ctx, *chunk_len, *chunk_row, *chunk_unit;
+  int prompt_rows, B, C, nblk, units, part_slots, prompt_max_len, max_pages, max_len;
+  const int32_t *pos, *slots, *prompt_table, *chunk_seq, *chunk_ctx, *chunk_len, *chunk_row;
+  const int32_t *chunk_unit, *chunk_part, *chunk_slot;
   const int32_t *blk_chunk, *blk_q0, *blk_part, *page_table, *lens;
   void *prompt_workspace, *workspace;
   int64_t prompt_workspace_bytes, workspace_bytes;

@@ -46,10 +46,10 @@ class PromptRows(ctypes.Structure):
 
 class Kv8Step(ctypes.Structure):
     """jit_kv8_step"""
-    _fields_ = [(n, _I) for n in ("prompt_rows", "B", "C", "nblk", "units", "pmax", "prompt_max_len", "max_pages",
+    _fields_ = [(n, _I) for n in ("prompt_rows", "B", "C", "nblk", "units", "part_slots", "prompt_max_len", "max_pages",
                                   "max_len")] + [
         (n, _P) for n in ("pos", "slots", "prompt_table", "chunk_seq", "chunk_ctx", "chunk_len", "chunk_row",
-                          "chunk_unit", "blk_chunk", "blk_q0", "blk_part", "page_table", "lens", "prompt_workspace",
+                          "chunk_unit", "chunk_part", "chunk_slot", "blk_chunk", "blk_q0", "blk_part", "page_table", "lens", "prompt_workspace",
                           "workspace")] + [("prompt_workspace_bytes", _L), ("workspace_bytes", _L)]
 
 
@@ -123,9 +123,12 @@ _SIGNATURES = {
     "jit_kv8_chunk_tokens": [_I],
     "jit_kv8_decode_workspace_bytes": [_I, _I, _I],
     "jit_paged_decode_attn_kv8": [_P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, ctypes.c_int64, _P, _P],
-    "jit_kv8_prefill_workspace_bytes": [_I, _I, _I, _I, _I],
-    "jit_paged_prefill_attn_kv8": [_P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F,
-                                   _P, ctypes.c_int64, _P, _P],
+    "jit_kv8_prefill_block_tokens": [_I, _I],
+    "jit_kv8_prefill_part_units": [_I, _I, _I, _I],
+    "jit_kv8_prefill_plan": [_P, _P, _I, _I, _I, _P, _P, _I],
+    "jit_kv8_prefill_workspace_bytes": [_I, _I, _I, _I],
+    "jit_paged_prefill_attn_kv8": [_P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I,
+                                   _F, _P, ctypes.c_int64, _P, _P],
 }
 _RESTYPES = {"jit_last_error": ctypes.c_char_p, "jit_attn_workspace_bytes": ctypes.c_int64,
              "jit_attn_split_workspace_bytes": ctypes.c_int64, "jit_layer_scratch_bytes": ctypes.c_int64,

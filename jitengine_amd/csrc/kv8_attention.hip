@@ -395,17 +395,18 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
 // Every row block of a chunk reads all of its keys, so the conversion is done once instead of once a block; inside the
 // attention loop it cost as many vector instructions as the softmax (2,048 rows after 8,192 keys: 344 us, now 328).
 //
-// The second: a workgroup owns WAVES x 32 rows (32 / G tokens x the G q heads of a kv head a wave) and walks the keys up
-// to its last token 64 (a unit) at a time, a unit's 32 KB going straight from memory into LDS.
+// The second: a workgroup owns 4 waves x 32 rows (32 / G tokens x the G q heads of a kv head a wave) and walks the keys
+// of a part, up to its last token, 64 (a unit) at a time, a unit's 32 KB going straight from memory into LDS.  Two
+// workgroups share a CU.
 //   S^T[32 keys x 32 rows] = K . Q^T        (8 MFMA 32x32x16 bf16)
 //   O^T[128 dims x 32 rows] += V^T . P^T    (4 MFMA 32x32x16 fp16 a page)
 // A lane owns one row throughout: its scores of a page are its P operand as they are, since the 16 keys of V's
 // operand are kept in the order in which the score tile holds them.
-constexpr int kRowsWave = 32, kBlockRows = 256;  // a row block (jit_prefill_block_tokens): 256 / G tokens
+constexpr int kPfWaves = 4, kStages = 2;  // waves a workgroup; units in LDS: the one in use, and those on their way
+constexpr int kRowsWave = 32, kBlockRows = kPfWaves * kRowsWave;  // a row block: 128 / G tokens
 constexpr int kUnitKeys = JIT_KV8_UNIT_KEYS, kUnitPages = kUnitKeys / kPage;
 constexpr int kUnitBytes = 2 * kUnitKeys * kD * 2;  // K, then V
-constexpr int kPartKeys = 6144;                  // key parts (jit_prefill_part_keys)
-constexpr int kPartUnits = kPartKeys / kUnitKeys;
+constexpr int kPartMax = 192;  // units of the longest part: every unit's workgroup looks through its part's scales
 constexpr int kPfSlot = kD + 4;                  // floats of a (token, part, head) partial: o, max, sum, 2 pad
 // Expanded values are relative to the loudest scale 2^E of the part's keys, times 2^7 (448 x 2^7 < 65,504): a value of
 // a token 2^22 times quieter than that still has all its bits.
@@ -428,12 +429,13 @@ struct PrefillArgs {
   const uint8_t *pool;
   const int32_t *page_table;
   const int32_t *blk_chunk, *blk_q0, *blk_part;
-  const int32_t *chunk_seq, *chunk_ctx, *chunk_len, *chunk_row, *chunk_unit;  // chunk_unit [C + 1]: first unit of each
+  const int32_t *chunk_seq, *chunk_ctx, *chunk_len, *chunk_row;
+  const int32_t *chunk_unit, *chunk_part, *chunk_slot;  // [C + 1]: first unit of each; units a part; first partial slot
   uint16_t *out;
   uint8_t *units;  // [units][Hkv][kUnitBytes]
   int32_t *info;   // [units][Hkv][2]: E of the unit's part, its pages outside the pool (4 bits; 16: some in the part)
   float *part;
-  int num_pages, max_pages, H, Hkv, G, C, pmax;
+  int num_pages, max_pages, H, Hkv, G, C;
   float qk_scale;
 };
 
@@ -469,9 +471,9 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
     sv[i] = *(const float4 *)(sc + kPage + 8 * i + 4 * vh);
   }
   // E: thread = page of the part x quarter of its slots
-  const int pg0 = u / kPartUnits * (kPartKeys / kPage), pg1 = min(pg0 + kPartKeys / kPage, npages);
+  const int part = a.chunk_part[lo], pg0 = u / part * part * kUnitPages, pg1 = min(pg0 + part * kUnitPages, npages);
   int e = 0, bad = 0;  // (positive powers of two are ordered as their bits)
-#pragma unroll 2
+#pragma unroll 4
   for (int i = threadIdx.x; i < 4 * (pg1 - pg0); i += 256) {
     const int p = pg0 + (i >> 2), id = prow[p];
     const bool off = (uint32_t)id >= (uint32_t)a.num_pages;
@@ -534,26 +536,20 @@ __device__ __forceinline__ void load_lds16(const uint8_t *base, uint32_t off, ui
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
 }
 
-// WAVES waves of 32 rows; STAGES units of K and of V in LDS: the one in use, and those on their way.
-template <int WAVES, int STAGES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(64 * kPfWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void kv8_prefill_kernel(const PrefillArgs a) {
-  constexpr int kSub = kBlockRows / (WAVES * kRowsWave);  // workgroups a row block
-  constexpr int kLoads = 16 / WAVES;                      // 1 KB loads of a wave for a unit's K (and V)
-  __shared__ __attribute__((aligned(16))) uint4 s_k[STAGES][16][64];              // [page pair, 16 dims][lane] 8 bf16
-  __shared__ __attribute__((aligned(16))) uint4 s_v[STAGES][kUnitPages * 4][64];  // [page, 32 dims][lane] 8 fp16
-  const int item = blockIdx.x / (kSub * a.Hkv), kvh = blockIdx.x % a.Hkv;
-  const int ch = a.blk_chunk[item], part = a.blk_part[item];
+  constexpr int kLoads = 16 / kPfWaves;  // 1 KB loads of a wave for a unit's K (and V)
+  __shared__ __attribute__((aligned(16))) uint4 s_k[kStages][16][64];              // [page pair, 16 dims][lane] 8 bf16
+  __shared__ __attribute__((aligned(16))) uint4 s_v[kStages][kUnitPages * 4][64];  // [page, 32 dims][lane] 8 fp16
+  const int item = blockIdx.x / a.Hkv, kvh = blockIdx.x % a.Hkv;
+  const int ch = a.blk_chunk[item], q0 = a.blk_q0[item], part = a.blk_part[item], part_units = a.chunk_part[ch];
   const int ctx = a.chunk_ctx[ch], len = a.chunk_len[ch], row0 = a.chunk_row[ch];
   const int G = a.G, tpw = kRowsWave / G;  // tokens a wave
-  int q0 = a.blk_q0[item];
-  if constexpr (kSub > 1) q0 += blockIdx.x / a.Hkv % kSub * WAVES * tpw;
-  if (q0 >= len) return;  // (uniform)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
   const int lr = l & 31, lh = l >> 5;
-  const int kend = ctx + min(q0 + WAVES * tpw, len);  // the workgroup's keys: [0, kend)
-  const int u0 = part * kPartUnits, u1 = min((kend + kUnitKeys - 1) / kUnitKeys, u0 + kPartUnits);
-  if (u0 >= u1) return;  // (uniform: a piece of a block whose last token alone reaches the part)
+  const int kend = ctx + min(q0 + kPfWaves * tpw, len);  // the workgroup's keys: [0, kend)
+  const int u0 = part * part_units, u1 = min((kend + kUnitKeys - 1) / kUnitKeys, u0 + part_units);
+  if (q0 >= len || u0 >= u1) return;  // (uniform: no such item in a plan)
   const long long first_unit = (long long)a.chunk_unit[ch] * a.Hkv + kvh;  // (units of a head lie Hkv apart)
   const uint8_t *units = a.units + first_unit * kUnitBytes;
   const int32_t *info = a.info + 2 * first_unit;
@@ -596,8 +592,8 @@ void kv8_prefill_kernel(const PrefillArgs a) {
     for (int i = 0; i < kLoads; i++) load_lds16(p, lane_at + 1024 * i, v_lds + 16384 * slot + 1024 * i);
   };
   // The loads of units up to the one that is next are there, for every wave, and the units behind it are read: the newest
-  // STAGES - 2 units' loads stay in flight (vmcnt is split over bits 3:0 and 15:14), and a bare barrier follows.
-  constexpr int kVm = (STAGES - 2) * 2 * kLoads;
+  // kStages - 2 units' loads stay in flight (vmcnt is split over bits 3:0 and 15:14), and a bare barrier follows.
+  constexpr int kVm = (kStages - 2) * 2 * kLoads;
   auto meet = [&]() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt((kVm & 15) | ((kVm >> 4) << 14) | (7 << 4) | (0 << 8));  // vmcnt(kVm) lgkmcnt(0)
@@ -656,7 +652,7 @@ void kv8_prefill_kernel(const PrefillArgs a) {
         for (int i = 0; i < 16; i++) o[c][i] *= alpha;
     }
   };
-  auto next = [](int slot, int by) { return slot + by >= STAGES ? slot + by - STAGES : slot + by; };
+  auto next = [](int slot, int by) { return slot + by >= kStages ? slot + by - kStages : slot + by; };
   int slot = 0;  // unit u's place in both rings
   // Unit u: its softmax beside the scores of unit u + 1, then its products with V beside the maximum of the new scores;
   // cut into groups of a matrix instruction and the vector work that runs during it.
@@ -667,8 +663,8 @@ void kv8_prefill_kernel(const PrefillArgs a) {
     FragH vf[kAhead], pf[kUnitPages];
 #pragma unroll
     for (int j = 0; j < kAhead; j++) kf[j] = read_k(k_slot, j);
-    request_k(u + STAGES, slot);  // (K(u)'s and V(u - 1)'s places are free)
-    request_v(u + STAGES - 1, next(slot, STAGES - 1));
+    request_k(u + kStages, slot);  // (K(u)'s and V(u - 1)'s places are free)
+    request_v(u + kStages - 1, next(slot, kStages - 1));
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < 16; j++) {
@@ -701,22 +697,14 @@ void kv8_prefill_kernel(const PrefillArgs a) {
     if (more) settle(u + 1, s_next);
   };
 
-  // K(u0) .. K(u0 + STAGES - 1) and V(u0) .. V(u0 + STAGES - 2), in the order of the loop's requests
+  // K(u0) .. K(u0 + kStages - 1) and V(u0) .. V(u0 + kStages - 2), in the order of the loop's requests
   request_k(u0, 0);
 #pragma unroll
-  for (int i = 1; i < STAGES; i++) {
+  for (int i = 1; i < kStages; i++) {
     request_k(u0 + i, i);
     request_v(u0 + i - 1, i - 1);
   }
-  if (STAGES > 2) {  // K(u0) alone is needed now: K(u0 + 1) and V(u0) at the loop's first barrier
-    asm volatile("" ::: "memory");
-    constexpr int kVm0 = (STAGES - 1) * 2 * kLoads;
-    __builtin_amdgcn_s_waitcnt((kVm0 & 15) | ((kVm0 >> 4) << 14) | (7 << 4) | (0 << 8));
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  } else {
-    meet();
-  }
+  meet();
 #pragma unroll
   for (int j = 0; j < 16; j++) score(sc[0], read_k(0, j), j);
   largest(sc[0]);
@@ -730,7 +718,7 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   __builtin_amdgcn_s_waitcnt(0);  // no load may still write the LDS when the workgroup ends
   const float unit = exp_bits(E - kVShift);
   const float l_tot = sum_xor32(l_run);
-  const int parts = pos / kPartKeys + 1;
+  const int parts = pos / (kUnitKeys * part_units) + 1;
   if (t >= len || part >= parts) return;  // (a token before this part's keys: finished by its own last part)
   const long long hrow = (long long)(row0 + tok) * a.H + kvh * G + lr % G;
   if (parts == 1) {
@@ -745,7 +733,8 @@ void kv8_prefill_kernel(const PrefillArgs a) {
         *(uint2 *)(a.out + hrow * kD + 32 * c + 8 * i + 4 * lh) = w;
       }
   } else {
-    float *ps = a.part + (((long long)(row0 + tok) * a.pmax + part) * a.H + kvh * G + lr % G) * kPfSlot;
+    const int most = (a.chunk_unit[ch + 1] - a.chunk_unit[ch] + part_units - 1) / part_units;
+    float *ps = a.part + ((a.chunk_slot[ch] + (long long)tok * most + part) * a.H + kvh * G + lr % G) * kPfSlot;
 #pragma unroll
     for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -756,33 +745,46 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   }
 }
 
-// The parts of a token's keys in order: one workgroup of 8 H threads a token, thread (h, d) 16 dims of head h.
-__global__ __launch_bounds__(512) void kv8_prefill_merge_kernel(const PrefillArgs a) {
-  const int c = blockIdx.y, t = blockIdx.x;
-  if (t >= a.chunk_len[c]) return;
-  const int parts = (a.chunk_ctx[c] + t) / kPartKeys + 1;
+// The parts of a token's keys in order, four at a time in flight: 16 heads a workgroup, thread (h, x) dims 32 i + 4 x .. + 3.
+__global__ __launch_bounds__(128) void kv8_prefill_merge_kernel(const PrefillArgs a) {
+  const int c = blockIdx.y, t = blockIdx.x, h = 16 * blockIdx.z + (threadIdx.x >> 3);
+  if (t >= a.chunk_len[c] || h >= a.H) return;
+  const int pu = a.chunk_part[c], parts = (a.chunk_ctx[c] + t) / (kUnitKeys * pu) + 1;
   if (parts < 2) return;
-  const long long row = a.chunk_row[c] + t;
-  const int h = threadIdx.x >> 3, d0 = 16 * (threadIdx.x & 7);
+  const int most = (a.chunk_unit[c + 1] - a.chunk_unit[c] + pu - 1) / pu, d0 = 4 * (threadIdx.x & 7);
+  const float *first = a.part + ((a.chunk_slot[c] + (long long)t * most) * a.H + h) * kPfSlot;
   float M = kLowest, ls = 0.0f, O[16];
 #pragma unroll
   for (int i = 0; i < 16; i++) O[i] = 0.0f;
-  for (int p = 0; p < parts; p++) {
-    const float *ps = a.part + ((row * a.pmax + p) * a.H + h) * kPfSlot;
-    const float2 ml = *(const float2 *)(ps + kD);
-    const float mn = fmaxf(M, ml.x), fa = exp2f(M - mn), fb = exp2f(ml.x - mn);
-    ls = fmaf(ls, fa, ml.y * fb);
+  constexpr int kBatch = 4;
+  for (int p0 = 0; p0 < parts; p0 += kBatch) {
+    float4 v[kBatch][4];
+    float2 ml[kBatch];
 #pragma unroll
-    for (int i = 0; i < 16; i++) O[i] = fmaf(O[i], fa, ps[d0 + i] * fb);
-    M = mn;
+    for (int j = 0; j < kBatch; j++) {
+      if (p0 + j >= parts) break;  // (uniform)
+      const float *ps = first + (long long)(p0 + j) * a.H * kPfSlot;
+      ml[j] = *(const float2 *)(ps + kD);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[j][i] = *(const float4 *)(ps + d0 + 32 * i);
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; j++) {
+      if (p0 + j >= parts) break;
+      const float mn = fmaxf(M, ml[j].x), fa = exp2f(M - mn), fb = exp2f(ml[j].x - mn);
+      ls = fmaf(ls, fa, ml[j].y * fb);
+      const float *x = (const float *)v[j];
+#pragma unroll
+      for (int i = 0; i < 16; i++) O[i] = fmaf(O[i], fa, x[i] * fb);
+      M = mn;
+    }
   }
   const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-  uint32_t w[8];
+  uint16_t *op = a.out + ((long long)(a.chunk_row[c] + t) * a.H + h) * kD + d0;
 #pragma unroll
-  for (int i = 0; i < 8; i++) w[i] = pack_bf16x2(O[2 * i] * inv, O[2 * i + 1] * inv);
-  uint4 *op = (uint4 *)(a.out + (row * a.H + h) * kD + d0);
-  op[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  op[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  for (int i = 0; i < 4; i++)
+    *(uint2 *)(op + 32 * i) = make_uint2(pack_bf16x2(O[4 * i] * inv, O[4 * i + 1] * inv),
+                                         pack_bf16x2(O[4 * i + 2] * inv, O[4 * i + 3] * inv));
 }
 
 int64_t decode_bytes(int B, int H, int max_len) {
@@ -843,59 +845,124 @@ extern "C" int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, in
 }
 
 namespace {
-int64_t units_bytes(int units, int Hkv) { return (int64_t)units * Hkv * (kUnitBytes + 8); }
+// (infos padded to 16 bytes: the partials behind them are read 16 bytes at a time)
+int64_t units_bytes(int units, int Hkv) { return (int64_t)units * Hkv * kUnitBytes + ((int64_t)units * Hkv * 8 + 15) / 16 * 16; }
 }  // namespace
 
-extern "C" int64_t jit_kv8_prefill_workspace_bytes(int T, int pmax, int H, int Hkv, int units) {
-  if (T < 0 || pmax < 1 || H <= 0 || Hkv <= 0 || units < 0) return -1;
-  return units_bytes(units, Hkv) + jit_prefill_workspace_bytes(T, pmax, H);
+extern "C" int jit_kv8_prefill_block_tokens(int H, int Hkv) {
+  if (H <= 0 || Hkv <= 0 || H % Hkv != 0 || 16 % (H / Hkv) != 0) return -1;
+  return kBlockRows / (H / Hkv);
+}
+
+// Keys are cut where a chunk has too few row blocks to fill 256 CUs evenly.  `lines` row blocks of n parts are
+// lines x n workgroups, whose time is that of the rounds they take on 256 CUs: about 1.88 us a unit for the two that
+// share a CU and 1.15 us for one alone, 4 units' time for a workgroup's start and end, and 3 us and 0.02 a workgroup for
+// the partials and their merge.  The n with the least of that, by the chunk alone, so that a row's bits do not depend on
+// the call's other chunks.  All three launches, against parts of a fixed 6,144 keys (32 query heads over 4): 16 rows after
+// 8,000 keys 35 us in 15 parts, 115 us; 512 rows after 8,000 96 us in 4, 116 us; 512 of 16 heads over 16 after 4,000 49 us
+// in 4, 92 us; 2,048 rows after 8,192 308 us in one, 318 us.
+extern "C" int jit_kv8_prefill_part_units(int ctx, int len, int H, int Hkv) {
+  const int bt = jit_kv8_prefill_block_tokens(H, Hkv);
+  if (bt < 0 || ctx < 0 || len < 1) return -1;
+  const int64_t lines = ((int64_t)len + bt - 1) / bt * Hkv, units = ((int64_t)ctx + len + kUnitKeys - 1) / kUnitKeys;
+  int64_t best = 0, pu = 0;
+  for (int64_t n = (units + kPartMax - 1) / kPartMax; n == 1 || 8 * n <= units; n++) {
+    const int64_t part = (units + n - 1) / n, jobs = lines * n, rounds = (jobs + 255) / 256;
+    const int64_t cost = (rounds / 2 * 188 + rounds % 2 * 115) * (part + 4) + (n > 1 ? 300 + 2 * jobs : 0);  // (us / 100)
+    if (!pu || cost < best) best = cost, pu = part;
+    if (jobs > 4 * 256) break;  // (more rounds of shorter workgroups: nothing left to even out)
+  }
+  return (int)pu;
+}
+
+extern "C" int jit_kv8_prefill_plan(const int32_t *ctx, const int32_t *len, int C, int H, int Hkv, int32_t *tables,
+                                    int32_t *blocks, int n) {
+  const int bt = jit_kv8_prefill_block_tokens(H, Hkv);
+  if (bt < 0)
+    return jit::fail(JIT_EUNSUPPORTED, "kv8_prefill_plan covers H / Hkv in {1, 2, 4, 8, 16}, got %d / %d", H, Hkv);
+  if (C < 0 || (C > 0 && (!ctx || !len)) || !tables) return jit::fail(JIT_EINVAL, "kv8_prefill_plan: null pointer or C=%d", C);
+  int64_t units = 0, slots = 0, at[kPartMax + 1] = {};  // at[w]: items of w units, then where the next of them goes
+  auto items = [&](auto &&f) {
+    for (int c = 0; c < C; c++) {
+      const int pu = tables[C + 1 + c];
+      for (int64_t q0 = 0; q0 < len[c]; q0 += bt) {
+        const int64_t keys = (int64_t)ctx[c] + (q0 + bt < len[c] ? q0 + bt : len[c]), nu = (keys + kUnitKeys - 1) / kUnitKeys;
+        for (int64_t u = 0; u < nu; u += pu) f(c, (int)q0, (int)(u / pu), (int)(nu - u < pu ? nu - u : pu));
+      }
+    }
+  };
+  for (int c = 0; c < C; c++) {
+    const int pu = jit_kv8_prefill_part_units(ctx[c], len[c], H, Hkv);
+    if (pu < 0) return jit::fail(JIT_EINVAL, "kv8_prefill_plan: chunk %d of %d rows after %d", c, len[c], ctx[c]);
+    const int64_t nu = ((int64_t)ctx[c] + len[c] + kUnitKeys - 1) / kUnitKeys, parts = (nu + pu - 1) / pu;
+    tables[c] = (int32_t)units, tables[C + 1 + c] = pu, tables[2 * (C + 1) + c] = (int32_t)slots;
+    units += nu;
+    slots += parts > 1 ? parts * len[c] : 0;
+    if (units > 0x7fffffff || slots > 0x7fffffff)
+      return jit::fail(JIT_EUNSUPPORTED, "kv8_prefill_plan covers up to 2^31 - 1 units and partials");
+  }
+  tables[C] = (int32_t)units, tables[2 * C + 1] = 0, tables[3 * C + 2] = (int32_t)slots;
+  int64_t total = 0;
+  items([&](int, int, int, int w) { at[w]++, total++; });
+  if (total > 0x7fffffff) return jit::fail(JIT_EUNSUPPORTED, "kv8_prefill_plan: %lld work items", (long long)total);
+  if (!blocks) return (int)total;
+  if (n != total) return jit::fail(JIT_EINVAL, "kv8_prefill_plan: %d work items, %lld needed", n, (long long)total);
+  for (int64_t w = kPartMax, next = 0; w > 0; w--) {  // the items with the most units first
+    const int64_t of = at[w];
+    at[w] = next;
+    next += of;
+  }
+  items([&](int c, int q0, int part, int w) {
+    const int64_t i = at[w]++;
+    blocks[i] = c, blocks[n + i] = q0, blocks[2 * (int64_t)n + i] = part;
+  });
+  return (int)total;
+}
+
+extern "C" int64_t jit_kv8_prefill_workspace_bytes(int H, int Hkv, int units, int slots) {
+  if (H <= 0 || Hkv <= 0 || units < 0 || slots < 0) return -1;
+  return units_bytes(units, Hkv) + (int64_t)slots * H * kPfSlot * (int64_t)sizeof(float);
 }
 
 extern "C" int jit_paged_prefill_attn_kv8(const uint16_t *q, const void *pool, int num_pages, const int32_t *page_table,
                                           int max_pages, const int32_t *chunk_seq, const int32_t *chunk_ctx,
                                           const int32_t *chunk_len, const int32_t *chunk_row, const int32_t *chunk_unit,
-                                          int C, int units, const int32_t *blk_chunk, const int32_t *blk_q0,
-                                          const int32_t *blk_part, int nblk, int T, int pmax, int max_len, int H, int Hkv,
-                                          float scale, void *workspace, int64_t workspace_bytes, uint16_t *out,
-                                          void *stream) {
-  if (C < 0 || nblk < 0 || T < 0 || units < 0 || H <= 0 || Hkv <= 0 || max_pages <= 0 || num_pages <= 0 || pmax < 1 ||
-      max_len < 0)
-    return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: bad dims C=%d nblk=%d T=%d H=%d Hkv=%d pmax=%d max_len=%d units=%d", C,
-                     nblk, T, H, Hkv, pmax, max_len, units);
+                                          const int32_t *chunk_part, const int32_t *chunk_slot, int C, int units,
+                                          int slots, const int32_t *blk_chunk, const int32_t *blk_q0,
+                                          const int32_t *blk_part, int nblk, int max_len, int H, int Hkv, float scale,
+                                          void *workspace, int64_t workspace_bytes, uint16_t *out, void *stream) {
+  if (C < 0 || nblk < 0 || units < 0 || slots < 0 || H <= 0 || Hkv <= 0 || max_pages <= 0 || num_pages <= 0 || max_len < 0)
+    return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: bad dims C=%d nblk=%d H=%d Hkv=%d max_len=%d units=%d slots=%d", C,
+                     nblk, H, Hkv, max_len, units, slots);
   if (H % Hkv != 0) return jit::fail(JIT_EINVAL, "%d query heads do not share %d KV heads evenly", H, Hkv);
   if (!(scale > 0.0f)) return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: the scale must be positive");
   if (16 % (H / Hkv) != 0)
     return jit::fail(JIT_EUNSUPPORTED, "paged_prefill_attn_kv8 covers H / Hkv in {1, 2, 4, 8, 16}, got %d", H / Hkv);
-  if (pmax > 1 && H > 64)
-    return jit::fail(JIT_EUNSUPPORTED, "paged_prefill_attn_kv8 merges key parts of up to 64 query heads, got %d", H);
-  if (C > 65535 || Hkv > 65535)
+  if (C > 65535 || Hkv > 65535 || (int64_t)nblk * Hkv > 0x7fffffff)
     return jit::fail(JIT_EUNSUPPORTED, "paged_prefill_attn_kv8 covers up to 65535 chunks and heads, got %d and %d", C, Hkv);
   if (C == 0 || nblk == 0) return JIT_OK;
-  const int64_t need = jit_kv8_prefill_workspace_bytes(T, pmax, H, Hkv, units);
+  const int64_t need = jit_kv8_prefill_workspace_bytes(H, Hkv, units, slots);
   if (units == 0 || workspace_bytes < need)
     return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: workspace of %lld bytes for %d units, %lld needed",
                      (long long)workspace_bytes, units, (long long)need);
-  if (!q || !pool || !page_table || !chunk_seq || !chunk_ctx || !chunk_len || !chunk_row || !chunk_unit || !blk_chunk ||
-      !blk_q0 || !blk_part || !out || !workspace)
+  if (!q || !pool || !page_table || !chunk_seq || !chunk_ctx || !chunk_len || !chunk_row || !chunk_unit || !chunk_part ||
+      !chunk_slot || !blk_chunk || !blk_q0 || !blk_part || !out || !workspace)
     return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: null pointer");
   if (((uintptr_t)q | (uintptr_t)pool | (uintptr_t)out | (uintptr_t)workspace) & 15)
     return jit::fail(JIT_EINVAL, "paged_prefill_attn_kv8: q, the pool, the workspace and out must be 16-byte aligned");
   uint8_t *ws = (uint8_t *)workspace;
   int32_t *info = (int32_t *)(ws + (int64_t)units * Hkv * kUnitBytes);
   const PrefillArgs a{q, (const uint8_t *)pool, page_table, blk_chunk, blk_q0, blk_part, chunk_seq, chunk_ctx, chunk_len,
-                      chunk_row, chunk_unit, out, ws, info, (float *)(ws + units_bytes(units, Hkv)), num_pages, max_pages,
-                      H, Hkv, H / Hkv, C, pmax, scale * 1.44269504088896341f};
+                      chunk_row, chunk_unit, chunk_part, chunk_slot, out, ws, info,
+                      (float *)(ws + units_bytes(units, Hkv)), num_pages, max_pages, H, Hkv, H / Hkv, C,
+                      scale * 1.44269504088896341f};
   const hipStream_t st = (hipStream_t)stream;
   kv8_expand_kernel<<<dim3(units, Hkv), 256, 0, st>>>(a);
   int rc = jit::check_launch("jit_paged_prefill_attn_kv8");
   if (rc) return rc;
-  // few work items leave CUs idle: their row blocks are cut in two
-  if (2ll * nblk * Hkv <= jit::cu_count())
-    kv8_prefill_kernel<4, 2><<<dim3(2 * nblk * Hkv), 64 * 4, 0, st>>>(a);
-  else
-    kv8_prefill_kernel<8, 3><<<dim3(nblk * Hkv), 64 * 8, 0, st>>>(a);
+  kv8_prefill_kernel<<<dim3(nblk * Hkv), 64 * kPfWaves, 0, st>>>(a);
   rc = jit::check_launch("jit_paged_prefill_attn_kv8");
-  if (rc || pmax == 1 || max_len == 0) return rc;
-  kv8_prefill_merge_kernel<<<dim3(max_len, C), 8 * H, 0, st>>>(a);
+  if (rc || slots == 0 || max_len == 0) return rc;
+  kv8_prefill_merge_kernel<<<dim3(max_len, C, (H + 15) / 16), 128, 0, st>>>(a);
   return jit::check_launch("jit_paged_prefill_attn_kv8");
 }

@@ -229,9 +229,9 @@ int attend_kv8(const jit_kv8_step &t, const jit_layer &L, const Scratch &s, void
                                       t.pos, t.slots, pool, num_pages, s.q, stream));
   if (t.prompt_rows)
     JIT_TRY(jit_paged_prefill_attn_kv8(s.q, pool, num_pages, t.prompt_table, t.max_pages, t.chunk_seq, t.chunk_ctx,
-                                       t.chunk_len, t.chunk_row, t.chunk_unit, t.C, t.units, t.blk_chunk, t.blk_q0,
-                                       t.blk_part, t.nblk, t.prompt_rows, t.pmax, t.prompt_max_len, L.H, L.Hkv, L.scale,
-                                       t.prompt_workspace, t.prompt_workspace_bytes, s.attn, stream));
+                                       t.chunk_len, t.chunk_row, t.chunk_unit, t.chunk_part, t.chunk_slot, t.C, t.units,
+                                       t.part_slots, t.blk_chunk, t.blk_q0, t.blk_part, t.nblk, t.prompt_max_len, L.H,
+                                       L.Hkv, L.scale, t.prompt_workspace, t.prompt_workspace_bytes, s.attn, stream));
   if (t.B) {
     const int64_t at = (int64_t)t.prompt_rows * L.H * JIT_HEAD_DIM;
     JIT_TRY(jit_paged_decode_attn_kv8(s.q + at, pool, num_pages, t.page_table, t.max_pages, t.lens, t.B, L.H, L.Hkv,

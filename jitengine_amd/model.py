@@ -379,13 +379,17 @@ class DecoderLayer:
         _kv8_decode_rows(p, cfg, ms.dec_table, ms.kv8.lens[C:], ms.max_len, ms.workspace)
         if ms.P:
             ops.prefill_contract(pf, ms.seq_table)
+            p8 = pf.kv8
+            if p8.heads != (cfg.heads, cfg.kv_heads):
+                raise ValueError(f"the plan is for {p8.heads} heads, the layer has {cfg.heads} over {cfg.kv_heads}")
             pws = torch.empty(ops.kv8_prefill_workspace_bytes(pf, cfg.heads, cfg.kv_heads), dtype=torch.uint8, device=dev)
-            tb, bl = pf.tables.data_ptr(), pf.blocks.data_ptr()
-            nblk = pf.blocks.shape[1]
-            p.C, p.nblk, p.units, p.pmax, p.prompt_max_len = C, nblk, pf.total_units, pf.pmax, pf.max_len
+            tb, u, bl = pf.tables.data_ptr(), p8.tables.data_ptr(), p8.blocks.data_ptr()
+            nblk = p8.blocks.shape[1]
+            p.C, p.nblk, p.units, p.part_slots, p.prompt_max_len = C, nblk, p8.units, p8.slots, pf.max_len
             p.prompt_table, p.max_pages = ms.seq_table.data_ptr(), ms.seq_table.shape[1]
             p.chunk_seq, p.chunk_ctx, p.chunk_len, p.chunk_row = tb, tb + 4 * C, tb + 8 * C, tb + 12 * C
-            p.chunk_unit, p.blk_chunk, p.blk_q0, p.blk_part = pf.units.data_ptr(), bl, bl + 4 * nblk, bl + 8 * nblk
+            p.chunk_unit, p.chunk_part, p.chunk_slot = u, u + 4 * (C + 1), u + 8 * (C + 1)
+            p.blk_chunk, p.blk_q0, p.blk_part = bl, bl + 4 * nblk, bl + 8 * nblk
             p.prompt_workspace, p.prompt_workspace_bytes = pws.data_ptr(), pws.nbytes
         lib = _lib.lib()
         scratch = _layer_scratch(lib, lay, T, 1, dev)

@@ -656,18 +656,25 @@ class PrefillPlan:
     rows: int
     pmax: int = 1  # most key parts of a token (jit_prefill_part_keys keys a part)
     max_len: int = 0  # the longest chunk
-    units: torch.Tensor | None = None  # [C + 1]: first unit of KV8_UNIT keys of each chunk, and their number
-    total_units: int = 0
+    kv8: Kv8Chunks | None = None  # what paged_prefill_attention_kv8 takes besides
 
 
-def _chunk_units(chunks) -> np.ndarray:
-    return np.cumsum([0] + [-(-(ctx + n) // KV8_UNIT) for _, ctx, n in chunks], dtype=np.int64).astype(np.int32)
+@dataclass
+class Kv8Chunks:
+    """The row blocks and key parts of a prefill plan over an 8-bit pool (jit_paged_prefill_attn_kv8)."""
+
+    tables: torch.Tensor  # int32 [3, C + 1]: chunk_unit, chunk_part, chunk_slot
+    blocks: torch.Tensor  # int32 [3, n]: blk_chunk, blk_q0, blk_part
+    units: int
+    slots: int
+    heads: tuple          # (H, Hkv)
 
 
 def prefill_plan(chunks, H: int, Hkv: int, device) -> PrefillPlan:
     """Plan of causal prefill attention over chunks [(seq, ctx, length), ...]: every chunk cut
     into row blocks of jit_prefill_block_tokens tokens, each block's keys cut at multiples of
-    jit_prefill_part_keys, one work item per (block, part), the items with the most key steps first."""
+    jit_prefill_part_keys, one work item per (block, part), the items with the most key steps first; and the blocks and
+    parts of an 8-bit pool (jit_kv8_prefill_plan)."""
     lib = _lib.lib()
     bt = int(lib.jit_prefill_block_tokens(H, Hkv))
     if bt <= 0:
@@ -689,12 +696,21 @@ def prefill_plan(chunks, H: int, Hkv: int, device) -> PrefillPlan:
             for p in range((nst - 1) // part_steps + 1):
                 items.append((min(nst, (p + 1) * part_steps) - p * part_steps, keys, c, q0, p))
     items.sort(key=lambda it: (-it[0], -it[1]))
-    C, units = len(tab), _chunk_units(chunks)
-    tables = upload(np.concatenate([np.array(tab, np.int32).T.reshape(-1), units]) if tab else units, device)
-    blocks = upload(np.array([it[2:] for it in items], np.int32).T.copy() if items
-                    else np.zeros((3, 0), np.int32), device)
-    return PrefillPlan(list(chunks), tables[:4 * C].view(4, C), blocks.contiguous(), rows, pmax, max_len, tables[4 * C:],
-                       int(units[-1]))
+    C, n = len(tab), len(items)
+    head = 4 * C + 3 * (C + 1)
+    buf = np.empty(head, np.int32)
+    if C:
+        buf[:4 * C] = np.array(tab, np.int32).T.reshape(-1)
+    at = buf.ctypes.data
+    args = at + 4 * C, at + 8 * C, C, H, Hkv, at + 16 * C
+    n8 = _lib.check(lib.jit_kv8_prefill_plan(*args, None, 0), "kv8_prefill_plan")
+    blk8 = np.empty(3 * n8, np.int32)
+    _lib.check(lib.jit_kv8_prefill_plan(*args, blk8.ctypes.data, n8), "kv8_prefill_plan")
+    # one upload; the tables are views of it
+    blk = np.array([it[2:] for it in items], np.int32).T.reshape(-1) if n else np.empty(0, np.int32)
+    t, t8, b, b8 = upload(np.concatenate([buf, blk, blk8]), device).split([4 * C, 3 * (C + 1), 3 * n, 3 * n8])
+    return PrefillPlan(list(chunks), t.view(4, C), b.view(3, n), rows, pmax, max_len,
+                       Kv8Chunks(t8.view(3, C + 1), b8.view(3, n8), int(buf[5 * C]), int(buf[head - 1]), (H, Hkv)))
 
 
 def prefill_workspace_bytes(plan: PrefillPlan, H: int) -> int:
@@ -1006,8 +1022,7 @@ def paged_decode_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: 
 
 
 def kv8_prefill_workspace_bytes(plan: PrefillPlan, H: int, Hkv: int) -> int:
-    total = plan.total_units if plan.units is not None else int(_chunk_units(plan.chunks)[-1])
-    return int(_lib.lib().jit_kv8_prefill_workspace_bytes(plan.rows, plan.pmax, int(H), int(Hkv), total))
+    return int(_lib.lib().jit_kv8_prefill_workspace_bytes(int(H), int(Hkv), plan.kv8.units, plan.kv8.slots))
 
 
 def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, plan: PrefillPlan,
@@ -1015,9 +1030,11 @@ def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table:
     """q [T, H, 128] bf16 (the plan's chunk rows) -> out [T, H, 128]: paged_prefill_attention over an 8-bit pool
     (jit_paged_prefill_attn_kv8; the same plans), through a workspace of kv8_prefill_workspace_bytes (allocated when not
     given) that the chunks' keys are expanded into."""
-    tb, bl = plan.tables, plan.blocks
+    tb, p8 = plan.tables, plan.kv8
+    if p8 is None:
+        raise ValueError("the plan has no row blocks for an 8-bit pool (prefill_plan makes them)")
     dev = _take((q, torch.bfloat16, "q"), (pool, torch.uint8, "pool"), (page_table, torch.int32, "page_table"),
-                (tb, torch.int32, "plan"), (bl, torch.int32, "plan"))
+                (tb, torch.int32, "plan"), (p8.tables, torch.int32, "plan"), (p8.blocks, torch.int32, "plan"))
     Hkv = _kv8_heads(pool)
     if q.dim() != 3 or page_table.dim() != 2:
         raise ValueError("q must be [T, H, 128] and page_table [S, W]")
@@ -1026,19 +1043,17 @@ def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table:
         raise _lib.UnsupportedShape(f"paged_prefill_attention_kv8 covers head_dim 128, got {Dh}")
     if T != plan.rows:
         raise ValueError(f"q has {T} rows, the plan's chunks {plan.rows}")
+    if p8.heads != (H, Hkv):
+        raise ValueError(f"the plan is for {p8.heads[0]} query heads over {p8.heads[1]}, the call's are {H} over {Hkv}")
     prefill_contract(plan, page_table)
-    units, total = plan.units, plan.total_units
-    if units is None:  # (a plan put together from its tables)
-        host = _chunk_units(plan.chunks)
-        units, total = upload(host, q.device), int(host[-1])
     lib = _lib.lib()
-    ws = _kv8_workspace(workspace, lib.jit_kv8_prefill_workspace_bytes(T, plan.pmax, H, Hkv, total), q.device)
+    ws = _kv8_workspace(workspace, lib.jit_kv8_prefill_workspace_bytes(H, Hkv, p8.units, p8.slots), q.device)
     out = torch.empty_like(q)
-    C, nblk, t, b = tb.shape[1], bl.shape[1], tb.data_ptr(), bl.data_ptr()
+    C, n, t, u, b = tb.shape[1], p8.blocks.shape[1], tb.data_ptr(), p8.tables.data_ptr(), p8.blocks.data_ptr()
     _launch(dev, lib.jit_paged_prefill_attn_kv8, "paged_prefill_attn_kv8", q.data_ptr(), pool.data_ptr(), pool.shape[0],
-            page_table.data_ptr(), page_table.shape[1], t, t + 4 * C, t + 8 * C, t + 12 * C, units.data_ptr(), C, total, b,
-            b + 4 * nblk, b + 8 * nblk, nblk, T, plan.pmax, plan.max_len, H, Hkv, float(scale), _ptr(ws),
-            0 if ws is None else ws.nbytes, out.data_ptr())
+            page_table.data_ptr(), page_table.shape[1], t, t + 4 * C, t + 8 * C, t + 12 * C, u, u + 4 * (C + 1),
+            u + 8 * (C + 1), C, p8.units, p8.slots, b, b + 4 * n, b + 8 * n, n, plan.max_len, H, Hkv, float(scale),
+            _ptr(ws), 0 if ws is None else ws.nbytes, out.data_ptr())
     return out
 
 

@@ -383,26 +383,26 @@ def _(q, pool, page_table, lens, max_len, scale, workspace):
 
 @torch.library.custom_op(f"{_NS}::paged_prefill_attention_kv8", mutates_args=("workspace",))
 def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, tables: torch.Tensor,
-                                blocks: torch.Tensor, units: torch.Tensor, chunks: list[int], pmax: int, max_len: int,
-                                scale: float, workspace: torch.Tensor) -> torch.Tensor:
+                                chunk_tables: torch.Tensor, blocks: torch.Tensor, chunks: list[int], units: int,
+                                slots: int, scale: float, workspace: torch.Tensor) -> torch.Tensor:
     """out bf16 [T, H, 128]: paged_prefill_attention over an 8-bit pool (jit_paged_prefill_attn_kv8; the plan by
     kv8_prefill_plan_args, workspace of kv8_prefill_workspace_bytes bytes)."""
     trip = [tuple(chunks[i:i + 3]) for i in range(0, len(chunks), 3)]
-    total = int(ops._chunk_units(trip)[-1])
-    plan = ops.PrefillPlan(trip, tables, blocks, sum(c[2] for c in trip), int(pmax), int(max_len), units, total)
+    p8 = ops.Kv8Chunks(chunk_tables, blocks, int(units), int(slots), (q.shape[1], pool.shape[1]))
+    plan = ops.PrefillPlan(trip, tables, blocks, sum(c[2] for c in trip), 1, max([c[2] for c in trip] + [0]), p8)
     return ops.paged_prefill_attention_kv8(q, pool, page_table, plan, scale, workspace)
 
 
 @paged_prefill_attention_kv8.register_fake
-def _(q, pool, page_table, tables, blocks, units, chunks, pmax, max_len, scale, workspace):
+def _(q, pool, page_table, tables, chunk_tables, blocks, chunks, units, slots, scale, workspace):
     return torch.empty_like(q)
 
 
 def kv8_prefill_plan_args(plan: ops.PrefillPlan) -> tuple:
-    """(tables, blocks, units, chunks, pmax, max_len) of a prefill plan, for
+    """(tables, chunk_tables, blocks, chunks, units, slots) of a prefill plan, for
     torch.ops.jitengine.paged_prefill_attention_kv8."""
-    t, b, *rest = prefill_plan_args(plan)
-    return t, b, plan.units, *rest
+    p8 = plan.kv8
+    return plan.tables, p8.tables, p8.blocks, [int(v) for c in plan.chunks for v in c], p8.units, p8.slots
 
 
 @torch.library.custom_op(f"{_NS}::kv8_copy_pages", mutates_args=("pool",))

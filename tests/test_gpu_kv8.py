@@ -533,3 +533,27 @@ def test_refusals_on_device_tensors():
     assert ops.paged_decode_attention_kv8(q[:0], pool, t[:0], i[:0], 64, SCALE).shape == (0, 32, 128)
     ops.kv8_append_paged(pool, kv[:0], kv[:0], i[:0])
     assert not bool(pool.any())
+
+
+@pytest.mark.parametrize("H, Hkv", [(32, 4), (128, 16), (16, 16)])
+def test_a_chunk_of_many_key_parts_does_not_depend_on_its_call(H, Hkv):
+    """Few rows after many keys are cut into many parts; a chunk's bits are those of the chunk alone."""
+    chunks = [(0, 3000, 9), (1, 0, 400), (2, 5001, 1), (3, 640, 130)]
+    lens = [c + n for _, c, n in chunks]
+    table, pages = _table(lens, H)
+    pool = ref.random_pool(pages, Hkv, H, DEV, v_spread=2.0)
+    _poison_stale(pool, table, lens)
+    t, T = _i32(table), sum(n for *_, n in chunks)
+    plan = ops.prefill_plan(chunks, H, Hkv, DEV)
+    assert plan.kv8.slots > 0 and int(plan.kv8.blocks[2].max()) >= 4
+    q = torch.randn((T, H, 128), generator=torch.Generator().manual_seed(H)).to(torch.bfloat16).to(DEV)
+    out = ops.paged_prefill_attention_kv8(q, pool, t, plan, SCALE)
+    _check_prefill(out, q, pool, torch.from_numpy(table).to(DEV), chunks, (H, Hkv))
+    row = 0
+    for s, c, n in chunks:
+        alone = ops.paged_prefill_attention_kv8(q[row:row + n].contiguous(), pool, t,
+                                                ops.prefill_plan([(s, c, n)], H, Hkv, DEV), SCALE)
+        assert torch.equal(_bits(alone), _bits(out[row:row + n])), (s, c, n)
+        row += n
+    with pytest.raises(ValueError, match="plan is for"):  # a plan of another geometry
+        ops.paged_prefill_attention_kv8(q, pool, t, ops.prefill_plan(chunks, H, Hkv * 2 if H > Hkv else 8, DEV), SCALE)

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
@@ -56,10 +57,10 @@ def _decode(q=X, pool=X, pages=8, W=4, B=2, H=32, Hkv=4, max_len=64, ws=None, nb
     return _lib.lib().jit_paged_decode_attn_kv8(q, pool, pages, X, W, lens, B, H, Hkv, max_len, 0.1, ws, nb, out, None)
 
 
-def _prefill(q=X, pool=X, pages=8, W=4, C=1, nblk=1, T=4, pmax=1, max_len=4, units=1, H=32, Hkv=4, scale=0.1, ws=X, nb=1 << 40,
-             out=X, unit=X):
-    return _lib.lib().jit_paged_prefill_attn_kv8(q, pool, pages, X, W, X, X, X, X, unit, C, units, X, X, X, nblk, T, pmax,
-                                                 max_len, H, Hkv, scale, ws, nb, out, None)
+def _prefill(q=X, pool=X, pages=8, W=4, C=1, nblk=1, slots=0, max_len=4, units=1, H=32, Hkv=4, scale=0.1, ws=X, nb=1 << 40,
+             out=X, unit=X, part=X, slot=X):
+    return _lib.lib().jit_paged_prefill_attn_kv8(q, pool, pages, X, W, X, X, X, X, unit, part, slot, C, units, slots, X, X, X,
+                                                 nblk, max_len, H, Hkv, scale, ws, nb, out, None)
 
 
 def _tables(S=2, W=4, rows=2, free=None, n_free=-1, ctx=X, row_start=X, pos=X, status=X):
@@ -78,10 +79,11 @@ def _tables(S=2, W=4, rows=2, free=None, n_free=-1, ctx=X, row_start=X, pos=X, s
     (lambda: _decode(W=4096, max_len=65536, ws=X, nb=16), EINVAL),  # a workspace too small for the chunks
     (lambda: _decode(q=ODD), EINVAL), (lambda: _decode(out=ODD), EINVAL), (lambda: _decode(pool=ODD), EINVAL),
     (lambda: _prefill(H=30), EINVAL), (lambda: _prefill(H=24, Hkv=8), EUNS), (lambda: _prefill(H=12, Hkv=4), EUNS),
-    (lambda: _prefill(pmax=0), EINVAL), (lambda: _prefill(ws=None), EINVAL), (lambda: _prefill(pmax=2, H=128, Hkv=16), EUNS),
-    (lambda: _prefill(nb=32776 * 4 - 1), EINVAL), (lambda: _prefill(nb=32776 * 4, pmax=2), EINVAL), (lambda: _prefill(units=0), EINVAL),
+    (lambda: _prefill(slots=-1), EINVAL), (lambda: _prefill(ws=None), EINVAL), (lambda: _prefill(nblk=1 << 30), EUNS),
+    (lambda: _prefill(nb=32776 * 4 - 1), EINVAL), (lambda: _prefill(nb=32776 * 4, slots=8), EINVAL), (lambda: _prefill(units=0), EINVAL),
+    (lambda: _prefill(part=None), EINVAL), (lambda: _prefill(slot=None), EINVAL), (lambda: _prefill(nblk=-1), EINVAL),
     (lambda: _prefill(scale=0.0), EINVAL), (lambda: _prefill(scale=-1.0), EINVAL), (lambda: _prefill(scale=float("nan")), EINVAL),
-    (lambda: _prefill(unit=None), EINVAL), (lambda: _prefill(T=-1), EINVAL),
+    (lambda: _prefill(unit=None), EINVAL), (lambda: _prefill(max_len=-1), EINVAL),
     (lambda: _prefill(C=0, q=None), OK), (lambda: _prefill(out=None), EINVAL), (lambda: _prefill(C=65536), EUNS),
     (lambda: _prefill(q=ODD), EINVAL), (lambda: _prefill(pool=ODD), EINVAL),
     (lambda: _tables(S=-1), EINVAL), (lambda: _tables(W=0), EINVAL), (lambda: _tables(rows=-1), EINVAL),
@@ -139,3 +141,59 @@ def test_tables_of_the_restatement_never_share_a_slot(seed):
     used = [s for s in t["slots"] if s >= 0]
     assert len(used) == len(set(used)) and t["row_start"][-1] == sum(new)
     assert sum(n - c for n, c in zip(t["lens"], ctx)) == len(used)
+
+
+def _plan(ctx, length, H=32, Hkv=4):
+    """(chunk_unit, chunk_part, chunk_slot, items in order) of jit_kv8_prefill_plan."""
+    lib, C = _lib.lib(), len(ctx)
+    a, b, tab = np.array(ctx, np.int32), np.array(length, np.int32), np.full((3, C + 1), -9, np.int32)
+    args = a.ctypes.data, b.ctypes.data, C, H, Hkv, tab.ctypes.data
+    n = lib.jit_kv8_prefill_plan(*args, None, 0)
+    assert n >= 0
+    blk = np.full((3, n), -9, np.int32)
+    assert lib.jit_kv8_prefill_plan(*args, blk.ctypes.data, n) == n
+    assert lib.jit_kv8_prefill_plan(*args, blk.ctypes.data, n + 1) == EINVAL
+    return (*(t.tolist() for t in tab), list(zip(*blk.tolist())))
+
+
+@pytest.mark.parametrize("H, Hkv", [(32, 4), (16, 16), (16, 1), (128, 16)])
+@pytest.mark.parametrize("ctx, length", [
+    ([0], [1]), ([8000], [16]), ([8192], [2048]), ([235, 0, 5834, 40000], [994, 3, 8, 700]), ([], []), ([262128], [16]),
+])
+def test_a_prompt_plan_covers_every_key_of_every_row_once(ctx, length, H, Hkv):
+    first, part, slot, items = _plan(ctx, length, H, Hkv)
+    bt = _lib.lib().jit_kv8_prefill_block_tokens(H, Hkv)
+    assert bt == 128 * Hkv // H
+    want, work = {}, []
+    for c, (k, n) in enumerate(zip(ctx, length)):
+        units = -(-(k + n) // 64)
+        assert first[c + 1] - first[c] == units and 1 <= part[c] <= 192
+        parts = -(-units // part[c])
+        assert slot[c + 1] - slot[c] == (n * parts if parts > 1 else 0)
+        for q0 in range(0, n, bt):
+            nu = -(-(k + min(q0 + bt, n)) // 64)
+            for p in range(-(-nu // part[c])):
+                want[c, q0, p] = min(part[c], nu - p * part[c])
+    assert first[0] == slot[0] == 0 and len(items) == len(want) and set(items) == set(want)
+    work = [want[i] for i in items]
+    assert work == sorted(work, reverse=True)
+
+
+def test_a_chunk_is_cut_by_its_own_shape():
+    alone = _plan([5834], [8])[1][0]
+    assert _plan([235, 5834, 40000], [994, 8, 700])[1][1] == alone
+    pu = _lib.lib().jit_kv8_prefill_part_units
+    assert pu(0, 1, 32, 4) == 1 and pu(0, 500, 32, 4) == 8     # short sequences: one part
+    assert pu(8000, 16, 32, 4) < 12                             # few rows, many keys: short parts
+    assert pu(8192, 2048, 32, 4) == 160                         # enough rows: whole
+    assert max(pu(c, 2048, 32, 4) for c in range(0, 262144, 4099)) <= 192
+    assert pu(-1, 3, 32, 4) == -1 and pu(0, 0, 32, 4) == -1 and pu(0, 4, 30, 4) == -1
+
+
+@pytest.mark.parametrize("ctx, length, H, want", [
+    ([0], [0], 32, EINVAL), ([-1], [4], 32, EINVAL), ([0], [4], 12, EUNS), ([2 ** 31 - 1] * 80, [2 ** 31 - 1] * 80, 32, EUNS),
+])
+def test_a_prompt_plan_refuses_what_it_cannot_cut(ctx, length, H, want):
+    a, b, tab = np.array(ctx, np.int32), np.array(length, np.int32), np.zeros((3, len(ctx) + 1), np.int32)
+    assert _lib.lib().jit_kv8_prefill_plan(a.ctypes.data, b.ctypes.data, len(ctx), H, 4, tab.ctypes.data, None, 0) == want
+    assert _lib.lib().jit_kv8_prefill_plan(None, b.ctypes.data, 1, 32, 4, tab.ctypes.data, None, 0) == EINVAL

@@ -92,7 +92,7 @@ def test_operators_are_registered_and_propagate_shapes():
                                   m((64,), torch.float32), t[2], t[3], pool)
     assert q.shape == (20, 32, 128) and q.dtype == bf
     assert J.paged_decode_attention_kv8(q[:3], pool, table, t[4], 99, 0.1, m((64,), torch.uint8)).shape == (3, 32, 128)
-    out = J.paged_prefill_attention_kv8(q, pool, table, m((4, 1), i32), m((3, 1), i32), m((2,), i32), [0, 0, 20], 1, 20,
+    out = J.paged_prefill_attention_kv8(q, pool, table, m((4, 1), i32), m((3, 2), i32), m((3, 2), i32), [0, 0, 20], 1, 0,
                                         0.1, m((64,), torch.uint8))
     assert out.shape == q.shape and out.dtype == bf
     assert J.kv8_append_paged(pool, m((20, 4, 128), bf), m((20, 4, 128), bf), t[3]) is None
