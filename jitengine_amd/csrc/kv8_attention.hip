@@ -433,7 +433,8 @@ struct PrefillArgs {
   const int32_t *chunk_unit, *chunk_part, *chunk_slot;  // [C + 1]: first unit of each; units a part; first partial slot
   uint16_t *out;
   uint8_t *units;  // [units][Hkv][kUnitBytes]
-  int32_t *info;   // [units][Hkv][2]: E of the unit's part, its pages outside the pool (4 bits; 16: some in the part)
+  int32_t *info;   // [units][Hkv][2]: E of the unit's part, its pages outside the pool (4 bits; 16: some in the part;
+                   // 32: NaN codes of V in the unit)
   float *part;
   int num_pages, max_pages, H, Hkv, G, C;
   float qk_scale;
@@ -487,7 +488,25 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o, 64));
   const int any = __any(bad), here = __any(out_of_pool && pg < npages);
-  if (l == 0) s_e[wave] = e, s_bad[wave] = (any ? 16 : 0) | (here ? 1 << wave : 0);
+  // What lies past the keys or in a page outside the pool may be anything (0 x NaN): it counts as 0.  So do NaN codes
+  // of V, which rows that do not see their key must not get either: kv8_prefill_kernel puts them back.
+  int keep[2];
+  uint32_t nan = 0;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    keep[i] = out_of_pool ? 0 : kend - (kPage * pg + 8 * i + 4 * vh);
+    const uint32_t km = keep_bytes(keep[i]);
+    uint32_t *w = (uint32_t *)&wv[i];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      w[j] &= km;
+      const uint32_t n = (((w[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in the bytes 0x7f and 0xff
+      w[j] &= ~(n * 255u);
+      nan |= n;
+    }
+  }
+  const int any_nan = __any(nan != 0);
+  if (l == 0) s_e[wave] = e, s_bad[wave] = (any ? 16 : 0) | (here ? 1 << wave : 0) | (any_nan ? 32 : 0);
   __syncthreads();
   e = max(max(s_e[0], s_e[1]), max(s_e[2], s_e[3]));
   const int E = min(max((e >> 23) - 127, kMinExp), kMaxExp);
@@ -509,13 +528,9 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
   f16x2_t fac[2][2];  // 2^(e - E + 7); below fp16's range 0
 #pragma unroll
   for (int i = 0; i < 2; i++) {
-    // what lies past the keys or in a page outside the pool may be anything (0 x NaN): it counts as 0
-    const int keep = out_of_pool ? 0 : kend - (kPage * pg + 8 * i + 4 * vh);
-    const uint32_t km = keep_bytes(keep);
-    wv[i].x &= km, wv[i].y &= km, wv[i].z &= km, wv[i].w &= km;
     const float *sp = (const float *)&sv[i];
 #pragma unroll
-    for (int j = 0; j < 4; j++) fac[i][j >> 1][j & 1] = (_Float16)(j < keep ? sp[j] * unit : 0.0f);
+    for (int j = 0; j < 4; j++) fac[i][j >> 1][j & 1] = (_Float16)(j < keep[i] ? sp[j] * unit : 0.0f);
   }
 #pragma unroll
   for (int c = 0; c < 4; c++) {
@@ -554,6 +569,9 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   const uint8_t *units = a.units + first_unit * kUnitBytes;
   const int32_t *info = a.info + 2 * first_unit;
   const int E = info[2 * (long long)u0 * a.Hkv], some_bad = info[2 * (long long)u0 * a.Hkv + 1] & 16;
+  int nan = 0;
+  for (int u = u0 + l; u < u1; u += 64) nan |= info[2 * (long long)u * a.Hkv + 1] & 32;
+  const bool some_nan = __any(nan);
 
   const int t = q0 + wave * tpw + lr / G, tok = min(t, len - 1), pos = ctx + tok;  // the lane's row
   const int first_pos = ctx + min(q0 + wave * tpw, len - 1);                       // the wave's first
@@ -716,6 +734,26 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   }
   if (u < u1) unit_step(u, sc[0], sc[1], false);
   __builtin_amdgcn_s_waitcnt(0);  // no load may still write the LDS when the workgroup ends
+  if (some_nan) {  // (rare) V's NaN codes, to the rows that see their keys
+    const int32_t *prow = a.page_table + (long long)a.chunk_seq[ch] * a.max_pages;
+    for (int u = u0; u < u1; u++) {
+      if (!(info[2 * (long long)u * a.Hkv + 1] & 32)) continue;
+      for (int k = 0; k < kUnitKeys; k++) {
+        const int key = kUnitKeys * u + k;
+        if (key > pos) break;
+        const int page = key / kPage < a.max_pages ? prow[key / kPage] : -1;
+        if ((uint32_t)page >= (uint32_t)a.num_pages) continue;
+        const uint8_t *v = record(a.pool, page, a.Hkv, kvh) + kVOff + (k % kPage / 4) * 256 + k % 4;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int d = 32 * c + 8 * (i >> 2) + 4 * lh + (i & 3);  // (byte of (slot, d): 16 (4 q + c) + r)
+            if ((v[(d >> 6) * 1024 + (d & 15) * 16 + ((d >> 4) & 3) * 4] & 127) == 127) o[c][i] = __builtin_nanf("");
+          }
+      }
+    }
+  }
   const float unit = exp_bits(E - kVShift);
   const float l_tot = sum_xor32(l_run);
   const int parts = pos / (kUnitKeys * part_units) + 1;
@@ -860,7 +898,7 @@ extern "C" int jit_kv8_prefill_block_tokens(int H, int Hkv) {
 // the partials and their merge.  The n with the least of that, by the chunk alone, so that a row's bits do not depend on
 // the call's other chunks.  All three launches, against parts of a fixed 6,144 keys (32 query heads over 4): 16 rows after
 // 8,000 keys 35 us in 15 parts, 115 us; 512 rows after 8,000 96 us in 4, 116 us; 512 of 16 heads over 16 after 4,000 49 us
-// in 4, 92 us; 2,048 rows after 8,192 308 us in one, 318 us.
+// in 4, 92 us; 2,048 rows after 8,192 308 to 321 us in one, 318 to 329 in two.
 extern "C" int jit_kv8_prefill_part_units(int ctx, int len, int H, int Hkv) {
   const int bt = jit_kv8_prefill_block_tokens(H, Hkv);
   if (bt < 0 || ctx < 0 || len < 1) return -1;

@@ -557,3 +557,54 @@ def test_a_chunk_of_many_key_parts_does_not_depend_on_its_call(H, Hkv):
         row += n
     with pytest.raises(ValueError, match="plan is for"):  # a plan of another geometry
         ops.paged_prefill_attention_kv8(q, pool, t, ops.prefill_plan(chunks, H, Hkv * 2 if H > Hkv else 8, DEV), SCALE)
+
+
+@pytest.mark.parametrize("ctx, n", [(20, 100), (3000, 9), (0, 70)])
+def test_keys_that_are_not_finite_reach_only_the_rows_that_see_them(ctx, n):
+    """NaN codes of later tokens of a chunk (and of what a recycled page holds past its end) leave a row as it is; a
+    row that sees one gets NaN: all of it from K, that dim from V."""
+    H, Hkv, L = 32, 4, ctx + n
+    table, pages = _table([L], n)
+    pool = ref.random_pool(pages, Hkv, n, DEV, v_spread=2.0)
+    _poison_stale(pool, table, [L])
+    t = torch.from_numpy(table).to(DEV)
+    nan_v = {0: (ctx + n // 2, [3, 70, 127]), 1: (L - 1, [0]), 3: (ctx // 2, [64, 65])}  # head: (key, dims)
+    nan_k = {2: ctx + n // 3}
+    for h, (key, dims) in nan_v.items():
+        pool[t[0, key // 16], h, ref.v_at(key % 16, torch.tensor(dims, device=DEV))] = 127 if h else 255
+    for h, key in nan_k.items():
+        pool[t[0, key // 16], h, ref.k_at(key % 16, torch.tensor([9], device=DEV))] = 255
+    q = torch.randn((n, H, 128), generator=torch.Generator().manual_seed(n)).to(torch.bfloat16).to(DEV)
+    out = ops.paged_prefill_attention_kv8(q, pool, _i32(table), ops.prefill_plan([(0, ctx, n)], H, Hkv, DEV), SCALE)
+    last = ops.paged_decode_attention_kv8(q[-1:].contiguous(), pool, _i32(table), _i32([L]), L, SCALE)
+    k, v = ref.read(pool, t[0])
+    k, v = torch.nan_to_num(k[:, :L]), torch.nan_to_num(v[:, :L])
+    seen = torch.arange(L, device=DEV)[None] <= ctx + torch.arange(n, device=DEV)[:, None]
+    G = H // Hkv
+    for h in range(Hkv):
+        want, tol = ref.attend(q[:, h * G:(h + 1) * G], k[h], v[h], SCALE, seen)
+        if h in nan_v:
+            key, dims = nan_v[h]
+            want[seen[:, key].nonzero()[:, 0][:, None], :, torch.tensor(dims, device=DEV)[None]] = float("nan")
+        if h in nan_k:
+            want[seen[:, nan_k[h]]] = float("nan")
+        for got, rows in ((out, slice(0, n)), (last, slice(n - 1, n))):
+            got, w, tl = got[:, h * G:(h + 1) * G].double(), want[rows], tol[rows]
+            assert torch.equal(got.isnan(), w.isnan()), (h, ctx)
+            assert bool(((got - w).abs() <= tl)[~w.isnan()].all()), (h, ctx)
+
+
+def test_decode_of_more_sequences_than_a_launch_covers():
+    B, H, Hkv = 4101, 8, 4
+    rng = np.random.default_rng(1)
+    lens = rng.integers(0, 40, B)
+    lens[4096], lens[4095] = 700, 1100
+    table, pages = _table(lens.tolist(), 1)
+    table[:, 4:] = np.where(np.arange(4, table.shape[1])[None] < -(-lens[:, None] // 16), table[:, 4:], 0)
+    pool = ref.random_pool(pages, Hkv, 1, DEV)
+    q = torch.randn((B, H, 128), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    out = ops.paged_decode_attention_kv8(q, pool, _i32(table), _i32(lens), 16 * table.shape[1], SCALE)
+    assert bool((out[torch.from_numpy(lens == 0).to(DEV)] == 0).all())
+    some = [0, 1, 4094, 4095, 4096, 4097, 4100] + rng.integers(0, B, 60).tolist()
+    some = [b for b in some if lens[b]]
+    _check_decode(out[some], q[some], pool, torch.from_numpy(table[some]).to(DEV), [int(lens[b]) for b in some], "many")
