@@ -18,7 +18,8 @@ constexpr float kLowest = -1e30f;  // the running maximum before any key: finite
 constexpr float kPShift = 15.0f;
 
 // ---------------------------------------------------------------- single tokens
-// A sequence is cut into chunks by its own length alone, a chunk into 4 runs of a wave each.
+// A sequence is cut into chunks by its own length alone, a chunk into 4 runs of a wave each.  512 keys: with 768 and
+// 1,024 64 sequences of 300 keys take 11.8 and 14.2 us instead of 9.8, 32 ragged ones 32 to 35 with any of the three.
 constexpr int kSplits = 4;
 constexpr int kChunk = 512, kLongChunks = 128, kChunkMax = 64 * kPage * kSplits;
 
@@ -83,6 +84,8 @@ struct Run {
 // lengths: sized by the host's bound (32 sequences of 128 to 32,768 keys: 8,448 workgroups for 1,003 chunks) most
 // workgroups only took a CU's place for the microsecond in which they found that they had nothing to do.  A
 // wave never runs dry: the first loads of its next chunk are in flight while it ends one.
+// Bound by memory: 262,144 keys of 4 kv heads (277 MB) in 45.9 us, 6.0 TB/s; the 32 sequences (133 MB) in 27.5, 4.8 TB/s;
+// one of 4,096 keys takes 7.5 us, the latency of a run.
 __global__ __launch_bounds__(64 * kSplits) __attribute__((amdgpu_waves_per_eu(kDecodeWgs, kDecodeWgs)))
 void kv8_decode_kernel(const DecodeArgs a) {
   __shared__ float xstate[kSplits][kStateFloats][64];
@@ -343,6 +346,7 @@ void kv8_decode_kernel(const DecodeArgs a) {
 }
 
 // The chunks of a (sequence, q head), in order: thread = chunk lane (16) x 4 dims; lane j takes chunks j, j + 16, ..
+// (3.8 to 5.7 us: an empty launch and two or three trips to memory)
 constexpr int kMergeLanes = 16;
 
 __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const DecodeArgs a) {
@@ -393,13 +397,16 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
 // Two launches (three where a token's keys have several parts).  The first expands the keys that the chunks see: K to
 // bf16 (times its scale) and V to fp16, in the order in which the second launch's matrix instructions take them.
 // Every row block of a chunk reads all of its keys, so the conversion is done once instead of once a block; inside the
-// attention loop it cost as many vector instructions as the softmax (2,048 rows after 8,192 keys: 344 us, now 328).
+// attention loop it cost as many vector instructions as the softmax (2,048 rows after 8,192 keys: 344 us, without it 328).
 //
 // The second: a workgroup owns 4 waves x 32 rows (32 / G tokens x the G q heads of a kv head a wave) and walks the keys
 // of a part, up to its last token, 64 (a unit) at a time, a unit's 32 KB going straight from memory into LDS.  Two
 // workgroups share a CU.
 //   S^T[32 keys x 32 rows] = K . Q^T        (8 MFMA 32x32x16 bf16)
 //   O^T[128 dims x 32 rows] += V^T . P^T    (4 MFMA 32x32x16 fp16 a page)
+// Bound by the matrix instructions and the clock they leave (2,048 rows after 8,192 keys: busy 60% of the cycles at 1.9 GHz,
+// 303 to 318 us, 1.0 PFLOP/s; a large bf16 product of the library 1.15 to 1.4).  Both workgroups of a CU are needed: with
+// one of four waves, however many units are on their way, the same takes 394 us.
 // A lane owns one row throughout: its scores of a page are its P operand as they are, since the 16 keys of V's
 // operand are kept in the order in which the score tile holds them.
 constexpr int kPfWaves = 4, kStages = 2;  // waves a workgroup; units in LDS: the one in use, and those on their way
@@ -440,7 +447,8 @@ struct PrefillArgs {
   float qk_scale;
 };
 
-// One workgroup expands a unit of one kv head, wave w its page w.  Its codes are requested first; meanwhile the part's
+// One workgroup expands a unit of one kv head, wave w its page w: 10,240 keys of 4 heads, 11 MB to 21 MB, in 18 us, most of
+// it the latency of its part's scales (parts of 96 units: 11 us).  Its codes are requested first; meanwhile the part's
 // loudest live V scale is found (by every workgroup of a part for itself: a line of 64 bytes a page).
 __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
   __shared__ int s_e[4], s_bad[4];
