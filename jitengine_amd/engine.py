@@ -76,6 +76,9 @@ class Engine:
             raise ValueError("prefill_chunk and max_step_tokens must be positive")
         if prefill_chunk > max_step_tokens:
             raise ValueError(f"a prompt chunk ({prefill_chunk} rows) must fit a step ({max_step_tokens} rows)")
+        if kv8 and max_step_tokens > ops.STEP_SEQS:
+            raise ValueError(f"a step over an 8-bit cache covers up to {ops.STEP_SEQS} sequences, max_step_tokens is "
+                             f"{max_step_tokens}")
         self.lm = lm
         cfg = lm.cfg
         dev = device if device is not None else lm.final_norm.device

@@ -844,6 +844,7 @@ def paged_decode_attention_noalloc(q: torch.Tensor, pool: torch.Tensor, page_tab
 
 
 # ----------------------------------------------------------------------------- 8-bit KV cache
+STEP_SEQS = 8192  # sequences of a step (jit_step_tables)
 KV8_UNIT = 64  # keys of a unit of prompt attention's expanded cache
 KV8_RECORD = 4224  # bytes of one page's 16 tokens of one kv head: K codes, V codes, 32 fp32 scales
 

@@ -608,3 +608,54 @@ def test_decode_of_more_sequences_than_a_launch_covers():
     some = [0, 1, 4094, 4095, 4096, 4097, 4100] + rng.integers(0, B, 60).tolist()
     some = [b for b in some if lens[b]]
     _check_decode(out[some], q[some], pool, torch.from_numpy(table[some]).to(DEV), [int(lens[b]) for b in some], "many")
+
+
+def test_pools_past_4_gib():
+    """Records whose offsets pass 32 bits: the same bits as in a small pool."""
+    H, Hkv, lens, big = 32, 4, [70, 33], 260_000
+    small_t, pages = _table(lens, 7, extra=0)
+    n = sum(lens)
+    far = np.random.default_rng(8).permutation(pages)
+    ids = np.where(far % 2, big - 1 - far, far)  # half of the pages at either end
+    pool, small = ops.kv8_pool(big, Hkv, DEV), ops.kv8_pool(pages, Hkv, DEV)
+    assert pool.nbytes > 2 ** 32
+    big_t = np.where(small_t < pages, ids[np.minimum(small_t, pages - 1)], 2 ** 31 - 1)
+    g = torch.Generator().manual_seed(9)
+    qkv = torch.randn((n, (H + 2 * Hkv) * 128), generator=g).to(torch.bfloat16).to(DEV)
+    w, inv = torch.ones(128, dtype=torch.bfloat16, device=DEV), torch.rand(64, generator=g).to(DEV)
+    outs = []
+    for p, t in ((pool, big_t), (small, small_t)):
+        t = _i32(t)
+        st = ops.step_tables(_i32([0, 0]), _i32(lens), t, n)
+        q = ops.qk_norm_rope_append_kv8(qkv, H, Hkv, w, w, 1e-6, inv, st.pos, st.slots, p)
+        plan = ops.prefill_plan([(i, 0, m) for i, m in enumerate(lens)], H, Hkv, DEV)
+        outs.append((_bits(q), _bits(ops.paged_prefill_attention_kv8(q, p, t, plan, SCALE)),
+                     _bits(ops.paged_decode_attention_kv8(q[:2].contiguous(), p, t, st.lens, max(lens), SCALE))))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert torch.equal(pool[torch.from_numpy(ids).to(DEV)], small)
+    src, dst = _i32([int(ids.max())]), _i32([big // 2])
+    ops.kv8_copy_pages(pool, src, dst)
+    assert torch.equal(pool[big // 2], pool[int(ids.max())]) and bool(pool[int(ids.max())].any())
+
+
+def test_prompt_rows_after_262140_keys_of_16_heads():
+    """The longest context: an expanded cache past 2 GiB, parts of the largest size."""
+    H, ctx, n = 16, 262140, 4
+    table, pages = _table([ctx + n], 5, extra=0)
+    pool = ops.kv8_pool(pages, H, DEV)
+    t = _i32(table)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    for at in range(0, ctx + n, 65536):  # (rows of at most 65,535 a call)
+        for lo, hi in ((at, at + 32768), (at + 32768, min(at + 65536, ctx + n))):
+            k, v = (torch.randn((hi - lo, H, 128), generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+            st = ops.step_tables(_i32([lo]), _i32([hi - lo]), t, hi - lo)
+            ops.kv8_append_paged(pool, k, v, st.slots)
+    plan = ops.prefill_plan([(0, ctx, n)], H, H, DEV)
+    assert ops.kv8_prefill_workspace_bytes(plan, H, H) > 2 ** 31
+    q = torch.randn((n, H, 128), generator=g, device=DEV).to(torch.bfloat16)
+    out = ops.paged_prefill_attention_kv8(q, pool, t, plan, SCALE)
+    keep = torch.arange(ctx + n, device=DEV)[None] <= ctx + torch.arange(n, device=DEV)[:, None]
+    for h in (0, 7, 15):
+        k, v = ref.read(pool[:, h:h + 1].contiguous(), torch.from_numpy(table).to(DEV)[0])
+        want, tol = ref.attend(q[:, h:h + 1], k[0], v[0], SCALE, keep)
+        assert bool(((out[:, h:h + 1].double() - want).abs() <= tol).all()), h

@@ -26,6 +26,9 @@ def test_pool_holds_records_and_charges_their_bytes():
                          final_norm=torch.zeros(1))
     e = Engine(lm, 8, prefill_chunk=8, allocate=False, kv8=True)
     assert e.pool.kv8 and not Engine(lm, 8, prefill_chunk=8, allocate=False).pool.kv8
+    with pytest.raises(ValueError, match="8192"):
+        Engine(lm, 8, prefill_chunk=8, max_step_tokens=8193, allocate=False, kv8=True)
+    Engine(lm, 8, prefill_chunk=8, max_step_tokens=8193, allocate=False)
 
 
 def test_a_state_of_the_other_kind_is_refused():
