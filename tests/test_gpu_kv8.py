@@ -659,3 +659,28 @@ def test_prompt_rows_after_262140_keys_of_16_heads():
         k, v = ref.read(pool[:, h:h + 1].contiguous(), torch.from_numpy(table).to(DEV)[0])
         want, tol = ref.attend(q[:, h:h + 1], k[0], v[0], SCALE, keep)
         assert bool(((out[:, h:h + 1].double() - want).abs() <= tol).all()), h
+
+
+def test_prompt_attention_replays_over_new_contents():
+    """A captured chunk (expansion, key parts, merge) replayed over other rows, keys and page tables."""
+    H, Hkv, chunks = 32, 4, [(0, 1500, 20), (1, 0, 70)]
+    lens = [c + n for _, c, n in chunks]
+    plan = ops.prefill_plan(chunks, H, Hkv, DEV)
+    assert plan.kv8.slots > 0
+    tables = [_table(lens, s, extra=0) for s in (1, 2, 3)]
+    pools = [ref.random_pool(tables[0][1], Hkv, s, DEV) for s in (4, 5, 6)]
+    g = torch.Generator().manual_seed(2)
+    qs = [torch.randn((90, H, 128), generator=g).to(torch.bfloat16).to(DEV) for _ in range(3)]
+    q, pool, t = qs[0].clone(), pools[0].clone(), _i32(tables[0][0])
+    ops.paged_prefill_attention_kv8(q, pool, t, plan, SCALE)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_prefill_attention_kv8(q, pool, t, plan, SCALE)
+    for i in (0, 1, 2, 0):
+        q.copy_(qs[i])
+        pool.copy_(pools[i])
+        t.copy_(_i32(tables[i][0]))
+        graph.replay()
+        want = ops.paged_prefill_attention_kv8(qs[i], pools[i], _i32(tables[i][0]), plan, SCALE)
+        assert torch.equal(_bits(out), _bits(want)), i
