@@ -576,30 +576,6 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   const long long first_unit = (long long)a.chunk_unit[ch] * a.Hkv + kvh;  // (units of a head lie Hkv apart)
   const uint8_t *units = a.units + first_unit * kUnitBytes;
   const int32_t *info = a.info + 2 * first_unit;
-  const int E = info[2 * (long long)u0 * a.Hkv], some_bad = info[2 * (long long)u0 * a.Hkv + 1] & 16;
-  int nan = 0;
-  for (int u = u0 + l; u < u1; u += 64) nan |= info[2 * (long long)u * a.Hkv + 1] & 32;
-  const bool some_nan = __any(nan);
-
-  const int t = q0 + wave * tpw + lr / G, tok = min(t, len - 1), pos = ctx + tok;  // the lane's row
-  const int first_pos = ctx + min(q0 + wave * tpw, len - 1);                       // the wave's first
-  Frag8 qf[8];
-  {
-    const uint16_t *qp = a.q + ((long long)(row0 + tok) * a.H + kvh * G + lr % G) * kD + 8 * lh;
-#pragma unroll
-    for (int s = 0; s < 8; s++) qf[s].q = *(const uint4 *)(qp + 16 * s);
-  }
-  // (q has landed before the first direct load: the compiler's waits for it would include those)
-#pragma unroll
-  for (int s = 0; s < 8; s++)
-    asm volatile("" ::"v"(qf[s].u[0]), "v"(qf[s].u[1]), "v"(qf[s].u[2]), "v"(qf[s].u[3]));
-  float m_run = kLowest, l_run = 0.0f, top = 0.0f;
-  f32x16 o[4];
-#pragma unroll
-  for (int c = 0; c < 4; c++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) o[c][i] = 0.0f;
-
   const uint32_t k_lds = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)&s_k[0][kLoads * wave][0]);
   const uint32_t v_lds = __builtin_amdgcn_readfirstlane(
@@ -617,6 +593,37 @@ void kv8_prefill_kernel(const PrefillArgs a) {
 #pragma unroll
     for (int i = 0; i < kLoads; i++) load_lds16(p, lane_at + 1024 * i, v_lds + 16384 * slot + 1024 * i);
   };
+  // K(u0) .. K(u0 + kStages - 1) and V(u0) .. V(u0 + kStages - 2), in the order of the loop's requests; q and the units'
+  // infos come in behind them, on one trip to memory
+  request_k(u0, 0);
+#pragma unroll
+  for (int i = 1; i < kStages; i++) {
+    request_k(u0 + i, i);
+    request_v(u0 + i - 1, i - 1);
+  }
+  const int t = q0 + wave * tpw + lr / G, tok = min(t, len - 1), pos = ctx + tok;  // the lane's row
+  const int first_pos = ctx + min(q0 + wave * tpw, len - 1);                       // the wave's first
+  Frag8 qf[8];
+  {
+    const uint16_t *qp = a.q + ((long long)(row0 + tok) * a.H + kvh * G + lr % G) * kD + 8 * lh;
+#pragma unroll
+    for (int s = 0; s < 8; s++) qf[s].q = *(const uint4 *)(qp + 16 * s);
+  }
+  const int E = info[2 * (long long)u0 * a.Hkv], some_bad = info[2 * (long long)u0 * a.Hkv + 1] & 16;
+  int nan = 0;
+  for (int u = u0 + l; u < u1; u += 64) nan |= info[2 * (long long)u * a.Hkv + 1] & 32;
+  const bool some_nan = __any(nan);
+  // (q is there before the loop, whose direct loads the compiler's waits for it would include)
+#pragma unroll
+  for (int s = 0; s < 8; s++)
+    asm volatile("" ::"v"(qf[s].u[0]), "v"(qf[s].u[1]), "v"(qf[s].u[2]), "v"(qf[s].u[3]));
+  float m_run = kLowest, l_run = 0.0f, top = 0.0f;
+  f32x16 o[4];
+#pragma unroll
+  for (int c = 0; c < 4; c++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[c][i] = 0.0f;
+
   // The loads of units up to the one that is next are there, for every wave, and the units behind it are read: the newest
   // kStages - 2 units' loads stay in flight (vmcnt is split over bits 3:0 and 15:14), and a bare barrier follows.
   constexpr int kVm = (kStages - 2) * 2 * kLoads;
@@ -723,13 +730,6 @@ void kv8_prefill_kernel(const PrefillArgs a) {
     if (more) settle(u + 1, s_next);
   };
 
-  // K(u0) .. K(u0 + kStages - 1) and V(u0) .. V(u0 + kStages - 2), in the order of the loop's requests
-  request_k(u0, 0);
-#pragma unroll
-  for (int i = 1; i < kStages; i++) {
-    request_k(u0 + i, i);
-    request_v(u0 + i - 1, i - 1);
-  }
   meet();
 #pragma unroll
   for (int j = 0; j < 16; j++) score(sc[0], read_k(0, j), j);
