@@ -447,11 +447,11 @@ struct PrefillArgs {
   float qk_scale;
 };
 
-// One workgroup expands a unit of one kv head, wave w its page w: 10,240 keys of 4 heads, 11 MB to 21 MB, in 18 us, most of
+// One workgroup expands a unit of one kv head, wave w its page w: 10,240 keys of 4 heads, 11 MB to 21 MB, in 14 to 18 us, most of
 // it the latency of its part's scales (parts of 96 units: 11 us).  Its codes are requested first; meanwhile the part's
 // loudest live V scale is found (by every workgroup of a part for itself: a line of 64 bytes a page).
 __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
-  __shared__ int s_e[4], s_bad[4];
+  __shared__ int s_e[4], s_bad[4], s_ids[kPartMax * kUnitPages];
   const int gu = blockIdx.x, kvh = blockIdx.y, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int lo = 0, hi = a.C - 1;  // the chunk whose units hold gu
   while (lo < hi) {
@@ -462,6 +462,10 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
   const int u = gu - a.chunk_unit[lo], kend = a.chunk_ctx[lo] + a.chunk_len[lo];
   const int32_t *prow = a.page_table + (long long)a.chunk_seq[lo] * a.max_pages;
   const int npages = min((kend + kPage - 1) / kPage, a.max_pages);
+  // the part's pages
+  const int part = min(a.chunk_part[lo], kPartMax), pg0 = u / part * part * kUnitPages;
+  const int np = min(part * kUnitPages, npages - pg0);
+  for (int i = threadIdx.x; i < np; i += 256) s_ids[i] = prow[pg0 + i];
   // this wave's page
   const int pg = kUnitPages * u + wave, page = pg < npages ? prow[pg] : -1;
   const bool out_of_pool = (uint32_t)page >= (uint32_t)a.num_pages;
@@ -479,12 +483,12 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
     wv[i] = *(const uint4 *)(rec + kVOff + 1024 * (l >> 5) + 512 * i + 16 * (l & 31));
     sv[i] = *(const float4 *)(sc + kPage + 8 * i + 4 * vh);
   }
-  // E: thread = page of the part x quarter of its slots
-  const int part = a.chunk_part[lo], pg0 = u / part * part * kUnitPages, pg1 = min(pg0 + part * kUnitPages, npages);
+  // E: thread = page of the part x quarter of its slots (a bare barrier: the codes stay in flight)
   int e = 0, bad = 0;  // (positive powers of two are ordered as their bits)
-#pragma unroll 4
-  for (int i = threadIdx.x; i < 4 * (pg1 - pg0); i += 256) {
-    const int p = pg0 + (i >> 2), id = prow[p];
+  lds_barrier();
+#pragma unroll 6
+  for (int i = threadIdx.x; i < 4 * np; i += 256) {
+    const int p = pg0 + (i >> 2), id = s_ids[i >> 2];
     const bool off = (uint32_t)id >= (uint32_t)a.num_pages;
     const float4 s = *(const float4 *)(record(a.pool, off ? 0 : id, a.Hkv, kvh) + kScaleOff + 4 * kPage + 16 * (i & 3));
     const int left = off ? 0 : kend - (kPage * p + 4 * (i & 3));
