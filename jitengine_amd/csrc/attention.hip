@@ -769,7 +769,8 @@ __global__ __launch_bounds__(64 * WAVES) void prefill_attn_kernel(const PrefillA
   // The loads are issued from inline assembly: the compiler then keeps no track of them (its
   // own waits would otherwise include them before every LDS read, as it cannot tell the
   // stages apart), and the explicit waits below order them; its waits for other loads only
-  // grow more conservative.
+  // grow more conservative.  (s_nop: the load takes M0 one wait state after a scalar write of it
+  // at the earliest, which the compiler does not see to inside a string)
   const uint32_t kvs_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&kvs[0][0];
 #define PF_STAGE(st, pv)                                                                                      \
   _Pragma("unroll") for (int i = 0; i < kPfPages / WAVES; i++) {                                              \
@@ -779,7 +780,7 @@ __global__ __launch_bounds__(64 * WAVES) void prefill_attn_kernel(const PrefillA
     const uint16_t *src = head_part(a.pool, pg, a.Hkv, kvh) + (u >> 2) * kPageHead + (u & 3) * 512 + 8 * l;   \
     const uint32_t dst = __builtin_amdgcn_readfirstlane(                                                      \
         kvs_lds + 2 * (((st) % kPfStages) * kPfHalves * 4 * kPageHead + 512 * c));                            \
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0"); \
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0"); \
   }                                                                                                           \
   }
   // the q fragments have landed before the first staged load is issued: the compiler's waits

@@ -558,9 +558,10 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
 }
 
 // 16 bytes a lane from base + off straight into LDS at byte dst + 16 lane.  Written in assembly, so that the compiler's
-// waits for LDS reads do not include these.
+// waits for LDS reads do not include these.  (s_nop: the load takes M0 one wait state after a scalar write of it at the
+// earliest, which the compiler does not see to inside a string)
 __device__ __forceinline__ void load_lds16(const uint8_t *base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
 }
 
 __global__ __launch_bounds__(64 * kPfWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))

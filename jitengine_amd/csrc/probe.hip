@@ -285,7 +285,8 @@ __global__ __launch_bounds__(64 * L) void probe_lds_ring_kernel(const uint8_t *_
     for (int c = 0; c < NL; c++) {
       const uint8_t *src = run + (long long)st * kStage + (w * NL + c) * 1024 + 16 * l;
       const uint32_t dst = __builtin_amdgcn_readfirstlane(base + slot * kStage + (w * NL + c) * 1024);
-      asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "s"(dst) : "memory", "m0");
+      // (s_nop: M0 is taken one wait state after a scalar write of it at the earliest)
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "s"(dst) : "memory", "m0");
     }
   };
   for (int st = 0; st < S - 1; st++) stage(st, st);

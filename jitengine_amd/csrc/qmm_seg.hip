@@ -164,13 +164,14 @@ __device__ __forceinline__ void seg_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// (the dword form: 256 B a wave)
+// (s_nop: the load takes M0 one wait state after a scalar write of it at the earliest, which the compiler does not see
+// to inside a string; the dword form: 256 B a wave)
 __device__ __forceinline__ void seg_load_lds4(const void *src, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
 }
 
 __device__ __forceinline__ void seg_load_lds(const void *src, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
 }
 
 // DENSE: one dense matrix (E = 1, cnt null), one token chunk per group.
