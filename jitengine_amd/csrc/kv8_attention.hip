@@ -414,7 +414,7 @@ constexpr int kRowsWave = 32, kBlockRows = kPfWaves * kRowsWave;  // a row block
 constexpr int kUnitKeys = JIT_KV8_UNIT_KEYS, kUnitPages = kUnitKeys / kPage;
 constexpr int kUnitBytes = 2 * kUnitKeys * kD * 2;  // K, then V
 constexpr int kPartMax = 192;  // units of the longest part: every unit's workgroup looks through its part's scales
-constexpr int kPfSlot = kD + 4;                  // floats of a (token, part, head) partial: o, max, sum, 2 pad
+constexpr int kPfSlot = kD + 4;                  // floats of a (token, part, head) partial: o / sum, max, sum, 2 pad
 // Expanded values are relative to the loudest scale 2^E of the part's keys, times 2^7 (448 x 2^7 < 65,504): a value of
 // a token 2^22 times quieter than that still has all its bits.
 constexpr int kVShift = 7;
@@ -442,7 +442,7 @@ struct PrefillArgs {
   uint8_t *units;  // [units][Hkv][kUnitBytes]
   int32_t *info;   // [units][Hkv][2]: E of the unit's part, its pages outside the pool (4 bits; 16: some in the part;
                    // 32: NaN codes of V in the unit)
-  float *part;
+  float *part;     // (token, part, head): o / sum, the maximum, the sum
   int num_pages, max_pages, H, Hkv, G, C;
   float qk_scale;
 };
@@ -772,8 +772,10 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   const int parts = pos / (kUnitKeys * part_units) + 1;
   if (t >= len || part >= parts) return;  // (a token before this part's keys: finished by its own last part)
   const long long hrow = (long long)(row0 + tok) * a.H + kvh * G + lr % G;
+  // (divided by the part's own sum, so that a partial, too, is a mean of values of the cache: the undivided sum of loud
+  // ones would pass fp32's range)
+  const float inv = l_tot == 0.0f ? 0.0f : unit / l_tot;
   if (parts == 1) {
-    const float inv = l_tot == 0.0f ? 0.0f : unit / l_tot;
 #pragma unroll
     for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -790,13 +792,14 @@ void kv8_prefill_kernel(const PrefillArgs a) {
     for (int c = 0; c < 4; c++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        *(float4 *)(ps + 32 * c + 8 * i + 4 * lh) = make_float4(o[c][4 * i] * unit, o[c][4 * i + 1] * unit,
-                                                                o[c][4 * i + 2] * unit, o[c][4 * i + 3] * unit);
+        *(float4 *)(ps + 32 * c + 8 * i + 4 * lh) = make_float4(o[c][4 * i] * inv, o[c][4 * i + 1] * inv,
+                                                                o[c][4 * i + 2] * inv, o[c][4 * i + 3] * inv);
     if (lh == 0) *(float2 *)(ps + kD) = make_float2(m_run, l_tot);
   }
 }
 
 // The parts of a token's keys in order, four at a time in flight: 16 heads a workgroup, thread (h, x) dims 32 i + 4 x .. + 3.
+// O is the mean over the parts so far throughout: a part with the share w of the weight moves it by w (o - O).
 __global__ __launch_bounds__(128) void kv8_prefill_merge_kernel(const PrefillArgs a) {
   const int c = blockIdx.y, t = blockIdx.x, h = 16 * blockIdx.z + (threadIdx.x >> 3);
   if (t >= a.chunk_len[c] || h >= a.H) return;
@@ -822,20 +825,19 @@ __global__ __launch_bounds__(128) void kv8_prefill_merge_kernel(const PrefillArg
 #pragma unroll
     for (int j = 0; j < kBatch; j++) {
       if (p0 + j >= parts) break;
-      const float mn = fmaxf(M, ml[j].x), fa = exp2f(M - mn), fb = exp2f(ml[j].x - mn);
-      ls = fmaf(ls, fa, ml[j].y * fb);
+      const float mn = fmaxf(M, ml[j].x), here = ml[j].y * exp2f(ml[j].x - mn);
+      ls = fmaf(ls, exp2f(M - mn), here);
+      const float w = ls == 0.0f ? 0.0f : here / ls;
       const float *x = (const float *)v[j];
 #pragma unroll
-      for (int i = 0; i < 16; i++) O[i] = fmaf(O[i], fa, x[i] * fb);
+      for (int i = 0; i < 16; i++) O[i] = fmaf(w, x[i] - O[i], O[i]);
       M = mn;
     }
   }
-  const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
   uint16_t *op = a.out + ((long long)(a.chunk_row[c] + t) * a.H + h) * kD + d0;
 #pragma unroll
   for (int i = 0; i < 4; i++)
-    *(uint2 *)(op + 32 * i) = make_uint2(pack_bf16x2(O[4 * i] * inv, O[4 * i + 1] * inv),
-                                         pack_bf16x2(O[4 * i + 2] * inv, O[4 * i + 3] * inv));
+    *(uint2 *)(op + 32 * i) = make_uint2(pack_bf16x2(O[4 * i], O[4 * i + 1]), pack_bf16x2(O[4 * i + 2], O[4 * i + 3]));
 }
 
 int64_t decode_bytes(int B, int H, int max_len) {
