@@ -395,7 +395,7 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
 
 // ---------------------------------------------------------------- causal prompt chunks
 // Two launches (three where a token's keys have several parts).  The first expands the keys that the chunks see: K to
-// bf16 (times its scale) and V to fp16, in the order in which the second launch's matrix instructions take them.
+// bf16 (times its scale) and V to fp16 (or bf16: kSpread), in the order in which the second launch's matrix instructions take them.
 // Every row block of a chunk reads all of its keys, so the conversion is done once instead of once a block; inside the
 // attention loop it cost as many vector instructions as the softmax (2,048 rows after 8,192 keys: 344 us, without it 328).
 //
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
 // of a part, up to its last token, 64 (a unit) at a time, a unit's 32 KB going straight from memory into LDS.  Two
 // workgroups share a CU.
 //   S^T[32 keys x 32 rows] = K . Q^T        (8 MFMA 32x32x16 bf16)
-//   O^T[128 dims x 32 rows] += V^T . P^T    (4 MFMA 32x32x16 fp16 a page)
+//   O^T[128 dims x 32 rows] += V^T . P^T    (4 MFMA 32x32x16 fp16 a page; 8 of bf16 in a part of uneven V)
 // Bound by the matrix instructions and the clock they leave (2,048 rows after 8,192 keys: busy 60% of the cycles at 1.9 GHz,
 // 303 to 318 us, 1.0 PFLOP/s; a large bf16 product of the library 1.15 to 1.4).  Both workgroups of a CU are needed: with
 // one of four waves, however many units are on their way, the same takes 394 us.
@@ -415,12 +415,18 @@ constexpr int kUnitKeys = JIT_KV8_UNIT_KEYS, kUnitPages = kUnitKeys / kPage;
 constexpr int kUnitBytes = 2 * kUnitKeys * kD * 2;  // K, then V
 constexpr int kPartMax = 192;  // units of the longest part: every unit's workgroup looks through its part's scales
 constexpr int kPfSlot = kD + 4;                  // floats of a (token, part, head) partial: o / sum, max, sum, 2 pad
-// Expanded values are relative to the loudest scale 2^E of the part's keys, times 2^7 (448 x 2^7 < 65,504): a value of
-// a token 2^22 times quieter than that still has all its bits.
-constexpr int kVShift = 7;
 // A row's reference for the exponentials moves when its maximum passes it by more than 2^4: most units then have no O
 // to rescale.  Probabilities are formed 2^11 times too large, at most 2^15: 11 bits down to 2^-25 of the reference.
 constexpr float kLazy = 4.0f, kPfShift = 11.0f;
+// Two forms of a part, by the scales of V's blocks that its keys hold:
+// * within 2^12 of each other: V in fp16 relative to the loudest scale 2^E, times 2^7 (448 x 2^7 < 65,504; the quietest
+//   block's least code is 2^-14 then, so every value has all its bits and no row depends on E), probabilities as one fp16.
+//   One below fp16's range is off by 2^-25, 2^-36 of the row's sum at least: 12,288 keys 2^12 times louder than what the
+//   row is made of lose it 2^(13.6 - 36 + 12), less than a fifth of a bf16 rounding.
+// * further apart: V in bf16 as it is (4 bits, 2^-109 .. 2^127: exact) and probabilities as a high and a low bf16 part, 16
+//   bits at any magnitude, 2^-20 of their size so that no sum passes fp32's range: half as many matrix instructions again.
+constexpr int kVShift = 7, kSpread = 12;
+constexpr float kWideShift = -20.0f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -441,7 +447,7 @@ struct PrefillArgs {
   uint16_t *out;
   uint8_t *units;  // [units][Hkv][kUnitBytes]
   int32_t *info;   // [units][Hkv][2]: E of the unit's part, its pages outside the pool (4 bits; 16: some in the part;
-                   // 32: NaN codes of V in the unit)
+                   // 32: NaN codes of V in the unit; 64: the part's V scales are more than 2^kSpread apart)
   float *part;     // (token, part, head): o / sum, the maximum, the sum
   int num_pages, max_pages, H, Hkv, G, C;
   float qk_scale;
@@ -449,9 +455,10 @@ struct PrefillArgs {
 
 // One workgroup expands a unit of one kv head, wave w its page w: 10,240 keys of 4 heads, 11 MB to 21 MB, in 14 to 18 us, most of
 // it the latency of its part's scales (parts of 96 units: 11 us).  Its codes are requested first; meanwhile the part's
-// loudest live V scale is found (by every workgroup of a part for itself: a line of 64 bytes a page).
-__global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
+// loudest and quietest live V scales are found (by every workgroup of a part for itself: a line of 64 bytes a page).
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8))) void kv8_expand_kernel(const PrefillArgs a) {
   __shared__ int s_e[4], s_bad[4], s_ids[kPartMax * kUnitPages];
+  __shared__ uint32_t s_least[4];
   const int gu = blockIdx.x, kvh = blockIdx.y, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int lo = 0, hi = a.C - 1;  // the chunk whose units hold gu
   while (lo < hi) {
@@ -484,7 +491,8 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
     sv[i] = *(const float4 *)(sc + kPage + 8 * i + 4 * vh);
   }
   // E: thread = page of the part x quarter of its slots (a bare barrier: the codes stay in flight)
-  int e = 0, bad = 0;  // (positive powers of two are ordered as their bits)
+  int e = 0, bad = 0;     // (positive powers of two are ordered as their bits)
+  uint32_t least = ~0u;   // (bits - 1: a slot never written, scale 0, is the last of all)
   lds_barrier();
 #pragma unroll 6
   for (int i = threadIdx.x; i < 4 * np; i += 256) {
@@ -495,10 +503,13 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
     const float *sp = (const float *)&s;
     bad |= off;
 #pragma unroll
-    for (int j = 0; j < 4; j++) e = j < left ? max(e, __float_as_int(sp[j])) : e;
+    for (int j = 0; j < 4; j++) {
+      e = j < left ? max(e, __float_as_int(sp[j])) : e;
+      least = j < left ? min(least, __float_as_uint(sp[j]) - 1u) : least;
+    }
   }
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o, 64));
+  for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o, 64)), least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
   const int any = __any(bad), here = __any(out_of_pool && pg < npages);
   // What lies past the keys or in a page outside the pool may be anything (0 x NaN): it counts as 0.  So do NaN codes
   // of V, which rows that do not see their key must not get either: kv8_prefill_kernel puts them back.
@@ -518,12 +529,15 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
     }
   }
   const int any_nan = __any(nan != 0);
-  if (l == 0) s_e[wave] = e, s_bad[wave] = (any ? 16 : 0) | (here ? 1 << wave : 0) | (any_nan ? 32 : 0);
+  if (l == 0) s_e[wave] = e, s_least[wave] = least, s_bad[wave] = (any ? 16 : 0) | (here ? 1 << wave : 0) | (any_nan ? 32 : 0);
   __syncthreads();
   e = max(max(s_e[0], s_e[1]), max(s_e[2], s_e[3]));
+  least = min(min(s_least[0], s_least[1]), min(s_least[2], s_least[3]));
   const int E = min(max((e >> 23) - 127, kMinExp), kMaxExp);
+  const bool wide = e && (e >> 23) - (int)((least + 1u) >> 23) > kSpread;
   if (threadIdx.x == 0)
-    *(int2 *)(a.info + 2 * ((long long)gu * a.Hkv + kvh)) = make_int2(E, s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]);
+    *(int2 *)(a.info + 2 * ((long long)gu * a.Hkv + kvh)) =
+        make_int2(E, s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3] | (wide ? 64 : 0));
   uint4 *dst_k = (uint4 *)(a.units + ((long long)gu * a.Hkv + kvh) * kUnitBytes), *dst_v = dst_k + kUnitBytes / 32;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
@@ -536,8 +550,28 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
     d[0] = f0;
     d[32] = f1;
   }
+  // value (i, j) of dims c: slot 8 i + 4 vh + j
+  auto v_out = [&](int c) { return dst_v + (4 * wave + 2 * (l >> 5) + (c >> 1)) * 64 + 32 * vh + 16 * (c & 1) + (l & 15); };
+  if (wide) {  // (uniform; rare)
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      uint32_t r[4];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const float *sp = (const float *)&sv[i];
+        uint32_t w[2];
+        to_bf16(((const uint32_t *)&wv[i])[c], 1.0f, w[0], w[1]);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          r[2 * i + j] = pack_bf16x2(2 * j < keep[i] ? bf2f(w[j] & 0xffffu) * sp[2 * j] : 0.0f,
+                                     2 * j + 1 < keep[i] ? bf2f_hi(w[j]) * sp[2 * j + 1] : 0.0f);
+      }
+      *v_out(c) = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+    return;
+  }
   const float unit = exp_bits(kVShift - E);
-  f16x2_t fac[2][2];  // 2^(e - E + 7); below fp16's range 0
+  f16x2_t fac[2][2];  // 2^(e - E + 7); of a slot never written 0
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const float *sp = (const float *)&sv[i];
@@ -552,8 +586,7 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(const PrefillArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
       r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, r[i]) * fac[i >> 1][i & 1]);
-    dst_v[(4 * wave + 2 * (l >> 5) + (c >> 1)) * 64 + 32 * vh + 16 * (c & 1) + (l & 15)] =
-        make_uint4(r[0], r[1], r[2], r[3]);
+    *v_out(c) = make_uint4(r[0], r[1], r[2], r[3]);
   }
 }
 
@@ -588,12 +621,12 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   const uint32_t lane_at = 1024 * kLoads * wave + 16 * l;
   const long long unit_step_bytes = (long long)a.Hkv * kUnitBytes;
   // (a unit past the last: the last again, whose place in LDS is free and never read)
-  auto request_k = [&](int u, int slot) {
+  auto request_k = [&](int u, int slot) __attribute__((always_inline)) {
     const uint8_t *p = units + min(u, u1 - 1) * unit_step_bytes;
 #pragma unroll
     for (int i = 0; i < kLoads; i++) load_lds16(p, lane_at + 1024 * i, k_lds + 16384 * slot + 1024 * i);
   };
-  auto request_v = [&](int u, int slot) {
+  auto request_v = [&](int u, int slot) __attribute__((always_inline)) {
     const uint8_t *p = units + min(u, u1 - 1) * unit_step_bytes + kUnitBytes / 2;
 #pragma unroll
     for (int i = 0; i < kLoads; i++) load_lds16(p, lane_at + 1024 * i, v_lds + 16384 * slot + 1024 * i);
@@ -614,7 +647,9 @@ void kv8_prefill_kernel(const PrefillArgs a) {
 #pragma unroll
     for (int s = 0; s < 8; s++) qf[s].q = *(const uint4 *)(qp + 16 * s);
   }
-  const int E = info[2 * (long long)u0 * a.Hkv], some_bad = info[2 * (long long)u0 * a.Hkv + 1] & 16;
+  const int E = info[2 * (long long)u0 * a.Hkv], flags = info[2 * (long long)u0 * a.Hkv + 1], some_bad = flags & 16;
+  const bool wide = __builtin_amdgcn_readfirstlane(flags & 64) != 0;
+  const float p_shift = wide ? kWideShift : kPfShift;
   int nan = 0;
   for (int u = u0 + l; u < u1; u += 64) nan |= info[2 * (long long)u * a.Hkv + 1] & 32;
   const bool some_nan = __any(nan);
@@ -632,30 +667,30 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   // The loads of units up to the one that is next are there, for every wave, and the units behind it are read: the newest
   // kStages - 2 units' loads stay in flight (vmcnt is split over bits 3:0 and 15:14), and a bare barrier follows.
   constexpr int kVm = (kStages - 2) * 2 * kLoads;
-  auto meet = [&]() {
+  auto meet = [&]() __attribute__((always_inline)) {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt((kVm & 15) | ((kVm >> 4) << 14) | (7 << 4) | (0 << 8));  // vmcnt(kVm) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
 
-  f32x16 sc[2][2];  // scores of two units (u % 2) of two page pairs; lane: key 32 g + 8 (i / 4) + 4 lh + i % 4
   constexpr int kAhead = 4;  // operand fragments requested from LDS ahead of their instructions
-  auto read_k = [&](int slot, int j) {  // page pair j % 2, dims 16 (j / 2)
+  f32x16 sc[2][2];  // scores of two units (u % 2) of two page pairs; lane: key 32 g + 8 (i / 4) + 4 lh + i % 4
+  auto read_k = [&](int slot, int j) __attribute__((always_inline)) {  // page pair j % 2, dims 16 (j / 2)
     Frag8 f;
     f.q = s_k[slot][8 * (j & 1) + (j >> 1)][l];
     return f;
   };
-  auto read_v = [&](int slot, int j) {  // page j / 4, dims 32 (j % 4)
+  auto read_v = [&](int slot, int j) __attribute__((always_inline)) {  // page j / 4, dims 32 (j % 4)
     FragH f;
     f.q = s_v[slot][j][l];
     return f;
   };
-  auto score = [&](f32x16 (&s)[2], const Frag8 &kf, int j) {
+  auto score = [&](f32x16 (&s)[2], const Frag8 &kf, int j) __attribute__((always_inline)) {
     const f32x16 z = {};
     s[j & 1] = mfma32x32x16(kf, qf[j >> 1], j < 2 ? z : s[j & 1]);
   };
-  auto largest = [&](const f32x16 (&s)[2]) {
+  auto largest = [&](const f32x16 (&s)[2]) __attribute__((always_inline)) {
     top = s[0][0];
 #pragma unroll
     for (int g = 0; g < 2; g++)
@@ -664,7 +699,7 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   };
   // What of unit u's softmax waits for its scores' maximum, and O's rescaling.
   float off = 0.0f;
-  auto settle = [&](int u, f32x16 (&s)[2]) {
+  auto settle = [&](int u, f32x16 (&s)[2]) __attribute__((always_inline)) {
     const int k0 = kUnitKeys * u;
     if (k0 + kUnitKeys - 1 > first_pos || some_bad) {
       const int bad = some_bad ? info[2 * (long long)u * a.Hkv + 1] : 0;
@@ -680,7 +715,7 @@ void kv8_prefill_kernel(const PrefillArgs a) {
     top = max_xor32(top) * a.qk_scale;
     const float m_new = top > m_run + kLazy ? top : m_run;
     const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-    off = kPfShift - m_new;
+    off = p_shift - m_new;
     l_run *= alpha;
     m_run = m_new;
     if (__any(alpha != 1.0f)) {
@@ -694,7 +729,7 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   int slot = 0;  // unit u's place in both rings
   // Unit u: its softmax beside the scores of unit u + 1, then its products with V beside the maximum of the new scores;
   // cut into groups of a matrix instruction and the vector work that runs during it.
-  auto unit_step = [&](int u, f32x16 (&s)[2], f32x16 (&s_next)[2], bool more) {
+  auto unit_step = [&](int u, f32x16 (&s)[2], f32x16 (&s_next)[2], bool more) __attribute__((always_inline)) {
     meet();
     const int k_slot = next(slot, 1);
     Frag8 kf[kAhead];
@@ -735,17 +770,60 @@ void kv8_prefill_kernel(const PrefillArgs a) {
     if (more) settle(u + 1, s_next);
   };
 
+  // unit_step of a part of uneven V: bf16 V, a page's probabilities in two parts at a time (all four pages' do not fit the
+  // registers)
+  auto wide_step = [&](int u, f32x16 (&s)[2], f32x16 (&s_next)[2], bool more) __attribute__((always_inline)) {
+    meet();
+    const int k_slot = next(slot, 1);
+    request_k(u + kStages, slot);
+    request_v(u + kStages - 1, next(slot, kStages - 1));
+#pragma unroll
+    for (int j = 0; j < 16; j++) score(s_next, read_k(k_slot, j), j);
+#pragma unroll
+    for (int pg = 0; pg < kUnitPages; pg++) {
+      Frag8 high, rest;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int i = 8 * (pg & 1) + 2 * j;
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[pg >> 1][i], a.qk_scale, off));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[pg >> 1][i + 1], a.qk_scale, off));
+        high.u[j] = pack_bf16x2(p0, p1);
+        rest.u[j] = pack_bf16x2(p0 - bf2f(high.u[j] & 0xffffu), p1 - bf2f_hi(high.u[j]));
+        l_run += p0 + p1;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        Frag8 v;
+        v.q = s_v[slot][4 * pg + c][l];
+        o[c] = mfma32x32x16(v, high, o[c]);
+        o[c] = mfma32x32x16(v, rest, o[c]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    largest(s_next);
+    slot = k_slot;
+    if (more) settle(u + 1, s_next);
+  };
+
   meet();
 #pragma unroll
   for (int j = 0; j < 16; j++) score(sc[0], read_k(0, j), j);
   largest(sc[0]);
   settle(u0, sc[0]);
   int u = u0;
-  for (; u + 1 < u1; u += 2) {
-    unit_step(u, sc[0], sc[1], true);
-    unit_step(u + 1, sc[1], sc[0], u + 2 < u1);
+  if (!wide) {
+    for (; u + 1 < u1; u += 2) {
+      unit_step(u, sc[0], sc[1], true);
+      unit_step(u + 1, sc[1], sc[0], u + 2 < u1);
+    }
+    if (u < u1) unit_step(u, sc[0], sc[1], false);
+  } else {
+    for (; u + 1 < u1; u += 2) {
+      wide_step(u, sc[0], sc[1], true);
+      wide_step(u + 1, sc[1], sc[0], u + 2 < u1);
+    }
+    if (u < u1) wide_step(u, sc[0], sc[1], false);
   }
-  if (u < u1) unit_step(u, sc[0], sc[1], false);
   __builtin_amdgcn_s_waitcnt(0);  // no load may still write the LDS when the workgroup ends
   if (some_nan) {  // (rare) V's NaN codes, to the rows that see their keys
     const int32_t *prow = a.page_table + (long long)a.chunk_seq[ch] * a.max_pages;
@@ -767,7 +845,7 @@ void kv8_prefill_kernel(const PrefillArgs a) {
       }
     }
   }
-  const float unit = exp_bits(E - kVShift);
+  const float unit = wide ? 1.0f : exp_bits(E - kVShift);
   const float l_tot = sum_xor32(l_run);
   const int parts = pos / (kUnitKeys * part_units) + 1;
   if (t >= len || part >= parts) return;  // (a token before this part's keys: finished by its own last part)
@@ -794,7 +872,8 @@ void kv8_prefill_kernel(const PrefillArgs a) {
       for (int i = 0; i < 4; i++)
         *(float4 *)(ps + 32 * c + 8 * i + 4 * lh) = make_float4(o[c][4 * i] * inv, o[c][4 * i + 1] * inv,
                                                                 o[c][4 * i + 2] * inv, o[c][4 * i + 3] * inv);
-    if (lh == 0) *(float2 *)(ps + kD) = make_float2(m_run, l_tot);
+    // (the sums of both forms at one size)
+    if (lh == 0) *(float2 *)(ps + kD) = make_float2(m_run, wide ? l_tot * 0x1p31f : l_tot);
   }
 }
 

@@ -91,3 +91,111 @@ def test_loud_values_stay_finite_however_a_chunk_is_cut(ctx, n, mag):
     assert (plan.kv8.slots > 0) == (ctx > 0)
     want, A = _rows(q.to(DEV), pool, table, ctx)
     _check(out, want, A, 11, L, _score_error(q, k), (ctx, n, mag))
+
+
+SHAPES = [(0, 2), (0, 70), (3000, 9), (20, 300), (8000, 16)]
+
+
+@pytest.mark.parametrize("ctx, n", SHAPES)
+@pytest.mark.parametrize("H, Hkv", [(32, 4), (16, 16)])
+@pytest.mark.parametrize("power", [12, 13, 23, 40, 110])
+def test_a_loud_value_leaves_the_rows_before_it_alone(ctx, n, H, Hkv, power):
+    """The chunk's last token has V 2^power times its neighbours': the other rows do not see it."""
+    L = ctx + n
+    q, k, v = _normal(L, H, Hkv, n + power)
+    q, k, v = q[:n].to(torch.bfloat16).to(DEV), k.to(torch.bfloat16), v.to(torch.bfloat16)
+    v[-1] *= 2.0 ** power
+    pool, table = _cache(k, v, power)
+    out, _ = _prompt(q, pool, table, ctx)
+    want, A = _rows(q, pool, table, ctx)
+    _check(out, want, A, 11, L, _score_error(q, k), (ctx, n, power))
+
+
+def test_a_quiet_first_row_is_its_own_value():
+    """Two tokens, V of 1e-6 and then of 1e5: the first row gives its token's V as the cache holds it."""
+    q, k, v = _normal(2, 8, 1, 5)
+    k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+    v[0] *= 1e-6
+    v[1] *= 1e5
+    pool, table = _cache(k, v)
+    out, _ = _prompt(q.to(torch.bfloat16).to(DEV), pool, table, 0)
+    _, held = ref.read(pool, table[0].to(DEV))
+    assert torch.equal(out[0].double(), held[0, :1].expand(8, 128))  # (4 significant bits: exact in bf16)
+
+
+@pytest.mark.parametrize("ctx, n", [(0, 70), (3000, 9), (20, 300)])
+@pytest.mark.parametrize("power", [-20, -40, -90])
+def test_a_row_whose_weight_is_on_a_quiet_value(ctx, n, power):
+    """Key 5 is 2^power as loud as the others and takes every row's weight but for some 2^-130."""
+    H, Hkv, L = 32, 4, ctx + n
+    q, k, v = _normal(L, H, Hkv, n)
+    k = (k - 2 * k[5:6] * (k * k[5:6]).sum(-1, keepdim=True).clamp(min=0) / (k[5:6] ** 2).sum(-1, keepdim=True))
+    k[5] = -k[5] / k[5].norm(dim=-1, keepdim=True) * 32  # (the others' products with it are zero or less)
+    k = k.to(torch.bfloat16)
+    q = (k[5].repeat_interleave(H // Hkv, 0)[None] * (1 + 0.01 * q[:n, :, :1])).to(torch.bfloat16).to(DEV)
+    v = v.to(torch.bfloat16)
+    v[5] *= 2.0 ** power
+    pool, table = _cache(k, v, n)
+    out, _ = _prompt(q, pool, table, ctx)
+    want, A = _rows(q, pool, table, ctx)
+    _check(out, want, A, 11, L, _score_error(q, k), (ctx, n, power))
+
+
+@pytest.mark.parametrize("ctx, n", [(0, 70), (3000, 9), (40, 300)])
+@pytest.mark.parametrize("power", [-8, -13, -30, -60, -85])
+def test_quiet_values_beside_rows_of_zeros(ctx, n, power):
+    """A block of zeros has scale 1, however quiet its neighbours are; slots that nothing was written to have scale 0."""
+    H, Hkv, L = 32, 4, ctx + n
+    q, k, v = _normal(L, H, Hkv, n)
+    v *= 2.0 ** power
+    v[torch.arange(0, L, 3)] = 0.0
+    q, k = q[:n].to(torch.bfloat16).to(DEV), k.to(torch.bfloat16)
+    pool, table = _cache(k, v.to(torch.bfloat16), n)
+    pool[table[0, 1]] = 0
+    out, _ = _prompt(q, pool, table, ctx)
+    want, A = _rows(q, pool, table, ctx)
+    _check(out, want, A, 11, L, _score_error(q, k), (ctx, n, power))
+
+
+def test_parts_of_even_and_of_uneven_values_meet():
+    """One of a chunk's 15 parts has values 2^30 louder than the others', with a weight that leaves both to be seen."""
+    ctx, n, H, Hkv = 8000, 16, 32, 4
+    L = ctx + n
+    q, k, v = _normal(L, H, Hkv, 9)
+    q, k, v = q[:n].to(torch.bfloat16).to(DEV), k.to(torch.bfloat16), v.to(torch.bfloat16)
+    v[4000] *= 2.0 ** 16
+    v[4001] *= 2.0 ** -14
+    pool, table = _cache(k, v)
+    out, plan = _prompt(q, pool, table, ctx)
+    assert plan.kv8.slots >= 8 * n
+    want, A = _rows(q, pool, table, ctx)
+    _check(out, want, A, 11, L, _score_error(q, k), "parts")
+
+
+def test_replays_over_even_and_uneven_values():
+    """A captured chunk takes whatever values the cache holds when it is replayed."""
+    ctx, n, H, Hkv = 640, 40, 32, 4
+    L = ctx + n
+    q, k, v = _normal(L, H, Hkv, 3)
+    q, k, v = q[:n].to(torch.bfloat16).to(DEV), k.to(torch.bfloat16).to(DEV), v.to(torch.bfloat16).to(DEV)
+    pool, table = _cache(k, v)
+    t = table.int().to(DEV)
+    at = torch.arange(L, device=DEV)
+    slots = t[0, at // 16] * 16 + (at % 16).int()
+    plan = ops.prefill_plan([(0, ctx, n)], H, Hkv, DEV)
+    ws = torch.empty(ops.kv8_prefill_workspace_bytes(plan, H, Hkv), dtype=torch.uint8, device=DEV)
+    ops.paged_prefill_attention_kv8(q, pool, t, plan, SCALE, ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_prefill_attention_kv8(q, pool, t, plan, SCALE, ws)
+    for power in (0, 30, 0, -40, 5):
+        v2 = v.clone()
+        v2[L - 7] *= 2.0 ** power
+        ops.kv8_append_paged(pool, k, v2, slots)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, A = _rows(q, pool, table, ctx)
+        _check(out, want, A, 11, L, _score_error(q, k), power)
+        eager = ops.paged_prefill_attention_kv8(q, pool, t, plan, SCALE)
+        assert torch.equal(eager.view(torch.int16), out.view(torch.int16))
