@@ -60,15 +60,11 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2v_t __attribute__((ext_vector_type(2)));
 
-union FragH {  // 8 fp16 = one 16x16x32 operand fragment of one lane
+union FragH {  // 8 fp16 = one 32x32x16 operand fragment of one lane
   f16x8_t v;
   uint32_t u[4];
   uint4 q;
 };
-
-__device__ __forceinline__ f32x4 mfma16x16x32_f16(const FragH &a, const FragH &b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v, b.v, c, 0, 0, 0);
-}
 
 // four codes -> two words of bf16 (times the power of two s) or fp16: exact, 4 significant bits
 __device__ __forceinline__ void to_bf16(uint32_t w, float s, uint32_t &lo, uint32_t &hi) {

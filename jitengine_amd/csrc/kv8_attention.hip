@@ -2,8 +2,9 @@
 // Records and number format: kv8.hpp.
 //
 // Scores are formed from the codes, K_codes . Q^T in bf16 matrix instructions (codes and q are exact there), and
-// take their key's scale afterwards; V's codes meet the probabilities in fp16 instructions (codes are exact, a
-// probability keeps 11 bits, 8 times what bf16 would, at half the instructions of a bf16 high and low part).
+// take their key's scale afterwards.  Single tokens, bound by memory, keep 16 bits of a probability times V's scale, as
+// a high and a low bf16 part (as the bf16 pool's attention does).  Prompt chunks, bound by the matrix instructions, take a
+// probability as one fp16, 11 bits: 16 of them would be twice the products with V.
 #include "kv8.hpp"
 
 #include <type_traits>
@@ -13,14 +14,14 @@ namespace {
 using namespace kv8;
 
 constexpr float kLowest = -1e30f;  // the running maximum before any key: finite, so that rows without a key stay 0
-// Probabilities are formed 2^15 times too large: fp16 then keeps 11 bits of those down to 2^-29 of a row's largest,
-// and the factor cancels in the division by their sum.
-constexpr float kPShift = 15.0f;
-
 // ---------------------------------------------------------------- single tokens
 // A sequence is cut into chunks by its own length alone, a chunk into 4 runs of a wave each.  512 keys: with 768 and
 // 1,024 64 sequences of 300 keys take 11.8 and 14.2 us instead of 9.8, 32 ragged ones 32 to 35 with any of the three.
 constexpr int kSplits = 4;
+// What meets in a product: a probability times V's scale times 2^8 (2^-92 .. 2^126: both parts are normal numbers down to
+// p = 2^-18 of the quietest block), and V's codes times 2^-28.  O is 2^-20 of its size: 2^20 keys of the loudest block
+// stay in fp32's range.
+constexpr float kVScaleUp = 256.0f, kCodeScale = 0x1p-28f, kOBack = 0x1p20f;
 constexpr int kChunk = 512, kLongChunks = 128, kChunkMax = 64 * kPage * kSplits;
 
 __host__ __device__ __forceinline__ int chunk_tokens(int len) {
@@ -210,20 +211,17 @@ void kv8_decode_kernel(const DecodeArgs a) {
           s[p] = mfma16x16x32(kf, qf[f], s[p]);
         }
       }
-      float t[2][4], iv[2][4];
+      float t[2][4], v8[2][4];  // scores, then weights; V's scales
 #pragma unroll
       for (int p = 0; p < 2; p++) {
-        // V's scale 2^e is part of the exponent, so a row's maximum is that of its contributions; the sum of the
-        // probabilities themselves takes 2^-e back out (a scale of 0, a slot never written, as 2^-100)
-        uint32_t vb = max(__float_as_uint(vs[p]), (uint32_t)(kMinExp + 127) << 23);
-        if (cut) vb = (l & 3) < keep[p] ? vb : 127u << 23;
-        const float kq = ks[p] * a.qk_scale, ev = (float)((int)(vb >> 23) - 127), inv = __uint_as_float((254u << 23) - vb);
+        float vb = vs[p] * kVScaleUp;
+        if (cut) vb = (l & 3) < keep[p] ? vb : 0.0f;
+        const float kq = ks[p] * a.qk_scale;
         const float kqs[4] = {quad<0>(kq), quad<1>(kq), quad<2>(kq), quad<3>(kq)};
-        const float evs[4] = {quad<0>(ev), quad<1>(ev), quad<2>(ev), quad<3>(ev)};
-        iv[p][0] = quad<0>(inv), iv[p][1] = quad<1>(inv), iv[p][2] = quad<2>(inv), iv[p][3] = quad<3>(inv);
+        v8[p][0] = quad<0>(vb), v8[p][1] = quad<1>(vb), v8[p][2] = quad<2>(vb), v8[p][3] = quad<3>(vb);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          t[p][i] = fmaf(s[p][i], kqs[i], evs[i]);
+          t[p][i] = s[p][i] * kqs[i];
           if (cut) t[p][i] = i < keep[p] ? t[p][i] : -INFINITY;
         }
       }
@@ -246,16 +244,15 @@ void kv8_decode_kernel(const DecodeArgs a) {
       for (int p = 0; p < 2; p++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          t[p][i] = __builtin_amdgcn_exp2f(t[p][i] - (m_new - kPShift));
-          psum = fmaf(t[p][i], iv[p][i], psum);
+          t[p][i] = __builtin_amdgcn_exp2f(t[p][i] - m_new);
+          psum += t[p][i];
+          t[p][i] *= v8[p][i];
         }
       l_run = fmaf(l_run, alpha, psum);
       m_run = m_new;
-      FragH pf;
-      pf.u[0] = pack_f16x2(t[0][0], t[0][1]);
-      pf.u[1] = pack_f16x2(t[0][2], t[0][3]);
-      pf.u[2] = pack_f16x2(t[1][0], t[1][1]);
-      pf.u[3] = pack_f16x2(t[1][2], t[1][3]);
+      Frag8 high, rest;
+#pragma unroll
+      for (int i = 0; i < 4; i++) split_bf16x2(t[i >> 1][2 * (i & 1)], t[i >> 1][2 * (i & 1) + 1], high.u[i], rest.u[i]);
       if (cut) {  // (a p of 0 does not cancel a NaN code)
 #pragma unroll
         for (int p = 0; p < 2; p++) {
@@ -272,10 +269,12 @@ void kv8_decode_kernel(const DecodeArgs a) {
       }
 #pragma unroll
       for (int cc = 0; cc < 8; cc++) {
-        FragH vf;
+        Frag8 vf;
 #pragma unroll
-        for (int p = 0; p < 2; p++) to_f16(((const uint32_t *)&vc[p][cc >> 2])[cc & 3], vf.u[2 * p], vf.u[2 * p + 1]);
-        o[cc] = mfma16x16x32_f16(vf, pf, o[cc]);
+        for (int p = 0; p < 2; p++)
+          to_bf16(((const uint32_t *)&vc[p][cc >> 2])[cc & 3], kCodeScale, vf.u[2 * p], vf.u[2 * p + 1]);
+        o[cc] = mfma16x16x32(vf, high, o[cc]);
+        o[cc] = mfma16x16x32(vf, rest, o[cc]);
       }
       asm volatile("" ::: "memory");
       if constexpr (!LAST) request_v(cur, st + 1);
@@ -319,7 +318,7 @@ void kv8_decode_kernel(const DecodeArgs a) {
         l_tot = fmaf(xstate[sp][33][l], f[sp], l_tot);
       }
       l_tot = sum_xor32(sum_xor16(l_tot));
-      const float inv = cur.n > 1 ? 1.0f : l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+      const float inv = cur.n > 1 ? 1.0f : l_tot == 0.0f ? 0.0f : kOBack / l_tot;
       const long long r = ((long long)cur.b * a.ncap + cur.c) * a.H + kvh * G + lr;
 #pragma unroll
       for (int x = 0; x < 2; x++) {
@@ -386,7 +385,7 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
     acc.w = fmaf(v.w, f, acc.w);
     l_tot = fmaf(s_l[j], f, l_tot);
   }
-  const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+  const float inv = l_tot == 0.0f ? 0.0f : kOBack / l_tot;
   uint2 w;
   w.x = pack_bf16x2(acc.x * inv, acc.y * inv);
   w.y = pack_bf16x2(acc.z * inv, acc.w * inv);

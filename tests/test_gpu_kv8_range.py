@@ -30,7 +30,9 @@ def _cache(k: torch.Tensor, v: torch.Tensor, seed: int = 0, spare: int = 2):
     pool = ref.random_pool(W + spare, Hkv, seed + n, DEV)
     pool[table.to(DEV)] = 0
     t = torch.arange(n)
-    ops.kv8_append_paged(pool, k.to(DEV), v.to(DEV), (table[t // 16] * 16 + t % 16).int().to(DEV))
+    slots = (table[t // 16] * 16 + t % 16).int()
+    for part in t.split(32768):  # (a write covers 65,535 rows)
+        ops.kv8_append_paged(pool, k[part].to(DEV), v[part].to(DEV), slots[part].to(DEV))
     return pool, table.view(1, W)
 
 
@@ -199,3 +201,55 @@ def test_replays_over_even_and_uneven_values():
         _check(out, want, A, 11, L, _score_error(q, k), power)
         eager = ops.paged_prefill_attention_kv8(q, pool, t, plan, SCALE)
         assert torch.equal(eager.view(torch.int16), out.view(torch.int16))
+
+
+def _decode(q, k, v, seed, tag, pool_edit=None):
+    """One sequence's single token over all of k, v, checked with 16 bits of a probability."""
+    L = k.shape[0]
+    pool, table = _cache(k, v, seed)
+    if pool_edit:
+        pool_edit(pool, table)
+    t, n = table.int().to(DEV), torch.tensor([L], dtype=torch.int32, device=DEV)
+    out = ops.paged_decode_attention_kv8(q, pool, t, n, L, SCALE)
+    want, A = _rows(q, pool, table, L - 1)
+    _check(out, want, A, 16, L, _score_error(q, k), tag)
+    return out
+
+
+@pytest.mark.parametrize("L", [1, 2, 33, 512, 513, 4096, 70001])
+@pytest.mark.parametrize("H, Hkv", [(32, 4), (12, 4)])
+def test_decode_keeps_16_bits_of_a_probability(L, H, Hkv):
+    q, k, v = _normal(L, H, Hkv, L)
+    _decode(q[:1].to(torch.bfloat16).to(DEV), k.to(torch.bfloat16), v.to(torch.bfloat16), L, L)
+
+
+@pytest.mark.parametrize("L", [70, 600, 4100])
+@pytest.mark.parametrize("power", [-8, -13, -30, -60, -85])
+def test_decode_of_quiet_values_beside_rows_of_zeros(L, power):
+    q, k, v = _normal(L, 32, 4, L)
+    v *= 2.0 ** power
+    v[torch.arange(0, L, 3)] = 0.0
+
+    def empty_page(pool, table):
+        pool[table[0, 1]] = 0
+    _decode(q[:1].to(torch.bfloat16).to(DEV), k.to(torch.bfloat16), v.to(torch.bfloat16), L, (L, power), empty_page)
+
+
+@pytest.mark.parametrize("L", [70, 4100, 40000])
+@pytest.mark.parametrize("mag", [2.0 ** -92, 1e-20, 1e30, 1e36, 3e38])
+def test_decode_of_even_values_of_any_magnitude(L, mag):
+    """Sums of values, and of probabilities, that stay in fp32's range."""
+    q, k, v = _normal(L, 32, 4, L)
+    v = ((1 + 0.05 * v.clamp(-1, 1)) * (mag / 1.06)).to(torch.bfloat16)
+    _decode((0.1 * q[:1]).to(torch.bfloat16).to(DEV), k.to(torch.bfloat16), v, L, (L, mag))
+
+
+@pytest.mark.parametrize("power", [-90, -40, 40, 110])
+def test_decode_of_one_value_far_from_the_others(power):
+    L = 900
+    q, k, v = _normal(L, 32, 4, 4)
+    k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+    v[37] *= 2.0 ** power
+    for on in (False, True):  # (with the weight on it, and as one of many)
+        qq = (8 * k[37]).repeat_interleave(8, 0)[None] if on else q[:1].to(torch.bfloat16)
+        _decode(qq.to(torch.bfloat16).to(DEV), k, v, 4, (power, on))
