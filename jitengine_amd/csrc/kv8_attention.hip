@@ -562,8 +562,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8))) void k
         to_bf16(((const uint32_t *)&wv[i])[c], 1.0f, w[0], w[1]);
 #pragma unroll
         for (int j = 0; j < 2; j++)
-          r[2 * i + j] = pack_bf16x2(2 * j < keep[i] ? bf2f(w[j] & 0xffffu) * sp[2 * j] : 0.0f,
-                                     2 * j + 1 < keep[i] ? bf2f_hi(w[j]) * sp[2 * j + 1] : 0.0f);
+          r[2 * i + j] = pack_bf16x2_rne(2 * j < keep[i] ? bf2f(w[j] & 0xffffu) * sp[2 * j] : 0.0f,
+                                         2 * j + 1 < keep[i] ? bf2f_hi(w[j]) * sp[2 * j + 1] : 0.0f);
       }
       *v_out(c) = make_uint4(r[0], r[1], r[2], r[3]);
     }
@@ -786,8 +786,7 @@ void kv8_prefill_kernel(const PrefillArgs a) {
         const int i = 8 * (pg & 1) + 2 * j;
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[pg >> 1][i], a.qk_scale, off));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[pg >> 1][i + 1], a.qk_scale, off));
-        high.u[j] = pack_bf16x2(p0, p1);
-        rest.u[j] = pack_bf16x2(p0 - bf2f(high.u[j] & 0xffffu), p1 - bf2f_hi(high.u[j]));
+        split_bf16x2(p0, p1, high.u[j], rest.u[j]);
         l_run += p0 + p1;
       }
 #pragma unroll
