@@ -407,6 +407,10 @@ int jit_paged_decode_attn_noalloc(const uint16_t *q, const uint16_t *pool, const
  * pmax > 1 (JIT_EUNSUPPORTED).  Any context length. */
 int jit_prefill_block_tokens(int H, int Hkv);
 int jit_prefill_part_keys(void);
+/* The work items of C chunks (host arrays): blocks [3][n] blk_chunk, blk_q0, blk_part, those of the most 128-key steps
+ * first, then those that reach furthest, then in chunk order.  Returns their number (blocks NULL: that alone) or an
+ * error. */
+int jit_prefill_plan(const int32_t *ctx, const int32_t *len, int C, int H, int Hkv, int32_t *blocks, int n);
 /* Bytes of the partials' workspace: T * pmax * H * 132 * 4 when pmax > 1, 0 when pmax == 1,
  * -1 for T < 0, pmax < 1 or H <= 0. */
 long long jit_prefill_workspace_bytes(int T, int pmax, int H);

@@ -125,6 +125,7 @@ _SIGNATURES = {
     "jit_paged_decode_attn_kv8": [_P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, ctypes.c_int64, _P, _P],
     "jit_kv8_prefill_block_tokens": [_I, _I],
     "jit_kv8_prefill_part_units": [_I, _I, _I, _I],
+    "jit_prefill_plan": [_P, _P, _I, _I, _I, _P, _I],
     "jit_kv8_prefill_plan": [_P, _P, _I, _I, _I, _P, _P, _I],
     "jit_kv8_prefill_workspace_bytes": [_I, _I, _I, _I],
     "jit_paged_prefill_attn_kv8": [_P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I,

@@ -27,7 +27,9 @@
 // attn_merge_kernel combines in chunk order.
 #include "common.hpp"
 
+#include <algorithm>
 #include <mutex>
+#include <new>
 #include <type_traits>
 
 namespace {
@@ -1047,6 +1049,51 @@ extern "C" int jit_prefill_block_tokens(int H, int Hkv) {
 }
 
 extern "C" int jit_prefill_part_keys(void) { return kPfPartKeys; }
+
+namespace {
+struct PrefillItem {
+  int steps, keys, chunk, q0, part;
+};
+}  // namespace
+
+extern "C" int jit_prefill_plan(const int32_t *ctx, const int32_t *len, int C, int H, int Hkv, int32_t *blocks, int n) {
+  const int bt = jit_prefill_block_tokens(H, Hkv);
+  if (bt < 0)
+    return jit::fail(JIT_EUNSUPPORTED, "prefill_plan covers H / Hkv in {1, 2, 4, 8, 16}, got %d / %d", H, Hkv);
+  if (C < 0 || n < 0 || (C > 0 && (!ctx || !len))) return jit::fail(JIT_EINVAL, "prefill_plan: null pointer, C=%d or n=%d", C, n);
+  constexpr int kStep = 32 * kPfHalves;  // keys of a step
+  auto items = [&](auto &&f) {
+    for (int c = 0; c < C; c++)
+      for (int64_t q0 = 0; q0 < len[c]; q0 += bt) {
+        const int64_t keys = (int64_t)ctx[c] + std::min<int64_t>(q0 + bt, len[c]);
+        const int64_t steps = (keys + kStep - 1) / kStep;
+        for (int64_t s0 = 0; s0 < steps; s0 += kPfPartSteps)
+          f(PrefillItem{(int)std::min<int64_t>(steps - s0, kPfPartSteps), (int)keys, c, (int)q0, (int)(s0 / kPfPartSteps)});
+      }
+  };
+  for (int c = 0; c < C; c++)
+    if (ctx[c] < 0 || len[c] < 1 || (int64_t)ctx[c] + len[c] > 0x7fffffff)
+      return jit::fail(JIT_EINVAL, "prefill_plan: chunk %d of %d rows after %d", c, len[c], ctx[c]);
+  int64_t total = 0;
+  items([&](const PrefillItem &) { total++; });
+  if (total > 0x7fffffff) return jit::fail(JIT_EUNSUPPORTED, "prefill_plan: %lld work items", (long long)total);
+  if (!blocks || total == 0) return (int)total;
+  if (n != total) return jit::fail(JIT_EINVAL, "prefill_plan: %d work items, %lld needed", n, (long long)total);
+  PrefillItem *list = new (std::nothrow) PrefillItem[total];
+  if (!list) return jit::fail(JIT_EINVAL, "prefill_plan: no memory for %lld work items", (long long)total);
+  int64_t at = 0;
+  items([&](const PrefillItem &it) { list[at++] = it; });
+  std::sort(list, list + total, [](const PrefillItem &a, const PrefillItem &b) {
+    if (a.steps != b.steps) return a.steps > b.steps;
+    if (a.keys != b.keys) return a.keys > b.keys;
+    if (a.chunk != b.chunk) return a.chunk < b.chunk;
+    return a.q0 != b.q0 ? a.q0 < b.q0 : a.part < b.part;
+  });
+  for (int64_t i = 0; i < total; i++)
+    blocks[i] = list[i].chunk, blocks[total + i] = list[i].q0, blocks[2 * total + i] = list[i].part;
+  delete[] list;
+  return (int)total;
+}
 
 extern "C" long long jit_prefill_workspace_bytes(int T, int pmax, int H) {
   if (T < 0 || pmax < 1 || H <= 0) return -1;

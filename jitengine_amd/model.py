@@ -159,7 +159,7 @@ def make_mixed_state(cfg: MoEConfig, chunks, seq_table_host, dec_pos_host, dec_t
         P = int(new[:C].sum())
         t = ops.step_tables(up[n:n + C + D], up[n + C + D:], table, P + D)
         ws = torch.empty(ops.kv8_decode_workspace_bytes(D, cfg.heads, max_len), dtype=torch.uint8, device=device)
-        plan = ops.prefill_plan([(i, c[1], c[2]) for i, c in enumerate(chunks)], cfg.heads, cfg.kv_heads, device)
+        plan = ops.prefill_plan([(i, c[1], c[2]) for i, c in enumerate(chunks)], cfg.heads, cfg.kv_heads, device, kv8=True)
         return MixedState(P, t.pos, None, table[:C], plan, table[C:], None, ws, t, max_len)
     pos, rows = [], []
     for seq, ctx, length in chunks:
@@ -174,7 +174,8 @@ def make_mixed_state(cfg: MoEConfig, chunks, seq_table_host, dec_pos_host, dec_t
                      device=device)
     # (pinned, asynchronous uploads: the host does not wait for the steps still queued)
     return MixedState(P, ops.upload(pos_rows, device), ops.upload(table_rows, device),
-                      ops.upload(seq_table_host, device), ops.prefill_plan(chunks, cfg.heads, cfg.kv_heads, device),
+                      ops.upload(seq_table_host, device),
+                      ops.prefill_plan(chunks, cfg.heads, cfg.kv_heads, device, kv8=False),
                       ops.upload(dec_table_host, device), dplan, ws)
 
 

@@ -652,7 +652,7 @@ class PrefillPlan:
 
     chunks: list
     tables: torch.Tensor  # [4, C] chunk_seq, chunk_ctx, chunk_len, chunk_row
-    blocks: torch.Tensor  # [3, nblk] blk_chunk, blk_q0, blk_part
+    blocks: torch.Tensor | None  # [3, nblk] blk_chunk, blk_q0, blk_part (None: a plan for 8-bit pools alone)
     rows: int
     pmax: int = 1  # most key parts of a token (jit_prefill_part_keys keys a part)
     max_len: int = 0  # the longest chunk
@@ -670,19 +670,17 @@ class Kv8Chunks:
     heads: tuple          # (H, Hkv)
 
 
-def prefill_plan(chunks, H: int, Hkv: int, device) -> PrefillPlan:
+def prefill_plan(chunks, H: int, Hkv: int, device, kv8: bool | None = None) -> PrefillPlan:
     """Plan of causal prefill attention over chunks [(seq, ctx, length), ...]: every chunk cut
     into row blocks of jit_prefill_block_tokens tokens, each block's keys cut at multiples of
-    jit_prefill_part_keys, one work item per (block, part), the items with the most key steps first; and the blocks and
-    parts of an 8-bit pool (jit_kv8_prefill_plan)."""
+    jit_prefill_part_keys, one work item per (block, part), the items with the most key steps first
+    (jit_prefill_plan); and the blocks and parts of an 8-bit pool (jit_kv8_prefill_plan).  kv8: False
+    plans for a bf16 pool alone, True for an 8-bit one, None for either."""
     lib = _lib.lib()
-    bt = int(lib.jit_prefill_block_tokens(H, Hkv))
-    if bt <= 0:
+    if int(lib.jit_prefill_block_tokens(H, Hkv)) <= 0:
         raise _lib.UnsupportedShape(f"prefill attention covers H / Hkv in (1, 2, 4, 8, 16), got {H}/{Hkv}")
     part_keys = int(lib.jit_prefill_part_keys())
-    step = 128
-    part_steps = part_keys // step
-    rows, tab, items, pmax, max_len = 0, [], [], 1, 0
+    rows, tab, pmax, max_len = 0, [], 1, 0
     for c, (seq, ctx, length) in enumerate(chunks):
         if seq < 0 or ctx < 0 or length < 1:
             raise ValueError(f"chunk {c}: seq {seq}, ctx {ctx}, length {length}")
@@ -690,27 +688,32 @@ def prefill_plan(chunks, H: int, Hkv: int, device) -> PrefillPlan:
         rows += length
         max_len = max(max_len, length)
         pmax = max(pmax, (ctx + length - 1) // part_keys + 1)
-        for q0 in range(0, length, bt):
-            keys = ctx + min(q0 + bt, length)
-            nst = (keys + step - 1) // step
-            for p in range((nst - 1) // part_steps + 1):
-                items.append((min(nst, (p + 1) * part_steps) - p * part_steps, keys, c, q0, p))
-    items.sort(key=lambda it: (-it[0], -it[1]))
-    C, n = len(tab), len(items)
-    head = 4 * C + 3 * (C + 1)
-    buf = np.empty(head, np.int32)
+    # one upload, whose views the tables are: [4, C] chunks, [3, C + 1] of the 8-bit pool, then both lists of items
+    C = len(tab)
+    top = 4 * C + (3 * (C + 1) if kv8 is not False else 0)
+    head = np.empty(top, np.int32)
     if C:
-        buf[:4 * C] = np.array(tab, np.int32).T.reshape(-1)
-    at = buf.ctypes.data
-    args = at + 4 * C, at + 8 * C, C, H, Hkv, at + 16 * C
-    n8 = _lib.check(lib.jit_kv8_prefill_plan(*args, None, 0), "kv8_prefill_plan")
-    blk8 = np.empty(3 * n8, np.int32)
-    _lib.check(lib.jit_kv8_prefill_plan(*args, blk8.ctypes.data, n8), "kv8_prefill_plan")
-    # one upload; the tables are views of it
-    blk = np.array([it[2:] for it in items], np.int32).T.reshape(-1) if n else np.empty(0, np.int32)
-    t, t8, b, b8 = upload(np.concatenate([buf, blk, blk8]), device).split([4 * C, 3 * (C + 1), 3 * n, 3 * n8])
-    return PrefillPlan(list(chunks), t.view(4, C), b.view(3, n), rows, pmax, max_len,
-                       Kv8Chunks(t8.view(3, C + 1), b8.view(3, n8), int(buf[5 * C]), int(buf[head - 1]), (H, Hkv)))
+        head[:4 * C].reshape(4, C).T[:] = tab
+    at, n, n8 = head.ctypes.data, 0, 0
+    ctx_at, len_at = at + 4 * C, at + 8 * C
+    if not kv8:
+        n = _lib.check(lib.jit_prefill_plan(ctx_at, len_at, C, H, Hkv, None, 0), "prefill_plan")
+    if kv8 is not False:
+        n8 = _lib.check(lib.jit_kv8_prefill_plan(ctx_at, len_at, C, H, Hkv, at + 16 * C, None, 0), "kv8_prefill_plan")
+    buf = np.empty(top + 3 * (n + n8), np.int32)
+    to = buf.ctypes.data + 4 * top
+    if n:
+        _lib.check(lib.jit_prefill_plan(ctx_at, len_at, C, H, Hkv, to, n), "prefill_plan")
+    if n8:
+        _lib.check(lib.jit_kv8_prefill_plan(ctx_at, len_at, C, H, Hkv, at + 16 * C, to + 12 * n, n8), "kv8_prefill_plan")
+    buf[:top] = head
+    dev = upload(buf, device)
+    blocks = None if kv8 else dev.as_strided((3, n), (n, 1), top)
+    p8 = None
+    if kv8 is not False:
+        p8 = Kv8Chunks(dev.as_strided((3, C + 1), (C + 1, 1), 4 * C), dev.as_strided((3, n8), (n8, 1), top + 3 * n),
+                       int(head[5 * C]), int(head[-1]), (H, Hkv))
+    return PrefillPlan(list(chunks), dev.as_strided((4, C), (C, 1), 0), blocks, rows, pmax, max_len, p8)
 
 
 def prefill_workspace_bytes(plan: PrefillPlan, H: int) -> int:
@@ -738,6 +741,8 @@ def paged_prefill_attention(q: torch.Tensor, pool: torch.Tensor, page_table: tor
         raise _lib.UnsupportedShape(f"paged_prefill_attention covers head_dim 128, got {Dh}")
     if T != plan.rows:
         raise ValueError(f"q has {T} rows, the plan's chunks {plan.rows}")
+    if plan.blocks is None:
+        raise ValueError("the plan has no row blocks for a bf16 pool (prefill_plan makes them without kv8=True)")
     prefill_contract(plan, page_table)
     need = prefill_workspace_bytes(plan, H)
     if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
@@ -1033,7 +1038,7 @@ def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table:
     given) that the chunks' keys are expanded into."""
     tb, p8 = plan.tables, plan.kv8
     if p8 is None:
-        raise ValueError("the plan has no row blocks for an 8-bit pool (prefill_plan makes them)")
+        raise ValueError("the plan has no row blocks for an 8-bit pool (prefill_plan makes them without kv8=False)")
     dev = _take((q, torch.bfloat16, "q"), (pool, torch.uint8, "pool"), (page_table, torch.int32, "page_table"),
                 (tb, torch.int32, "plan"), (p8.tables, torch.int32, "plan"), (p8.blocks, torch.int32, "plan"))
     Hkv = _kv8_heads(pool)
