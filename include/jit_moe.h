@@ -576,7 +576,8 @@ int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, int num_pages
  *   chunk_part  the units of each chunk's key parts, jit_kv8_prefill_part_units of its ctx and len;
  *   chunk_slot  first partial slot of each chunk, len x its parts in a chunk of more than one; their number `slots` last.
  * Work items: (blk_chunk, blk_q0, blk_part) for every jit_kv8_prefill_block_tokens tokens of a chunk and every part that
- * holds keys of theirs, in any order.  max_len: the longest chunk.  Keys of page ids outside the pool are left out; a row
+ * holds keys of theirs, in any order; an item, unit or slot that is not the chunks' is left out, and the rows it was for with
+ * it.  max_len: the longest chunk.  Keys of page ids outside the pool are left out; a row
  * without a key gives zeros.  A row's bits depend on its sequence and its chunk's ctx and len alone.
  * Contract: H / Hkv in {1, 2, 4, 8, 16} (JIT_EUNSUPPORTED), scale > 0, a workspace of jit_kv8_prefill_workspace_bytes
  * bytes (32,776 bytes a unit and kv head, and the partials) (JIT_EINVAL). */

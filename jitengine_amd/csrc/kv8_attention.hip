@@ -448,9 +448,19 @@ struct PrefillArgs {
   int32_t *info;   // [units][Hkv][2]: E of the unit's part, its pages outside the pool (4 bits; 16: some in the part;
                    // 32: NaN codes of V in the unit; 64: the part's V scales are more than 2^kSpread apart)
   float *part;     // (token, part, head): o / sum, the maximum, the sum
-  int num_pages, max_pages, H, Hkv, G, C;
+  int num_pages, max_pages, H, Hkv, G, C, num_units, num_slots;
   float qk_scale;
 };
+
+// The tables of the units, parts, slots and work items come from the caller's device memory: an entry that does not
+// belong to these chunks is left out here, before it becomes an address.
+// first slot of token t's partials (-1: not its chunk's)
+__device__ __forceinline__ long long first_slot(const PrefillArgs &a, int ch, int part_units, int t, int parts) {
+  const uint32_t units = (uint32_t)a.chunk_unit[ch + 1] - (uint32_t)a.chunk_unit[ch];
+  const uint32_t most = (units + (uint32_t)part_units - 1u) / (uint32_t)part_units;
+  const long long s = a.chunk_slot[ch] + (long long)t * most;
+  return most >= (uint32_t)parts && s >= 0 && s + parts <= a.num_slots ? s : -1;
+}
 
 // One workgroup expands a unit of one kv head, wave w its page w: 10,240 keys of 4 heads, 11 MB to 21 MB, in 14 to 18 us, most of
 // it the latency of its part's scales (parts of 96 units: 11 us).  Its codes are requested first; meanwhile the part's
@@ -466,10 +476,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8))) void k
     else hi = mid - 1;
   }
   const int u = gu - a.chunk_unit[lo], kend = a.chunk_ctx[lo] + a.chunk_len[lo];
+  if (u < 0 || u > (kend - 1) / kUnitKeys) return;  // (uniform: no such unit of a chunk)
   const int32_t *prow = a.page_table + (long long)a.chunk_seq[lo] * a.max_pages;
   const int npages = min((kend + kPage - 1) / kPage, a.max_pages);
   // the part's pages
-  const int part = min(a.chunk_part[lo], kPartMax), pg0 = u / part * part * kUnitPages;
+  const int part = min(max(a.chunk_part[lo], 1), kPartMax), pg0 = u / part * part * kUnitPages;
   const int np = min(part * kUnitPages, npages - pg0);
   for (int i = threadIdx.x; i < np; i += 256) s_ids[i] = prow[pg0 + i];
   // this wave's page
@@ -602,15 +613,19 @@ void kv8_prefill_kernel(const PrefillArgs a) {
   __shared__ __attribute__((aligned(16))) uint4 s_k[kStages][16][64];              // [page pair, 16 dims][lane] 8 bf16
   __shared__ __attribute__((aligned(16))) uint4 s_v[kStages][kUnitPages * 4][64];  // [page, 32 dims][lane] 8 fp16
   const int item = blockIdx.x / a.Hkv, kvh = blockIdx.x % a.Hkv;
-  const int ch = a.blk_chunk[item], q0 = a.blk_q0[item], part = a.blk_part[item], part_units = a.chunk_part[ch];
+  const int ch = a.blk_chunk[item], q0 = a.blk_q0[item], part = a.blk_part[item];
+  if (ch < 0 || ch >= a.C || q0 < 0 || part < 0) return;  // (uniform, as below)
+  const int part_units = a.chunk_part[ch], unit0 = a.chunk_unit[ch];  // (loads on one trip to memory)
   const int ctx = a.chunk_ctx[ch], len = a.chunk_len[ch], row0 = a.chunk_row[ch];
   const int G = a.G, tpw = kRowsWave / G;  // tokens a wave
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
   const int lr = l & 31, lh = l >> 5;
   const int kend = ctx + min(q0 + kPfWaves * tpw, len);  // the workgroup's keys: [0, kend)
-  const int u0 = part * part_units, u1 = min((kend + kUnitKeys - 1) / kUnitKeys, u0 + part_units);
-  if (q0 >= len || u0 >= u1) return;  // (uniform: no such item in a plan)
-  const long long first_unit = (long long)a.chunk_unit[ch] * a.Hkv + kvh;  // (units of a head lie Hkv apart)
+  const int all = (kend + kUnitKeys - 1) / kUnitKeys;
+  if ((q0 >= len) | (unit0 < 0) | (all > a.num_units - unit0) | (part_units < 1) | (part_units > kPartMax)) return;
+  if ((long long)part * part_units >= all) return;  // (no such item)
+  const int u0 = part * part_units, u1 = min(all, u0 + part_units);
+  const long long first_unit = (long long)unit0 * a.Hkv + kvh;  // (units of a head lie Hkv apart)
   const uint8_t *units = a.units + first_unit * kUnitBytes;
   const int32_t *info = a.info + 2 * first_unit;
   const uint32_t k_lds = __builtin_amdgcn_readfirstlane(
@@ -862,8 +877,9 @@ void kv8_prefill_kernel(const PrefillArgs a) {
         *(uint2 *)(a.out + hrow * kD + 32 * c + 8 * i + 4 * lh) = w;
       }
   } else {
-    const int most = (a.chunk_unit[ch + 1] - a.chunk_unit[ch] + part_units - 1) / part_units;
-    float *ps = a.part + ((a.chunk_slot[ch] + (long long)tok * most + part) * a.H + kvh * G + lr % G) * kPfSlot;
+    const long long slot0 = first_slot(a, ch, part_units, tok, parts);
+    if (slot0 < 0) return;
+    float *ps = a.part + ((slot0 + part) * a.H + kvh * G + lr % G) * kPfSlot;
 #pragma unroll
     for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -880,10 +896,13 @@ void kv8_prefill_kernel(const PrefillArgs a) {
 __global__ __launch_bounds__(128) void kv8_prefill_merge_kernel(const PrefillArgs a) {
   const int c = blockIdx.y, t = blockIdx.x, h = 16 * blockIdx.z + (threadIdx.x >> 3);
   if (t >= a.chunk_len[c] || h >= a.H) return;
-  const int pu = a.chunk_part[c], parts = (a.chunk_ctx[c] + t) / (kUnitKeys * pu) + 1;
+  const int pu = a.chunk_part[c], d0 = 4 * (threadIdx.x & 7);
+  if (pu < 1 || pu > kPartMax) return;
+  const int parts = (a.chunk_ctx[c] + t) / (kUnitKeys * pu) + 1;
   if (parts < 2) return;
-  const int most = (a.chunk_unit[c + 1] - a.chunk_unit[c] + pu - 1) / pu, d0 = 4 * (threadIdx.x & 7);
-  const float *first = a.part + ((a.chunk_slot[c] + (long long)t * most) * a.H + h) * kPfSlot;
+  const long long slot0 = first_slot(a, c, pu, t, parts);
+  if (slot0 < 0) return;
+  const float *first = a.part + (slot0 * a.H + h) * kPfSlot;
   float M = kLowest, ls = 0.0f, O[16];
 #pragma unroll
   for (int i = 0; i < 16; i++) O[i] = 0.0f;
@@ -1084,7 +1103,7 @@ extern "C" int jit_paged_prefill_attn_kv8(const uint16_t *q, const void *pool, i
   int32_t *info = (int32_t *)(ws + (int64_t)units * Hkv * kUnitBytes);
   const PrefillArgs a{q, (const uint8_t *)pool, page_table, blk_chunk, blk_q0, blk_part, chunk_seq, chunk_ctx, chunk_len,
                       chunk_row, chunk_unit, chunk_part, chunk_slot, out, ws, info,
-                      (float *)(ws + units_bytes(units, Hkv)), num_pages, max_pages, H, Hkv, H / Hkv, C,
+                      (float *)(ws + units_bytes(units, Hkv)), num_pages, max_pages, H, Hkv, H / Hkv, C, units, slots,
                       scale * 1.44269504088896341f};
   const hipStream_t st = (hipStream_t)stream;
   kv8_expand_kernel<<<dim3(units, Hkv), 256, 0, st>>>(a);

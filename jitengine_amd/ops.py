@@ -1031,6 +1031,22 @@ def kv8_prefill_workspace_bytes(plan: PrefillPlan, H: int, Hkv: int) -> int:
     return int(_lib.lib().jit_kv8_prefill_workspace_bytes(int(H), int(Hkv), plan.kv8.units, plan.kv8.slots))
 
 
+def kv8_plan_contract(plan: PrefillPlan) -> None:
+    """A plan put together from its parts: the 8-bit pool's tables have the sizes that the plan's chunks give
+    (ValueError)."""
+    C, p8 = len(plan.chunks), plan.kv8
+    if plan.rows != sum(c[2] for c in plan.chunks) or plan.max_len != max([c[2] for c in plan.chunks] + [0]):
+        raise ValueError("the plan's rows or longest chunk are not its chunks'")
+    host = np.array([[c[1] for c in plan.chunks], [c[2] for c in plan.chunks]], np.int32)
+    tables = np.empty((3, C + 1), np.int32)
+    n = _lib.check(_lib.lib().jit_kv8_prefill_plan(host.ctypes.data, host.ctypes.data + 4 * C, C, *p8.heads,
+                                                   tables.ctypes.data, None, 0), "kv8_prefill_plan")
+    want = ((4, C), (3, C + 1), (3, n), int(tables[0, C]), int(tables[2, C]))
+    got = (tuple(plan.tables.shape), tuple(p8.tables.shape), tuple(p8.blocks.shape), p8.units, p8.slots)
+    if got != want:
+        raise ValueError(f"the plan's tables, blocks, units and slots {got} are not those of its chunks, {want}")
+
+
 def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, plan: PrefillPlan,
                                 scale: float, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """q [T, H, 128] bf16 (the plan's chunk rows) -> out [T, H, 128]: paged_prefill_attention over an 8-bit pool

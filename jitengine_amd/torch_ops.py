@@ -387,9 +387,12 @@ def paged_prefill_attention_kv8(q: torch.Tensor, pool: torch.Tensor, page_table:
                                 slots: int, scale: float, workspace: torch.Tensor) -> torch.Tensor:
     """out bf16 [T, H, 128]: paged_prefill_attention over an 8-bit pool (jit_paged_prefill_attn_kv8; the plan by
     kv8_prefill_plan_args, workspace of kv8_prefill_workspace_bytes bytes)."""
+    if len(chunks) % 3:
+        raise ValueError(f"chunks are (seq, ctx, length) triples, got {len(chunks)} numbers")
     trip = [tuple(chunks[i:i + 3]) for i in range(0, len(chunks), 3)]
     p8 = ops.Kv8Chunks(chunk_tables, blocks, int(units), int(slots), (q.shape[1], pool.shape[1]))
     plan = ops.PrefillPlan(trip, tables, blocks, sum(c[2] for c in trip), 1, max([c[2] for c in trip] + [0]), p8)
+    ops.kv8_plan_contract(plan)
     return ops.paged_prefill_attention_kv8(q, pool, page_table, plan, scale, workspace)
 
 

@@ -87,3 +87,34 @@ def test_a_plan_serves_the_pools_that_it_is_made_for():
         run(q, pool, table, plans[True], 0.1)
     with pytest.raises(ValueError, match="no row blocks for an 8-bit pool"):
         run8(q, pool8, table, plans[False], 0.1)
+
+
+def test_the_registered_operator_refuses_tables_of_another_plan():
+    """Its plan comes as tensors and numbers; what they are sized for has to be the chunks."""
+    from jitengine_amd import torch_ops
+
+    H, Hkv, chunks = 32, 4, [(0, 3000, 9), (1, 0, 400)]
+    T = sum(n for *_, n in chunks)
+    q, pool, table = torch.zeros((T, H, 128), dtype=torch.bfloat16), ops.kv8_pool(2, Hkv, "cpu"), torch.zeros((2, 200), dtype=torch.int32)
+    plan = ops.prefill_plan(chunks, H, Hkv, "cpu")
+    assert plan.kv8.slots > 0
+    ws = torch.empty(16, dtype=torch.uint8)
+    args = dict(zip(("tables", "chunk_tables", "blocks", "chunks", "units", "slots"), torch_ops.kv8_prefill_plan_args(plan)))
+    call = lambda **other: torch.ops.jitengine.paged_prefill_attention_kv8(  # noqa: E731
+        q, pool, table, *{**args, **other}.values(), 0.1, ws)
+    ops.kv8_plan_contract(plan)
+    with pytest.raises(ValueError, match="device tensor"):  # (the plan passes; the tensors here are the host's)
+        call()
+    for other in (
+        {"units": plan.kv8.units + 1}, {"units": 1}, {"slots": 0}, {"slots": plan.kv8.slots - 1}, {"slots": -1},
+        {"blocks": plan.kv8.blocks[:, :-1].contiguous()}, {"blocks": plan.kv8.blocks[:2].contiguous()},
+        {"blocks": plan.blocks}, {"chunk_tables": plan.kv8.tables[:, :-1].contiguous()},
+        {"chunk_tables": plan.tables}, {"tables": plan.tables[:, :1].contiguous()}, {"chunks": [0, 3000, 9]},
+        {"chunks": [0, 3000, 9, 1, 0, 401]}, {"chunks": [0, 6000, 9, 1, 0, 400]}, {"chunks": []},
+    ):
+        with pytest.raises(ValueError, match="the plan's tables"):
+            call(**other)
+    with pytest.raises(ValueError, match="triples"):
+        call(chunks=[0, 3000, 9, 1])
+    with pytest.raises(ValueError):
+        call(chunks=[0, 3000, 9, 1, 0, 0])
