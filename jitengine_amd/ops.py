@@ -929,6 +929,11 @@ def step_tables(ctx: torch.Tensor, new: torch.Tensor, page_table: torch.Tensor, 
     more, built on the device in one launch (jit_step_tables).  With `free` (int32 page ids) page_table grows in
     place: each sequence's new pages come from the list in sequence order, from index free_at[0] on (0 without).  A
     sequence that does not fit its table, the `rows` or the list is refused (slots -1, lens = ctx; status counts them)."""
+    return _step_tables(ctx, new, page_table, rows, free, free_at, False)
+
+
+def _step_tables(ctx, new, page_table, rows, free, free_at, apart: bool) -> StepTables:
+    """step_tables into views of one allocation, or (apart) into six of their own."""
     i32 = torch.int32
     dev = _take((ctx, i32, "ctx"), (new, i32, "new"), (page_table, i32, "page_table"), (free, i32, "free"),
                 (free_at, i32, "free_at"))
@@ -942,14 +947,19 @@ def step_tables(ctx: torch.Tensor, new: torch.Tensor, page_table: torch.Tensor, 
         raise ValueError("free_at is one index into free")
     if rows < 0 or rows >= 1 << 29:
         raise ValueError(f"rows must lie in [0, 2^29), got {rows}")
-    buf = torch.empty(2 * S + 5 + 3 * rows, dtype=i32, device=ctx.device)
-    at = buf.data_ptr()
-    p_seq = at + 4 * (S + 1)
-    p_len = p_seq + 12 * rows
+    sizes = [S + 1, rows, rows, rows, S, 4]
+    if apart:
+        out = [ctx.new_empty((n,)) for n in sizes]
+        to = [t.data_ptr() for t in out]
+    else:
+        buf = torch.empty(2 * S + 5 + 3 * rows, dtype=i32, device=ctx.device)
+        at = buf.data_ptr()
+        p_seq = at + 4 * (S + 1)
+        p_len = p_seq + 12 * rows
+        to = at, p_seq, p_seq + 4 * rows, p_seq + 8 * rows, p_len, p_len + 4 * S
     _launch(dev, _lib.lib().jit_step_tables, "step_tables", ctx.data_ptr(), new.data_ptr(), S, page_table.data_ptr(),
-            page_table.shape[1], rows, _ptr(free), -1 if free is None else free.numel(), _ptr(free_at), at, p_seq,
-            p_seq + 4 * rows, p_seq + 8 * rows, p_len, p_len + 4 * S)
-    return StepTables(*buf.split_with_sizes([S + 1, rows, rows, rows, S, 4]))
+            page_table.shape[1], rows, _ptr(free), -1 if free is None else free.numel(), _ptr(free_at), *to)
+    return StepTables(*(out if apart else buf.split_with_sizes(sizes)))
 
 
 def kv8_append_paged(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:

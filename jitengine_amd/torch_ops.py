@@ -332,9 +332,9 @@ def step_tables(ctx: torch.Tensor, new: torch.Tensor, page_table: torch.Tensor, 
                 free_at: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
                                                        torch.Tensor, torch.Tensor]:
     """(row_start, row_seq, pos, slots, lens, status) of a step (jit_step_tables; page_table grows with `free`)."""
-    t = ops.step_tables(ctx, new, page_table, rows, free, free_at)
     # (six tensors of their own: an operator's outputs share no storage)
-    return tuple(x.clone() for x in (t.row_start, t.row_seq, t.pos, t.slots, t.lens, t.status))
+    t = ops._step_tables(ctx, new, page_table, rows, free, free_at, True)
+    return t.row_start, t.row_seq, t.pos, t.slots, t.lens, t.status
 
 
 @step_tables.register_fake

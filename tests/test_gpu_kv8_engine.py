@@ -196,3 +196,17 @@ def test_registered_operators_equal_the_library_calls():
     assert {op._qualified_op_name.split("::")[1] for op, _ in cases} == set(torch_ops.OPS_KV8)
     for op, op_args in cases:
         torch.library.opcheck(op, op_args)
+
+
+def test_the_registered_step_tables_is_one_launch():
+    """Into outputs of their own: no copies after it."""
+    ctx, new, table = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([3, 40], [5, 1], [[0, 1, 2], [3, 4, 5]]))
+    J = torch.ops.jitengine
+    got = J.step_tables(ctx, new, table, 6, None, None)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        got = J.step_tables(ctx, new, table, 6, None, None)
+        torch.cuda.synchronize()
+    names = [e.key for e in prof.key_averages() for _ in range(e.count) if e.self_device_time_total > 0]
+    assert len(names) == 1 and "step_tables_kernel" in names[0], names
+    assert len({t.untyped_storage().data_ptr() for t in got}) == 6
+    assert got[3].tolist() == [3, 4, 5, 6, 7, 16 * 5 + 8] and got[4].tolist() == [8, 41]
