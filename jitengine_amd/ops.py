@@ -693,7 +693,7 @@ def prefill_plan(chunks, H: int, Hkv: int, device, kv8: bool | None = None) -> P
     top = 4 * C + (3 * (C + 1) if kv8 is not False else 0)
     head = np.empty(top, np.int32)
     if C:
-        head[:4 * C].reshape(4, C).T[:] = tab
+        head[:4 * C] = np.array(tab, np.int32).T.reshape(-1)
     at, n, n8 = head.ctypes.data, 0, 0
     ctx_at, len_at = at + 4 * C, at + 8 * C
     if not kv8:

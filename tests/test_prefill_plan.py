@@ -59,6 +59,9 @@ def test_what_a_plan_refuses():
             ops.prefill_plan([(0, 0, 5), chunk], 32, 4, "cpu")
     with pytest.raises(_lib.UnsupportedShape, match="H / Hkv"):
         ops.prefill_plan([(0, 0, 5)], 24, 8, "cpu", kv8=False)
+    for chunk in ((0, 2 ** 32 + 5, 1), (2 ** 32, 0, 1)):  # (not what is left of it in 32 bits)
+        with pytest.raises(OverflowError):
+            ops.prefill_plan([chunk], 32, 4, "cpu")
     a, b, out = (np.array(x, np.int32) for x in ([0, 9], [5, 300], [0] * 99))
     call = lambda ctx, n, C=2, H=32, to=None, m=0: _lib.lib().jit_prefill_plan(  # noqa: E731
         ctx.ctypes.data if ctx is not None else None, n.ctypes.data if n is not None else None, C, H, 4,
