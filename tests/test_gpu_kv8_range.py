@@ -244,6 +244,21 @@ def test_decode_of_even_values_of_any_magnitude(L, mag):
     _decode((0.1 * q[:1]).to(torch.bfloat16).to(DEV), k.to(torch.bfloat16), v, L, (L, mag))
 
 
+@pytest.mark.parametrize("L", [1, 40, 700])
+@pytest.mark.parametrize("mag", [-1e30, -1e33, 1e33])
+def test_decode_of_scores_of_any_magnitude(L, mag):
+    """Keys that are all alike have the same weight, whatever their score."""
+    q, k, v = _normal(L, 32, 4, L)
+    k = torch.full((L, 4, 128), 2.0 ** 50).to(torch.bfloat16)
+    q = torch.full((1, 32, 128), mag / 2.0 ** 50).to(torch.bfloat16).to(DEV)  # (scores about 11 mag)
+    v = v.to(torch.bfloat16)
+    pool, table = _cache(k, v, L)
+    out = ops.paged_decode_attention_kv8(q, pool, table.int().to(DEV), torch.tensor([L], dtype=torch.int32, device=DEV), L, SCALE)
+    _, held = ref.read(pool, table[0].to(DEV))
+    held = held[:, :L].repeat_interleave(8, 0)
+    _check(out, held.mean(1)[None], held.abs().mean(1)[None], 16, L, 0.0, (L, mag))
+
+
 @pytest.mark.parametrize("power", [-90, -40, 40, 110])
 def test_decode_of_one_value_far_from_the_others(power):
     L = 900
