@@ -8,9 +8,10 @@
 //                 keys in each of 4 output tiles.
 //   [4096, 4224)  fp32 scales, K of the 16 slots, then V: one line, read as the float4 of a lane's 4 keys.
 // A block is one token of one kv head (K and V apart).  Tokens arrive one at a time: a longer block would be rounded
-// again whenever a louder token joins it, and a row's bits would depend on how its prompt was cut.  Its scale is a
-// power of two: e4m3 keeps its relative precision at any scale, code x scale is exact in bf16, and the
-// conversions that take a power of two apply it for nothing.
+// again whenever a louder token joins it, and what the cache holds of given k and v would depend on how they arrived.
+// (Attention's own bits are another matter: a prompt chunk's key parts are chosen by the chunk.)  Its scale is a power
+// of two: e4m3 keeps its relative precision at any scale, code x scale is exact in bf16, and the conversions that take a
+// power of two apply it for nothing.
 #pragma once
 
 #include "common.hpp"

@@ -268,3 +268,18 @@ def test_decode_of_one_value_far_from_the_others(power):
     for on in (False, True):  # (with the weight on it, and as one of many)
         qq = (8 * k[37]).repeat_interleave(8, 0)[None] if on else q[:1].to(torch.bfloat16)
         _decode(qq.to(torch.bfloat16).to(DEV), k, v, 4, (power, on))
+
+
+def test_rows_of_a_chunk_in_parts_are_those_of_a_larger_chunk():
+    """16 rows after 8,000 keys are cut into parts, the same rows inside a chunk of 1,016 into others: the bits may
+    differ, the values do not."""
+    H, Hkv, L, n, more = 32, 4, 8016, 16, 1016
+    q, k, v = _normal(L, H, Hkv, 6)
+    q, k, v = q[:more].to(torch.bfloat16).to(DEV), k.to(torch.bfloat16), v.to(torch.bfloat16)
+    pool, table = _cache(k, v)
+    whole, wide = _prompt(q, pool, table, L - more)
+    last, cut = _prompt(q[-n:].contiguous(), pool, table, L - n)
+    assert int(cut.kv8.tables[1, 0]) != int(wide.kv8.tables[1, 0])  # (keys of a part)
+    want, A = _rows(q[-n:], pool, table, L - n)
+    for got in (last, whole[-n:]):
+        _check(got, want, A, 11, L, _score_error(q, k), "cut")
