@@ -562,8 +562,8 @@ int64_t jit_kv8_decode_workspace_bytes(int B, int H, int max_len);
 
 /* Paged GQA decode attention over an 8-bit pool, one query per row: out[b, h] = softmax(scale * q[b, h] . K_b^T) .
  * V_b over the first lens[b] tokens (device values; at most max_len and 16 max_pages count) of the values the cache
- * holds.  No keys: zeros.  Keys of page ids outside the pool are left out; what the other slots of a page hold does
- * not matter.  q, out [B, H, 128] bf16; page_table [B, max_pages].
+ * holds, of any magnitude.  No keys: zeros.  Keys of page ids outside the pool are left out; what the other slots of a
+ * page hold does not matter.  A probability keeps 16 bits.  q, out [B, H, 128] bf16; page_table [B, max_pages].
  * Contract: H % Hkv == 0 (JIT_EINVAL), H / Hkv <= 16 (JIT_EUNSUPPORTED). */
 int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, int num_pages, const int32_t *page_table,
                               int max_pages, const int32_t *lens, int B, int H, int Hkv, int max_len, float scale,
@@ -576,9 +576,11 @@ int jit_paged_decode_attn_kv8(const uint16_t *q, const void *pool, int num_pages
  *   chunk_part  the units of each chunk's key parts, jit_kv8_prefill_part_units of its ctx and len;
  *   chunk_slot  first partial slot of each chunk, len x its parts in a chunk of more than one; their number `slots` last.
  * Work items: (blk_chunk, blk_q0, blk_part) for every jit_kv8_prefill_block_tokens tokens of a chunk and every part that
- * holds keys of theirs, in any order; an item, unit or slot that is not the chunks' is left out, and the rows it was for with
- * it.  max_len: the longest chunk.  Keys of page ids outside the pool are left out; a row
- * without a key gives zeros.  A row's bits depend on its sequence and its chunk's ctx and len alone.
+ * holds keys of theirs, in any order; an item, unit or slot that is not its chunk's is left out, and the rows it was for
+ * are not defined.  max_len: the longest chunk.  Keys of page ids outside the pool are left out; a row without a key
+ * gives zeros.  A row's bits depend on its sequence and its chunk's ctx and len alone.  Values may have any magnitude; a
+ * probability keeps 11 bits, or 16 in the key parts whose V scales lie more than 2^12 apart (a third slower).  A row's
+ * largest score lies below 2^24: past that fp32 does not tell its keys apart, and the row may be NaN or zeros.
  * Contract: H / Hkv in {1, 2, 4, 8, 16} (JIT_EUNSUPPORTED), scale > 0, a workspace of jit_kv8_prefill_workspace_bytes
  * bytes (32,776 bytes a unit and kv head, and the partials) (JIT_EINVAL). */
 #define JIT_KV8_UNIT_KEYS 64

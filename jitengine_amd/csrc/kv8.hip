@@ -8,8 +8,9 @@ using namespace kv8;
 // A wave writes one head of 4 consecutive rows (tokens), 16 lanes a row: lane x of a row has dims 4 x .. + 3 and 64 + 4 x ..
 // + 3, so RoPE's pairs (i, i + 64) are its own, and a norm or a largest magnitude is four lane exchanges.  Bound by
 // latency up to some hundred rows (32 rows of 32 + 2 x 4 heads: 3.4 us, an empty launch 2.5), past that by memory: 2,108
-// such rows read 21.6 MB and write 17.3 MB of q and 2.2 MB of codes in 12.2 us (3.4 TB/s; a copy reaches 4.8).  A wave a
-// row, two dims a lane, took 20.7 us: its V codes went out two bytes a lane, and every wave formed 64 sines.
+// such rows read 21.6 MB and write 17.3 MB of q and 2.2 MB of codes in 12.4 us (3.3 TB/s; a copy reaches 4.8), 11.3 to 11.7 at
+// consecutive slots: V's byte stores are 1 us of it.  A wave a row, two dims a lane, took 20.7 us: its V codes went out
+// two bytes a lane, and every wave formed 64 sines.
 
 // Sum or maximum over the 16 lanes of a row (lanes l ^ 1, l ^ 2, then mirrored in 8 and in 16).
 template <bool MAX>
@@ -85,7 +86,8 @@ __device__ __forceinline__ uint32_t lane_of_quad(uint32_t v) {
 
 // The wave's blocks into their records: rec and slot of the lane's row (on: whether it is written); quad: the rows are
 // the 4 slots of one of V's words (uniform), which then go as words of 4 slots, else V's codes go byte by byte (1,001
-// rows of 16 + 16 heads at consecutive slots: 4.8 us as words, at scattered ones 7.1 as bytes).
+// rows of 16 + 16 heads at consecutive slots: 4.9 us as words; 6.0 as bytes, where the run's first row of the call is not a
+// word's first slot; at scattered slots 7.0).
 __device__ __forceinline__ void store_blocks(uint8_t *rec, int slot, bool on, bool is_v, bool quad, int l, const float (&v)[8]) {
   const int x = l & 15, k = l >> 4;
   float amax = 0.0f;
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(256) void kv8_copy_pages_kernel(uint4 *__restrict__
 // ---------------------------------------------------------------- step tables
 // Every workgroup scans all S sequences itself (a few thousand integers out of L2) and then writes the entries of
 // its own rows: no workgroup waits for another, and the tables take one launch.  Bound by latency (the lengths, two
-// scans, a table entry): 4.8 us for one sequence, 6.2 for 1,024 with 9,208 rows; an empty launch takes 2.5.
+// scans, a table entry): 4.1 us for one sequence, 6.1 for 1,024 with 9,208 rows; an empty launch takes 2.5.
 constexpr int kTabThreads = 1024, kTabRows = 1024, kTabSeqs = JIT_STEP_TABLES_MAX_SEQS;
 
 struct TableArgs {

@@ -17,7 +17,8 @@ using namespace kv8;
 constexpr float kLowest = -3.402823466e38f;
 // ---------------------------------------------------------------- single tokens
 // A sequence is cut into chunks by its own length alone, a chunk into 4 runs of a wave each.  512 keys: with 768 and
-// 1,024 64 sequences of 300 keys take 11.8 and 14.2 us instead of 9.8, 32 ragged ones 32 to 35 with any of the three.
+// 1,024 64 sequences of 300 keys take 9.9 and 11.5 us a call instead of 8.3, one of 4,096 13.1 and 13.0 instead of 11.1,
+// 32 ragged ones 29 to 32 with any of the three.
 constexpr int kSplits = 4;
 // What meets in a product: a probability times V's scale times 2^8 (2^-92 .. 2^126: both parts are normal numbers down to
 // p = 2^-18 of the quietest block), and V's codes times 2^-28.  O is 2^-20 of its size: 2^20 keys of the loudest block
@@ -86,8 +87,8 @@ struct Run {
 // lengths: sized by the host's bound (32 sequences of 128 to 32,768 keys: 8,448 workgroups for 1,003 chunks) most
 // workgroups only took a CU's place for the microsecond in which they found that they had nothing to do.  A
 // wave never runs dry: the first loads of its next chunk are in flight while it ends one.
-// Bound by memory: 262,144 keys of 4 kv heads (277 MB) in 45.9 us, 6.0 TB/s; the 32 sequences (133 MB) in 27.5, 4.8 TB/s;
-// one of 4,096 keys takes 7.5 us, the latency of a run.
+// Bound by memory: 262,144 keys of 4 kv heads (277 MB) in 45.8 us, 6.0 TB/s; the 32 sequences (133 MB) in 28.4, 4.7 TB/s;
+// one of 4,096 keys takes 7.7 us, the latency of a run.  (Reads alone reach 7.1 TB/s here.)
 __global__ __launch_bounds__(64 * kSplits) __attribute__((amdgpu_waves_per_eu(kDecodeWgs, kDecodeWgs)))
 void kv8_decode_kernel(const DecodeArgs a) {
   __shared__ float xstate[kSplits][kStateFloats][64];
@@ -346,7 +347,7 @@ void kv8_decode_kernel(const DecodeArgs a) {
 }
 
 // The chunks of a (sequence, q head), in order: thread = chunk lane (16) x 4 dims; lane j takes chunks j, j + 16, ..
-// (3.8 to 5.7 us: an empty launch and two or three trips to memory)
+// (3.4 to 5.6 us: an empty launch and two or three trips to memory)
 constexpr int kMergeLanes = 16;
 
 __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const DecodeArgs a) {
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
 //   S^T[32 keys x 32 rows] = K . Q^T        (8 MFMA 32x32x16 bf16)
 //   O^T[128 dims x 32 rows] += V^T . P^T    (4 MFMA 32x32x16 fp16 a page; 8 of bf16 in a part of uneven V)
 // Bound by the matrix instructions and the clock they leave (2,048 rows after 8,192 keys: busy 60% of the cycles at 1.9 GHz,
-// 303 to 318 us, 1.0 PFLOP/s; a large bf16 product of the library 1.15 to 1.4).  Both workgroups of a CU are needed: with
+// LDS reads 30%, 298 to 312 us, 1.0 PFLOP/s; a large bf16 product of the library 1.14 to 1.4).  Both workgroups of a CU are needed: with
 // one of four waves, however many units are on their way, the same takes 394 us.
 // A lane owns one row throughout: its scores of a page are its P operand as they are, since the 16 keys of V's
 // operand are kept in the order in which the score tile holds them.
@@ -424,7 +425,8 @@ constexpr float kLazy = 4.0f, kPfShift = 11.0f;
 //   One below fp16's range is off by 2^-25, 2^-36 of the row's sum at least: 12,288 keys 2^12 times louder than what the
 //   row is made of lose it 2^(13.6 - 36 + 12), less than a fifth of a bf16 rounding.
 // * further apart: V in bf16 as it is (4 bits, 2^-109 .. 2^127: exact) and probabilities as a high and a low bf16 part, 16
-//   bits at any magnitude, 2^-20 of their size so that no sum passes fp32's range: half as many matrix instructions again.
+//   bits at any magnitude, 2^-20 of their size so that no sum passes fp32's range: half as many matrix instructions again
+//   (2,048 rows after 8,192 keys: 408 us instead of 298).
 constexpr int kVShift = 7, kSpread = 12;
 constexpr float kWideShift = -20.0f;
 
@@ -463,7 +465,7 @@ __device__ __forceinline__ long long first_slot(const PrefillArgs &a, int ch, in
   return most >= (uint32_t)parts && s >= 0 && s + parts <= a.num_slots ? s : -1;
 }
 
-// One workgroup expands a unit of one kv head, wave w its page w: 10,240 keys of 4 heads, 11 MB to 21 MB, in 14 to 18 us, most of
+// One workgroup expands a unit of one kv head, wave w its page w: 10,240 keys of 4 heads, 11 MB to 21 MB, in 16 to 18 us, most of
 // it the latency of its part's scales (parts of 96 units: 11 us).  Its codes are requested first; meanwhile the part's
 // loudest and quietest live V scales are found (by every workgroup of a part for itself: a line of 64 bytes a page).
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8))) void kv8_expand_kernel(const PrefillArgs a) {
@@ -1009,8 +1011,8 @@ extern "C" int jit_kv8_prefill_block_tokens(int H, int Hkv) {
 // share a CU and 1.15 us for one alone, 4 units' time for a workgroup's start and end, and 3 us and 0.02 a workgroup for
 // the partials and their merge.  The n with the least of that, by the chunk alone, so that a row's bits do not depend on
 // the call's other chunks.  All three launches, against parts of a fixed 6,144 keys (32 query heads over 4): 16 rows after
-// 8,000 keys 35 us in 15 parts, 115 us; 512 rows after 8,000 96 us in 4, 116 us; 512 of 16 heads over 16 after 4,000 49 us
-// in 4, 92 us; 2,048 rows after 8,192 308 to 321 us in one, 318 to 329 in two.
+// 8,000 keys 35 us in 15 parts, 115 us; 512 rows after 8,000 90 us in 4, 116 us; 512 of 16 heads over 16 after 4,000 49 us
+// in 4, 92 us; 2,048 rows after 8,192 305 to 316 us in one, 318 to 329 in two.
 extern "C" int jit_kv8_prefill_part_units(int ctx, int len, int H, int Hkv) {
   const int bt = jit_kv8_prefill_block_tokens(H, Hkv);
   if (bt < 0 || ctx < 0 || len < 1) return -1;
