@@ -15,6 +15,7 @@ using namespace kv8;
 
 // The running maximum before any key: finite, so that rows without a key stay 0, and no finite score lies below it.
 constexpr float kLowest = -3.402823466e38f;
+
 // ---------------------------------------------------------------- single tokens
 // A sequence is cut into chunks by its own length alone, a chunk into 4 runs of a wave each.  512 keys: with 768 and
 // 1,024 64 sequences of 300 keys take 9.9 and 11.5 us a call instead of 8.3, one of 4,096 13.1 and 13.0 instead of 11.1,
@@ -396,7 +397,8 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
 
 // ---------------------------------------------------------------- causal prompt chunks
 // Two launches (three where a token's keys have several parts).  The first expands the keys that the chunks see: K to
-// bf16 (times its scale) and V to fp16 (or bf16: kSpread), in the order in which the second launch's matrix instructions take them.
+// bf16 (times its scale) and V to fp16 (or bf16: kSpread), in the order in which the second launch's matrix instructions
+// take them.
 // Every row block of a chunk reads all of its keys, so the conversion is done once instead of once a block; inside the
 // attention loop it cost as many vector instructions as the softmax (2,048 rows after 8,192 keys: 344 us, without it 328).
 //
@@ -406,8 +408,8 @@ __global__ __launch_bounds__(32 * kMergeLanes) void kv8_merge_kernel(const Decod
 //   S^T[32 keys x 32 rows] = K . Q^T        (8 MFMA 32x32x16 bf16)
 //   O^T[128 dims x 32 rows] += V^T . P^T    (4 MFMA 32x32x16 fp16 a page; 8 of bf16 in a part of uneven V)
 // Bound by the matrix instructions and the clock they leave (2,048 rows after 8,192 keys: busy 60% of the cycles at 1.9 GHz,
-// LDS reads 30%, 298 to 312 us, 1.0 PFLOP/s; a large bf16 product of the library 1.14 to 1.4).  Both workgroups of a CU are needed: with
-// one of four waves, however many units are on their way, the same takes 394 us.
+// LDS reads 30%, 298 to 312 us, 1.0 PFLOP/s; a large bf16 product of the library 1.14 to 1.4).  Both workgroups of a CU are
+// needed: with one of four waves, however many units are on their way, the same takes 394 us.
 // A lane owns one row throughout: its scores of a page are its P operand as they are, since the 16 keys of V's
 // operand are kept in the order in which the score tile holds them.
 constexpr int kPfWaves = 4, kStages = 2;  // waves a workgroup; units in LDS: the one in use, and those on their way
@@ -455,9 +457,8 @@ struct PrefillArgs {
   float qk_scale;
 };
 
-// The tables of the units, parts, slots and work items come from the caller's device memory: an entry that does not
-// belong to these chunks is left out here, before it becomes an address.
-// first slot of token t's partials (-1: not its chunk's)
+// The tables of units, parts, slots and work items lie in the caller's device memory: each kernel leaves out an entry that
+// does not belong to its chunk before it becomes an address.  Here: the first slot of token t's partials, or -1.
 __device__ __forceinline__ long long first_slot(const PrefillArgs &a, int ch, int part_units, int t, int parts) {
   const uint32_t units = (uint32_t)a.chunk_unit[ch + 1] - (uint32_t)a.chunk_unit[ch];
   const uint32_t most = (units + (uint32_t)part_units - 1u) / (uint32_t)part_units;
@@ -465,8 +466,8 @@ __device__ __forceinline__ long long first_slot(const PrefillArgs &a, int ch, in
   return most >= (uint32_t)parts && s >= 0 && s + parts <= a.num_slots ? s : -1;
 }
 
-// One workgroup expands a unit of one kv head, wave w its page w: 10,240 keys of 4 heads, 11 MB to 21 MB, in 16 to 18 us, most of
-// it the latency of its part's scales (parts of 96 units: 11 us).  Its codes are requested first; meanwhile the part's
+// One workgroup expands a unit of one kv head, wave w its page w: 10,240 keys of 4 heads, 11 MB to 21 MB, in 16 to 18 us,
+// most of it the latency of its part's scales (parts of 96 units: 11 us).  Its codes are requested first; meanwhile the part's
 // loudest and quietest live V scales are found (by every workgroup of a part for itself: a line of 64 bytes a page).
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8))) void kv8_expand_kernel(const PrefillArgs a) {
   __shared__ int s_e[4], s_bad[4], s_ids[kPartMax * kUnitPages];
@@ -504,8 +505,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8))) void k
     sv[i] = *(const float4 *)(sc + kPage + 8 * i + 4 * vh);
   }
   // E: thread = page of the part x quarter of its slots (a bare barrier: the codes stay in flight)
-  int e = 0, bad = 0;     // (positive powers of two are ordered as their bits)
-  uint32_t least = ~0u;   // (bits - 1: a slot never written, scale 0, is the last of all)
+  int e = 0, bad = 0;    // (positive powers of two are ordered as their bits)
+  uint32_t least = ~0u;  // (bits - 1: a slot never written, scale 0, is the last of all)
   lds_barrier();
 #pragma unroll 6
   for (int i = threadIdx.x; i < 4 * np; i += 256) {
@@ -522,7 +523,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(8))) void k
     }
   }
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o, 64)), least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
+  for (int o = 1; o < 64; o <<= 1) {
+    e = max(e, __shfl_xor(e, o, 64));
+    least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
+  }
   const int any = __any(bad), here = __any(out_of_pool && pg < npages);
   // What lies past the keys or in a page outside the pool may be anything (0 x NaN): it counts as 0.  So do NaN codes
   // of V, which rows that do not see their key must not get either: kv8_prefill_kernel puts them back.

@@ -95,6 +95,19 @@ def test_loud_values_stay_finite_however_a_chunk_is_cut(ctx, n, mag):
     _check(out, want, A, 11, L, _score_error(q, k), (ctx, n, mag))
 
 
+@pytest.mark.parametrize("ctx, n", [(3000, 9), (0, 40)])
+@pytest.mark.parametrize("mag", [2.0 ** -92, 1e-20])
+def test_quiet_values_keep_their_bits_however_a_chunk_is_cut(ctx, n, mag):
+    L, H, Hkv = ctx + n, 32, 4
+    q, k, v = _normal(L, H, Hkv, n)
+    q, k = (0.1 * q[:n]).to(torch.bfloat16), k.to(torch.bfloat16)
+    v = ((1 + 0.05 * v.clamp(-1, 1)) * mag / 1.06).to(torch.bfloat16)
+    pool, table = _cache(k, v)
+    out, _ = _prompt(q.to(DEV), pool, table, ctx)
+    want, A = _rows(q.to(DEV), pool, table, ctx)
+    _check(out, want, A, 11, L, _score_error(q, k), (ctx, n, mag))
+
+
 SHAPES = [(0, 2), (0, 70), (3000, 9), (20, 300), (8000, 16)]
 
 
