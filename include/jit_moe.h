@@ -506,6 +506,70 @@ int jit_threefry_uniform(const uint32_t *keys, int B, float *u, void *stream);
 int jit_kv_copy_pages(uint16_t *pool, int num_pages, int Hkv, const int32_t *src, const int32_t *dst, int n,
                       void *stream);
 
+/* ------------------------------------------------------------ scoring, continued sequences --
+ * Log-probabilities of given tokens for rows of logits [B, V] (bf16, or fp32 with fp32 = 1; row b begins row_stride
+ * elements after row b - 1, at any address that its type allows).  No counterpart in the reference, whose sampler keeps
+ * whole rows of bf16 log-probabilities (Q36/sampler.py:295-297); here everything is fp32 or more from the logits on.
+ * With m the largest logit of a row, l = sum e^(x - m), t = sum (x - m) e^(x - m):
+ *   logprob [B, n_tokens]  (x_v - m) - ln l of the tokens v = tokens [B, n_tokens]; 0 for a v outside [0, V);
+ *   rank    [B, n_tokens]  logits before x_v in the order (value descending, index ascending); -1 outside [0, V);
+ *   entropy [B]            ln l - t / l, in nats;
+ *   top_ids, top_logprobs [B, top]  the first `top` of that order.
+ * -inf logits have probability 0; a row of nothing else has log-probabilities -inf and entropy 0.  A row with a NaN or
+ * +inf has NaN log-probabilities and entropy; a NaN is no alternative (id -1 where numbers are missing, rank -1).
+ * The bits repeat; they depend on B through the slices of a row.
+ * Contract: top <= V, top <= 64, n_tokens <= 64, V <= 2^30 (the last three JIT_EUNSUPPORTED); a workspace of
+ * jit_token_logprobs_workspace_bytes (16-byte aligned, contents do not matter, none where that is 0). */
+long long jit_token_logprobs_workspace_bytes(int B, int V, int n_tokens, int top);
+int jit_token_logprobs(const void *logits, int fp32, int B, int V, long long row_stride, const int32_t *tokens,
+                       int n_tokens, int top, float *logprob, int32_t *rank, float *entropy, int32_t *top_ids,
+                       float *top_logprobs, void *workspace, long long workspace_bytes, void *stream);
+
+/* The same of one token a row straight from hidden rows x [T, K] bf16 and a packed 4-bit head [V, K] (jit_q4_prepack),
+ * with no logits in memory: logit = x . (s q + b) in fp32, not rounded to bf16 as jit_qmm_packed's are.
+ *   logprob, entropy, lse [T]  of tokens [T] (logprob 0 for a token outside [0, V)); lse = m + ln l.
+ * Contract: K % 128 == 0, V % 16 == 0, T <= 2^20 (JIT_EUNSUPPORTED); x, w and the workspace 16-byte aligned. */
+long long jit_head_logprobs_workspace_bytes(int T, int K, int V);
+int jit_head_logprobs(const uint16_t *x, int T, int K, const void *w, int V, const int32_t *tokens, float *logprob,
+                      float *entropy, float *lse, void *workspace, long long workspace_bytes, void *stream);
+
+/* The best continuations of each group's beams.  scores [groups, beams]; logprobs, ids [groups, beams, alternatives];
+ * done [groups, beams] (NULL: none has ended); eos [n_eos].  Candidates of a group: alternative j of beam b with
+ * score_b + logprob_bj (one fp32 sum) where its id is >= 0; of a beam with done != 0 only its score, as alternative 0
+ * without a token.  A NaN or -inf is no candidate.  The first `width` in the order (score descending, b * alternatives + j
+ * ascending) are written: parents (the beam's row, group * beams + b), tokens (-1 of an ended beam), out_scores, and
+ * out_done = 1 where the parent had ended or the token is one of eos; -1, -1, -inf, 1 past the last candidate.
+ * Contract: beams * alternatives <= 4096, width <= 64 (JIT_EUNSUPPORTED). */
+int jit_beam_select(const float *scores, const float *logprobs, const int32_t *ids, const int32_t *done,
+                    const int32_t *eos, int n_eos, int groups, int beams, int alternatives, int width,
+                    int32_t *parents, int32_t *tokens, float *out_scores, int32_t *out_done, void *stream);
+
+/* Sequences continued by others: the tables, counts and free list of a paged cache after sequence parents[i] (-1: none)
+ * went on as sequence i, for i < N.  Sequence s < S holds the first ceil(lens[s] / 16) pages of page_table[s] (at most
+ * max_pages); refs [num_pages] counts the holders of each page; free_pages [n_free] is jit_step_tables' list, going on at
+ * *free_at.  The old sequences give up their pages and the new ones take theirs:
+ *   full pages are shared; a last page that is part full stays with the first child where refs is 1, every other child
+ *   takes the list's next page for it, and (src[i], dst[i]) says what to copy (-1, -1 without; jit_kv_copy_pages_layers);
+ *   pages whose last reference went are put back before the list's next page, in ascending order from the new *free_at on.
+ * new_table [N, max_pages] (0 past the pages held), new_lens [N]; refs and free_pages change in place.
+ *   status [4]  pages copied, where the free list goes on, children refused, pages that found no room in the list.
+ * A child is refused (length 0, no pages) where the list ends or holds an id outside the pool.  A page id outside
+ * [0, num_pages) in a table is handed on as it is, without a count.  A list of num_pages entries always has room.
+ * Contract: S, N <= JIT_STEP_TABLES_MAX_SEQS (JIT_EUNSUPPORTED); a workspace of jit_pages_fork_workspace_bytes, 16-byte
+ * aligned; outputs apart from inputs. */
+long long jit_pages_fork_workspace_bytes(int S, int N, int num_pages);
+int jit_pages_fork(const int32_t *page_table, const int32_t *lens, int S, int max_pages, const int32_t *parents, int N,
+                   int32_t *refs, int num_pages, int32_t *free_pages, int n_free, const int32_t *free_at,
+                   int32_t *new_table, int32_t *new_lens, int32_t *src, int32_t *dst, int32_t *status, void *workspace,
+                   long long workspace_bytes, void *stream);
+
+/* jit_kv_copy_pages (or jit_kv8_copy_pages) in every layer by one launch (one for every 128 layers): page src[i] to
+ * page dst[i], i < n, of each of the `layers` pools; `pools` is a host array of device pointers, page_bytes the bytes of
+ * a page in one layer.  A page id outside [0, num_pages) copies nothing.  No page is copied to twice, and none of those
+ * copied to is copied from.  Contract: 16-byte aligned pools, page_bytes % 16 == 0. */
+int jit_kv_copy_pages_layers(void *const *pools, int layers, int num_pages, long long page_bytes, const int32_t *src,
+                             const int32_t *dst, int n, void *stream);
+
 /* ------------------------------------------------------------ 8-bit KV cache --
  * A KV pool held in 8 bits with a scale for each token and kv head, at 0.516 of the bf16 pool's bytes.  No
  * counterpart in the reference, whose caches are bf16 (Q36/kvcache/kv_cache.py:27-85).  A layer's pool is

@@ -116,6 +116,14 @@ _SIGNATURES = {
     "jit_argmax_rows_ws": [_P, _I, _I, _P, _P, ctypes.c_int64, _P],
     "jit_sample_rows_ws": [_P, _I, _I, ctypes.c_double, ctypes.c_double, _I, _P, _P, _P, ctypes.c_int64, _P],
     "jit_kv_copy_pages": [_P, _I, _I, _P, _P, _I, _P],
+    "jit_token_logprobs_workspace_bytes": [_I, _I, _I, _I],
+    "jit_token_logprobs": [_P, _I, _I, _I, _L, _P, _I, _I, _P, _P, _P, _P, _P, _P, _L, _P],
+    "jit_head_logprobs_workspace_bytes": [_I, _I, _I],
+    "jit_head_logprobs": [_P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _L, _P],
+    "jit_beam_select": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P],
+    "jit_pages_fork_workspace_bytes": [_I, _I, _I],
+    "jit_pages_fork": [_P, _P, _I, _I, _P, _I, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _P],
+    "jit_kv_copy_pages_layers": [_P, _I, _I, _L, _P, _P, _I, _P],
     "jit_step_tables": [_P, _P, _I, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P],
     "jit_kv8_append_paged": [_P, _P, _I, _I, _P, _P, _I, _P],
     "jit_qk_norm_rope_append_kv8": [_P, _I, _I, _I, _P, _P, _F, _P, _P, _P, _P, _I, _P, _P],
@@ -136,7 +144,8 @@ _RESTYPES = {"jit_last_error": ctypes.c_char_p, "jit_attn_workspace_bytes": ctyp
              "jit_prefill_workspace_bytes": ctypes.c_int64,
              "jit_q4_packed_bytes": ctypes.c_int64, "jit_moe_pack_workspace_bytes": ctypes.c_int64,
              "jit_sampler_workspace_bytes": ctypes.c_int64, "jit_kv8_decode_workspace_bytes": ctypes.c_int64,
-             "jit_kv8_prefill_workspace_bytes": ctypes.c_int64}
+             "jit_kv8_prefill_workspace_bytes": ctypes.c_int64, "jit_token_logprobs_workspace_bytes": _L,
+             "jit_head_logprobs_workspace_bytes": _L, "jit_pages_fork_workspace_bytes": _L}
 
 _lib = None
 

@@ -42,6 +42,9 @@ SOURCES = {
     "block.hip": [],
     "head.hip": [],
     "sampler.hip": ["-ffp-contract=off"],
+    "score.hip": [],
+    "score_head.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "beam.hip": [],
     "kv8.hip": [],
     "kv8_attention.hip": [],
 }

@@ -1099,6 +1099,215 @@ def kv8_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> 
             dst.data_ptr(), src.shape[0])
 
 
+# ----------------------------------------------------------------------------- scoring, continued sequences
+@dataclass
+class TokenLogprobs:
+    """What rows of logits say of given tokens (jit_token_logprobs); the members of what was not asked for are None."""
+
+    logprob: torch.Tensor | None       # fp32, the tokens' shape
+    rank: torch.Tensor | None          # int32, the tokens' shape: 0 is the most likely
+    entropy: torch.Tensor              # fp32 [B], nats
+    top_ids: torch.Tensor | None       # int32 [B, top], the most likely first
+    top_logprobs: torch.Tensor | None  # fp32 [B, top]
+
+
+def _workspace(workspace, need: int, device, name: str) -> torch.Tensor | None:
+    """The caller's workspace of `need` bytes (ValueError where it is too small or lies elsewhere), or a new one; None for no bytes."""
+    if need <= 0:
+        return None
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace.device != device or not workspace.is_contiguous() or workspace.nbytes < need or workspace.data_ptr() % 16:
+        raise ValueError(f"{name} needs a contiguous workspace of {need} bytes on {device}, 16-byte aligned")
+    return workspace
+
+
+def token_logprobs_workspace_bytes(B: int, V: int, n_tokens: int = 1, top: int = 0) -> int:
+    return int(_lib.lib().jit_token_logprobs_workspace_bytes(int(B), int(V), int(n_tokens), int(top)))
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0,
+                   workspace: torch.Tensor | None = None) -> TokenLogprobs:
+    """Log-probability and rank of tokens [B] or [B, m] (int32, m <= 64) in rows of logits [B, V] (bf16 or fp32, rows at
+    any stride), the rows' entropy, and their `top` <= 64 most likely tokens with log-probabilities, equal logits by the
+    lowest index (jit_token_logprobs).  A token outside [0, V), as padding, has log-probability 0 and rank -1."""
+    f32, i32, lib = torch.float32, torch.int32, _lib.lib()
+    if logits.dtype not in (torch.bfloat16, f32):
+        raise ValueError(f"logits must be bf16 or fp32, got {logits.dtype}")
+    if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError(f"logits must be [B, V] with adjacent values in a row, got {tuple(logits.shape)}")
+    dev = logits.get_device()
+    if dev < 0:
+        raise ValueError("logits must be a device tensor")
+    (B, V), top, m, shape = logits.shape, int(top), 0, None
+    stride = logits.stride(0) if B > 1 else V
+    if V < 1 or stride < V:
+        raise ValueError(f"rows of {V} logits at a stride of {stride}")
+    if tokens is not None:
+        if _take((tokens, i32, "tokens")) != dev:
+            raise ValueError(f"tokens is on device {tokens.get_device()}, logits on {dev}")
+        shape = tokens.shape
+        if tokens.dim() not in (1, 2) or shape[0] != B or (tokens.dim() == 2 and shape[1] < 1):
+            raise ValueError(f"tokens must be [{B}] or [{B}, m], got {tuple(shape)}")
+        m = 1 if tokens.dim() == 1 else shape[1]
+    need = lib.jit_token_logprobs_workspace_bytes(B, V, m, max(top, 0))
+    ws = _workspace(workspace, need, logits.device, "token_logprobs")
+    ent = torch.empty(B, dtype=f32, device=logits.device)
+    lp = rank = ids = tlp = None
+    if m:
+        lp, rank = ent.new_empty(shape), torch.empty(shape, dtype=i32, device=logits.device)
+    if top > 0:
+        ids, tlp = torch.empty((B, top), dtype=i32, device=logits.device), ent.new_empty((B, top))
+    _launch(dev, lib.jit_token_logprobs, "token_logprobs", logits.data_ptr(), int(logits.dtype == f32), B, V, stride,
+            _ptr(tokens), m, top, _ptr(lp), _ptr(rank), ent.data_ptr(), _ptr(ids), _ptr(tlp), _ptr(ws),
+            0 if ws is None else ws.nbytes)
+    return TokenLogprobs(lp, rank, ent, ids, tlp)
+
+
+@dataclass
+class HeadLogprobs:
+    """What hidden rows and a head say of a given token a row (jit_head_logprobs), fp32 [T]."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    lse: torch.Tensor  # the log of the sum of the exponentials of a row's logits
+
+
+def head_logprobs_workspace_bytes(T: int, K: int, V: int) -> int:
+    return int(_lib.lib().jit_head_logprobs_workspace_bytes(int(T), int(K), int(V)))
+
+
+def head_logprobs(x: torch.Tensor, head: PackedQ4, tokens: torch.Tensor,
+                  workspace: torch.Tensor | None = None) -> HeadLogprobs:
+    """Log-probabilities of tokens [T] int32 for (normed) hidden rows x [T, K] bf16 against a packed head [V, K], with the
+    rows' entropies, and no logits in memory (jit_head_logprobs).  The logits are fp32 here, where qmm rounds them to
+    bf16: token_logprobs of qmm's differ by that rounding."""
+    if not isinstance(head, PackedQ4) or head.stacked:
+        raise _lib.UnsupportedShape("head_logprobs takes one packed [V, K] matrix (ops.prepack)")
+    dev = _take((x, torch.bfloat16, "x"), (tokens, torch.int32, "tokens"), (head.data, torch.uint8, "head"))
+    if x.dim() != 2 or x.shape[1] != head.K or tokens.shape != x.shape[:1]:
+        raise ValueError(f"head_logprobs takes x [T, {head.K}] and tokens [T], got {tuple(x.shape)} and {tuple(tokens.shape)}")
+    T, lib = x.shape[0], _lib.lib()
+    ws = _workspace(workspace, lib.jit_head_logprobs_workspace_bytes(T, head.K, head.N), x.device, "head_logprobs")
+    out = torch.empty((3, T), dtype=torch.float32, device=x.device)
+    at = out.data_ptr()
+    _launch(dev, lib.jit_head_logprobs, "head_logprobs", x.data_ptr(), T, head.K, head.data.data_ptr(), head.N,
+            tokens.data_ptr(), at, at + 4 * T, at + 8 * T, _ptr(ws), 0 if ws is None else ws.nbytes)
+    return HeadLogprobs(*out.unbind(0))
+
+
+@dataclass
+class Beams:
+    """The continuations that a step keeps, [G, width], the best first (jit_beam_select); -1, -1, -inf, 1 where a group has
+    no more."""
+
+    parents: torch.Tensor  # int32: rows of the [G * n] beams
+    tokens: torch.Tensor   # int32 (-1: of a beam that had ended)
+    scores: torch.Tensor   # fp32
+    done: torch.Tensor     # int32
+
+
+def beam_select(scores: torch.Tensor, logprobs: torch.Tensor, ids: torch.Tensor, width: int | None = None,
+                done: torch.Tensor | None = None, eos: torch.Tensor | None = None) -> Beams:
+    """The `width` (n without) best continuations of each group of n beams: scores [G, n] fp32, their alternatives'
+    logprobs fp32 and ids int32 [G, n, m], the beams that have ended (done [G, n] int32), the ids that end one (eos int32
+    list).  An ended beam goes on as itself; ties go to the lowest beam, then alternative (jit_beam_select)."""
+    f32, i32 = torch.float32, torch.int32
+    dev = _take((scores, f32, "scores"), (logprobs, f32, "logprobs"), (ids, i32, "ids"), (done, i32, "done"), (eos, i32, "eos"))
+    if scores.dim() != 2 or logprobs.dim() != 3 or logprobs.shape[:2] != scores.shape or ids.shape != logprobs.shape or \
+            (done is not None and done.shape != scores.shape) or (eos is not None and eos.dim() != 1):
+        raise ValueError(f"beam_select takes scores and done [G, n], logprobs and ids [G, n, m], eos [e], got "
+                         f"{tuple(scores.shape)}, {tuple(logprobs.shape)}, {tuple(ids.shape)}")
+    G, n, m = logprobs.shape
+    w = n if width is None else int(width)
+    if w < 1:
+        raise ValueError(f"width must be positive, got {w}")
+    buf = torch.empty((4, G, w), dtype=i32, device=scores.device)
+    at, step = buf.data_ptr(), 4 * G * w
+    _launch(dev, _lib.lib().jit_beam_select, "beam_select", scores.data_ptr(), logprobs.data_ptr(), ids.data_ptr(), _ptr(done),
+            _ptr(eos), 0 if eos is None else eos.numel(), G, n, m, w, at, at + step, at + 2 * step, at + 3 * step)
+    p, t, s, d = buf.unbind(0)
+    return Beams(p, t, s.view(f32), d)
+
+
+@dataclass
+class Fork:
+    """Sequences after others were continued (jit_pages_fork), int32 on the device."""
+
+    page_table: torch.Tensor  # [N, W]
+    lens: torch.Tensor        # [N]
+    src: torch.Tensor         # [N]: pages to copy from (-1: none), for kv_copy_pages_layers
+    dst: torch.Tensor         # [N]
+    status: torch.Tensor      # [4]: pages copied, where the free list goes on, children refused, pages without room
+
+
+def pages_fork(page_table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, refs: torch.Tensor, free: torch.Tensor,
+               free_at: torch.Tensor, workspace: torch.Tensor | None = None) -> Fork:
+    """The sequences page_table [S, W], lens [S] give way to children: child i goes on from parents[i] (-1: an empty row).
+    Full pages are shared, a part full last page is copied unless its one holder's first child keeps it; the counts refs
+    [num_pages] and the free list (step_tables' list and position; status[1:2] is the next one) change in place, and what
+    nobody holds comes back (jit_pages_fork).  All tensors int32."""
+    i32 = torch.int32
+    dev = _take((page_table, i32, "page_table"), (lens, i32, "lens"), (parents, i32, "parents"), (refs, i32, "refs"),
+                (free, i32, "free"), (free_at, i32, "free_at"))
+    if page_table.dim() != 2 or page_table.shape[1] < 1 or lens.shape != page_table.shape[:1] or parents.dim() != 1 or \
+            refs.dim() != 1 or refs.numel() < 1 or free.dim() != 1 or free_at.numel() != 1:
+        raise ValueError(f"pages_fork takes page_table [S, W], lens [S], parents [N], refs [P], free [F], free_at [1], got "
+                         f"{[tuple(t.shape) for t in (page_table, lens, parents, refs, free, free_at)]}")
+    (S, W), N, P, lib = page_table.shape, parents.numel(), refs.numel(), _lib.lib()
+    ws = _workspace(workspace, lib.jit_pages_fork_workspace_bytes(S, N, P), refs.device, "pages_fork")
+    buf = torch.empty(N * (W + 3) + 4, dtype=i32, device=refs.device)
+    at = buf.data_ptr()
+    p_len = at + 4 * N * W
+    _launch(dev, lib.jit_pages_fork, "pages_fork", page_table.data_ptr(), lens.data_ptr(), S, W, parents.data_ptr(), N,
+            refs.data_ptr(), P, free.data_ptr(), free.numel(), free_at.data_ptr(), at, p_len, p_len + 4 * N, p_len + 8 * N,
+            p_len + 12 * N, ws.data_ptr(), ws.nbytes)
+    table, *rest = buf.split_with_sizes([N * W, N, N, N, 4])
+    return Fork(table.view(N, W), *rest)
+
+
+@dataclass
+class PoolLayers:
+    """A model's layers' pools for calls that work on all of them (pool_layers)."""
+
+    pools: list
+    pointers: object  # ctypes array of the pools' addresses
+    num_pages: int
+    page_bytes: int
+    device: int
+
+
+def pool_layers(pools) -> PoolLayers:
+    """The pools of a model's layers (all bf16 or all 8-bit, of one shape and device) as one handle; made once."""
+    pools = list(pools)
+    if not pools:
+        raise ValueError("pool_layers takes at least one pool")
+    first = pools[0]
+    (_kv8_heads if is_kv8(first) else _pool_heads)(first)
+    dev = _take(*((p, torch.uint8 if is_kv8(first) else torch.bfloat16, f"pool {i}") for i, p in enumerate(pools)))
+    for i, p in enumerate(pools):
+        if p.shape != first.shape:
+            raise ValueError(f"pool {i} is {tuple(p.shape)}, pool 0 {tuple(first.shape)}")
+        if p.data_ptr() % 16:
+            raise ValueError(f"pool {i} is not 16-byte aligned")
+    if len({p.data_ptr() for p in pools}) != len(pools):
+        raise ValueError("a pool is given twice")
+    ptrs = (ctypes.c_void_p * len(pools))(*(p.data_ptr() for p in pools))
+    return PoolLayers(pools, ptrs, first.shape[0], first[0].numel() * first.element_size(), dev)
+
+
+def kv_copy_pages_layers(layers: PoolLayers, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copy pages src[i] -> dst[i] (int32 device tensors; -1: none) in every layer by one launch
+    (jit_kv_copy_pages_layers).  No page may be copied to twice, nor both to and from."""
+    dev = _take((src, torch.int32, "src"), (dst, torch.int32, "dst"))
+    if dev != layers.device:
+        raise ValueError(f"src is on device {dev}, the pools on {layers.device}")
+    if src.shape != dst.shape or src.dim() != 1:
+        raise ValueError("src and dst must be equal-length 1-D page lists")
+    _launch(dev, _lib.lib().jit_kv_copy_pages_layers, "kv_copy_pages_layers", layers.pointers, len(layers.pools),
+            layers.num_pages, layers.page_bytes, src.data_ptr(), dst.data_ptr(), src.numel())
+
+
 # ----------------------------------------------------------------------------- step ends, KV pages
 def embed_q4(ids: torch.Tensor, table: QLinear) -> torch.Tensor:
     """Embedding rows [B, D] bf16 of token ids [B] int32 from an MLX 4-bit table [V, D]
