@@ -44,6 +44,7 @@ SOURCES = {
     "sampler.hip": ["-ffp-contract=off"],
     "score.hip": [],
     "score_head.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "score_head_mid.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "beam.hip": [],
     "kv8.hip": [],
     "kv8_attention.hip": [],

@@ -8,51 +8,11 @@
 // and the nearer the offset, the less the two sums cancel.)
 #include <type_traits>
 
-#include "qtile.hpp"
+#include "score_head.hpp"
 
 namespace {
 
-constexpr int kThreads = 512, kWaves = 8;
-constexpr float kLowest = -3.402823466e38f, kFloor = -1000.0f, kLog2e = 1.44269504088896341f;
-constexpr float kDead = -1.7e38f;  // the logit of a row that is not there (its product with log2 e is finite)
-
-struct HeadArgs {
-  const uint16_t *x;
-  const uint8_t *w;
-  const int32_t *tokens;
-  const uint16_t *xs;  // [3][T16][G32] the groups' sums of x
-  float *part;     // [parts][segs][3][32 TT]: a run's states of each tile it meets
-  float *picked;   // [T] the given tokens' logits
-  float *logprob, *entropy, *lse;
-  int T, K, V, parts, segs, tiles, T16, G32;
-};
-
-// A token's softmax in base 2 against a reference m near its largest logit: with y = x log2 e - m, l = sum 2^y and
-// t = sum y 2^y.  (m is what every y was formed with, so its own rounding cancels.)
-struct Stat {
-  float m, l, t;
-};
-
-__device__ __forceinline__ Stat rebase(const Stat &s, float m) {
-  const float d = fmaxf(s.m - m, kFloor), e = __builtin_amdgcn_exp2f(d);
-  return {m, s.l * e, fmaf(s.l, d, s.t) * e};
-}
-
-__device__ __forceinline__ Stat join(const Stat &a, const Stat &b) {
-  const float m = fmaxf(a.m, b.m);
-  const Stat p = rebase(a, m), q = rebase(b, m);
-  return {m, p.l + q.l, p.t + q.t};
-}
-
-// The 8 values of a packed word as bf16 q + 16.
-__device__ __forceinline__ Frag8 unpack16(uint32_t w, uint32_t m, uint32_t c) {
-  Frag8 f;
-  f.u[0] = ((w << 3) & m) | c;
-  f.u[1] = ((w >> 1) & m) | c;
-  f.u[2] = ((w >> 5) & m) | c;
-  f.u[3] = ((w >> 9) & m) | c;
-  return f;
-}
+using namespace head;
 
 // Lane exchanges within each half of a wave: lane l ^ 16, mirrored in 16, in 8, then lanes l ^ 2 and l ^ 1.
 template <int STEP>
@@ -124,26 +84,6 @@ __global__ __launch_bounds__(64) void head_xsum_kernel(const uint16_t *__restric
 }
 
 // ------------------------------------------------------------------ many rows
-// s_waitcnt vmcnt(N) alone; the fence keeps the reads of what has landed behind it.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | (7 << 4) | (15 << 8));
-  asm volatile("" ::: "memory");
-}
-__device__ __forceinline__ void bare_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-// 1 KB straight into LDS (16 bytes a lane; M0 wants a wait state before the load that takes it), and 256 bytes
-__device__ __forceinline__ void load_lds(const void *base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
-}
-
-__device__ __forceinline__ void load_lds4(const void *base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
-}
-
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kRB = 2;               // 32-row blocks of a wave
@@ -498,20 +438,203 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   }
 }
 
+// ------------------------------------------------------------------ few rows
+// Up to 16 rows, held in LDS: 8 waves a workgroup, one workgroup a CU, each wave streaming 16-row blocks of the head of
+// its own with RING KB of weights in flight (16 x 16 x 32 products, tokens on the rows).  Bound by the head's bytes.
+constexpr int kFewBytes = 128 * 1024;  // LDS for the rows
+constexpr int kFewChunks = 2;          // 32-group chunks of a row at most (K <= 4096)
+
+template <int RING>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void head_few_kernel(const HeadArgs a) {
+  constexpr int NT = 16;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ float s_state[kWaves][3][NT];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), lr = l & 15, lg = l >> 4;
+  const int n = blockIdx.x, GP = a.K >> 7, blocks = a.V >> 4, row_bytes = 2 * a.K;
+  const int r0 = (int)((long long)blocks * n / a.parts), r1 = (int)((long long)blocks * (n + 1) / a.parts);
+  const long long blk_bytes = (long long)GP * qtile::kTileBytes;
+  uint32_t um = 0x00780078u, uc = 0x41804180u;
+  asm volatile("" : "+v"(um), "+s"(uc));
+
+  uint4 ring[RING];
+  uint2 sb[kFewChunks][4], sn[kFewChunks][4];  // scale and bias pairs of pair 16 c + 4 lg + j, this block's and the next's
+  const int chunks = a.G32 / 32;
+  auto blk = [&](int b) { return a.w + min(b, blocks - 1) * blk_bytes; };  // (past the run: loaded and unused)
+  auto load_pair = [&](int b, int p) { return ld_stream16(blk(b) + p * qtile::kNibbleBytes + 16 * l); };
+  auto load_scales = [&](int b, uint2 (&to)[kFewChunks][4]) {
+    const uint8_t *sp = blk(b) + (long long)GP * qtile::kNibbleBytes + 8 * lr;
+#pragma unroll
+    for (int c = 0; c < kFewChunks; c++)
+      if (c < chunks) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) to[c][j] = *(const uint2 *)(sp + min(16 * c + 4 * lg + j, GP - 1) * qtile::kScaleBytes);
+      }
+  };
+  // The rows (zeros past T, piece c of a pair in slot c ^ row) are asked for ahead of the weights: loads come back in
+  // order, and nothing starts without them.
+  const int per_row = row_bytes / 16, pieces = NT * per_row;
+  auto row_piece = [&](int c) {
+    const int row = c / per_row, piece = c % per_row;
+    return c < pieces && row < a.T ? *(const uint4 *)(a.x + (long long)row * a.K + 8 * piece) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  auto put_piece = [&](int c, const uint4 &q) {
+    const int row = c / per_row, piece = c % per_row;
+    if (c < pieces) *(uint4 *)(lds + row * row_bytes + 16 * ((piece & ~15) | ((piece ^ row) & 15))) = q;
+  };
+  uint4 xq[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) xq[i] = row_piece(threadIdx.x + i * kThreads);
+  asm volatile("" ::: "memory");
+  int b = r0 + wave;
+#pragma unroll
+  for (int j = 0; j < RING; j++) ring[j] = load_pair(b, min(j, GP - 1));
+  load_scales(b, sb);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; i++) put_piece(threadIdx.x + i * kThreads, xq[i]);
+  for (int c = threadIdx.x + 8 * kThreads; c < pieces; c += kThreads) put_piece(c, row_piece(c));
+  // then each group's sum in three bf16 pieces [3][NT][G32]
+  __syncthreads();
+  uint16_t *xs = (uint16_t *)(lds + NT * row_bytes);
+  for (int c = threadIdx.x; c < NT * a.G32; c += kThreads) {
+    const int row = c / a.G32, g = c % a.G32;
+    float s = 0.0f;
+    if (64 * g < a.K)
+      for (int i = 0; i < 8; i++) {
+        const uint4 q = *(const uint4 *)(lds + row * row_bytes + 256 * (g >> 1) + 16 * ((8 * (g & 1) + i) ^ (row & 15)));
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) s += bf2f(w[j] & 0xffffu) + bf2f_hi(w[j]);
+      }
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+      const float v = bf2f(f2bf(s));
+      xs[i * NT * a.G32 + c] = (uint16_t)(__float_as_uint(v) >> 16);
+      s -= v;
+    }
+  }
+  __syncthreads();
+
+  int tok[4];
+  Stat st[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    tok[i] = 4 * lg + i < a.T ? a.tokens[4 * lg + i] : -1;
+    st[i] = {kLowest, 0.0f, 0.0f};
+  }
+  const uint8_t *xrow = lds + lr * row_bytes;
+  for (; b < r1; b += kWaves) {
+    load_scales(b + kWaves, sn);
+    asm volatile("" ::: "memory");
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 < GP; p0 += RING) {
+#pragma unroll
+      for (int j = 0; j < RING; j++) {
+        // (every load goes out, pairs past the last for nothing, so that the waits know how many are in flight)
+        const int p = p0 + j;
+        const uint4 q = ring[j];
+        const bool more = p + RING < GP;
+        ring[j] = load_pair(more ? b : b + kWaves, more ? p + RING : min(j, GP - 1));
+        asm volatile("" ::: "memory");
+        if (p < GP) {
+          const uint32_t su = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * ((p & 12) * 4 + lr), (int)(p < 16 ? sb[0][j & 3].x : sb[1][j & 3].x));
+#pragma unroll
+          for (int g = 0; g < 2; g++) {
+            const Frag8 w0 = unpack16(g ? q.z : q.x, um, uc), w1 = unpack16(g ? q.w : q.y, um, uc);
+            const float s = g ? bf2f_hi(su) : bf2f(su & 0xffffu);
+            Frag8 x0, x1;
+            x0.q = *(const uint4 *)(xrow + 256 * p + 16 * ((8 * g + 2 * lg) ^ lr));
+            x1.q = *(const uint4 *)(xrow + 256 * p + 16 * ((8 * g + 2 * lg + 1) ^ lr));
+            f32x4 c = mfma16x16x32(x0, w0, f32x4{0.f, 0.f, 0.f, 0.f});
+            c = mfma16x16x32(x1, w1, c);
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = fmaf(s, c[i], acc[i]);
+          }
+        }
+      }
+    }
+    // biases, as in head_tile_kernel
+#pragma unroll
+    for (int c = 0; c < kFewChunks; c++)
+      if (c < chunks) {
+        Frag8 fs, fb;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const bool in = 16 * c + 4 * lg + j < GP;
+          fs.u[j] = in ? sb[c][j].x : 0u;
+          fb.u[j] = in ? sb[c][j].y : 0u;
+        }
+        f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 2; i >= 0; i--) {
+          Frag8 x;
+          x.q = *(const uint4 *)(xs + (i * NT + lr) * a.G32 + 32 * c + 8 * lg);
+          d = mfma16x16x32(x, fs, d);
+          acc = mfma16x16x32(x, fb, acc);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = fmaf(-16.0f, d[i], acc[i]);
+      }
+#pragma unroll
+    for (int c = 0; c < kFewChunks; c++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) sb[c][j] = sn[c][j];
+    // acc[i]: head row 16 b + lr, token 4 lg + i; every lane keeps its own rows' state
+    bool over = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (tok[i] == 16 * b + lr) a.picked[4 * lg + i] = acc[i];
+      over |= fmaf(acc[i], kLog2e, -st[i].m) > 64.0f;
+    }
+    if (__any(over)) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) st[i] = rebase(st[i], fmaxf(st[i].m, acc[i] * kLog2e));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float y = fmaf(acc[i], kLog2e, -st[i].m), e = __builtin_amdgcn_exp2f(y);
+      st[i].l += e;
+      st[i].t = fmaf(e, y, st[i].t);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    Stat s = st[i];
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) s = join(s, {shfl_xor_f(s.m, o), shfl_xor_f(s.l, o), shfl_xor_f(s.t, o)});
+    if (lr == 0) s_state[wave][0][4 * lg + i] = s.m, s_state[wave][1][4 * lg + i] = s.l, s_state[wave][2][4 * lg + i] = s.t;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < NT; c += kThreads) {
+    Stat s{s_state[0][0][c], s_state[0][1][c], s_state[0][2][c]};
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) s = join(s, {s_state[w][0][c], s_state[w][1][c], s_state[w][2][c]});
+    float *p = a.part + (long long)n * a.segs * 3 * NT + c;
+    p[0] = s.m, p[NT] = s.l, p[2 * NT] = s.t;
+  }
+}
+
 // One wave a token: the runs that met its tile, put together in a fixed order.
 __global__ __launch_bounds__(64) void head_merge_kernel(const HeadArgs a, int NT) {
   const int tok = blockIdx.x, l = lane_id(), tile = tok / NT;
   const long long blocks = a.V >> 4, line = blocks * a.tiles, lo = tile * blocks, hi = lo + blocks;
-  int n0 = (int)(lo * a.parts / line);  // the first run that ends past lo
-  while (line * (n0 + 1) / a.parts <= lo) n0++;
-  while (n0 > 0 && line * n0 / a.parts > lo) n0--;
   Stat s{kLowest, 0.0f, 0.0f};
-  for (int n = n0 + l; n < a.parts; n += 64) {
-    const long long from = line * n / a.parts, to = line * (n + 1) / a.parts;
-    if (from >= hi) break;
-    if (to <= from) continue;
-    const float *q = a.part + ((long long)n * a.segs + tile - (int)(from / blocks)) * 3 * NT + tok % NT;
-    s = join(s, {q[0], q[NT], q[2 * NT]});
+  if (a.tiles == 1) {  // (every run)
+    const float *q = a.part + tok;
+    const long long step = (long long)a.segs * 3 * NT;
+#pragma unroll 4
+    for (int n = l; n < a.parts; n += 64) s = join(s, {q[n * step], q[n * step + NT], q[n * step + 2 * NT]});
+  } else {
+    int n0 = (int)(lo * a.parts / line);  // the first run that ends past lo
+    while (line * (n0 + 1) / a.parts <= lo) n0++;
+    while (n0 > 0 && line * n0 / a.parts > lo) n0--;
+    for (int n = n0 + l; n < a.parts; n += 64) {
+      const long long from = line * n / a.parts, to = line * (n + 1) / a.parts;
+      if (from >= hi) break;
+      if (to <= from) continue;
+      const float *q = a.part + ((long long)n * a.segs + tile - (int)(from / blocks)) * 3 * NT + tok % NT;
+      s = join(s, {q[0], q[NT], q[2 * NT]});
+    }
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) s = join(s, {shfl_xor_f(s.m, o), shfl_xor_f(s.l, o), shfl_xor_f(s.t, o)});
@@ -528,23 +651,54 @@ __global__ __launch_bounds__(64) void head_merge_kernel(const HeadArgs a, int NT
 
 // Token tiles of a launch: 32 TT tokens each, TT as even as they come.
 struct Shape {
-  int tt, tiles, parts, segs, T16, G32;
+  bool few, mid;  // up to 16 rows that fit LDS; one tile of up to 96
+  int tt, tile, tiles, parts, segs, T16, G32;
   long long part_at, picked_at, bytes;
 };
 Shape shape_of(long long T, int K, int V) {
   Shape s;
-  const long long n32 = (T + 31) / 32;
-  s.tiles = (int)((n32 + kMaxTT - 1) / kMaxTT);
-  s.tt = s.tiles ? (int)((n32 + s.tiles - 1) / s.tiles) : 1;
-  const long long line = s.tiles * (long long)(V / 16), fill = (line + 3) / 4;  // (a run of four blocks at least)
-  s.parts = fill < 256 ? (int)(fill < 1 ? 1 : fill) : 256;
-  s.segs = s.tiles / s.parts + 2;
-  s.T16 = s.tiles * s.tt * 32;
+  const int blocks = V / 16;
   s.G32 = (K / 64 + 31) / 32 * 32;
+  s.mid = mid_tile(T, K) > 0;
+  s.few = T <= 16 && 32LL * K <= kFewBytes;
+  if (s.few) {
+    s.tt = 0;
+    s.tile = 16;
+    s.tiles = s.segs = 1;
+    s.parts = (blocks + kWaves - 1) / kWaves < 256 ? (blocks + kWaves - 1) / kWaves : 256;
+    s.T16 = 0;  // (their sums stay in LDS)
+  } else if (s.mid) {
+    s.tt = 0;
+    s.tile = mid_tile(T, K);
+    s.tiles = s.segs = 1;
+    s.parts = mid_parts(V);
+    s.T16 = 0;
+  } else {
+    const long long n32 = (T + 31) / 32;
+    s.tiles = (int)((n32 + kMaxTT - 1) / kMaxTT);
+    s.tt = s.tiles ? (int)((n32 + s.tiles - 1) / s.tiles) : 1;
+    s.tile = 32 * s.tt;
+    const long long fill = (s.tiles * (long long)blocks + 3) / 4;  // (a run of four blocks at least)
+    s.parts = fill < 256 ? (int)(fill < 1 ? 1 : fill) : 256;
+    s.segs = s.tiles / s.parts + 2;
+    s.T16 = s.tiles * s.tile;
+  }
   s.part_at = ((long long)3 * s.T16 * s.G32 * 2 + 15) / 16 * 16;
-  s.picked_at = s.part_at + 4LL * 3 * s.parts * s.segs * 32 * s.tt;
+  s.picked_at = s.part_at + 4LL * 3 * s.parts * s.segs * s.tile;
   s.bytes = s.picked_at + 4 * T;
   return s;
+}
+
+template <int RING>
+int launch_few(const HeadArgs &a, hipStream_t st) {
+  static const bool wide = [] {  // (more than the static limit)
+    (void)hipFuncSetAttribute((const void *)&head_few_kernel<RING>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                              kFewBytes + 3 * 16 * 32 * kFewChunks * 2);
+    return true;
+  }();
+  (void)wide;
+  head_few_kernel<RING><<<a.parts, kThreads, (size_t)16 * (2 * a.K + 6 * a.G32), st>>>(a);
+  return jit::check_launch("jit_head_logprobs");
 }
 
 template <int TT>
@@ -584,16 +738,22 @@ extern "C" int jit_head_logprobs(const uint16_t *x, int T, int K, const void *w,
   HeadArgs a{x, (const uint8_t *)w, tokens, (uint16_t *)ws, (float *)(ws + s.part_at), (float *)(ws + s.picked_at),
              logprob, entropy, lse, T, K, V, s.parts, s.segs, s.tiles, s.T16, s.G32};
   const hipStream_t st = (hipStream_t)stream;
-  head_xsum_kernel<<<dim3(s.T16, s.G32 / 32), 64, 0, st>>>(x, T, K, s.T16, s.G32, (uint16_t *)ws);
-  int rc = jit::check_launch("jit_head_logprobs (sums)");
-  if (rc != JIT_OK) return rc;
-  switch (s.tt) {
-    case 1: rc = launch_tile<1>(a, st); break;
-    case 2: rc = launch_tile<2>(a, st); break;
-    case 3: rc = launch_tile<3>(a, st); break;
-    default: rc = launch_tile<4>(a, st); break;
+  int rc;
+  if (s.few) {
+    rc = K % 2048 == 0 ? launch_few<16>(a, st) : launch_few<8>(a, st);
+  } else if (s.mid) {
+    rc = launch_mid(a, st);
+  } else {
+    head_xsum_kernel<<<dim3(s.T16, s.G32 / 32), 64, 0, st>>>(x, T, K, s.T16, s.G32, (uint16_t *)ws);
+    if ((rc = jit::check_launch("jit_head_logprobs (sums)")) != JIT_OK) return rc;
+    switch (s.tt) {
+      case 1: rc = launch_tile<1>(a, st); break;
+      case 2: rc = launch_tile<2>(a, st); break;
+      case 3: rc = launch_tile<3>(a, st); break;
+      default: rc = launch_tile<4>(a, st); break;
+    }
   }
   if (rc != JIT_OK) return rc;
-  head_merge_kernel<<<T, 64, 0, st>>>(a, 32 * s.tt);
+  head_merge_kernel<<<T, 64, 0, st>>>(a, s.tile);
   return jit::check_launch("jit_head_logprobs (merge)");
 }
