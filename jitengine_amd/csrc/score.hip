@@ -1,26 +1,32 @@
 // Scoring of given tokens from rows of logits for gfx950: log-probability, rank, entropy and the most likely
 // alternatives in one pass over each row.
 //
-// With m = max x, l = sum e^(x - m) and t = sum (x - m) e^(x - m) over a row:
-//   log-probability of v = (x_v - m) - ln l,   entropy = ln l - t / l,
+// With m = max x over a row and, in base 2, y = (x - m) log2 e, l = sum 2^y, t = sum y 2^y:
+//   log-probability of v = (y_v - log2 l) ln 2,   entropy = (log2 l - t / l) ln 2,
 //   rank of v = #{j : x_j > x_v, or x_j = x_v and j < v}.
-// Every lane keeps its own (m, l, t), rescaled where its largest value grows:
-//   l' = l e^(m - m'),   t' = (t + l (m - m')) e^(m - m'),
-// and lanes, waves and slices meet by the same rule with sums in a fixed order, so a call's bits repeat.  m starts at
-// the lowest finite value and x - m is kept above -1000 (e^-1000 is 0 in fp32): masked entries (-inf, or the type's
-// lowest value beside larger ones) add 0 to l and t, and a row of nothing but lowest values is uniform.
+// Every lane keeps its own (m, l, t), rescaled where its largest value grows; lanes, waves and slices meet by the same
+// rule in a fixed order, so a call's bits repeat.  y is one fused multiply-add x log2 e - (m log2 e), whose second term's
+// rounding is the same for every y and cancels; rows whose largest magnitude would overflow there take (x - m) log2 e.
+// Masked entries (-inf, or the type's lowest value beside larger ones) add 0; a row of nothing but lowest values is uniform.
 //
-// A row is cut into slices (one workgroup each) until the launch fills the chip; the slices' results meet in a second,
-// small launch.  Alternatives: each wave keeps its `top` best (value, index) in order, one a lane, and looks at a lane's
-// values one by one only where the lane's largest (which the softmax has formed anyway) passes the wave's last.
+// A row is cut into slices, one workgroup each, until the launch fills the chip; a second, small launch puts a row's
+// slices together.  Alternatives: a wave keeps the values that pass a threshold in LDS (the threshold is the `top`-th
+// largest of its lanes' largest, found bit by bit with ballots, later of what it has kept), and what is kept at the end is
+// put in order by counting, for each, those that stand before it.  Lists kept in order by insertion cost 4 times as much
+// (32 rows, 20 alternatives: 67 + 19 us).
+//
+// What bounds it: many rows, the vector ALU (a value takes 5 1/2 instructions of 4 cycles and an exponential of 16, one
+// instruction more for the rank: 2,048 rows of 151,936 bf16 values, 622 MB, in 165 us, 3.8 TB/s; a large copy reaches 4.8);
+// few rows, latency: 1 row of 151,936 in 6.5 + 5.4 us of two launches, 32 rows of 248,320 under a mask in 17.4 + 5.8.
 #include "common.hpp"
 
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxTop = 64, kMaxTokens = 64, kMaxSlices = 64;
-constexpr float kLowest = -3.402823466e38f, kFloor = -1000.0f, kLog2e = 1.44269504088896341f;
-constexpr int kNone = 0x7fffffff;  // the index of an alternative that is not there
+constexpr int kRoom = 128;  // values a wave keeps: at least kMaxTop + 64
+constexpr float kLowest = -3.402823466e38f, kFloor = -2000.0f, kLog2e = 1.44269504088896341f;
+constexpr double kLn2 = 0.693147180559945309;
 
 struct ScoreArgs {
   const void *x;
@@ -28,7 +34,7 @@ struct ScoreArgs {
   const int32_t *tokens;  // [B, nt]
   float *logprob, *entropy, *top_lp;
   int32_t *rank, *top_ids;
-  float *part;  // [B, ns, words]: m, l, t, -, nt counts, top (value, index)
+  float *part;  // [B, ns, words]: m, l, t, -, nt counts, then top keys
   int B, V, nt, top, ns, slice, words;
 };
 
@@ -37,6 +43,7 @@ struct Elems;  // 16 bytes of a row's values
 template <>
 struct Elems<uint16_t> {
   static constexpr int N = 8;
+  static constexpr uint32_t kLowestWord = 0xff80ff80u;  // -inf
   static __device__ __forceinline__ float one(const uint16_t *p) { return bf2f(*p); }
   static __device__ __forceinline__ void widen(const uint4 &q, float *v) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -47,113 +54,211 @@ struct Elems<uint16_t> {
 template <>
 struct Elems<float> {
   static constexpr int N = 4;
+  static constexpr uint32_t kLowestWord = 0xff800000u;
   static __device__ __forceinline__ float one(const float *p) { return *p; }
   static __device__ __forceinline__ void widen(const uint4 &q, float *v) {
     v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
   }
 };
 
+// One of four.
+__device__ __forceinline__ uint32_t pick(uint4 q, int i) {
+  const uint32_t lo = i & 1 ? q.y : q.x, hi = i & 1 ? q.w : q.z;
+  return i & 2 ? hi : lo;
+}
+
+// Value j of a lane's words.
+template <typename T>
+__device__ __forceinline__ float value_at(uint4 q0, uint4 q1, int j) {
+  constexpr int P = 4 / sizeof(T);
+  const uint32_t a = pick(q0, j / P), b = pick(q1, j / P), w = j / P & 4 ? b : a;
+  if constexpr (sizeof(T) == 2)
+    return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+  else
+    return __uint_as_float(w);
+}
+
+// The largest value below x > -inf (so that v >= x is v > prev(x)).
+__device__ __forceinline__ float prev(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return __uint_as_float(u == 0 ? 0x80000001u : u & 0x80000000u ? u + 1 : u - 1);
+}
+
+// ------------------------------------------------------------------ a row's softmax
 struct Stat {
   float m, l, t;
 };
 
-// e^d for a d that is at most 0 (or NaN, which stays).
-__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+// y from one reference to a larger one: between the two rounded terms, so that it adds no error (floor at -2000, where
+// 2^y is 0; a NaN stays one).
+__device__ __forceinline__ float between(float a, float b) {
+#pragma clang fp contract(off)
+  const float ra = a * kLog2e, rb = b * kLog2e, r = fabsf(rb) < __builtin_inff() ? ra - rb : (a - b) * kLog2e;
+  return r < kFloor ? kFloor : r;
+}
+
+__device__ __forceinline__ Stat rebase(const Stat &s, float m) {
+  const float d = s.m == m ? 0.0f : between(s.m, m), e = __builtin_amdgcn_exp2f(d);
+  return {m, s.l * e, fmaf(s.l, d, s.t) * e};
+}
 
 __device__ __forceinline__ Stat join(const Stat &a, const Stat &b) {
   const float m = fmaxf(a.m, b.m);
-  const float da = fmaxf(a.m - m, kFloor), db = fmaxf(b.m - m, kFloor);
-  const float ea = exp_of(da), eb = exp_of(db);
-  return {m, fmaf(a.l, ea, b.l * eb), fmaf(fmaf(a.l, da, a.t), ea, fmaf(b.l, db, b.t) * eb)};
+  const Stat p = rebase(a, m), q = rebase(b, m);
+  return {m, p.l + q.l, p.t + q.t};
 }
 
 __device__ __forceinline__ Stat wave_join(Stat s) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) s = join(s, {shfl_xor_f(s.m, o), shfl_xor_f(s.l, o), shfl_xor_f(s.t, o)});
-  return s;
+  const Stat r = rebase(s, wave_butterfly<true>(s.m));
+  return {r.m, wave_butterfly<false>(r.l), wave_butterfly<false>(r.t)};
 }
 
-// Whether (v, i) stands before (w, j): larger value, then lower index.  A NaN stands before nothing.
-__device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+// The log-probability of a logit x in a row of state s, log_l = log2 l.
+__device__ __forceinline__ float logprob_of(float x, const Stat &s, double log_l) {
+  if (s.l != s.l) return __builtin_nanf("");  // a NaN or +inf in the row
+  if (!(x > -__builtin_inff())) return x;     // (-inf, also in a row of nothing else; or a NaN)
+  const float mb = s.m * kLog2e;
+  const double y = fabsf(mb) < __builtin_inff() ? (double)x * (double)kLog2e - (double)mb
+                                                : ((double)x - (double)s.m) * (double)kLog2e;
+  return (float)((y - log_l) * kLn2);
+}
 
-__device__ __forceinline__ float lane_f(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
+// ------------------------------------------------------------------ order
+// A value and its index as one number, larger for what stands before: the larger value, then the lower index.  0 is none.
+__device__ __forceinline__ uint64_t key_of(float v, int i) {
+  const uint32_t u = __float_as_uint(v + 0.0f);  // (-0 ties +0)
+  return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+__device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k; }
 
-// A wave's best alternatives, lane i the i-th (lanes from `top` on hold what fell off).
-struct Best {
-  float v;
-  int i;
-  float last_v;  // of lane top - 1 (uniform)
-  int last_i;
-  __device__ __forceinline__ void clear() { v = last_v = -__builtin_inff(), i = last_i = kNone; }
-  __device__ __forceinline__ void insert(float nv, int ni, int top) {  // (uniform)
-    const int p = __builtin_popcountll(__ballot(before(v, i, nv, ni)));
-    const int l = lane_id();
-    const float pv = __shfl_up(v, 1, 64);
-    const int pi = __shfl_up(i, 1, 64);
-    v = l < p ? v : l == p ? nv : pv;
-    i = l < p ? i : l == p ? ni : pi;
-    last_v = lane_f(v, top - 1);
-    last_i = __builtin_amdgcn_readlane(i, top - 1);
+// The n-th largest of the lanes' values (-inf where fewer are numbers): bit by bit from the top over order-preserving keys;
+// a bf16 is decided by its 16 bits.
+template <int BITS>
+__device__ __forceinline__ float nth_of_lanes(float v, int n) {
+  const uint32_t u = __float_as_uint(v + 0.0f), k = v == v ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
+  uint32_t least = 0;
+  for (int bit = 31; bit >= 32 - BITS; bit--) {
+    const uint32_t at = least | 1u << bit;
+    if (__builtin_popcountll(__ballot(k >= at)) >= n) least = at;
+  }
+  const float r = __uint_as_float((least & 0x80000000u ? least ^ 0x80000000u : ~least) & ~(uint32_t)0 << (32 - BITS));
+  return r == r && least ? r : -__builtin_inff();
+}
+
+// What a wave keeps of its values: keys in LDS (kRoom, and space for the first kMaxTop of them in order).  `top` of the
+// values met are not below `bar`; what ties it may stand before them in the step that set it, and stands behind them later.
+struct Kept {
+  uint64_t *at;
+  int count;  // (uniform)
+  float bar, least;  // a value passes that is larger than `least`: bar, or the value before it
+  __device__ __forceinline__ void raise(float v) { bar = fmaxf(bar, v), least = prev(bar); }
+  // Takes the values that pass of every lane's words x (as bits q), of indices i + j + u step.
+  template <typename T, int U, int N>
+  __device__ __forceinline__ void put(const float (&x)[U][N], const uint4 (&q)[U], int i, int step, int top) {
+    uint32_t bits = 0;  // the first value's on top
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int j = 0; j < N; j++) bits = bits + bits + (x[u][j] > least);
+    uint64_t mask;
+    while ((mask = __ballot(bits != 0))) {
+      if (count + __builtin_popcountll(mask) > kRoom) squeeze(top);
+      const int at_bit = 31 - __builtin_clz(bits | 1), j = U * N - 1 - at_bit;
+      if (bits) {
+        const int lower = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+        at[count + lower] = key_of(value_at<T>(q[0], q[U - 1], j), i + (j / N) * step + j % N);
+        bits ^= 1u << at_bit;
+      }
+      count += __builtin_popcountll(mask);
+    }
+  }
+  // Leaves the `top` first, in order.
+  __device__ __forceinline__ void squeeze(int top) {
+    uint64_t *to = at + kRoom;
+    for (int e = lane_id(); e < (count + 63) / 64 * 64; e += 64) {
+      const uint64_t k = e < count ? at[e] : 0;
+      int r = 0;
+#pragma unroll 4
+      for (int j = 0; j < count; j++) r += at[j] > k;
+      if (k && r < top) to[r] = k;
+    }
+    count = min(count, top);
+    if (lane_id() < count) at[lane_id()] = to[lane_id()];
+    if (count == top) raise(key_value(to[top - 1]));
   }
 };
 
-// The `top` best of n sorted lists (n <= 64), lane j walking list j: at(j, k) is its k-th entry.  Called by a whole
-// wave; put(k, v, i) by every lane with the k-th best.
-template <typename At, typename Put>
-__device__ __forceinline__ void merge_lists(int n, int top, At &&at, Put &&put) {
-  const int l = lane_id();
-  int k = 0;
-  float v = -__builtin_inff();
-  int i = kNone;
-  if (l < n) at(l, 0, v, i);
-  for (int r = 0; r < top; r++) {
-    float bv = v;
-    int bi = i;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const float ov = shfl_xor_f(bv, o);
-      const int oi = __shfl_xor(bi, o, 64);
-      if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
-    }
-    put(r, bv, bi);
-    if (bi != kNone && i == bi) {  // (indices differ between the lists)
-      k++;
-      v = -__builtin_inff(), i = kNone;
-      if (k < top) at(l, k, v, i);
-    }
+// The first `top` of n keys in LDS, put(r, key) by the thread that has the r-th; every thread of the workgroup calls it.
+template <typename Put>
+__device__ __forceinline__ void rank_keys(const uint64_t *keys, int n, int top, Put &&put) {
+  for (int e = threadIdx.x; e < n; e += kThreads) {
+    const uint64_t k = keys[e];
+    int r = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; j++) r += keys[j] > k;
+    if (k && r < top) put(r, k);
   }
 }
 
-// The outputs of row b from its state, its tokens' counts and its alternatives.
-__device__ __forceinline__ float logprob_of(float x, const Stat &s, double ln_l) {
-  if (s.l != s.l) return __builtin_nanf("");       // a NaN or +inf in the row
-  if (!(x > -__builtin_inff())) return x;          // (-inf, also in a row of nothing else; or a NaN)
-  return (float)((double)x - (double)s.m - ln_l);
-}
-
-template <typename T>
-__device__ __forceinline__ void write_row(const ScoreArgs &a, int b, const Stat &s, int tid, int threads, const int *counts) {
+// Outputs of row b that need its whole state; counts of the values before each token.
+template <typename T, typename Count>
+__device__ __forceinline__ void write_row(const ScoreArgs &a, int b, const Stat &s, double log_l, int tid, int threads,
+                                          Count &&count_of) {
   const T *row = (const T *)a.x + (long long)b * a.stride;
-  const double ln_l = log((double)s.l);
-  if (tid == 0) a.entropy[b] = s.l != s.l ? __builtin_nanf("") : s.l > 0.0f ? (float)fmax(ln_l - (double)s.t / (double)s.l, 0.0) : 0.0f;
+  if (tid == 0) {
+    const float h = s.l > 0.0f ? (float)(fmax(log_l - (double)s.t / (double)s.l, 0.0) * kLn2) : 0.0f;
+    a.entropy[b] = s.l != s.l ? __builtin_nanf("") : h;
+  }
   for (int q = tid; q < a.nt; q += threads) {
     const int tok = a.tokens[(long long)b * a.nt + q];
     const bool in = tok >= 0 && tok < a.V;
     const float x = in ? Elems<T>::one(row + tok) : 0.0f;
-    a.logprob[(long long)b * a.nt + q] = in ? logprob_of(x, s, ln_l) : 0.0f;
-    a.rank[(long long)b * a.nt + q] = in && x == x ? counts[q] : -1;
+    a.logprob[(long long)b * a.nt + q] = in ? logprob_of(x, s, log_l) : 0.0f;
+    a.rank[(long long)b * a.nt + q] = in && x == x ? count_of(q) : -1;
   }
 }
 
+__device__ __forceinline__ void write_alternative(const ScoreArgs &a, int b, const Stat &s, double log_l, int r, uint64_t k) {
+  a.top_ids[(long long)b * a.top + r] = key_index(k);
+  a.top_lp[(long long)b * a.top + r] = logprob_of(key_value(k), s, log_l);
+}
+
+// Fewer than `top` logits of row b are numbers above -inf: its -inf entries follow in order of index (log-probability
+// -inf, or NaN in a NaN row), -1 and NaN past the last number.  One wave.
+template <typename T>
+__device__ __forceinline__ void write_rest(const ScoreArgs &a, int b, const Stat &s, int have) {
+  const T *row = (const T *)a.x + (long long)b * a.stride;
+  const int l = lane_id();
+  for (int i0 = 0; i0 < a.V && have < a.top; i0 += 64) {
+    const bool is = i0 + l < a.V && Elems<T>::one(row + i0 + l) == -__builtin_inff();
+    const uint64_t mask = __ballot(is);
+    const int r = have + __builtin_popcountll(mask & (((uint64_t)1 << l) - 1));
+    if (is && r < a.top) {
+      a.top_ids[(long long)b * a.top + r] = i0 + l;
+      a.top_lp[(long long)b * a.top + r] = s.l != s.l ? __builtin_nanf("") : -__builtin_inff();
+    }
+    have += __builtin_popcountll(mask);
+  }
+  for (int r = have + l; r < a.top; r += 64) {
+    a.top_ids[(long long)b * a.top + r] = -1;
+    a.top_lp[(long long)b * a.top + r] = __builtin_nanf("");
+  }
+}
+
+// ------------------------------------------------------------------ a slice of a row
 // U: 16-byte words a thread takes of a step.
 template <typename T, int U>
 __global__ __launch_bounds__(kThreads) void score_rows_kernel(const ScoreArgs a) {
-  constexpr int N = Elems<T>::N, kStep = kThreads * U;  // values of a word, words of a step
+  constexpr int N = Elems<T>::N, kStep = kThreads * U, kBits = sizeof(T) * 8;  // values of a word, words of a step
+  constexpr float kInf = __builtin_inff();
   __shared__ Stat s_stat[kWaves];
-  __shared__ float s_x[kMaxTokens];
-  __shared__ int s_tok[kMaxTokens], s_cnt[kMaxTokens];
-  __shared__ float s_v[kWaves][kMaxTop];
-  __shared__ int s_i[kWaves][kMaxTop];
+  __shared__ float s_x[kMaxTokens], s_bar[kWaves];
+  __shared__ int s_tok[kMaxTokens], s_cnt[kWaves][kMaxTokens], s_n;
+  __shared__ uint64_t s_keep[kWaves * (kRoom + kMaxTop)];
   const int b = blockIdx.x / a.ns, sl = blockIdx.x % a.ns;
   const int tid = threadIdx.x, wave = tid >> 6;
   const T *row = (const T *)a.x + (long long)b * a.stride;
@@ -161,201 +266,294 @@ __global__ __launch_bounds__(kThreads) void score_rows_kernel(const ScoreArgs a)
   const int off = (int)(((uintptr_t)row & 15) / sizeof(T));
   const int words = (a.V + off + N - 1) / N;
   const int w0 = sl * a.slice, w1 = min(words, w0 + a.slice);
-  for (int q = tid; q < a.nt; q += kThreads) {
-    const int tok = a.tokens[(long long)b * a.nt + q];
-    const bool in = tok >= 0 && tok < a.V;
-    s_tok[q] = in ? tok : -1;
-    s_x[q] = in ? Elems<T>::one(row + tok) : __builtin_nanf("");
-    s_cnt[q] = 0;
-  }
-  __syncthreads();
-  const float xt = a.nt ? s_x[0] : __builtin_nanf("");
-  const int tok = a.nt ? s_tok[0] : -1;
-  Stat st{kLowest, 0.0f, 0.0f};
-  Best best;
-  best.clear();
-  int count = 0;  // the wave's values before the first token's (uniform)
-
-  auto step = [&](int base) {
-    float x[U][N];
-    bool whole = true;
+  uint4 raw[U];
+  auto load = [&](int base) {
+    if (base + kStep <= w1 && base * N >= off && (base + kStep) * N - off <= a.V) {
+#pragma unroll
+      for (int u = 0; u < U; u++) raw[u] = *(const uint4 *)(row + ((base + u * kThreads + tid) * N - off));
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int w = base + u * kThreads + tid, i0 = w * N - off;
-      if (w < w1 && i0 >= 0 && i0 + N <= a.V) {
-        Elems<T>::widen(*(const uint4 *)(row + i0), x[u]);
-      } else {  // past the slice, or a word that the row's ends cut
-        whole = false;
-#pragma unroll
-        for (int j = 0; j < N; j++)
-          x[u][j] = w < w1 && i0 + j >= 0 && i0 + j < a.V ? Elems<T>::one(row + i0 + j) : -__builtin_inff();
+      constexpr uint32_t kLow = Elems<T>::kLowestWord;
+      raw[u] = {kLow, kLow, kLow, kLow};
+      if (w >= w1) continue;
+      if (i0 >= 0 && i0 + N <= a.V) {
+        raw[u] = *(const uint4 *)(row + i0);
+      } else {  // a word that the row's ends cut
+        uint64_t h[2] = {kLow | (uint64_t)kLow << 32, kLow | (uint64_t)kLow << 32};
+#pragma unroll 1
+        for (int j = 0; j < N; j++) {
+          if (i0 + j < 0 || i0 + j >= a.V) continue;
+          const int at = j * kBits & 63;
+          const uint64_t ones = (((uint64_t)1 << kBits) - 1) << at;
+          uint64_t v;
+          if constexpr (sizeof(T) == 2)
+            v = row[i0 + j];
+          else
+            v = __float_as_uint(row[i0 + j]);
+          if (j * 2 < N)
+            h[0] = (h[0] & ~ones) | v << at;
+          else
+            h[1] = (h[1] & ~ones) | v << at;
+        }
+        raw[u] = {(uint32_t)h[0], (uint32_t)(h[0] >> 32), (uint32_t)h[1], (uint32_t)(h[1] >> 32)};
       }
     }
-    float top = -__builtin_inff();
+  };
+  load(w0);
+  float xt = __builtin_nanf("");
+  int tok = -1, count = 0;  // the wave's values before the only token's (uniform)
+  if (a.nt == 1) {
+    tok = a.tokens[b];
+    if (tok >= 0 && tok < a.V) {
+      // (and what equals it in its own word)
+      const int wt = (tok + off) / N, i = wt * N - off + tid;
+      xt = Elems<T>::one(row + tok);
+      if (wt >= w0 && wt < w1 && wave == 0) count = __builtin_popcountll(__ballot(i >= 0 && i < tok && Elems<T>::one(row + i) == xt));
+    } else {
+      tok = -1;
+    }
+  } else if (a.nt) {
+    for (int q = tid; q < a.nt; q += kThreads) {
+      const int t = a.tokens[(long long)b * a.nt + q];
+      const bool in = t >= 0 && t < a.V;
+      s_tok[q] = in ? t : -1;
+      s_x[q] = in ? Elems<T>::one(row + t) : __builtin_nanf("");
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) s_cnt[w][q] = 0;
+    }
+    __syncthreads();
+  }
+  Stat st{kLowest, 0.0f, 0.0f};
+  Kept kept{s_keep + wave * (kRoom + kMaxTop), 0, -kInf, -kInf};
+
+  for (int base = w0; base < w1; base += kStep) {
+    float x[U][N];
+    uint4 cur[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) cur[u] = raw[u], Elems<T>::widen(raw[u], x[u]);
+    if (base + kStep < w1) load(base + kStep);
+    float top = -kInf;
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int j = 0; j < N; j++) top = fmaxf(top, x[u][j]);
-    if (top > st.m) {
-      const float d = fmaxf(st.m - top, kFloor), e = exp_of(d);
-      st.t = fmaf(st.l, d, st.t) * e;
-      st.l *= e;
-      st.m = top;
+    if (top > st.m) st = rebase(st, top);
+    // a lane that has met nothing but masked values takes the wave's largest
+    if (!__all(fabsf(st.m * kLog2e) < kInf)) {
+      st = rebase(st, wave_butterfly<true>(st.m));
     }
+    const float ref = st.m * kLog2e;
+    const bool huge = !__all(fabsf(ref) < kInf);
+    float l = st.l, t = st.t;
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int j = 0; j < N; j++) {
-        // (not fmaxf: a NaN has to stay one)
-        const float r = x[u][j] - st.m, d = r < kFloor ? kFloor : r, e = exp_of(d);
-        st.l += e;
-        st.t = fmaf(e, d, st.t);
+        const float y = fmaf(x[u][j], kLog2e, -ref), e = __builtin_amdgcn_exp2f(y);
+        l += e;
+        t = fmaf(e, y, t);
       }
-    const bool all = __all(whole);
-    // ranks: a step behind or before the token compares one way
-    const int i_lo = base * N - off, i_hi = (base + kStep) * N - off;
-    if (a.nt == 1 && all && (i_hi <= tok || i_lo > tok)) {
-      if (i_lo > tok) {
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-          for (int j = 0; j < N; j++) count += __builtin_popcountll(__ballot(x[u][j] > xt));
-      } else {
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-          for (int j = 0; j < N; j++) count += __builtin_popcountll(__ballot(x[u][j] >= xt));
-      }
-    } else {
-      for (int q = 0; q < a.nt; q++) {
-        const float xq = s_x[q];
-        const int tq = s_tok[q];
-        int c = 0;
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-          for (int j = 0; j < N; j++) {
-            const int w = base + u * kThreads + tid, i = w * N - off + j;
-            const bool in = w < w1 && i >= 0 && i < a.V;
-            c += __builtin_popcountll(__ballot(in && before(x[u][j], i, xq, tq)));
-          }
-        if (a.nt == 1) count += c;
-        else if (lane_id() == 0 && c) atomicAdd(&s_cnt[q], c);
-      }
-    }
-    if (a.top && __any(top > best.last_v || best.last_i == kNone)) {
+    // once more where a masked value (0 times -inf) or a NaN is among them, or y overflows (one instruction a value less
+    // for rows without)
+    if (huge || __any(t != t)) {
+      l = st.l, t = st.t;
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
         for (int j = 0; j < N; j++) {
-          const int w = base + u * kThreads + tid, i = w * N - off + j;
-          const bool in = w < w1 && i >= 0 && i < a.V;
-          const float v = x[u][j];
-          uint64_t mask = __ballot(in && before(v, i, best.last_v, best.last_i));
-          while (mask) {
-            const int l = __builtin_ctzll(mask);
-            best.insert(lane_f(v, l), __builtin_amdgcn_readlane(i, l), a.top);
-            mask &= mask - 1;
-            mask &= __ballot(before(v, i, best.last_v, best.last_i));
-          }
+          const float r = huge ? (x[u][j] - st.m) * kLog2e : fmaf(x[u][j], kLog2e, -ref), y = r < kFloor ? kFloor : r;
+          const float e = __builtin_amdgcn_exp2f(y);
+          l += e;
+          t = fmaf(e, y, t);
         }
     }
-  };
-  for (int base = w0; base < w1; base += kStep) step(base);
+    st.l = l, st.t = t;
+    // ranks: a value equal to a token's counts where it is in a word before the token's (the token's own word below;
+    // -inf, what fills words up, never passes)
+    for (int q = 0; q < a.nt; q++) {
+      const float xq = a.nt == 1 ? xt : s_x[q];
+      const int wq = ((a.nt == 1 ? tok : s_tok[q]) + off) / N;
+      const float pq = xq > -kInf ? prev(xq) : xq;
+      int c = 0;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const float least = base + u * kThreads + tid < wq ? pq : xq;
+#pragma unroll
+        for (int j = 0; j < N; j++) c += __builtin_popcountll(__ballot(x[u][j] > least));
+      }
+      if (a.nt == 1)
+        count += c;
+      else if (lane_id() == 0)
+        s_cnt[wave][q] += c;
+    }
+    if (a.top && __any(top > kept.least)) {
+      if (__builtin_popcountll(__ballot(top > kept.least)) >= a.top) kept.raise(nth_of_lanes<kBits>(top, a.top));
+      kept.put<T>(x, cur, (base + tid) * N - off, kThreads * N, a.top);
+      kept.least = kept.bar;
+    }
+  }
 
+  // what equals one of several tokens in its own word before it; of a -inf token, all that is -inf before it
+  if (a.nt > 1 || xt == -kInf) {
+    for (int q = wave; q < a.nt; q += kWaves) {
+      const float xq = a.nt == 1 ? xt : s_x[q];
+      const int tq = a.nt == 1 ? tok : s_tok[q], wq = (tq + off) / N;
+      const int from = xq == -kInf ? w0 : max(w0, wq), to = min(w1, a.nt == 1 ? wq : wq + 1);
+      const int i1 = min(tq, to * N - off);
+      int c = 0;
+      for (int i0 = max(0, from * N - off); i0 < i1; i0 += 64) {
+        const int i = i0 + lane_id();
+        c += __builtin_popcountll(__ballot(i < i1 && Elems<T>::one(row + i) == xq));
+      }
+      if (a.nt == 1)
+        count += c;
+      else if (lane_id() == 0)
+        s_cnt[wave][q] += c;
+    }
+  }
   st = wave_join(st);
+  if (kept.count > kMaxTop) kept.squeeze(a.top);
   if (lane_id() == 0) {
     s_stat[wave] = st;
-    if (a.nt == 1 && count) atomicAdd(&s_cnt[0], count);
+    s_bar[wave] = kept.bar;
+    if (a.nt == 1) s_cnt[wave][0] = count;
   }
-  if (lane_id() < a.top) s_v[wave][lane_id()] = best.v, s_i[wave][lane_id()] = best.i;
+  if (tid == 0) s_n = 0;
   __syncthreads();
   st = s_stat[0];
 #pragma unroll
   for (int w = 1; w < kWaves; w++) st = join(st, s_stat[w]);
-  const double ln_l = log((double)st.l);
+  float *part = a.part + (long long)blockIdx.x * a.words;
+  auto count_of = [&](int q) {
+    int c = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) c += s_cnt[w][q];
+    return c;
+  };
+  double log_l = 0.0;
   if (a.ns == 1) {
-    write_row<T>(a, b, st, tid, kThreads, s_cnt);
+    log_l = log2((double)st.l);
+    write_row<T>(a, b, st, log_l, tid, kThreads, count_of);
   } else {
-    float *p = a.part + (long long)blockIdx.x * a.words;
-    if (tid == 0) p[0] = st.m, p[1] = st.l, p[2] = st.t;
-    for (int q = tid; q < a.nt; q += kThreads) ((int *)p)[4 + q] = s_cnt[q];
+    if (tid == 0) part[0] = st.m, part[1] = st.l, part[2] = st.t;
+    for (int q = tid; q < a.nt; q += kThreads) ((int *)part)[4 + q] = count_of(q);
   }
-  if (a.top && wave == 0) {
-    merge_lists(
-        kWaves, a.top, [&](int w, int k, float &v, int &i) { v = s_v[w][k], i = s_i[w][k]; },
-        [&](int r, float v, int i) {
-          if (lane_id() != 0) return;
-          if (a.ns == 1) {
-            a.top_ids[(long long)b * a.top + r] = i == kNone ? -1 : i;
-            a.top_lp[(long long)b * a.top + r] = i == kNone ? __builtin_nanf("") : logprob_of(v, st, ln_l);
-          } else {
-            float *p = a.part + (long long)blockIdx.x * a.words + 4 + a.nt + 2 * r;
-            p[0] = v;
-            ((int *)p)[1] = i;
-          }
-        });
+  if (!a.top) return;
+  // what the waves have kept, but for what is below the largest bar
+  __shared__ uint64_t s_all[kWaves * kMaxTop];
+  float bar = s_bar[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; w++) bar = fmaxf(bar, s_bar[w]);
+  if (lane_id() < kept.count) {
+    const uint64_t k = kept.at[lane_id()];
+    if (key_value(k) >= bar) s_all[atomicAdd(&s_n, 1)] = k;  // (in any order: they are ranked)
+  }
+  __syncthreads();
+  const int n = s_n;
+  uint64_t *to = (uint64_t *)(part + 4 + a.nt + (a.nt & 1));
+  rank_keys(s_all, n, a.top, [&](int r, uint64_t k) {
+    if (a.ns == 1)
+      write_alternative(a, b, st, log_l, r, k);
+    else
+      to[r] = k;
+  });
+  if (a.ns == 1) {
+    if (n < a.top && wave == 0) write_rest<T>(a, b, st, n);
+  } else {
+    for (int r = n + tid; r < a.top; r += kThreads) to[r] = 0;
   }
 }
 
-// The slices of a row put together by one wave.
+// ------------------------------------------------------------------ the slices of a row put together
 template <typename T>
-__global__ __launch_bounds__(64) void score_merge_kernel(const ScoreArgs a) {
-  __shared__ int s_cnt[kMaxTokens];
-  extern __shared__ float s_list[];  // [ns][top] values, then indices
-  const int b = blockIdx.x, l = lane_id();
+__global__ __launch_bounds__(kThreads) void score_merge_kernel(const ScoreArgs a) {
+  __shared__ Stat s_stat;
+  __shared__ int s_cnt[kMaxTokens], s_n;
+  __shared__ uint64_t s_least;
+  extern __shared__ uint64_t s_keys[];  // [ns top] the slices' keys, then those that pass
+  const int b = blockIdx.x, tid = threadIdx.x, l = lane_id(), wave = tid >> 6, all = a.ns * a.top;
   const float *part = a.part + (long long)b * a.ns * a.words;
-  Stat st{kLowest, 0.0f, 0.0f};
-  if (l < a.ns) st = {part[l * a.words], part[l * a.words + 1], part[l * a.words + 2]};
-  int *s_idx = (int *)s_list + a.ns * a.top;
-  for (int e = l; e < a.ns * a.top; e += 64) {
-    const int s = e / a.top, k = e % a.top;
-    const float *p = part + s * a.words + 4 + a.nt + 2 * k;
-    s_list[e] = p[0];
-    s_idx[e] = ((const int *)p)[1];
+  const int keys_at = 4 + a.nt + (a.nt & 1);
+  if (tid == 0) s_n = 0, s_least = 0;
+  for (int e = tid; e < all; e += kThreads)
+    s_keys[e] = *(const uint64_t *)(part + (long long)(e / a.top) * a.words + keys_at + 2 * (e % a.top));
+  if (wave == 0) {
+    Stat st{kLowest, 0.0f, 0.0f};
+    const float *p = part + (long long)l * a.words;
+    if (l < a.ns) st = {p[0], p[1], p[2]};
+    st = wave_join(st);
+    if (l == 0) s_stat = st;
   }
-  for (int q = 0; q < a.nt; q++) {
-    int c = l < a.ns ? ((const int *)part)[l * a.words + 4 + q] : 0;
+  for (int q = wave; q < a.nt; q += kWaves) {
+    int c = 0;
+    if (l < a.ns) c = ((const int *)part)[(long long)l * a.words + 4 + q];
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) c += __shfl_xor(c, o, 64);
     if (l == 0) s_cnt[q] = c;
   }
-  st = wave_join(st);
   __syncthreads();
-  write_row<T>(a, b, st, l, 64, s_cnt);
+  const Stat st = s_stat;
+  const double log_l = log2((double)st.l);
+  write_row<T>(a, b, st, log_l, tid, kThreads, [&](int q) { return s_cnt[q]; });
   if (!a.top) return;
-  const double ln_l = log((double)st.l);
-  merge_lists(
-      a.ns, a.top, [&](int s, int k, float &v, int &i) { v = s_list[s * a.top + k], i = s_idx[s * a.top + k]; },
-      [&](int r, float v, int i) {
-        if (l != 0) return;
-        a.top_ids[(long long)b * a.top + r] = i == kNone ? -1 : i;
-        a.top_lp[(long long)b * a.top + r] = i == kNone ? __builtin_nanf("") : logprob_of(v, st, ln_l);
-      });
+  // `top` keys are at least this: the top-th of the slices' first, or the least of their d-th where d each make `top`
+  const int d = (a.top + a.ns - 1) / a.ns;
+  if (d == 1) {
+    if (tid < a.ns) {
+      const uint64_t k = s_keys[tid * a.top];
+      int r = 0;
+#pragma unroll 4
+      for (int j = 0; j < a.ns; j++) r += s_keys[j * a.top] > k;
+      if (r == a.top - 1 && k) s_least = k;
+    }
+  } else if (wave == 0) {
+    uint64_t k = l < a.ns ? s_keys[l * a.top + d - 1] : ~0ull;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t y = (uint64_t)__shfl_xor((long long)k, o, 64);
+      k = y < k ? y : k;
+    }
+    if (l == 0) s_least = k;
+  }
+  __syncthreads();
+  const uint64_t least = s_least ? s_least : 1;
+  uint64_t *pass = s_keys + all;
+  for (int e = tid; e < all; e += kThreads) {
+    const uint64_t k = s_keys[e];
+    if (k >= least) pass[atomicAdd(&s_n, 1)] = k;  // (in any order: they are ranked)
+  }
+  __syncthreads();
+  const int n = s_n;
+  rank_keys(pass, n, a.top, [&](int r, uint64_t k) { write_alternative(a, b, st, log_l, r, k); });
+  if (n < a.top && wave == 0) write_rest<T>(a, b, st, n);
 }
 
-// Slices of a row: enough workgroups to fill the chip eight times over, none of fewer than 2,048 values.
+// Slices of a row: 1,024 workgroups or so (32 rows of 248,320 bf16: 23 us; 26 with 2,048, 30 with 512), none of fewer
+// than 2,048 values.
 int slices_of(long long B, int V) {
-  const long long want = 2048 / (B > 0 ? B : 1), most = ((long long)V + 2047) / 2048;
+  const long long want = 1024 / (B > 0 ? B : 1), most = ((long long)V + 2047) / 2048;
   const long long n = want < most ? want : most;
   return n < 1 ? 1 : n > kMaxSlices ? kMaxSlices : (int)n;
 }
 
-int part_words(int nt, int top) { return 4 + nt + 2 * top; }
+int part_words(int nt, int top) { return (4 + nt + (nt & 1) + 2 * top + 3) / 4 * 4; }
 
 template <typename T>
 int launch(ScoreArgs a, hipStream_t st) {
   constexpr int N = Elems<T>::N;
   const long long words = ((long long)a.V + 2 * N - 2) / N;  // (of a row that begins anywhere)
-  const long long blocks = (long long)a.B * a.ns;
+  const unsigned blocks = (unsigned)((long long)a.B * a.ns);
   a.slice = (int)((words + a.ns - 1) / a.ns);
-  if (a.slice <= 2 * kThreads)
-    score_rows_kernel<T, 1><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+  if (a.slice <= kThreads)
+    score_rows_kernel<T, 1><<<blocks, kThreads, 0, st>>>(a);
   else
-    score_rows_kernel<T, 4><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+    score_rows_kernel<T, 2><<<blocks, kThreads, 0, st>>>(a);
   int rc = jit::check_launch("jit_token_logprobs");
   if (rc != JIT_OK || a.ns == 1) return rc;
-  score_merge_kernel<T><<<a.B, 64, (size_t)a.ns * a.top * 8, st>>>(a);
+  score_merge_kernel<T><<<a.B, kThreads, (size_t)a.ns * a.top * 16, st>>>(a);
   return jit::check_launch("jit_token_logprobs (merge)");
 }
 
