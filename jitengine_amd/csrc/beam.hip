@@ -7,8 +7,9 @@ namespace {
 // ------------------------------------------------------------------ choice of continuations
 // A group's candidates are (beam b, alternative j), c = b m + j, with score_b + logprob_bj (score_b alone, as alternative
 // 0, for a beam that has ended).  One wave a group, candidate c in lane c % 64: the w-th largest score is found bit by bit
-// from the top (32 counts by ballot over order-preserving keys), candidates that tie with it are taken from the lowest c
-// on, and the w chosen ones count how many of them stand before each.
+// from the top (up to 32 counts by ballot over order-preserving keys, until just w are left), candidates that tie with it
+// are taken from the lowest c on, and the w chosen ones count how many of them stand before each.  Latency bounds it: one
+// group of 4 x 8 candidates 3 us, 64 groups of 16 x 32 12 us.
 constexpr int kMaxWidth = 64, kMaxCands = 4096;
 
 struct BeamArgs {
@@ -31,22 +32,30 @@ template <int NV>
 __global__ __launch_bounds__(64) void beam_select_kernel(const BeamArgs a) {
   __shared__ uint32_t s_key[kMaxWidth];
   __shared__ int s_c[kMaxWidth];
+  __shared__ float s_score[64 * NV];
+  __shared__ bool s_done[64 * NV];
   const int g = blockIdx.x, l = lane_id(), cands = a.n * a.m;
   uint32_t key[NV];
+  // (every load before the first use: clamped addresses in place of branches)
+  float lp[NV];
+  int32_t id[NV];
 #pragma unroll
   for (int i = 0; i < NV; i++) {
-    const int c = 64 * i + l;
-    key[i] = 0u;
-    if (c < cands) {
-      const int b = c / a.m;
-      const float s = a.scores[(long long)g * a.n + b];
-      const bool ended = a.done && a.done[(long long)g * a.n + b] != 0;
-      const long long at = (long long)g * cands + c;
-      if (ended)
-        key[i] = c == b * a.m ? key_of(s) : 0u;
-      else
-        key[i] = a.ids[at] >= 0 ? key_of(s + a.lp[at]) : 0u;
-    }
+    const long long at = (long long)g * cands + min(64 * i + l, cands - 1);
+    lp[i] = a.lp[at];
+    id[i] = a.ids[at];
+  }
+  for (int b = l; b < a.n; b += 64) {  // (a beam that has ended: its score, and no other candidate)
+    s_score[b] = a.scores[(long long)g * a.n + b];
+    s_done[b] = a.done && a.done[(long long)g * a.n + b] != 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int c = 64 * i + l, b = min(c, cands - 1) / a.m;
+    const float s = s_score[b];
+    const bool ended = s_done[b], is = ended ? c == b * a.m : id[i] >= 0;
+    key[i] = c < cands && is ? key_of(ended ? s : s + lp[i]) : 0u;
   }
   auto count = [&](uint32_t least) {
     int n = 0;
@@ -56,11 +65,15 @@ __global__ __launch_bounds__(64) void beam_select_kernel(const BeamArgs a) {
   };
   uint32_t least = 0u;  // the w-th largest key, or 1 where there are fewer candidates
   if (count(1u) > a.w) {
-    for (int bit = 31; bit >= 0; bit--)
-      if (count(least | (1u << bit)) >= a.w) least |= 1u << bit;
+    for (int bit = 31; bit >= 0; bit--) {
+      const int n = count(least | (1u << bit));
+      if (n >= a.w) least |= 1u << bit;
+      if (n == a.w) break;
+    }
   } else {
     least = 1u;
   }
+  // (left early, all that is not below `least` is wanted: ties are none too many then)
   int above = 0;
 #pragma unroll
   for (int i = 0; i < NV; i++) above += __builtin_popcountll(__ballot(key[i] > least));
@@ -87,7 +100,7 @@ __global__ __launch_bounds__(64) void beam_select_kernel(const BeamArgs a) {
     int r = 0;
     for (int j = 0; j < at; j++) r += s_key[j] > k || (s_key[j] == k && s_c[j] < c) ? 1 : 0;
     const int b = c / a.m;
-    const bool ended = a.done && a.done[(long long)g * a.n + b] != 0;
+    const bool ended = s_done[b];
     const int tok = ended ? -1 : a.ids[(long long)g * cands + c];
     bool end = ended;
     for (int e = 0; e < a.n_eos; e++) end |= tok == a.eos[e];
@@ -108,8 +121,10 @@ __global__ __launch_bounds__(64) void beam_select_kernel(const BeamArgs a) {
 // child if no one else holds it, and the other children get copies from the free list.  A table's entry gives its page
 // (the children that keep it) - 1 references; pages that lost their last one go back before the list's next free page,
 // in ascending order.  Three launches: the children (one workgroup), the tables' entries (every workgroup), the pages
-// that came free (one workgroup).
+// that came free (one workgroup); one launch for small tables.  Latency and the order among the parts bound it: 8 tables of 272
+// pages 12 us (13 as three launches, each of which costs the host some 3 more), 512 of 544 pages 5 + 8 + 11.
 constexpr int kForkThreads = 1024, kPage = JIT_PAGE_TOKENS;
+constexpr int kSmallFork = 8192;  // entries of the tables that one workgroup takes
 
 struct ForkArgs {
   const int32_t *table, *lens, *parents, *free_at;
@@ -148,9 +163,7 @@ __device__ __forceinline__ int fork_len(const ForkArgs &a, int s) {
   return n / kPage >= a.W ? a.W * kPage : n;  // (positions past the table are not there)
 }
 
-__global__ __launch_bounds__(kForkThreads) void fork_children_kernel(const ForkArgs a) {
-  extern __shared__ int s_first[];  // [S] first child
-  __shared__ int red[kForkThreads / 64];
+__device__ __forceinline__ void fork_children(const ForkArgs &a, int *s_first, int *red) {  // s_first [S]: first child
   const int t = threadIdx.x;
   for (int w = t; w < (a.P + 31) / 32; w += kForkThreads) a.lost[w] = 0u;
   for (int s = t; s < a.S; s += kForkThreads) s_first[s] = a.N, a.kids[s] = a.kids[a.S + s] = 0;
@@ -199,19 +212,16 @@ __global__ __launch_bounds__(kForkThreads) void fork_children_kernel(const ForkA
 }
 
 // Entry (row, j) of the old tables changes its page's count; of the new ones is copied.
-__global__ __launch_bounds__(256) void fork_entries_kernel(const ForkArgs a) {
-  const int cols = (a.W + 255) / 256;
-  const int row = blockIdx.x / cols, j = (blockIdx.x % cols) * 256 + threadIdx.x;
-  if (j >= a.W) return;
+__device__ __forceinline__ void fork_entry(const ForkArgs &a, int row, int j) {
   if (row < a.S) {
     const int n = fork_len(a, row), held = (n + kPage - 1) / kPage;
     if (j < held) {
       const int page = a.table[(long long)row * a.W + j];
-      const int gain = a.kids[n % kPage != 0 && j == held - 1 ? a.S + row : row] - 1;
-      if (page >= 0 && page < a.P && gain != 0) {
-        atomicAdd(&a.refs[page], gain);
-        if (gain < 0) atomicOr(&a.lost[page >> 5], 1u << (page & 31));
-      }
+      const int gain = load_now(&a.kids[n % kPage != 0 && j == held - 1 ? a.S + row : row]) - 1;
+      if (page >= 0 && page < a.P && gain > 0) atomicAdd(&a.refs[page], gain);
+      // (whoever takes the last reference sees a count that is not above 0 after it)
+      if (page >= 0 && page < a.P && gain < 0 && atomicAdd(&a.refs[page], gain) + gain <= 0)
+        atomicOr(&a.lost[page >> 5], 1u << (page & 31));
     }
   }
   if (row < a.N) {
@@ -225,21 +235,27 @@ __global__ __launch_bounds__(256) void fork_entries_kernel(const ForkArgs a) {
   }
 }
 
-__global__ __launch_bounds__(kForkThreads) void fork_free_kernel(const ForkArgs a) {
-  __shared__ int red[kForkThreads / 64];
+__device__ __forceinline__ void fork_free(const ForkArgs &a, int *red) {
   const int t = threadIdx.x, words = (a.P + 31) / 32;
   int gone = 0;  // pages that came free, all rounds
   const int here = a.status[1];
   // the count first: the list ends where it went on before
   for (int w0 = 0; w0 < words; w0 += kForkThreads) {
     const int w = w0 + t;
-    uint32_t bits = w < words ? a.lost[w] : 0u, kept = 0u;
-    while (bits) {
-      const int i = __builtin_ctz(bits);
-      bits &= bits - 1;
-      if (load_now(&a.refs[32 * w + i]) == 0) kept |= 1u << i;
+    const uint32_t bits = w < words ? load_now((const int32_t *)&a.lost[w]) : 0u;
+    uint32_t kept = 0u;
+    if (__any(bits != 0)) {  // a wave's 64 words, two at a time: the counts of 64 pages next to each other by one load
+      const int l = lane_id(), first = 32 * (w - l);
+      int32_t refs[32];
+#pragma unroll
+      for (int i = 0; i < 32; i++) refs[i] = load_now(&a.refs[min(first + 64 * i + l, a.P - 1)]);
+#pragma unroll
+      for (int i = 0; i < 32; i++) {
+        const uint64_t free = __ballot(refs[i] == 0);
+        if (l >> 1 == i) kept = bits & (uint32_t)(l & 1 ? free >> 32 : free);
+      }
+      if (w < words) a.lost[w] = kept;
     }
-    if (w < words) a.lost[w] = kept;
     int total;
     block_incl(__builtin_popcount(kept), red, total);
     gone += total;
@@ -249,7 +265,7 @@ __global__ __launch_bounds__(kForkThreads) void fork_free_kernel(const ForkArgs 
   int before = 0;
   for (int w0 = 0; w0 < words; w0 += kForkThreads) {
     const int w = w0 + t;
-    uint32_t bits = w < words ? a.lost[w] : 0u;
+    uint32_t bits = w < words ? load_now((const int32_t *)&a.lost[w]) : 0u;
     int total;
     int k = before + block_incl(__builtin_popcount(bits), red, total) - __builtin_popcount(bits);
     before += total;
@@ -272,8 +288,38 @@ __global__ __launch_bounds__(kForkThreads) void fork_free_kernel(const ForkArgs 
   }
 }
 
+__global__ __launch_bounds__(kForkThreads) void fork_children_kernel(const ForkArgs a) {
+  extern __shared__ int s_first[];
+  __shared__ int red[kForkThreads / 64];
+  fork_children(a, s_first, red);
+}
+
+__global__ __launch_bounds__(256) void fork_entries_kernel(const ForkArgs a) {
+  const int cols = (a.W + 255) / 256;
+  const int row = blockIdx.x / cols, j = (blockIdx.x % cols) * 256 + threadIdx.x;
+  if (j < a.W) fork_entry(a, row, j);
+}
+
+__global__ __launch_bounds__(kForkThreads) void fork_free_kernel(const ForkArgs a) {
+  __shared__ int red[kForkThreads / 64];
+  fork_free(a, red);
+}
+
+// The three by one workgroup, for tables of few entries.  What atomics changed is read by load_now, past the L1.
+__global__ __launch_bounds__(kForkThreads) void fork_small_kernel(const ForkArgs a) {
+  extern __shared__ int s_first[];
+  __shared__ int red[kForkThreads / 64];
+  fork_children(a, s_first, red);
+  __syncthreads();
+  const int rows = max(a.S, a.N);
+  for (int e = threadIdx.x; e < rows * a.W; e += kForkThreads) fork_entry(a, e / a.W, e % a.W);
+  __syncthreads();
+  fork_free(a, red);
+}
+
 // ------------------------------------------------------------------ page copies in every layer
-// A workgroup copies one part of one page of one layer, 16 bytes a thread and step.
+// A workgroup copies one part of one page of one layer, 16 bytes a thread and step.  256 pages of 48 layers (805 MB read
+// and written) take 166 us, 4.85 TB/s, what a large copy reaches; 7 pages 5.5 us.
 constexpr int kMaxLayers = 128;  // of a launch: the layers' pointers are its arguments
 
 struct CopyArgs {
@@ -349,6 +395,10 @@ extern "C" int jit_pages_fork(const int32_t *page_table, const int32_t *lens, in
   const ForkArgs a{page_table, lens, parents, free_at, refs, free_pages, new_table, new_lens, src, dst, status,
                    ws, ws + 2 * S, (uint32_t *)(ws + 2 * S + N), S, max_pages, N, num_pages, n_free};
   const hipStream_t st = (hipStream_t)stream;
+  if ((long long)(S > N ? S : N) * max_pages <= kSmallFork) {
+    fork_small_kernel<<<1, kForkThreads, (size_t)S * 4, st>>>(a);
+    return jit::check_launch("jit_pages_fork");
+  }
   fork_children_kernel<<<1, kForkThreads, (size_t)S * 4, st>>>(a);
   int rc = jit::check_launch("jit_pages_fork (children)");
   if (rc != JIT_OK) return rc;
@@ -375,8 +425,10 @@ extern "C" int jit_kv_copy_pages_layers(void *const *pools, int layers, int num_
   CopyArgs a;
   a.src = src, a.dst = dst, a.num_pages = num_pages;
   a.page_words = (int)(page_bytes / 16);
-  a.parts = 1;
-  a.part_words = a.page_words;
+  // parts of a page, none of fewer than 1,024 words, until 1,024 workgroups copy
+  const long long pages = (long long)n * (layers < kMaxLayers ? layers : kMaxLayers), most_parts = (a.page_words + 1023) / 1024;
+  a.parts = (int)(pages >= 1024 ? 1 : (1024 + pages - 1) / pages < most_parts ? (1024 + pages - 1) / pages : most_parts);
+  a.part_words = (a.page_words + a.parts - 1) / a.parts;
   const long long most = 0x7fffffffLL;
   for (int at = 0; at < layers; at += kMaxLayers) {
     a.layers = layers - at < kMaxLayers ? layers - at : kMaxLayers;
