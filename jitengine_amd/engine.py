@@ -37,12 +37,22 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from . import ops
+from . import ops, search
 from . import selfcheck as _selfcheck
 from .kvpool import KVPool, PoolExhausted, PrefixStore, pages_for
 from .ops import PAGE
 from .model import CausalLM, make_mixed_state, make_step_state
 from .sampler import Sampler, sample_rows
+
+
+@dataclass
+class TokenChoice:
+    """What the model said of a generated token: its log-probability and rank (0: the most likely) among the logits that
+    its sampler drew from (before temperature, top-p and top-k), and the most likely (token, log-probability) pairs."""
+
+    logprob: float
+    rank: int
+    top: list
 
 
 @dataclass
@@ -58,6 +68,9 @@ class Request:
     finish_reason: str | None = None
     reserved: int = 0      # pages charged at admission and not yet allocated
     sampler: Sampler | None = None  # (None: greedy)
+    top: int | None = None  # alternatives asked for with each token's log-probability (None: no log-probabilities)
+    logprobs: list = field(default_factory=list)  # a TokenChoice per token, where asked for
+    unread: deque = field(default_factory=deque, repr=False)  # drawn tokens' (host copies, row), the oldest first
 
     @property
     def length(self) -> int:
@@ -102,9 +115,12 @@ class Engine:
 
     # ------------------------------------------------------------------ requests
     def submit(self, prompt, max_tokens: int, eos=None, temperature: float = 0.0, top_p: float | None = None,
-               top_k: int | None = None, seed: int | None = None) -> Request:
+               top_k: int | None = None, seed: int | None = None, logprobs: int | None = None) -> Request:
         """Queue a request; temperature > 0 samples with top_p / top_k under `seed`'s key stream
-        (Sampler, Q36/scheduler/admission.py:104-113), else its tokens are greedy."""
+        (Sampler, Q36/scheduler/admission.py:104-113), else its tokens are greedy.  logprobs=n: each token's
+        log-probability and rank, and the n <= 64 most likely tokens, in Request.logprobs."""
+        if logprobs is not None and not 0 <= logprobs <= min(ops.BEAMS_MAX, self.lm.vocab):
+            raise ValueError(f"logprobs must lie in [0, {min(ops.BEAMS_MAX, self.lm.vocab)}], got {logprobs}")
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise ValueError("empty prompt")
@@ -118,7 +134,8 @@ class Engine:
                                 f"the pool has {self.pool.num_pages}")
         eos = frozenset(self.lm.eos_ids if eos is None else eos)
         r = Request(next(self._ids), prompt, int(max_tokens), eos,
-                    sampler=Sampler(temperature, top_p, top_k, seed, int(max_tokens), self.lm.vocab))
+                    sampler=Sampler(temperature, top_p, top_k, seed, int(max_tokens), self.lm.vocab),
+                    top=None if logprobs is None else int(logprobs))
         self.queue.append(r)
         return r
 
@@ -130,11 +147,11 @@ class Engine:
         while self.queue:
             r = self.queue[0]
             total = pages_for(len(r.prompt) + r.max_tokens)
-            n, pages = self._lookup(r.prompt)
+            n, pages = self.lookup(r.prompt)
             need = total - n // PAGE  # a shared partial page is copied before it is written
             if self.pool.free_pages - self.outstanding < need and self.store is not None:
                 self.store.make_room(need + self.outstanding)
-                n, pages = self._lookup(r.prompt)  # (the entry may have been evicted)
+                n, pages = self.lookup(r.prompt)  # (the entry may have been evicted)
                 need = total - n // PAGE
             if self.pool.free_pages - self.outstanding < need:
                 self.deferred += 1
@@ -147,7 +164,7 @@ class Engine:
             r.state = "prefill"
             self.rows.append(r)
 
-    def _lookup(self, prompt) -> tuple:
+    def lookup(self, prompt) -> tuple:
         """The longest stored prefix of the prompt, cut back to a multiple of prefill_chunk (the chunk
         grid), so the rest of the prompt is computed in the same chunks as a cold run's."""
         if self.store is None:
@@ -179,16 +196,37 @@ class Engine:
         (DecodingMixin._draw / _draw_groups, Q36/scheduler/decode.py:116-176)."""
         samplers = [r.sampler for r in rows]
         keys = [s.rows_key() for s in samplers]
-        if all(k is None for k in keys):
+        noted = any(r.top is not None for r in rows)
+        if all(k is None for k in keys) and not noted:
             return self.lm.greedy(h)
         logits = self.lm.logits(h)
-        out = torch.empty(len(rows), dtype=torch.int32, device=logits.device)
+        out = self._draw_from(logits, samplers, keys, steps)
+        if noted:
+            self._note(rows, logits, out)
+        return out
+
+    def _note(self, rows: list, logits: torch.Tensor, toks: torch.Tensor) -> None:
+        """The log-probabilities of drawn tokens, copied to the host behind the step; read when the tokens are."""
+        lp = ops.token_logprobs(logits, toks, max(r.top or 0 for r in rows))
+        host = []
+        for t in (lp.logprob, lp.rank, lp.top_ids, lp.top_logprobs):
+            host.append(None if t is None else torch.empty(t.shape, dtype=t.dtype, pin_memory=True))
+            if t is not None:
+                host[-1].copy_(t, non_blocking=True)
+        for i, r in enumerate(rows):
+            if r.top is not None:
+                r.unread.append((host, i))
+
+    def _draw_from(self, logits: torch.Tensor, samplers: list, keys: list, steps: list) -> torch.Tensor:
+        if all(k is None for k in keys):
+            return ops.argmax_rows(logits)
+        out = torch.empty(len(samplers), dtype=torch.int32, device=logits.device)
         groups: dict = {}
         for i, k in enumerate(keys):
             groups.setdefault(k, []).append(i)
         for members in groups.values():
             idx = ops.upload(members, logits.device, torch.int64)
-            sel = logits if len(members) == len(rows) else logits.index_select(0, idx).contiguous()
+            sel = logits if len(members) == len(samplers) else logits.index_select(0, idx).contiguous()
             tok = sample_rows(sel, [samplers[i] for i in members], [steps[i] for i in members])
             out.index_copy_(0, idx, tok)
         return out
@@ -239,6 +277,10 @@ class Engine:
         for r, t in drawn:
             r.tokens.append(int(t))
             r.state = "decode"
+            if r.top is not None:
+                (lp, rank, ids, tlp), i = r.unread.popleft()
+                top = list(zip(ids[i, :r.top].tolist(), tlp[i, :r.top].tolist())) if r.top else []
+                r.logprobs.append(TokenChoice(float(lp[i]), int(rank[i]), top))
         for r in list(self.rows):
             if r.state == "decode" and r.tokens:
                 self.pool.lengths[r.rid] = r.length
@@ -305,18 +347,33 @@ class Engine:
         return min(self.prefill_chunk - r.done_prompt % self.prefill_chunk, len(r.prompt) - r.done_prompt)
 
     def _prefill_chunk(self, r: Request, c: int, n: int):
-        """Prompt positions c .. c + n - 1 of request r as a forward of their own (the chunked-prefill
-        layer step over one chunk); returns the drawn token when the chunk ends the prompt."""
-        lm, dev = self.lm, self.device
-        seq_table = self.pool.page_table_host([r.rid])
-        ms = make_mixed_state(lm.cfg, [(0, c, n)], seq_table, np.zeros(0, np.int32),
-                              np.zeros((0, seq_table.shape[1]), np.int32), dev, self.pool.kv8)
-        x = lm.embed_tokens(ops.upload(np.asarray(r.prompt[c:c + n], np.int32), dev))
-        for layer, pool in zip(lm.layers, self.pool.pools):
-            x = layer.mixed(x, pool, ms)
+        """Prompt positions c .. c + n - 1 of request r (forward_chunk); returns the drawn token when the chunk ends the
+        prompt."""
+        x = self.forward_chunk(r.rid, r.prompt, c, n)
         if c + n < len(r.prompt):
             return None
         return int(self._draw([r], x[n - 1:n].contiguous(), [len(r.tokens)]).item())
+
+    def forward_chunk(self, seq_id, prompt: list, c: int, n: int) -> torch.Tensor:
+        """The last layer's rows of positions c .. c + n - 1 of `prompt`, whose pages sequence seq_id holds, as a forward
+        of their own (the chunked-prefill layer step over one chunk)."""
+        lm, dev = self.lm, self.device
+        seq_table = self.pool.page_table_host([seq_id])
+        ms = make_mixed_state(lm.cfg, [(0, c, n)], seq_table, np.zeros(0, np.int32),
+                              np.zeros((0, seq_table.shape[1]), np.int32), dev, self.pool.kv8)
+        x = lm.embed_tokens(ops.upload(np.asarray(prompt[c:c + n], np.int32), dev))
+        for layer, pool in zip(lm.layers, self.pool.pools):
+            x = layer.mixed(x, pool, ms)
+        return x
+
+    def score(self, tokens) -> list:
+        """The log-probability of each token of a text but the first, given those before it (search.score)."""
+        return search.score(self, tokens)
+
+    def beam_search(self, prompts, beams: int, max_tokens: int, eos=None) -> list:
+        """The `beams` most likely continuations of each prompt found by a search of that width, the best first
+        (search.beam_search); queued and running requests wait meanwhile."""
+        return search.beam_search(self, prompts, beams, max_tokens, eos)
 
     def run(self, max_steps: int | None = None) -> None:
         """Step until every submitted request is done (or max_steps rounds)."""

@@ -11,7 +11,7 @@ operand layouts the attention kernels read), or, with kv8=True, [num_pages, Hkv,
 scale a token, 0.516 of the bytes; ops.kv8_pool).  A sequence owns a list of pages, the same page ids
 in every layer; token t sits in page pages[t // 16], slot t % 16.  Sharing a prefix is sharing its
 pages: each page carries a reference count, and a sequence about to write into a page that someone
-else also holds first copies it (jit_kv_copy_pages, jit_kv8_copy_pages), so a shared page is never written.  The pool
+else also holds first copies it (jit_kv_copy_pages_layers, every layer in one launch), so a shared page is never written.  The pool
 is zero-initialised, so every slot of an allocated page always holds finite values.
 """
 
@@ -60,6 +60,7 @@ class KVPool:
              for _ in range(n_layers)]
             if allocate else []
         )
+        self._layers: ops.PoolLayers | None = None
 
     # ------------------------------------------------------------------ pages
     @property
@@ -99,8 +100,14 @@ class KVPool:
             return
         s = ops.upload(np.asarray(src, np.int32), self.device)
         d = ops.upload(np.asarray(dst, np.int32), self.device)
-        for pool in self.pools:
-            (ops.kv8_copy_pages if self.kv8 else ops.kv_copy_pages)(pool, s, d)
+        ops.kv_copy_pages_layers(self.layers(), s, d)
+
+    def layers(self) -> ops.PoolLayers:
+        """The layers' pools as one handle, for calls that work on every layer at once."""
+        h = self._layers
+        if h is None or len(h.pools) != len(self.pools) or any(a is not b for a, b in zip(h.pools, self.pools)):
+            h = self._layers = ops.pool_layers(self.pools)
+        return h
 
     # -------------------------------------------------------------- sequences
     def open(self, seq_id, pages=(), length: int = 0) -> None:

@@ -580,6 +580,11 @@ class CausalLM:
         logits do not depend on the batch)."""
         return ops.qmm(ops.rmsnorm(h, self.final_norm, self.cfg.eps), self.lm_head, seg=False)
 
+    def score(self, h: torch.Tensor, tokens: torch.Tensor) -> ops.HeadLogprobs:
+        """Last-layer rows [T, D] -> the log-probability of tokens [T] int32 in each and its entropy, with no logits in
+        memory (ops.head_logprobs: fp32 logits, where `logits` rounds them to bf16)."""
+        return ops.head_logprobs(ops.rmsnorm(h, self.final_norm, self.cfg.eps), self.lm_head, tokens)
+
     def greedy(self, h: torch.Tensor) -> torch.Tensor:
         """Last-layer rows -> the greedy token of each row, int32 [B]."""
         return ops.argmax_rows(self.logits(h))

@@ -1196,6 +1196,9 @@ def head_logprobs(x: torch.Tensor, head: PackedQ4, tokens: torch.Tensor,
     return HeadLogprobs(*out.unbind(0))
 
 
+BEAMS_MAX = 64  # beams that beam_select keeps of a group, and alternatives that token_logprobs gives
+
+
 @dataclass
 class Beams:
     """The continuations that a step keeps, [G, width], the best first (jit_beam_select); -1, -1, -inf, 1 where a group has

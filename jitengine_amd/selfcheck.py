@@ -218,9 +218,31 @@ def _sampler(dev) -> None:
     _equal("greedy draw", ops.argmax_rows(x.to(torch.bfloat16)), torch.tensor([417, 3], dtype=torch.int32, device=dev))
 
 
+def _scoring(dev) -> None:
+    """Log-probabilities from logits and from the packed head, the choice of continuations."""
+    g = torch.Generator(device=dev).manual_seed(9)
+    x = torch.randn((3, 5000), generator=g, device=dev) * 3
+    tok = torch.tensor([7, 4999, 0], dtype=torch.int32, device=dev)
+    lp = torch.log_softmax(x.double(), -1)
+    r = ops.token_logprobs(x, tok, top=8)
+    _close("log-probabilities", r.logprob, lp.gather(1, tok.long()[:, None])[:, 0])
+    _close("entropy", r.entropy, torch.special.entr(lp.exp()).sum(-1))
+    best = x.topk(8, -1)
+    _equal("alternatives", r.top_ids, best.indices.to(torch.int32))
+    b = ops.beam_select(r.logprob[None], r.top_logprobs[None], r.top_ids[None], 4)
+    want = (r.logprob[:, None] + r.top_logprobs).flatten().topk(4).indices
+    _equal("continuations", b.parents[0], (want // 8).to(torch.int32))
+    _equal("their tokens", b.tokens[0], r.top_ids.flatten()[want])
+    lin = random_quantized((512, 256), 11, 0.1, dev)
+    h = torch.randn((5, 256), generator=g, device=dev).to(torch.bfloat16)
+    tok = torch.arange(5, dtype=torch.int32, device=dev) * 100
+    lp = torch.log_softmax(h.double() @ dequantize4(lin).double().t().contiguous(), -1)
+    _close("head log-probabilities", ops.head_logprobs(h, ops.prepack(lin), tok).logprob, lp.gather(1, tok.long()[:, None])[:, 0])
+
+
 CASES = (("router + packing", _router_and_pack), ("projections + experts", _projections),
          ("rmsnorm + attention", _norm_and_attention), ("prefill attention", _prefill),
-         ("8-bit cache", _kv8), ("segment GEMMs", _segment), ("sampler", _sampler))
+         ("8-bit cache", _kv8), ("segment GEMMs", _segment), ("sampler", _sampler), ("scoring", _scoring))
 
 
 def run(device=None, force: bool = False) -> list:

@@ -464,9 +464,86 @@ def _(keys):
     return keys.new_empty((keys.shape[0],), dtype=torch.float32)
 
 
+# ----------------------------------------------------------------------------- scoring, continued sequences
+@torch.library.custom_op(f"{_NS}::token_logprobs", mutates_args=())
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int) -> tuple[
+        torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(logprob fp32, rank int32 in the shape of tokens; entropy fp32 [B]; top_ids int32, top_logprobs fp32 [B, top]) of
+    tokens [B] or [B, m] in rows of logits [B, V] (jit_token_logprobs)."""
+    r = ops.token_logprobs(logits, tokens, top)
+    B = logits.shape[0]
+    none = (logits.new_empty((B, 0), dtype=torch.int32), logits.new_empty((B, 0), dtype=torch.float32))
+    ids, lp = (r.top_ids, r.top_logprobs) if top > 0 else none
+    return r.logprob, r.rank, r.entropy, ids, lp
+
+
+@token_logprobs.register_fake
+def _(logits, tokens, top):
+    B, f32, i32 = logits.shape[0], torch.float32, torch.int32
+    return (tokens.new_empty(tokens.shape, dtype=f32), torch.empty_like(tokens), logits.new_empty((B,), dtype=f32),
+            logits.new_empty((B, top), dtype=i32), logits.new_empty((B, top), dtype=f32))
+
+
+@torch.library.custom_op(f"{_NS}::head_logprobs", mutates_args=())
+def head_logprobs(x: torch.Tensor, w: torch.Tensor, N: int, K: int, tokens: torch.Tensor) -> torch.Tensor:
+    """fp32 [3, T]: log-probability of tokens [T], entropy and log-sum of rows x [T, K] against a packed head [N, K]
+    (jit_head_logprobs)."""
+    r = ops.head_logprobs(x, _packed(w, 1, N, K), tokens)
+    return torch.stack((r.logprob, r.entropy, r.lse))
+
+
+@head_logprobs.register_fake
+def _(x, w, N, K, tokens):
+    return x.new_empty((3, x.shape[0]), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::beam_select", mutates_args=())
+def beam_select(scores: torch.Tensor, logprobs: torch.Tensor, ids: torch.Tensor, width: int,
+                done: torch.Tensor | None, eos: torch.Tensor | None) -> tuple[
+        torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(parents int32, tokens int32, scores fp32, done int32) [G, width] of the best continuations (jit_beam_select)."""
+    r = ops.beam_select(scores, logprobs, ids, width, done, eos)
+    return r.parents.clone(), r.tokens.clone(), r.scores.clone(), r.done.clone()  # (outputs must not share storage)
+
+
+@beam_select.register_fake
+def _(scores, logprobs, ids, width, done, eos):
+    i32, shape = torch.int32, (scores.shape[0], width)
+    return (scores.new_empty(shape, dtype=i32), scores.new_empty(shape, dtype=i32), scores.new_empty(shape),
+            scores.new_empty(shape, dtype=i32))
+
+
+@torch.library.custom_op(f"{_NS}::pages_fork", mutates_args=("refs", "free"))
+def pages_fork(page_table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, refs: torch.Tensor,
+               free: torch.Tensor, free_at: torch.Tensor) -> tuple[
+        torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(page_table [N, W], lens, src, dst [N], status [4]) int32 of the children of parents [N] (jit_pages_fork)."""
+    r = ops.pages_fork(page_table, lens, parents, refs, free, free_at)
+    return r.page_table.clone(), r.lens.clone(), r.src.clone(), r.dst.clone(), r.status.clone()
+
+
+@pages_fork.register_fake
+def _(page_table, lens, parents, refs, free, free_at):
+    n = parents.shape[0]
+    return (page_table.new_empty((n, page_table.shape[1])), lens.new_empty((n,)), lens.new_empty((n,)),
+            lens.new_empty((n,)), lens.new_empty((4,)))
+
+
+@torch.library.custom_op(f"{_NS}::kv_copy_pages_layers", mutates_args=("pools",))
+def kv_copy_pages_layers(pools: list[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Pages src[i] copied to dst[i] in every layer's pool (jit_kv_copy_pages_layers)."""
+    ops.kv_copy_pages_layers(ops.pool_layers(pools), src, dst)
+
+
+@kv_copy_pages_layers.register_fake
+def _(pools, src, dst):
+    return None
+
+
 OPS = ("router_topk", "moe_pack", "route_pack", "expert_gate_up", "route_gate_up", "expert_down", "moe_combine",
        "moe_combine_rmsnorm", "qmm", "rmsnorm", "rmsnorm_add", "qmm_add_rmsnorm", "qmm_combine_rmsnorm",
        "qk_norm_rope_append", "paged_decode_attention", "paged_decode_attention_qkv", "paged_prefill_attention",
        "kv_append_paged", "kv_copy_pages", "logprobs_rows", "argmax_rows", "sample_rows", "threefry_uniform")
 OPS_KV8 = ("step_tables", "kv8_append_paged", "qk_norm_rope_append_kv8", "paged_decode_attention_kv8",
            "paged_prefill_attention_kv8", "kv8_copy_pages")
+OPS_SCORING = ("token_logprobs", "head_logprobs", "beam_select", "pages_fork", "kv_copy_pages_layers")
