@@ -1,10 +1,10 @@
 // Scoring of given tokens from rows of logits for gfx950: log-probability, rank, entropy and the most likely
 // alternatives in one pass over each row.
 //
-// With m = max x over a row and, in base 2, y = (x - m) log2 e, l = sum 2^y, t = sum y 2^y:
+// With m about max x over a row and, in base 2, y = (x - m) log2 e, l = sum 2^y, t = sum y 2^y:
 //   log-probability of v = (y_v - log2 l) ln 2,   entropy = (log2 l - t / l) ln 2,
 //   rank of v = #{j : x_j > x_v, or x_j = x_v and j < v}.
-// Every lane keeps its own (m, l, t), rescaled where its largest value grows; lanes, waves and slices meet by the same
+// Every lane keeps its own (m, l, t), rescaled where its values grow well past m; lanes, waves and slices meet by the same
 // rule in a fixed order, so a call's bits repeat.  y is one fused multiply-add x log2 e - (m log2 e), whose second term's
 // rounding is the same for every y and cancels; rows whose largest magnitude would overflow there take (x - m) log2 e.
 // Masked entries (-inf, or the type's lowest value beside larger ones) add 0; a row of nothing but lowest values is uniform.
@@ -16,8 +16,8 @@
 // (32 rows, 20 alternatives: 67 + 19 us).
 //
 // What bounds it: many rows, the vector ALU (a value takes 5 1/2 instructions of 4 cycles and an exponential of 16, one
-// instruction more for the rank: 2,048 rows of 151,936 bf16 values, 622 MB, in 165 us, 3.8 TB/s; a large copy reaches 4.8);
-// few rows, latency: 1 row of 151,936 in 6.5 + 5.4 us of two launches, 32 rows of 248,320 under a mask in 17.4 + 5.8.
+// instruction more for the rank: 2,048 rows of 151,936 bf16 values, 622 MB, in 138 us, 4.5 TB/s; a large copy reaches 4.8);
+// few rows, latency: 1 row of 151,936 in 6.4 + 5.3 us of two launches, 32 rows of 248,320 under a mask in 17.0 + 5.7.
 #include "common.hpp"
 
 namespace {
@@ -340,7 +340,9 @@ __global__ __launch_bounds__(kThreads) void score_rows_kernel(const ScoreArgs a)
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int j = 0; j < N; j++) top = fmaxf(top, x[u][j]);
-    if (top > st.m) st = rebase(st, top);
+    // (a reference that lags by up to 8 costs nothing: 2^y stays below 2^12; following every larger value took 40
+    // instructions a step)
+    if (top > st.m + 8.0f) st = rebase(st, top);
     // a lane that has met nothing but masked values takes the wave's largest
     if (!__all(fabsf(st.m * kLog2e) < kInf)) {
       st = rebase(st, wave_butterfly<true>(st.m));
@@ -392,6 +394,7 @@ __global__ __launch_bounds__(kThreads) void score_rows_kernel(const ScoreArgs a)
     if (a.top && __any(top > kept.least)) {
       if (__builtin_popcountll(__ballot(top > kept.least)) >= a.top) kept.raise(nth_of_lanes<kBits>(top, a.top));
       kept.put<T>(x, cur, (base + tid) * N - off, kThreads * N, a.top);
+      if (kept.count > 2 * a.top) kept.squeeze(a.top);  // (raises the bar, so that few steps come here)
       kept.least = kept.bar;
     }
   }

@@ -1152,16 +1152,20 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         m = 1 if tokens.dim() == 1 else shape[1]
     need = lib.jit_token_logprobs_workspace_bytes(B, V, m, max(top, 0))
     ws = _workspace(workspace, need, logits.device, "token_logprobs")
-    ent = torch.empty(B, dtype=f32, device=logits.device)
-    lp = rank = ids = tlp = None
-    if m:
-        lp, rank = ent.new_empty(shape), torch.empty(shape, dtype=i32, device=logits.device)
-    if top > 0:
-        ids, tlp = torch.empty((B, top), dtype=i32, device=logits.device), ent.new_empty((B, top))
+    n, k = B * m, B * max(top, 0)  # (two allocations: a row's launches are a few microseconds, and so is the host's side)
+    floats = torch.empty(B + n + k, dtype=f32, device=logits.device)
+    ints = torch.empty(n + k, dtype=i32, device=logits.device)
+    at, to = floats.data_ptr(), ints.data_ptr()
     _launch(dev, lib.jit_token_logprobs, "token_logprobs", logits.data_ptr(), int(logits.dtype == f32), B, V, stride,
-            _ptr(tokens), m, top, _ptr(lp), _ptr(rank), ent.data_ptr(), _ptr(ids), _ptr(tlp), _ptr(ws),
-            0 if ws is None else ws.nbytes)
-    return TokenLogprobs(lp, rank, ent, ids, tlp)
+            _ptr(tokens), m, top, at + 4 * B if m else None, to if m else None, at, to + 4 * n if k else None,
+            at + 4 * (B + n) if k else None, _ptr(ws), 0 if ws is None else ws.nbytes)
+    ent, lp, tlp = floats.split_with_sizes([B, n, k])
+    rank, ids = ints.split_with_sizes([n, k])
+    if not m:
+        lp = rank = None
+    elif tokens.dim() == 2:
+        lp, rank = lp.view(shape), rank.view(shape)
+    return TokenLogprobs(lp, rank, ent, *((ids.view(B, top), tlp.view(B, top)) if top > 0 else (None, None)))
 
 
 @dataclass

@@ -473,8 +473,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int) -> tupl
     r = ops.token_logprobs(logits, tokens, top)
     B = logits.shape[0]
     none = (logits.new_empty((B, 0), dtype=torch.int32), logits.new_empty((B, 0), dtype=torch.float32))
-    ids, lp = (r.top_ids, r.top_logprobs) if top > 0 else none
-    return r.logprob, r.rank, r.entropy, ids, lp
+    ids, lp = (r.top_ids.clone(), r.top_logprobs.clone()) if top > 0 else none
+    return r.logprob.clone(), r.rank.clone(), r.entropy.clone(), ids, lp  # (outputs must not share storage)
 
 
 @token_logprobs.register_fake
@@ -503,7 +503,7 @@ def beam_select(scores: torch.Tensor, logprobs: torch.Tensor, ids: torch.Tensor,
         torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(parents int32, tokens int32, scores fp32, done int32) [G, width] of the best continuations (jit_beam_select)."""
     r = ops.beam_select(scores, logprobs, ids, width, done, eos)
-    return r.parents.clone(), r.tokens.clone(), r.scores.clone(), r.done.clone()  # (outputs must not share storage)
+    return r.parents.clone(), r.tokens.clone(), r.scores.clone(), r.done.clone()
 
 
 @beam_select.register_fake
