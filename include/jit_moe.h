@@ -510,14 +510,14 @@ int jit_kv_copy_pages(uint16_t *pool, int num_pages, int Hkv, const int32_t *src
  * Log-probabilities of given tokens for rows of logits [B, V] (bf16, or fp32 with fp32 = 1; row b begins row_stride
  * elements after row b - 1, at any address that its type allows).  No counterpart in the reference, whose sampler keeps
  * whole rows of bf16 log-probabilities (Q36/sampler.py:295-297); here everything is fp32 or more from the logits on.
- * With m the largest logit of a row, l = sum e^(x - m), t = sum (x - m) e^(x - m):
+ * With any reference m near the largest logit of a row, l = sum e^(x - m), t = sum (x - m) e^(x - m):
  *   logprob [B, n_tokens]  (x_v - m) - ln l of the tokens v = tokens [B, n_tokens]; 0 for a v outside [0, V);
  *   rank    [B, n_tokens]  logits before x_v in the order (value descending, index ascending); -1 outside [0, V);
  *   entropy [B]            ln l - t / l, in nats;
  *   top_ids, top_logprobs [B, top]  the first `top` of that order.
  * -inf logits have probability 0; a row of nothing else has log-probabilities -inf and entropy 0.  A row with a NaN or
  * +inf has NaN log-probabilities and entropy; a NaN is no alternative (id -1 where numbers are missing, rank -1).
- * The bits repeat; they depend on B through the slices of a row.
+ * The bits repeat; they depend on B and top through the slices of a row, and on where a row begins in its 16 bytes.
  * Contract: top <= V, top <= 64, n_tokens <= 64, V <= 2^30 (the last three JIT_EUNSUPPORTED); a workspace of
  * jit_token_logprobs_workspace_bytes (16-byte aligned, contents do not matter, none where that is 0). */
 long long jit_token_logprobs_workspace_bytes(int B, int V, int n_tokens, int top);
@@ -528,7 +528,9 @@ int jit_token_logprobs(const void *logits, int fp32, int B, int V, long long row
 /* The same of one token a row straight from hidden rows x [T, K] bf16 and a packed 4-bit head [V, K] (jit_q4_prepack),
  * with no logits in memory: logit = x . (s q + b) in fp32, not rounded to bf16 as jit_qmm_packed's are.
  *   logprob, entropy, lse [T]  of tokens [T] (logprob 0 for a token outside [0, V)); lse = m + ln l.
- * Contract: K % 128 == 0, V % 16 == 0, T <= 2^20 (JIT_EUNSUPPORTED); x, w and the workspace 16-byte aligned. */
+ * A row with a logit that is not finite, or of a magnitude past 2^127 / log2 e, is NaN in all three.
+ * Contract: K % 128 == 0, V % 16 == 0, T <= 2^20, T K < 2^31 (JIT_EUNSUPPORTED); x, w and the workspace 16-byte aligned;
+ * a workspace of jit_head_logprobs_workspace_bytes. */
 long long jit_head_logprobs_workspace_bytes(int T, int K, int V);
 int jit_head_logprobs(const uint16_t *x, int T, int K, const void *w, int V, const int32_t *tokens, float *logprob,
                       float *entropy, float *lse, void *workspace, long long workspace_bytes, void *stream);
@@ -555,8 +557,8 @@ int jit_beam_select(const float *scores, const float *logprobs, const int32_t *i
  *   status [4]  pages copied, where the free list goes on, children refused, pages that found no room in the list.
  * A child is refused (length 0, no pages) where the list ends or holds an id outside the pool.  A page id outside
  * [0, num_pages) in a table is handed on as it is, without a count.  A list of num_pages entries always has room.
- * Contract: S, N <= JIT_STEP_TABLES_MAX_SEQS (JIT_EUNSUPPORTED); a workspace of jit_pages_fork_workspace_bytes, 16-byte
- * aligned; outputs apart from inputs. */
+ * Contract: S, N <= JIT_STEP_TABLES_MAX_SEQS, max_pages <= 2^26, num_pages <= 2^27 (JIT_EUNSUPPORTED); a workspace of
+ * jit_pages_fork_workspace_bytes, 16-byte aligned; outputs apart from inputs. */
 long long jit_pages_fork_workspace_bytes(int S, int N, int num_pages);
 int jit_pages_fork(const int32_t *page_table, const int32_t *lens, int S, int max_pages, const int32_t *parents, int N,
                    int32_t *refs, int num_pages, int32_t *free_pages, int n_free, const int32_t *free_at,

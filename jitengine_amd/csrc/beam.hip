@@ -380,9 +380,9 @@ extern "C" int jit_pages_fork(const int32_t *page_table, const int32_t *lens, in
   if (S < 0 || N < 0 || max_pages <= 0 || num_pages <= 0 || n_free < 0)
     return jit::fail(JIT_EINVAL, "pages_fork: bad dims S=%d N=%d max_pages=%d num_pages=%d n_free=%d", S, N, max_pages,
                      num_pages, n_free);
-  if (S > JIT_STEP_TABLES_MAX_SEQS || N > JIT_STEP_TABLES_MAX_SEQS || max_pages > (1 << 26))
-    return jit::fail(JIT_EUNSUPPORTED, "pages_fork covers up to %d sequences and children of up to 2^26 pages, got %d, %d and %d",
-                     JIT_STEP_TABLES_MAX_SEQS, S, N, max_pages);
+  if (S > JIT_STEP_TABLES_MAX_SEQS || N > JIT_STEP_TABLES_MAX_SEQS || max_pages > (1 << 26) || num_pages > (1 << 27))
+    return jit::fail(JIT_EUNSUPPORTED, "pages_fork covers up to %d sequences and children of up to 2^26 pages of 2^27, got %d, %d, %d and %d",
+                     JIT_STEP_TABLES_MAX_SEQS, S, N, max_pages, num_pages);
   const long long blocks = (long long)(S > N ? S : N) * ((max_pages + 255) / 256);
   if (blocks > 0x7fffffffLL) return jit::fail(JIT_EUNSUPPORTED, "pages_fork: tables of %d x %d", S > N ? S : N, max_pages);
   if (!refs || !free_at || !status || (S && (!page_table || !lens)) || (N && (!parents || !new_table || !new_lens || !src || !dst)) ||

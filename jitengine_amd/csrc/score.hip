@@ -535,11 +535,11 @@ __global__ __launch_bounds__(kThreads) void score_merge_kernel(const ScoreArgs a
 }
 
 // Slices of a row: 1,024 workgroups or so (32 rows of 248,320 bf16: 23 us; 26 with 2,048, 30 with 512), none of fewer
-// than 2,048 values.
-int slices_of(long long B, int V) {
+// than 2,048 values.  (Of many alternatives, as many as the second launch's LDS holds keys of.)
+int slices_of(long long B, int V, int top) {
   const long long want = 1024 / (B > 0 ? B : 1), most = ((long long)V + 2047) / 2048;
-  const long long n = want < most ? want : most;
-  return n < 1 ? 1 : n > kMaxSlices ? kMaxSlices : (int)n;
+  const long long n = want < most ? want : most, cap = top > kMaxTop / 2 ? kMaxSlices / 2 : kMaxSlices;
+  return n < 1 ? 1 : n > cap ? (int)cap : (int)n;
 }
 
 int part_words(int nt, int top) { return (4 + nt + (nt & 1) + 2 * top + 3) / 4 * 4; }
@@ -564,7 +564,7 @@ int launch(ScoreArgs a, hipStream_t st) {
 
 extern "C" long long jit_token_logprobs_workspace_bytes(int B, int V, int n_tokens, int top) {
   if (B < 0 || V <= 0 || n_tokens < 0 || top < 0) return -1;
-  const int ns = slices_of(B, V);
+  const int ns = slices_of(B, V, top);
   return ns == 1 ? 0 : (long long)B * ns * part_words(n_tokens, top) * 4;
 }
 
@@ -580,7 +580,7 @@ extern "C" int jit_token_logprobs(const void *logits, int fp32, int B, int V, lo
     return jit::fail(JIT_EUNSUPPORTED, "token_logprobs covers up to %d alternatives and %d tokens a row, got %d and %d",
                      kMaxTop, kMaxTokens, top, n_tokens);
   if (V > (1 << 30)) return jit::fail(JIT_EUNSUPPORTED, "token_logprobs covers rows of up to 2^30 values, got %d", V);
-  const int ns = slices_of(B, V);
+  const int ns = slices_of(B, V, top);
   if ((long long)B * ns > 0x7fffffffLL)
     return jit::fail(JIT_EUNSUPPORTED, "token_logprobs covers up to 2^31 - 1 workgroups, got %d rows", B);
   if (B == 0) return JIT_OK;

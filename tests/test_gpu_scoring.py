@@ -120,6 +120,21 @@ def test_token_logprobs_of_rows_at_a_stride(at, dtype):
     _check_rows(x, tok, 9, ops.token_logprobs(wide.to(DEV)[:, at:at + V], tok.to(DEV), top=9))
 
 
+@pytest.mark.parametrize("top", [1, 31, 32, 33, 63, 64])
+@pytest.mark.parametrize("kind", ["normal", "ties", "constant", "ascending", "descending", "masked"])
+def test_token_logprobs_of_every_number_of_alternatives(kind, top):
+    """Of a row in as many slices as there are, and of rows of several steps a workgroup."""
+    for B, V, slices in ((1, 200000, 32), (600, 20001, 1)):
+        x = _rows(kind, 3 if B > 1 else 1, V, torch.bfloat16, top)
+        tok = torch.randint(0, V, (x.shape[0],), generator=torch.Generator().manual_seed(top), dtype=torch.int32)
+        n = B // x.shape[0]
+        r = ops.token_logprobs(x.repeat(n, 1).to(DEV), tok.repeat(n).to(DEV), top)
+        k = x.shape[0]
+        _check_rows(x, tok, top, ops.TokenLogprobs(*(t[-k:] for t in (r.logprob, r.rank, r.entropy, r.top_ids, r.top_logprobs))), slices)
+        if B > 1:  # (24 rows on, a row of any length begins at the same place in its 16 bytes: the same sums in the same order)
+            assert torch.equal(r.top_ids[:k], r.top_ids[24:24 + k]) and torch.equal(r.logprob[:k], r.logprob[24:24 + k])
+
+
 def test_token_logprobs_without_rows_tokens_or_alternatives():
     r = ops.token_logprobs(torch.zeros((0, 50), device=DEV), _i32([]), top=3)
     assert r.logprob.shape == (0,) and r.top_ids.shape == (0, 3)

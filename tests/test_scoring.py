@@ -69,7 +69,7 @@ def test_pages_fork_contract():
 
     E, U = _lib.JIT_EINVAL, _lib.JIT_EUNSUPPORTED
     assert call(S=-1) == call(N=-1) == call(W=0) == call(P=0) == call(F=-1) == E
-    assert call(S=8193) == call(N=8193) == call(W=(1 << 26) + 1) == U
+    assert call(S=8193) == call(N=8193) == call(W=(1 << 26) + 1) == call(P=(1 << 27) + 1) == U
     assert call(table=None) == call(refs=None) == call(ws=None) == call(nb=8) == call(ws=ctypes.c_void_p(264)) == E
     assert lib.jit_pages_fork_workspace_bytes(2, 2, 0) == -1
 
