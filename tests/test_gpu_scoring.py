@@ -152,6 +152,28 @@ def test_token_logprobs_without_rows_tokens_or_alternatives():
         ops.token_logprobs(torch.zeros((1, 90000), device=DEV), workspace=torch.empty(16, dtype=torch.uint8, device=DEV))
 
 
+def test_token_logprobs_of_very_long_rows_and_of_very_many():
+    x = _rows("normal", 2, 3000001, torch.float32, 3)
+    tok = torch.tensor([[2999999, 0], [7, 3000000]], dtype=torch.int32)
+    _check_rows(x, tok, 9, ops.token_logprobs(x.to(DEV), tok.to(DEV), 9), 64)
+    x = _rows("normal", 70000, 33, torch.bfloat16, 4)
+    tok = (torch.arange(70000) % 35 - 1).to(torch.int32)
+    r = ops.token_logprobs(x.to(DEV), tok.to(DEV), 3)
+    at = torch.tensor([0, 1, 34, 35, 2047, 2048, 65535, 65536, 69998, 69999])
+    _check_rows(x[at], tok[at], 3, ops.TokenLogprobs(*(t[at.to(DEV)] for t in (r.logprob, r.rank, r.entropy, r.top_ids, r.top_logprobs))))
+
+
+def test_token_logprobs_of_rows_whose_largest_grows_slowly():
+    """References lag behind values that grow by less than a step's worth; one value then has everything."""
+    V = 40000
+    for top in (7.9, 8.1, 40.0):
+        x = torch.stack([torch.linspace(0, top, V), torch.linspace(0, top, V).flip(0), torch.cat([torch.zeros(V - 1), torch.tensor([top])])])
+        tok = torch.tensor([V - 1, 0, V - 1], dtype=torch.int32)
+        for rows in (x, x.repeat(400, 1)):  # (split rows, and whole ones)
+            r = ops.token_logprobs(rows.to(DEV), tok.repeat(rows.shape[0] // 3).to(DEV), 5)
+            _check_rows(x, tok, 5, ops.TokenLogprobs(*(t[:3] for t in (r.logprob, r.rank, r.entropy, r.top_ids, r.top_logprobs))))
+
+
 def test_token_logprobs_past_4_gib():
     """Row offsets past 32 bits: the last row of logits of 4.2 GiB."""
     B, V = 15000, 151936

@@ -60,6 +60,14 @@ def test_searches_and_scores_past_the_pool_are_refused_and_hold_nothing():
     assert eng.pool.free_pages == 8 and not eng.pool.pages
 
 
+def test_a_search_that_fails_gives_its_pages_back():
+    eng = _engine(64)
+    for call in (lambda: eng.beam_search([[1, 2]], 2, 4), lambda: eng.score([1, 2, 3])):
+        with pytest.raises(AttributeError):  # (a model without weights)
+            call()
+        assert eng.pool.free_pages == 64 and not eng.pool.pages and not eng.pool.refs.any()
+
+
 def test_score_of_a_single_token_and_of_none():
     assert _engine().score([5]) == []
     with pytest.raises(ValueError, match="empty"):
