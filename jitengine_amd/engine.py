@@ -55,6 +55,23 @@ class TokenChoice:
     top: list
 
 
+class _Note:
+    """A step's log-probabilities on their way to the host: rows of (log-probability, rank, alternatives, their
+    log-probabilities) as 32-bit words, made lists of once, when the step's tokens have landed."""
+
+    def __init__(self, host: torch.Tensor, top: int):
+        self.host, self.top, self.lists = host, top, None
+
+    def choice(self, i: int, top: int) -> TokenChoice:
+        if self.lists is None:
+            ints = self.host.numpy()
+            floats = ints.view(np.float32)
+            self.lists = (floats[:, 0].tolist(), ints[:, 1].tolist(), ints[:, 2:2 + self.top].tolist(),
+                          floats[:, 2 + self.top:].tolist())
+        lp, rank, ids, tlp = (x[i] for x in self.lists)
+        return TokenChoice(lp, rank, list(zip(ids[:top], tlp[:top])))
+
+
 @dataclass
 class Request:
     rid: int
@@ -70,7 +87,7 @@ class Request:
     sampler: Sampler | None = None  # (None: greedy)
     top: int | None = None  # alternatives asked for with each token's log-probability (None: no log-probabilities)
     logprobs: list = field(default_factory=list)  # a TokenChoice per token, where asked for
-    unread: deque = field(default_factory=deque, repr=False)  # drawn tokens' (host copies, row), the oldest first
+    unread: deque = field(default_factory=deque, repr=False)  # drawn tokens' (note, row), the oldest first
 
     @property
     def length(self) -> int:
@@ -207,15 +224,17 @@ class Engine:
 
     def _note(self, rows: list, logits: torch.Tensor, toks: torch.Tensor) -> None:
         """The log-probabilities of drawn tokens, copied to the host behind the step; read when the tokens are."""
-        lp = ops.token_logprobs(logits, toks, max(r.top or 0 for r in rows))
-        host = []
-        for t in (lp.logprob, lp.rank, lp.top_ids, lp.top_logprobs):
-            host.append(None if t is None else torch.empty(t.shape, dtype=t.dtype, pin_memory=True))
-            if t is not None:
-                host[-1].copy_(t, non_blocking=True)
+        i32, top = torch.int32, max(r.top or 0 for r in rows)
+        lp = ops.token_logprobs(logits, toks, top)
+        cols = [lp.logprob.view(i32)[:, None], lp.rank[:, None]]
+        if top:
+            cols += [lp.top_ids, lp.top_logprobs.view(i32)]
+        dev = torch.cat(cols, 1)
+        note = _Note(torch.empty(dev.shape, dtype=i32, pin_memory=True), top)
+        note.host.copy_(dev, non_blocking=True)
         for i, r in enumerate(rows):
             if r.top is not None:
-                r.unread.append((host, i))
+                r.unread.append((note, i))
 
     def _draw_from(self, logits: torch.Tensor, samplers: list, keys: list, steps: list) -> torch.Tensor:
         if all(k is None for k in keys):
@@ -278,9 +297,8 @@ class Engine:
             r.tokens.append(int(t))
             r.state = "decode"
             if r.top is not None:
-                (lp, rank, ids, tlp), i = r.unread.popleft()
-                top = list(zip(ids[i, :r.top].tolist(), tlp[i, :r.top].tolist())) if r.top else []
-                r.logprobs.append(TokenChoice(float(lp[i]), int(rank[i]), top))
+                note, i = r.unread.popleft()
+                r.logprobs.append(note.choice(i, r.top))
         for r in list(self.rows):
             if r.state == "decode" and r.tokens:
                 self.pool.lengths[r.rid] = r.length
