@@ -124,7 +124,8 @@ __global__ __launch_bounds__(64) void beam_select_kernel(const BeamArgs a) {
 // that came free (one workgroup); one launch for small tables.  Latency and the order among the parts bound it: 8 tables of 272
 // pages 12 us (13 as three launches, each of which costs the host some 3 more), 512 of 544 pages 5 + 8 + 11.
 constexpr int kForkThreads = 1024, kPage = JIT_PAGE_TOKENS;
-constexpr int kSmallFork = 8192;  // entries of the tables that one workgroup takes
+constexpr int kSmallFork = 4096;  // entries of the tables that one workgroup takes (2,176: 10.0 us in a graph, 10.7 as three
+                                  // launches; 8,160: 17.5 and 11.2)
 
 struct ForkArgs {
   const int32_t *table, *lens, *parents, *free_at;
@@ -425,7 +426,8 @@ extern "C" int jit_kv_copy_pages_layers(void *const *pools, int layers, int num_
   CopyArgs a;
   a.src = src, a.dst = dst, a.num_pages = num_pages;
   a.page_words = (int)(page_bytes / 16);
-  // parts of a page, none of fewer than 1,024 words, until 1,024 workgroups copy
+  // parts of a page, none of fewer than 1,024 words, until 1,024 workgroups copy (1 page of 64 KB in 48 layers: 2.6 us in a
+  // graph, 4.4 whole; 7 of 32 KB: 3.8 and 4.1)
   const long long pages = (long long)n * (layers < kMaxLayers ? layers : kMaxLayers), most_parts = (a.page_words + 1023) / 1024;
   a.parts = (int)(pages >= 1024 ? 1 : (1024 + pages - 1) / pages < most_parts ? (1024 + pages - 1) / pages : most_parts);
   a.part_words = (a.page_words + a.parts - 1) / a.parts;

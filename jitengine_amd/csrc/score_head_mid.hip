@@ -5,7 +5,8 @@
 // blocks keep their sums over all of K in registers (16 x 16 x 32 products, tokens on the rows, head rows on the columns:
 // a lane's scale is its own row's), so biases, softmax and the meeting of lanes and waves come once a pass.  What bounds
 // it: the head's bytes below some 50 rows, past that the issue of products and the sums behind them (a 16 x 16 x 32
-// product holds the issue port for some 11 of its 16 cycles).
+// product holds the issue port for some 11 of its 16 cycles).  77 rows x 151,936 x 2,048 take 83 to 90 us (head_tile_kernel:
+// 127), 17 rows x 4,096 86 us (122), 96 rows x 4,096 190 us (222), 32 rows x 2,048 49 us.
 #include "score_head.hpp"
 
 namespace {
@@ -13,6 +14,7 @@ namespace {
 using namespace head;
 
 constexpr int kPairs = 2;  // of a step
+constexpr int kMaxK = 4096;
 
 template <int STEP>
 __device__ __forceinline__ float row_swap(float v) {  // mirrored in 16, in 8, then lanes l ^ 2 and l ^ 1
@@ -52,8 +54,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   uint32_t um = 0x00780078u, uc = 0x41804180u;
   asm volatile("" : "+v"(um), "+s"(uc));
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds);
-  uint16_t *xs = (uint16_t *)(lds + 2 * kStage);  // [3][NT][32]
-  int *toks = (int *)(xs + 3 * NT * 32);          // [NT]
+  uint16_t *xs = (uint16_t *)(lds + 2 * kStage);  // [3][NT][G32]
+  int *toks = (int *)(xs + 3 * NT * a.G32);       // [NT]
 
   // a wave's load j brings 4 rows of 256 bytes: number q = wave + 8 j is pair q / (4 T16), token tile q / 4 % T16, rows
   // 4 (q % 4) ..; row r's piece c sits in slot c ^ r % 16.  (Rows past T read the last row again, see head_tile_kernel.)
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   load_x(0, 0);
 #pragma unroll
   for (int i = 0; i < NB; i++) load_w(0, 0, i);
-  for (int c = threadIdx.x; c < 3 * NT * 16; c += kThreads) ((uint32_t *)xs)[c] = 0u;
+  for (int c = threadIdx.x; c < 3 * NT * a.G32 / 2; c += kThreads) ((uint32_t *)xs)[c] = 0u;
   for (int c = threadIdx.x; c < NT; c += kThreads) toks[c] = c < a.T ? a.tokens[c] : -1;
   __syncthreads();
 
@@ -170,29 +172,32 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
           for (int i = 0; i < 3; i++) {
             const float v = bf2f(f2bf(s));
-            xs[(i * NT + row) * 32 + grp] = (uint16_t)(__float_as_uint(v) >> 16);
+            xs[(i * NT + row) * a.G32 + grp] = (uint16_t)(__float_as_uint(v) >> 16);
             s -= v;
           }
         }
       }
       stage ^= 1;
     }
-    // biases: sum_g (b - 16 s)_g X_g over the 32 groups, X in its three pieces, the smallest first
-    uint2 sb[NB][4];  // of pairs 4 lg .. + 3, all asked for at once
+    // biases: sum_g (b - 16 s)_g X_g over 32 groups at a time, X in its three pieces, the smallest first
+    for (int c0 = 0; c0 < a.G32 / 2; c0 += 16) {
+    uint2 sb[NB][4];  // of pairs c0 + 4 lg .. + 3, all asked for at once
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const uint8_t *sp = a.w + min(block(pass, i), r1 - 1) * blk_bytes + (long long)GP * qtile::kNibbleBytes;
 #pragma unroll
-      for (int j = 0; j < 4; j++) sb[i][j] = *(const uint2 *)(sp + (uint32_t)(min(4 * lg + j, GP - 1) * qtile::kScaleBytes + 8 * lr));
+      for (int j = 0; j < 4; j++) sb[i][j] = *(const uint2 *)(sp + (uint32_t)(min(c0 + 4 * lg + j, GP - 1) * qtile::kScaleBytes + 8 * lr));
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    bare_barrier();  // the sums are there, and the last step's rows have been read
+    if (!c0) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      bare_barrier();  // the sums are there, and the last step's rows have been read
+    }
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       Frag8 fs, fb;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const bool in = 4 * lg + j < GP;
+        const bool in = c0 + 4 * lg + j < GP;
         fs.u[j] = in ? sb[i][j].x : 0u;
         fb.u[j] = in ? sb[i][j].y : 0u;
       }
@@ -202,13 +207,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int k = 2; k >= 0; k--) {
           Frag8 x;
-          x.q = *(const uint4 *)(xs + (k * NT + 16 * t + lr) * 32 + 8 * lg);
+          x.q = *(const uint4 *)(xs + (k * NT + 16 * t + lr) * a.G32 + 2 * c0 + 8 * lg);
           d = mfma16x16x32(x, fs, d);
           acc[i][t] = mfma16x16x32(x, fb, acc[i][t]);
         }
 #pragma unroll
         for (int k = 0; k < 4; k++) acc[i][t][k] = fmaf(-16.0f, d[k], acc[i][t][k]);
       }
+    }
     }
 #pragma unroll
     for (int i = 0; i < NB; i++)
@@ -279,14 +285,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 
 template <int T16, int NB>
 int launch(const HeadArgs &a, hipStream_t st) {
-  constexpr int lds = 16 * T16 * (4 * 256 + 3 * 64 + 4);
-  static_assert(lds <= 160 * 1024, "gfx950 gives a workgroup at most 160 KB of LDS");
+  constexpr int most = 16 * T16 * (4 * 256 + 6 * (kMaxK / 64) + 4);
+  static_assert(most <= 160 * 1024, "gfx950 gives a workgroup at most 160 KB of LDS");
   static const bool wide = [] {  // (more than the static limit)
-    (void)hipFuncSetAttribute((const void *)&head_mid_kernel<T16, NB>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    (void)hipFuncSetAttribute((const void *)&head_mid_kernel<T16, NB>, hipFuncAttributeMaxDynamicSharedMemorySize, most);
     return true;
   }();
   (void)wide;
-  head_mid_kernel<T16, NB><<<a.parts, kThreads, lds, st>>>(a);
+  head_mid_kernel<T16, NB><<<a.parts, kThreads, 16 * T16 * (4 * 256 + 6 * a.G32 + 4), st>>>(a);
   return jit::check_launch("jit_head_logprobs");
 }
 
@@ -308,7 +314,7 @@ int launch_even(const HeadArgs &a, hipStream_t st) {
 namespace head {
 
 int mid_tile(long long T, int K) {
-  if (T <= 16 || T > 96 || K > 2048) return 0;
+  if (T <= 16 || T > 96 || K > kMaxK) return 0;
   return (int)(T + 15) / 16 * 16;
 }
 

@@ -251,6 +251,15 @@ def test_head_logprobs_of_every_head(T, K, V):
     _check_head(x, lin, tok)
 
 
+@pytest.mark.parametrize("K", [1920, 2176, 4096])
+@pytest.mark.parametrize("T", [17, 50, 77, 96])
+def test_head_logprobs_of_one_tile_over_several_passes(T, K):
+    g = torch.Generator(device=DEV).manual_seed(T + K)
+    lin = _head(30000, K, T)
+    tok = torch.randint(0, 30000, (T,), generator=g, device=DEV, dtype=torch.int32)
+    _check_head((2 * torch.randn((T, K), generator=g, device=DEV)).to(torch.bfloat16), lin, tok)
+
+
 @pytest.mark.parametrize("T", [1, 20, 130])
 def test_head_logprobs_over_a_vocabulary(T):
     V, K = 151936, 512
