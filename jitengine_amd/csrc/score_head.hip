@@ -88,6 +88,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kRB = 2;               // 32-row blocks of a wave
 constexpr int kMaxTT = 4;            // token tiles of 32
+constexpr int kUnit = 2 * kWaves * kRB;  // 16-row blocks that the waves take at a time
 constexpr int kWStage = 2 * kRB * qtile::kTileBytes;  // a wave's weights of a step: its 16-row blocks' nibbles, then scales
 constexpr int kWLoads = 3 * kRB;     // loads of them
 
@@ -103,9 +104,10 @@ struct Lds {
 
 // A workgroup of 8 waves, one a CU, walks 64 kWaves rows of the head at a time (a wave 32 RB of them) against 32 TT tokens.
 // Products are 32 x 32 x 16: tokens on the rows, head rows on the columns, so a lane's scale is its own row's.  The work
-// is the line of (token tile, 16-row block) pairs, tiles first to last, cut into equal runs, one a workgroup.  What bounds
+// is the line of (token tile, unit of 32 or 16 blocks) pairs, tiles first to last, cut into equal runs, one a workgroup (the 8
+// waves do a unit at a time, so that no run has a part of one but at a tile's end).  What bounds
 // it: the issue slots that products (11 of their 32 cycles), scaling and unpacking share, at a clock that power holds near
-// 1.7 GHz: 2,048 rows of 248,320 x 2,048 take 2.05 ms, 1.02 PFLOP/s (a bare bf16 product of the library 1.68 ms).  Of a
+// 1.7 GHz: 2,048 rows of 248,320 x 2,048 take 2.05 to 2.16 ms, 1 PFLOP/s (a bare bf16 product of the library 1.68 ms).  Of a
 // tile's cycles 65% are its steps, 15% their barriers, 10% the biases and 10% the softmax.
 template <int TT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void head_tile_kernel(const HeadArgs a) {
@@ -135,13 +137,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   const uint8_t *wmine = lds + L::kW + wave * kWStage + (l >> 4 & 1) * qtile::kNibbleBytes + 16 * (32 * h + lr);
   const uint8_t *smine = lds + L::kW + wave * kWStage + 2 * kRB * qtile::kNibbleBytes + row * 8;
 
-  const long long line = (long long)a.tiles * blocks;
+  const int units = (blocks + a.unit - 1) / a.unit;  // of a tile
+  const long long line = (long long)a.tiles * units;
   long long at0 = line * n / a.parts;
   const long long at1 = line * (n + 1) / a.parts;
   if (n >= a.parts) return;
   for (int seg = 0; at0 < at1; seg++) {
-    const int tile = (int)(at0 / blocks), r0 = (int)(at0 % blocks), r1 = (int)min((long long)blocks, r0 + (at1 - at0));
-    at0 += r1 - r0;
+    const int tile = (int)(at0 / units), u0 = (int)(at0 % units), u1 = (int)min((long long)units, u0 + (at1 - at0));
+    const int r0 = u0 * a.unit, r1 = min(blocks, u1 * a.unit);
+    at0 += u1 - u0;
     const int t0 = NT * tile;
     if (seg) __syncthreads();  // (the last tile's states are read)
     for (int c = l; c < NT; c += 64) st[c] = kLowest, st[NT + c] = st[2 * NT + c] = 0.0f;
@@ -422,7 +426,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     asm volatile("" ::: "memory");
     }
   };
-  const int span = 2 * kWaves * kRB, n_full = (r1 - r0) / span, rest = (r1 - r0) % span;
+  constexpr int span = kUnit;
+  const int n_full = (r1 - r0) / span, rest = (r1 - r0) % span;
   walk(std::integral_constant<int, kRB>{}, r0, n_full + (rest > span / 2 ? 1 : 0));
   if (rest > 0 && rest <= span / 2) walk(std::integral_constant<int, 1>{}, r0 + span * n_full, 1);
     wait_loads<0>();  // (the last stages that were asked for)
@@ -621,7 +626,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 // One wave a token: the runs that met its tile, put together in a fixed order.
 __global__ __launch_bounds__(64) void head_merge_kernel(const HeadArgs a, int NT) {
   const int tok = blockIdx.x, l = lane_id(), tile = tok / NT;
-  const long long blocks = a.V >> 4, line = blocks * a.tiles, lo = tile * blocks, hi = lo + blocks;
+  const long long units = ((a.V >> 4) + a.unit - 1) / a.unit, line = units * a.tiles, lo = tile * units, hi = lo + units;
   Stat s{kLowest, 0.0f, 0.0f};
   if (a.tiles == 1) {  // (every run)
     const float *q = a.part + tok;
@@ -636,7 +641,7 @@ __global__ __launch_bounds__(64) void head_merge_kernel(const HeadArgs a, int NT
       const long long from = line * n / a.parts, to = line * (n + 1) / a.parts;
       if (from >= hi) break;
       if (to <= from) continue;
-      const float *q = a.part + ((long long)n * a.segs + tile - (int)(from / blocks)) * 3 * NT + tok % NT;
+      const float *q = a.part + ((long long)n * a.segs + tile - (int)(from / units)) * 3 * NT + tok % NT;
       s = join(s, {q[0], q[NT], q[2 * NT]});
     }
   }
@@ -653,10 +658,13 @@ __global__ __launch_bounds__(64) void head_merge_kernel(const HeadArgs a, int NT
   a.logprob[tok] = !in ? 0.0f : nan ? __builtin_nanf("") : (float)(((double)a.picked[tok] * kLog2 - (double)s.m - log_l) * kLn2);
 }
 
-// Token tiles of a launch: 32 TT tokens each, TT as even as they come.
+// Token tiles of a launch: 32 TT tokens each, TT as even as they come, so many that the last workgroup ends first.
+// (Always the largest tiles, runs of any number of blocks: 500 rows x 2,000 x 512 58 us, x 20,000 x 1,024 66, x 40,000 x
+// 2,048 135, 200 rows x 40,000 x 2,048 95, 129 x 151,936 x 2,048 176; so 17, 49, 128, 74, 167.)
+constexpr int kHalfCost[kMaxTT] = {43, 63, 95, 103};  // of 16 blocks of a tile of 1 .. 4 (3: more of it in spilled registers)
 struct Shape {
   bool few, mid;  // up to 16 rows that fit LDS; one tile of up to 96
-  int tt, tile, tiles, parts, segs, T16, G32;
+  int tt, tile, tiles, parts, segs, T16, G32, unit = kUnit;
   long long part_at, picked_at, bytes;
 };
 Shape shape_of(long long T, int K, int V) {
@@ -678,12 +686,22 @@ Shape shape_of(long long T, int K, int V) {
     s.parts = mid_parts(V);
     s.T16 = 0;
   } else {
-    const long long n32 = (T + 31) / 32;
-    s.tiles = (int)((n32 + kMaxTT - 1) / kMaxTT);
-    s.tt = s.tiles ? (int)((n32 + s.tiles - 1) / s.tiles) : 1;
+    const long long n32 = (T + 31) / 32, halves = (blocks + kUnit / 2 - 1) / (kUnit / 2);
+    long long best = 0;
+    for (int most = kMaxTT; most > 0; most--) {
+      const long long tiles = (n32 + most - 1) / most;
+      const int tt = tiles ? (int)((n32 + tiles - 1) / tiles) : 1;
+      const long long cost = (tiles * halves + 255) / 256 * kHalfCost[tt - 1];
+      if (most < kMaxTT && cost >= best) continue;
+      best = cost;
+      s.tiles = (int)tiles;
+      s.tt = tt;
+    }
     s.tile = 32 * s.tt;
-    const long long fill = (s.tiles * (long long)blocks + 3) / 4;  // (a run of four blocks at least)
-    s.parts = fill < 256 ? (int)(fill < 1 ? 1 : fill) : 256;
+    const long long whole = s.tiles * (long long)((blocks + kUnit - 1) / kUnit);
+    s.unit = s.tiles * halves > 256 && whole <= 256 ? kUnit : kUnit / 2;  // (whole walks where each has a workgroup)
+    const long long line = s.tiles * (long long)((blocks + s.unit - 1) / s.unit);
+    s.parts = line < 256 ? (int)(line < 1 ? 1 : line) : 256;
     s.segs = s.tiles / s.parts + 2;
     s.T16 = s.tiles * s.tile;
   }
@@ -740,7 +758,7 @@ extern "C" int jit_head_logprobs(const uint16_t *x, int T, int K, const void *w,
     return jit::fail(JIT_EINVAL, "head_logprobs: a workspace of %lld bytes, 16-byte aligned, is needed", s.bytes);
   uint8_t *ws = (uint8_t *)workspace;
   HeadArgs a{x, (const uint8_t *)w, tokens, (uint16_t *)ws, (float *)(ws + s.part_at), (float *)(ws + s.picked_at),
-             logprob, entropy, lse, T, K, V, s.parts, s.segs, s.tiles, s.T16, s.G32};
+             logprob, entropy, lse, T, K, V, s.parts, s.segs, s.tiles, s.T16, s.G32, s.unit};
   const hipStream_t st = (hipStream_t)stream;
   int rc;
   if (s.few) {

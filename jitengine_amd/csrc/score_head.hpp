@@ -21,6 +21,7 @@ struct HeadArgs {
   float *picked;   // [T] the given tokens' logits
   float *logprob, *entropy, *lse;
   int T, K, V, parts, segs, tiles, T16, G32;
+  int unit;  // 16-row blocks that stay together where a tile of many rows is cut into runs
 };
 
 // A token's softmax in base 2 against a reference m near its largest logit: with y = x log2 e - m, l = sum 2^y and
