@@ -260,6 +260,15 @@ def test_head_logprobs_of_one_tile_over_several_passes(T, K):
     _check_head((2 * torch.randn((T, K), generator=g, device=DEV)).to(torch.bfloat16), lin, tok)
 
 
+@pytest.mark.parametrize("T,V", [(1000, 48), (5000, 528), (40000, 32), (40001, 272)])
+def test_head_logprobs_of_many_rows_and_a_small_head(T, V):
+    """More token tiles than workgroups, whose runs meet several of them."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    lin = _head(V, 256, V)
+    tok = torch.randint(-1, V + 1, (T,), generator=g, device=DEV, dtype=torch.int32)
+    _check_head((2 * torch.randn((T, 256), generator=g, device=DEV)).to(torch.bfloat16), lin, tok)
+
+
 @pytest.mark.parametrize("T", [1, 20, 130])
 def test_head_logprobs_over_a_vocabulary(T):
     V, K = 151936, 512
