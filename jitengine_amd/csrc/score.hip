@@ -6,7 +6,8 @@
 //   rank of v = #{j : x_j > x_v, or x_j = x_v and j < v}.
 // Every lane keeps its own (m, l, t), rescaled where its values grow well past m; lanes, waves and slices meet by the same
 // rule in a fixed order, so a call's bits repeat.  y is one fused multiply-add x log2 e - (m log2 e), whose second term's
-// rounding is the same for every y and cancels; rows whose largest magnitude would overflow there take (x - m) log2 e.
+// rounding is the same for every y and cancels; where that rounding would itself be many powers of two (m far from 0, as in
+// a row of nothing but mask values of -1e9 or -1e30), y is (x - m) log2 e.
 // Masked entries (-inf, or the type's lowest value beside larger ones) add 0; a row of nothing but lowest values is uniform.
 //
 // A row is cut into slices, one workgroup each, until the launch fills the chip; a second, small launch puts a row's
@@ -26,6 +27,7 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxTop = 64, kMaxTokens = 64, kMaxSlices = 64;
 constexpr int kRoom = 128;  // values a wave keeps: at least kMaxTop + 64
 constexpr float kLowest = -3.402823466e38f, kFloor = -2000.0f, kLog2e = 1.44269504088896341f;
+constexpr float kNear = 1048576.0f;  // |m log2 e| up to which it is rounded: by at most 2^-4 there
 constexpr double kLn2 = 0.693147180559945309;
 
 struct ScoreArgs {
@@ -89,11 +91,16 @@ struct Stat {
   float m, l, t;
 };
 
-// y from one reference to a larger one: between the two rounded terms, so that it adds no error (floor at -2000, where
-// 2^y is 0; a NaN stays one).
+// Whether y is formed with m log2 e rounded, or with the difference to m.
+__device__ __forceinline__ bool is_near(float m) { return fabsf(m * kLog2e) < kNear; }
+
+// y from one reference to a larger one: between the two terms that were subtracted, rounded or not, so that it adds no error
+// (floor at -2000, where 2^y is 0; a NaN stays one).
 __device__ __forceinline__ float between(float a, float b) {
 #pragma clang fp contract(off)
-  const float ra = a * kLog2e, rb = b * kLog2e, r = fabsf(rb) < __builtin_inff() ? ra - rb : (a - b) * kLog2e;
+  const float ra = a * kLog2e, rb = b * kLog2e;
+  const float r = is_near(b) ? (is_near(a) ? ra - rb : fmaf(a, kLog2e, -rb))
+                             : (is_near(a) ? -fmaf(b, kLog2e, -ra) : (a - b) * kLog2e);
   return r < kFloor ? kFloor : r;
 }
 
@@ -117,10 +124,9 @@ __device__ __forceinline__ Stat wave_join(Stat s) {
 __device__ __forceinline__ float logprob_of(float x, const Stat &s, double log_l) {
   if (s.l != s.l) return __builtin_nanf("");  // a NaN or +inf in the row
   if (!(x > -__builtin_inff())) return x;     // (-inf, also in a row of nothing else; or a NaN)
+  if (!is_near(s.m)) return (float)((double)x - (double)s.m - log_l * kLn2);
   const float mb = s.m * kLog2e;
-  const double y = fabsf(mb) < __builtin_inff() ? (double)x * (double)kLog2e - (double)mb
-                                                : ((double)x - (double)s.m) * (double)kLog2e;
-  return (float)((y - log_l) * kLn2);
+  return (float)(((double)x * (double)kLog2e - (double)mb - log_l) * kLn2);
 }
 
 // ------------------------------------------------------------------ order
@@ -344,12 +350,13 @@ __global__ __launch_bounds__(kThreads) void score_rows_kernel(const ScoreArgs a)
     // (a reference that lags by up to 8 costs nothing: 2^y stays below 2^12; following every larger value took 40
     // instructions a step)
     if (top > st.m + 8.0f) st = rebase(st, top);
-    // a lane that has met nothing but masked values takes the wave's largest
-    if (!__all(fabsf(st.m * kLog2e) < kInf)) {
+    // a lane that has met nothing but masked values takes the wave's largest; where that one is far from 0 too, all lanes
+    // have it, and form y alike
+    if (!__all(is_near(st.m))) {
       st = rebase(st, wave_butterfly<true>(st.m));
     }
     const float ref = st.m * kLog2e;
-    const bool huge = !__all(fabsf(ref) < kInf);
+    const bool far = !__all(is_near(st.m));
     float l = st.l, t = st.t;
 #pragma unroll
     for (int u = 0; u < U; u++)
@@ -359,15 +366,15 @@ __global__ __launch_bounds__(kThreads) void score_rows_kernel(const ScoreArgs a)
         l += e;
         t = fmaf(e, y, t);
       }
-    // once more where a masked value (0 times -inf) or a NaN is among them, or y overflows (one instruction a value less
-    // for rows without)
-    if (huge || __any(t != t)) {
+    // once more where a masked value (0 times -inf) or a NaN is among them, or y is the other one (one instruction a value
+    // less for rows without)
+    if (far || __any(t != t)) {
       l = st.l, t = st.t;
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
         for (int j = 0; j < N; j++) {
-          const float r = huge ? (x[u][j] - st.m) * kLog2e : fmaf(x[u][j], kLog2e, -ref), y = r < kFloor ? kFloor : r;
+          const float r = far ? (x[u][j] - st.m) * kLog2e : fmaf(x[u][j], kLog2e, -ref), y = r < kFloor ? kFloor : r;
           const float e = __builtin_amdgcn_exp2f(y);
           l += e;
           t = fmaf(e, y, t);
