@@ -99,8 +99,9 @@ __device__ __forceinline__ bool is_near(float m) { return fabsf(m * kLog2e) < kN
 __device__ __forceinline__ float between(float a, float b) {
 #pragma clang fp contract(off)
   const float ra = a * kLog2e, rb = b * kLog2e;
-  const float r = is_near(b) ? (is_near(a) ? ra - rb : fmaf(a, kLog2e, -rb))
-                             : (is_near(a) ? -fmaf(b, kLog2e, -ra) : (a - b) * kLog2e);
+  float r = ra - rb;
+  if (__builtin_expect(!(fmaxf(fabsf(ra), fabsf(rb)) < kNear), 0))
+    r = is_near(b) ? fmaf(a, kLog2e, -rb) : is_near(a) ? -fmaf(b, kLog2e, -ra) : (a - b) * kLog2e;
   return r < kFloor ? kFloor : r;
 }
 
@@ -124,9 +125,9 @@ __device__ __forceinline__ Stat wave_join(Stat s) {
 __device__ __forceinline__ float logprob_of(float x, const Stat &s, double log_l) {
   if (s.l != s.l) return __builtin_nanf("");  // a NaN or +inf in the row
   if (!(x > -__builtin_inff())) return x;     // (-inf, also in a row of nothing else; or a NaN)
-  if (!is_near(s.m)) return (float)((double)x - (double)s.m - log_l * kLn2);
-  const float mb = s.m * kLog2e;
-  return (float)(((double)x * (double)kLog2e - (double)mb - log_l) * kLn2);
+  const bool near = is_near(s.m);
+  const float by = near ? kLog2e : 1.0f, mb = near ? s.m * kLog2e : s.m;
+  return (float)(((double)x * (double)by - (double)mb) * (near ? kLn2 : 1.0) - log_l * kLn2);
 }
 
 // ------------------------------------------------------------------ order
