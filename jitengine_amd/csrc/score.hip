@@ -121,13 +121,14 @@ __device__ __forceinline__ Stat wave_join(Stat s) {
   return {r.m, wave_butterfly<false>(r.l), wave_butterfly<false>(r.t)};
 }
 
-// The log-probability of a logit x in a row of state s, log_l = log2 l.
+// The log-probability of a logit x in a row of state s, log_l = log2 l.  (l is rounded, so that of a token with nearly all
+// of the probability can come out above 0 by some 2^-24: it is 0 then.)
 __device__ __forceinline__ float logprob_of(float x, const Stat &s, double log_l) {
   if (s.l != s.l) return __builtin_nanf("");  // a NaN or +inf in the row
   if (!(x > -__builtin_inff())) return x;     // (-inf, also in a row of nothing else; or a NaN)
   const bool near = is_near(s.m);
   const float by = near ? kLog2e : 1.0f, mb = near ? s.m * kLog2e : s.m;
-  return (float)(((double)x * (double)by - (double)mb) * (near ? kLn2 : 1.0) - log_l * kLn2);
+  return (float)fmin(((double)x * (double)by - (double)mb) * (near ? kLn2 : 1.0) - log_l * kLn2, 0.0);
 }
 
 // ------------------------------------------------------------------ order

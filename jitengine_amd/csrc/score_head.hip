@@ -655,7 +655,8 @@ __global__ __launch_bounds__(64) void head_merge_kernel(const HeadArgs a, int NT
   const bool in = v >= 0 && v < a.V;
   a.lse[tok] = nan ? __builtin_nanf("") : (float)(((double)s.m + log_l) * kLn2);
   a.entropy[tok] = nan ? __builtin_nanf("") : (float)(fmax(log_l - (double)s.t / (double)s.l, 0.0) * kLn2);
-  a.logprob[tok] = !in ? 0.0f : nan ? __builtin_nanf("") : (float)(((double)a.picked[tok] * kLog2 - (double)s.m - log_l) * kLn2);
+  // (not above 0, where the rounding of l would put a token that has nearly everything)
+  a.logprob[tok] = !in ? 0.0f : nan ? __builtin_nanf("") : (float)fmin(((double)a.picked[tok] * kLog2 - (double)s.m - log_l) * kLn2, 0.0);
 }
 
 // Token tiles of a launch: 32 TT tokens each, TT as even as they come, so many that the last workgroup ends first.

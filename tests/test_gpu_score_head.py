@@ -1,0 +1,87 @@
+"""Scoring from hidden rows and the packed head: running softmax states that must follow the logits upwards."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from jitengine_amd import ops
+from jitengine_amd.quant import random_quantized
+from tests.test_gpu_scoring import DEV, U
+
+pytestmark = pytest.mark.gpu
+
+# Tolerances of the softmax over logits that are exact, in half steps U of fp32.  A logit's exponential is off by ln 2 of
+# its exponent's rounding, whose magnitude is below 72 + 16 (a reference lags by up to 64), and by 2 for the instruction; a
+# join scales a state by another such exponential.  A wave folds up to 16 tiles, the 16 or 32 lanes of a row meet in 5
+# additions, 8 waves in 8 joins, the runs in 4 + 6.
+EXP = 0.7 * 88 + 2
+JOINS = 18
+REL = 16 + 5 + EXP + JOINS * (EXP + 2)  # of the sum of exponentials
+OWN = 88 * (16 + 5 + 3 * JOINS)         # of the weighted sum alone, for roundings that it does not share with the other
+
+
+def _softmax(z: torch.Tensor, tok: torch.Tensor):
+    """(logprob, entropy, log of the sum, standard deviation of the logits under their distribution) of fp64 logits."""
+    lse = torch.logsumexp(z, -1)
+    p = torch.exp(z - lse[:, None])
+    mean = (p * z).sum(-1)
+    sd = torch.sqrt((p * (z - mean[:, None]) ** 2).sum(-1))
+    return z.gather(1, tok.long()[:, None])[:, 0] - lse, torch.special.entr(p).sum(-1), lse, sd
+
+
+def _check(r, lp, h, lse, sd, bound=0.0):
+    """`bound`: how far the logits may be off."""
+    tol = REL * U + 2 * bound
+    assert torch.all((r.logprob.double() - lp).abs() <= tol + 1.25 * U * lp.abs())  # (log2 e is off by a quarter)
+    assert torch.all((r.lse.double() - lse).abs() <= tol + 1.25 * U * lse.abs())
+    # what both sums share moves the entropy by the logits' spread, the rest by the weighted sum's own roundings
+    assert torch.all((r.entropy.double() - h).abs() <= (REL * U + bound) * (2 + 2 * sd) + OWN * U + U * h)
+    assert float(r.logprob.max()) <= 0
+
+
+def _exact_head(target: torch.Tensor, K: int):
+    """A head whose rows' logits against rows of a constant are exact: q of any value with scale 2^-8, biases that bring row v
+    to about target[v] for a hidden row of ones (every term and sum is a multiple of 2^-10 below 2^9: fp32 loses nothing)."""
+    V = target.numel()
+    lin = random_quantized((V, K), 5, 0.02, DEV)
+    lin.scales = torch.full_like(lin.scales, 2.0 ** -8)
+    b = (target.double() / K - 7.5 / 256)[:, None].expand(V, K // 64)
+    lin.biases = (torch.round(b * 2 ** 8) / 2 ** 8).to(torch.bfloat16).contiguous()
+    q = (lin.weight.view(V, K // 8, 1) >> (4 * torch.arange(8, device=DEV, dtype=torch.int32))) & 15
+    z = q.reshape(V, K).double().sum(-1) / 256 + 64 * lin.biases.double().sum(-1)
+    return lin, z
+
+
+def _along(kind: str, V: int, most: float) -> torch.Tensor:
+    v = torch.arange(V, device=DEV) / V
+    if kind == "rising":
+        return most * v
+    if kind == "falling":
+        return most * (1 - v)
+    if kind == "steps":  # a wave meets each part after the one before it
+        return most * torch.floor(4 * v) / 4
+    x = torch.zeros(V, device=DEV)
+    x[-V // 50] = most  # one row near the end
+    return x
+
+
+@pytest.mark.parametrize("most", [20.0, 44.0, 60.0, 200.0])  # (a reference lags by up to 44.4)
+@pytest.mark.parametrize("kind", ["rising", "falling", "steps", "one"])
+@pytest.mark.parametrize("T", [1, 16, 50, 130, 300])
+def test_states_follow_rising_logits(T, kind, most):
+    """Sums that a wave already holds when larger logits come, in each kernel: hidden rows of ones, halves and quarters give
+    the same shape at three heights."""
+    V, K = 400000, 256
+    lin, z = _exact_head(_along(kind, V, most), K)
+    a = torch.tensor([1.0, 0.5, 0.25], device=DEV)[torch.arange(T, device=DEV) % 3]
+    x = a[:, None].expand(T, K).to(torch.bfloat16).contiguous()
+    g = torch.Generator(device=DEV).manual_seed(T)
+    tok = torch.randint(0, V, (T,), generator=g, device=DEV, dtype=torch.int32)
+    tok[::2] = int(z.argmax())
+    r = ops.head_logprobs(x, ops.prepack(lin), tok)
+    for c in (1.0, 0.5, 0.25):
+        at = torch.nonzero(a == c)[:, 0]
+        if at.numel():
+            ref = _softmax((c * z).expand(at.numel(), V), tok[at])
+            _check(ops.HeadLogprobs(r.logprob[at], r.entropy[at], r.lse[at]), *ref)

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from jitengine_amd import ops
-from tests.test_gpu_scoring import DEV, _check_rows
+from tests.test_gpu_scoring import DEV, U, _check_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,21 @@ def test_token_logprobs_of_rows_far_from_zero(V, slices, kind, dtype):
     many = x.repeat(200, 1)  # (one workgroup a row)
     r = ops.token_logprobs(many.to(DEV), tok.repeat(200).to(DEV), top=9)
     _check_rows(x, tok, 9, ops.TokenLogprobs(*(t[-6:] for t in (r.logprob, r.rank, r.entropy, r.top_ids, r.top_logprobs))))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("V", [100, 40000])
+def test_token_logprobs_are_never_above_zero(V, dtype):
+    """Rows whose mask leaves one token, and rows in which one has nearly everything: probabilities of 1, rounded."""
+    B = 300
+    g = torch.Generator().manual_seed(V)
+    x = torch.full((B, V), -math.inf)
+    tok = torch.randint(0, V, (B,), generator=g, dtype=torch.int32)
+    x[torch.arange(B), tok.long()] = torch.linspace(2, 100, B)
+    x[B // 2:] = torch.where(torch.isinf(x[B // 2:]), torch.linspace(-30, -20, V), x[B // 2:])
+    x = x.to(dtype)
+    r = ops.token_logprobs(x.to(DEV), tok.to(DEV), top=2)
+    assert float(r.logprob.max()) <= 0 and float(r.top_logprobs.max()) <= 0 and float(r.entropy.min()) >= 0
+    # (the sums hold one number of note: its exponential, up to a few joins, and the logarithm's argument are rounded)
+    assert float(r.logprob.min()) >= -64 * U
+    assert torch.equal(r.rank, torch.zeros_like(r.rank)) and torch.equal(r.top_ids[:, 0], tok.to(DEV))
