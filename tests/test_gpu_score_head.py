@@ -1,4 +1,5 @@
-"""Scoring from hidden rows and the packed head: running softmax states that must follow the logits upwards."""
+"""Scoring from hidden rows and the packed head: each of its kernels over long K and long runs of the head, and running
+softmax states that must follow the logits upwards."""
 
 from __future__ import annotations
 
@@ -7,7 +8,7 @@ import torch
 
 from jitengine_amd import ops
 from jitengine_amd.quant import random_quantized
-from tests.test_gpu_scoring import DEV, U
+from tests.test_gpu_scoring import DEV, U, _head, _head_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -38,6 +39,38 @@ def _check(r, lp, h, lse, sd, bound=0.0):
     # what both sums share moves the entropy by the logits' spread, the rest by the weighted sum's own roundings
     assert torch.all((r.entropy.double() - h).abs() <= (REL * U + bound) * (2 + 2 * sd) + OWN * U + U * h)
     assert float(r.logprob.max()) <= 0
+
+
+def _tiles(T: int, K: int, V: int) -> int:
+    """Token tiles of 32 that a workgroup of the kernel for many rows takes, from the workspace's size."""
+    need, n32, found = ops.head_logprobs_workspace_bytes(T, K, V), (T + 31) // 32, set()
+    for tt in range(1, 5):
+        for tiles in range(-(-n32 // tt), -(-n32 // tt) + 1):
+            t16 = 32 * tt * tiles
+            g32 = (K // 64 + 31) // 32 * 32
+            if need == (6 * t16 * g32 + 15) // 16 * 16 + 12 * 256 * (tiles // 256 + 2) * 32 * tt + 4 * T:
+                assert tiles * (V // 16) // 256 >= 64  # (a run holds several walks of 32 blocks)
+                found.add(tt)
+    assert len(found) == 1
+    return found.pop()
+
+
+@pytest.mark.parametrize("K", [1920, 2048, 2176, 4224])
+@pytest.mark.parametrize("T,V,tt", [(130, 151936, 2), (282, 151936, 3), (300, 151936, 4), (512, 151936, 4), (24, 302000, 1)])
+def test_many_rows_over_long_runs(T, V, tt, K):
+    """Every tile of the kernel for many rows, over K below and above where the groups' sums fit LDS, with rows left over."""
+    if tt == 1 and K <= 4096:
+        pytest.skip("so few rows of this K are another kernel's")
+    assert _tiles(T, K, V) == tt
+    lin = _head(V, K, T + K)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = (1.5 * torch.randn((T, K), generator=g, device=DEV)).to(torch.bfloat16)
+    tok = torch.randint(0, V, (T,), generator=g, device=DEV, dtype=torch.int32)
+    tok[:3] = torch.tensor([0, V - 1, V // 2])
+    r = ops.head_logprobs(x, ops.prepack(lin), tok)
+    lp, h, lse, bound = _head_ref(x, lin, tok)
+    # (the spread: logits of standard deviation below 4 under any of these distributions)
+    _check(r, lp, h, lse, 4.0, bound)
 
 
 def _exact_head(target: torch.Tensor, K: int):
