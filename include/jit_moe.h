@@ -528,7 +528,9 @@ int jit_token_logprobs(const void *logits, int fp32, int B, int V, long long row
 /* The same of one token a row straight from hidden rows x [T, K] bf16 and a packed 4-bit head [V, K] (jit_q4_prepack),
  * with no logits in memory: logit = x . (s q + b) in fp32, not rounded to bf16 as jit_qmm_packed's are.
  *   logprob, entropy, lse [T]  of tokens [T] (logprob 0 for a token outside [0, V)); lse = m + ln l.
- * A row with a logit that is not finite, or of a magnitude past 2^127 / log2 e, is NaN in all three.
+ * A row is NaN in all three where its largest logit lies past +-2^28 / log2 e (fp32 logits are 16 apart there), and where
+ * one of its logits is not finite or has a sum on the way to it that is not: products are with q + 16 before the scale, 64
+ * of them a sum, so that no x of a magnitude below 2^117 overflows there.
  * Contract: K % 128 == 0, V % 16 == 0, T <= 2^20, T K < 2^31 (JIT_EUNSUPPORTED); x, w and the workspace 16-byte aligned;
  * a workspace of jit_head_logprobs_workspace_bytes. */
 long long jit_head_logprobs_workspace_bytes(int T, int K, int V);

@@ -650,7 +650,8 @@ __global__ __launch_bounds__(64) void head_merge_kernel(const HeadArgs a, int NT
   if (l) return;
   constexpr double kLn2 = 0.693147180559945309, kLog2 = (double)kLog2e;  // (log2 e as the states were formed with it)
   const double log_l = log2((double)s.l);
-  const bool nan = s.l != s.l;
+  // NaN (or +inf) among the logits leaves l NaN, -inf leaves t NaN; past kFar a reference's rounding is many powers of two
+  const bool nan = !(s.l > 0x1p-20f && s.t == s.t && fabsf(s.m) <= kFar);
   const int v = a.tokens[tok];
   const bool in = v >= 0 && v < a.V;
   a.lse[tok] = nan ? __builtin_nanf("") : (float)(((double)s.m + log_l) * kLn2);

@@ -1,5 +1,5 @@
-"""Scoring from hidden rows and the packed head: each of its kernels over long K and long runs of the head, and running
-softmax states that must follow the logits upwards."""
+"""Scoring from hidden rows and the packed head: each of its kernels over long K and long runs of the head, running softmax
+states that must follow the logits upwards, and rows whose sums overflow or lie far from 0."""
 
 from __future__ import annotations
 
@@ -118,3 +118,48 @@ def test_states_follow_rising_logits(T, kind, most):
         if at.numel():
             ref = _softmax((c * z).expand(at.numel(), V), tok[at])
             _check(ops.HeadLogprobs(r.logprob[at], r.entropy[at], r.lse[at]), *ref)
+
+
+@pytest.mark.parametrize("T", [1, 16, 50, 130])
+@pytest.mark.parametrize("value", [1e36, 1.1e37, 3e38])
+def test_rows_whose_sums_overflow_are_nan(T, value):
+    """Products are formed before the scale: sums that overflow on the way, or logits far past 2^28, make their row NaN and
+    no other."""
+    V, K = 5008, 256
+    lin = _head(V, K, 3)
+    lin.scales = lin.scales.abs()  # (positive and negative values overflow to one side each)
+    head = ops.prepack(lin)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn((T, K), generator=g, device=DEV).to(torch.bfloat16)
+    tok = torch.randint(0, V, (T,), generator=g, device=DEV, dtype=torch.int32)
+    want = ops.head_logprobs(x, head, tok)
+    for sign in (1, -1):
+        bad = x.clone()
+        bad[T // 2, 3] = sign * value
+        r = ops.head_logprobs(bad, head, tok)
+        keep = [i for i in range(T) if i != T // 2]
+        for w, t in zip((want.logprob, want.entropy, want.lse), (r.logprob, r.entropy, r.lse)):
+            assert torch.isnan(t[T // 2]) and torch.equal(t[keep], w[keep])
+
+
+@pytest.mark.parametrize("T", [1, 16, 50, 130])
+def test_logits_far_from_zero(T):
+    """Rows whose largest logit lies past +-2^28 / log2 e are NaN, nearer ones numbers."""
+    V, K = 5008, 256
+    g = torch.Generator(device=DEV).manual_seed(T)
+    tok = torch.randint(0, V, (T,), generator=g, device=DEV, dtype=torch.int32)
+    for top, rest, nan in ((1.5e8, 1.5e8, False), (-1.5e8, -1.5e8, False), (2e8, 0.0, True),
+                           (-2e8, -2e8, True), (1e12, 1e12, True), (1e30, 0.0, True), (-1e30, -1e30, True)):
+        lin = random_quantized((V, K), 5, 0.02, DEV)
+        lin.scales = torch.zeros_like(lin.scales)
+        b = torch.full((V, 1), rest / K, device=DEV)
+        b[V // 3] = top / K
+        lin.biases = b.expand(V, K // 64).to(torch.bfloat16).contiguous()
+        x = torch.ones((T, K), dtype=torch.bfloat16, device=DEV)
+        r = ops.head_logprobs(x, ops.prepack(lin), tok)
+        if nan:
+            assert all(torch.isnan(t).all() for t in (r.logprob, r.entropy, r.lse))
+        else:  # (sums of 256 equal bf16 numbers: exact)
+            z = K * lin.biases[:, 0].double()
+            lp, h, lse, sd = _softmax(z.expand(T, V), tok)
+            _check(r, lp, h, lse, sd)
