@@ -148,7 +148,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     at0 += u1 - u0;
     const int t0 = NT * tile;
     if (seg) __syncthreads();  // (the last tile's states are read)
-    for (int c = l; c < NT; c += 64) st[c] = kLowest, st[NT + c] = st[2 * NT + c] = 0.0f;
+    for (int c = l; c < NT; c += 64) st[c] = kStart, st[NT + c] = st[2 * NT + c] = 0.0f;
     for (int c = threadIdx.x; c < NT; c += kThreads) toks[c] = t0 + c < a.T ? a.tokens[t0 + c] : -1;
     if (short_k)
       for (int c = threadIdx.x; c < 3 * NT * 4; c += kThreads)
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     tok[i] = 4 * lg + i < a.T ? a.tokens[4 * lg + i] : -1;
-    st[i] = {kLowest, 0.0f, 0.0f};
+    st[i] = {kStart, 0.0f, 0.0f};
   }
   const uint8_t *xrow = lds + lr * row_bytes;
   for (; b < r1; b += kWaves) {
@@ -627,7 +627,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 __global__ __launch_bounds__(64) void head_merge_kernel(const HeadArgs a, int NT) {
   const int tok = blockIdx.x, l = lane_id(), tile = tok / NT;
   const long long units = ((a.V >> 4) + a.unit - 1) / a.unit, line = units * a.tiles, lo = tile * units, hi = lo + units;
-  Stat s{kLowest, 0.0f, 0.0f};
+  Stat s{kStart, 0.0f, 0.0f};
   if (a.tiles == 1) {  // (every run)
     const float *q = a.part + tok;
     const long long step = (long long)a.segs * 3 * NT;

@@ -11,7 +11,10 @@ namespace head {
 constexpr int kThreads = 512, kWaves = 8;
 constexpr float kLowest = -3.402823466e38f, kFloor = -1000.0f, kLog2e = 1.44269504088896341f;
 constexpr float kFar = 0x1p28f;  // |m| up to which a row is a distribution: m is rounded by at most 8 there
-constexpr float kDead = -1.7e38f;  // the logit of a row that is not there (its product with log2 e is finite)
+// Where references begin: a tile of logits that all lie below it (in a row whose others do not) adds 0, instead of
+// exponentials of its reference's own rounding.  So do the rows that are not there, whose logit is kDead.
+constexpr float kStart = -kFar;
+constexpr float kDead = -0x1p127f;  // (its product with log2 e is finite)
 
 struct HeadArgs {
   const uint16_t *x;

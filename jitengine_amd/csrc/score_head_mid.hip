@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   for (int c = threadIdx.x; c < NT; c += kThreads) toks[c] = c < a.T ? a.tokens[c] : -1;
   __syncthreads();
 
-  Stat total{kLowest, 0.0f, 0.0f};  // thread c: token c
+  Stat total{kStart, 0.0f, 0.0f};  // thread c: token c
   int stage = 0;
   for (int pass = 0; pass < passes; pass++) {
     f32x4 acc[NB][T16];
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
           if (v[k] == 16 * block(pass, i) + lr && block(pass, i) < r1) a.picked[16 * t + 4 * lg + k] = acc[i][t][k];
           x = fmaxf(x, acc[i][t][k]);
         }
-        const float m = row_max(x) * kLog2e;
+        const float m = fmaxf(row_max(x) * kLog2e, kStart);
         float p = 0.0f, q = 0.0f;
 #pragma unroll
         for (int i = 0; i < NB; i++) {
