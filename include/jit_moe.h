@@ -531,7 +531,7 @@ int jit_token_logprobs(const void *logits, int fp32, int B, int V, long long row
  * A row is NaN in all three where its largest logit lies past +-2^28 / log2 e (fp32 logits are 16 apart there), and where
  * one of its logits is not finite or has a sum on the way to it that is not: products are with q + 16 before the scale, 64
  * of them a sum, so that no x of a magnitude below 2^117 overflows there.
- * Contract: K % 128 == 0, V % 16 == 0, T <= 2^20, T K < 2^31 (JIT_EUNSUPPORTED); x, w and the workspace 16-byte aligned;
+ * Contract: K % 128 == 0, V % 16 == 0, T <= 2^20, K <= 2^24, T K < 2^31 (JIT_EUNSUPPORTED); x, w and the workspace 16-byte aligned;
  * a workspace of jit_head_logprobs_workspace_bytes. */
 long long jit_head_logprobs_workspace_bytes(int T, int K, int V);
 int jit_head_logprobs(const uint16_t *x, int T, int K, const void *w, int V, const int32_t *tokens, float *logprob,

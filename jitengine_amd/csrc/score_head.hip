@@ -750,8 +750,9 @@ extern "C" int jit_head_logprobs(const uint16_t *x, int T, int K, const void *w,
   if (T < 0 || K <= 0 || V <= 0) return jit::fail(JIT_EINVAL, "head_logprobs: bad dims T=%d K=%d V=%d", T, K, V);
   if (K % 128 != 0 || V % 16 != 0)
     return jit::fail(JIT_EUNSUPPORTED, "head_logprobs covers K %% 128 == 0 and V %% 16 == 0, got K=%d V=%d", K, V);
-  if (T > (1 << 20) || (long long)T * K > 0x7fffffffLL)
-    return jit::fail(JIT_EUNSUPPORTED, "head_logprobs covers up to 2^20 rows and 2^31 - 1 values of x, got %d x %d", T, K);
+  // (a 16-row block's bytes, K / 128 tiles of 1,152, are offsets of 32 bits)
+  if (T > (1 << 20) || K > (1 << 24) || (long long)T * K > 0x7fffffffLL)
+    return jit::fail(JIT_EUNSUPPORTED, "head_logprobs covers up to 2^20 rows of up to 2^24 and 2^31 - 1 values of x, got %d x %d", T, K);
   if (T == 0) return JIT_OK;
   if (!x || !w || !tokens || !logprob || !entropy || !lse) return jit::fail(JIT_EINVAL, "head_logprobs: null pointer");
   if (((uintptr_t)x | (uintptr_t)w) & 15) return jit::fail(JIT_EINVAL, "head_logprobs: x and the head must be 16-byte aligned");
