@@ -518,7 +518,7 @@ int jit_kv_copy_pages(uint16_t *pool, int num_pages, int Hkv, const int32_t *src
  * -inf logits have probability 0; a row of nothing else has log-probabilities -inf and entropy 0.  A row with a NaN or
  * +inf has NaN log-probabilities and entropy; a NaN is no alternative (id -1 where numbers are missing, rank -1).
  * The bits repeat; they depend on B and top through the slices of a row, and on where a row begins in its 16 bytes.
- * Contract: top <= V, top <= 64, n_tokens <= 64, V <= 2^30 (the last three JIT_EUNSUPPORTED); a workspace of
+ * Contract: top <= V, top <= 64, n_tokens <= 64, V <= 2^30, B < 2^24 (all but the first JIT_EUNSUPPORTED); a workspace of
  * jit_token_logprobs_workspace_bytes (16-byte aligned, contents do not matter, none where that is 0). */
 long long jit_token_logprobs_workspace_bytes(int B, int V, int n_tokens, int top);
 int jit_token_logprobs(const void *logits, int fp32, int B, int V, long long row_stride, const int32_t *tokens,
@@ -543,7 +543,7 @@ int jit_head_logprobs(const uint16_t *x, int T, int K, const void *w, int V, con
  * without a token.  A NaN or -inf is no candidate.  The first `width` in the order (score descending, b * alternatives + j
  * ascending) are written: parents (the beam's row, group * beams + b), tokens (-1 of an ended beam), out_scores, and
  * out_done = 1 where the parent had ended or the token is one of eos; -1, -1, -inf, 1 past the last candidate.
- * Contract: beams * alternatives <= 4096, width <= 64 (JIT_EUNSUPPORTED). */
+ * Contract: beams * alternatives <= 4096, width <= 64, groups < 2^26, groups * beams < 2^31 (JIT_EUNSUPPORTED). */
 int jit_beam_select(const float *scores, const float *logprobs, const int32_t *ids, const int32_t *done,
                     const int32_t *eos, int n_eos, int groups, int beams, int alternatives, int width,
                     int32_t *parents, int32_t *tokens, float *out_scores, int32_t *out_done, void *stream);
@@ -559,15 +559,15 @@ int jit_beam_select(const float *scores, const float *logprobs, const int32_t *i
  *   status [4]  pages copied, where the free list goes on, children refused, pages that found no room in the list.
  * A child is refused (length 0, no pages) where the list ends or holds an id outside the pool.  A page id outside
  * [0, num_pages) in a table is handed on as it is, without a count.  A list of num_pages entries always has room.
- * Contract: S, N <= JIT_STEP_TABLES_MAX_SEQS, max_pages <= 2^26, num_pages <= 2^27 (JIT_EUNSUPPORTED); a workspace of
- * jit_pages_fork_workspace_bytes, 16-byte aligned; outputs apart from inputs. */
+ * Contract: S, N <= JIT_STEP_TABLES_MAX_SEQS, max_pages <= 2^26, num_pages <= 2^27, max(S, N) ceil(max_pages / 256) < 2^24
+ * (JIT_EUNSUPPORTED); a workspace of jit_pages_fork_workspace_bytes, 16-byte aligned; outputs apart from inputs. */
 long long jit_pages_fork_workspace_bytes(int S, int N, int num_pages);
 int jit_pages_fork(const int32_t *page_table, const int32_t *lens, int S, int max_pages, const int32_t *parents, int N,
                    int32_t *refs, int num_pages, int32_t *free_pages, int n_free, const int32_t *free_at,
                    int32_t *new_table, int32_t *new_lens, int32_t *src, int32_t *dst, int32_t *status, void *workspace,
                    long long workspace_bytes, void *stream);
 
-/* jit_kv_copy_pages (or jit_kv8_copy_pages) in every layer by one launch (one for every 128 layers): page src[i] to
+/* jit_kv_copy_pages (or jit_kv8_copy_pages) in every layer by one launch (one for every 128 layers and 2^24 copies): page src[i] to
  * page dst[i], i < n, of each of the `layers` pools; `pools` is a host array of device pointers, page_bytes the bytes of
  * a page in one layer.  A page id outside [0, num_pages) copies nothing.  No page is copied to twice, and none of those
  * copied to is copied from.  Contract: 16-byte aligned pools, page_bytes % 16 == 0. */

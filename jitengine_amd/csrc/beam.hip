@@ -11,6 +11,7 @@ namespace {
 // are taken from the lowest c on, and the w chosen ones count how many of them stand before each.  Latency bounds it: one
 // group of 4 x 8 candidates 3 us, 64 groups of 16 x 32 12 us.
 constexpr int kMaxWidth = 64, kMaxCands = 4096;
+constexpr long long kMaxLaunch = 0xffffffffLL;  // threads of a launch
 
 struct BeamArgs {
   const float *scores, *lp;
@@ -351,8 +352,8 @@ extern "C" int jit_beam_select(const float *scores, const float *logprobs, const
   if (cands > kMaxCands || width > kMaxWidth)
     return jit::fail(JIT_EUNSUPPORTED, "beam_select covers up to %d candidates a group and a width of %d, got %lld and %d",
                      kMaxCands, kMaxWidth, cands, width);
-  if ((long long)groups * beams > 0x7fffffffLL)
-    return jit::fail(JIT_EUNSUPPORTED, "beam_select covers up to 2^31 - 1 beams, got %d x %d", groups, beams);
+  if ((long long)groups * beams > 0x7fffffffLL || (long long)groups * 64 > kMaxLaunch)
+    return jit::fail(JIT_EUNSUPPORTED, "beam_select covers up to 2^31 - 1 beams of 2^26 - 1 groups, got %d x %d", groups, beams);
   if (groups == 0) return JIT_OK;
   if (!scores || !logprobs || !ids || (n_eos && !eos) || !parents || !tokens || !out_scores || !out_done)
     return jit::fail(JIT_EINVAL, "beam_select: null pointer");
@@ -385,7 +386,7 @@ extern "C" int jit_pages_fork(const int32_t *page_table, const int32_t *lens, in
     return jit::fail(JIT_EUNSUPPORTED, "pages_fork covers up to %d sequences and children of up to 2^26 pages of 2^27, got %d, %d, %d and %d",
                      JIT_STEP_TABLES_MAX_SEQS, S, N, max_pages, num_pages);
   const long long blocks = (long long)(S > N ? S : N) * ((max_pages + 255) / 256);
-  if (blocks > 0x7fffffffLL) return jit::fail(JIT_EUNSUPPORTED, "pages_fork: tables of %d x %d", S > N ? S : N, max_pages);
+  if (blocks * 256 > kMaxLaunch) return jit::fail(JIT_EUNSUPPORTED, "pages_fork: tables of %d x %d", S > N ? S : N, max_pages);
   if (!refs || !free_at || !status || (S && (!page_table || !lens)) || (N && (!parents || !new_table || !new_lens || !src || !dst)) ||
       (n_free && !free_pages))
     return jit::fail(JIT_EINVAL, "pages_fork: null pointer");
@@ -424,22 +425,24 @@ extern "C" int jit_kv_copy_pages_layers(void *const *pools, int layers, int num_
     if (!pools[i] || ((uintptr_t)pools[i] & 15))
       return jit::fail(JIT_EINVAL, "kv_copy_pages_layers: layer %d's pool must be 16-byte aligned and not null", i);
   CopyArgs a;
-  a.src = src, a.dst = dst, a.num_pages = num_pages;
+  a.num_pages = num_pages;
   a.page_words = (int)(page_bytes / 16);
   // parts of a page, none of fewer than 1,024 words, until 1,024 workgroups copy (1 page of 64 KB in 48 layers: 2.6 us in a
   // graph, 4.4 whole; 7 of 32 KB: 3.8 and 4.1)
   const long long pages = (long long)n * (layers < kMaxLayers ? layers : kMaxLayers), most_parts = (a.page_words + 1023) / 1024;
   a.parts = (int)(pages >= 1024 ? 1 : (1024 + pages - 1) / pages < most_parts ? (1024 + pages - 1) / pages : most_parts);
   a.part_words = (a.page_words + a.parts - 1) / a.parts;
-  const long long most = 0x7fffffffLL;
   for (int at = 0; at < layers; at += kMaxLayers) {
     a.layers = layers - at < kMaxLayers ? layers - at : kMaxLayers;
     for (int i = 0; i < a.layers; i++) a.pool[i] = (uint4 *)pools[at + i];
-    const long long blocks = (long long)n * a.layers * a.parts;
-    if (blocks > most) return jit::fail(JIT_EUNSUPPORTED, "kv_copy_pages_layers: %d pages of %d layers", n, layers);
-    copy_layers_kernel<<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>(a);
-    const int rc = jit::check_launch("jit_kv_copy_pages_layers");
-    if (rc != JIT_OK) return rc;
+    const long long most = kMaxLaunch / 256 / ((long long)a.layers * a.parts);  // pages of a launch
+    for (long long i0 = 0; i0 < n; i0 += most) {
+      const long long m = n - i0 < most ? n - i0 : most;
+      a.src = src + i0, a.dst = dst + i0;
+      copy_layers_kernel<<<(unsigned)(m * a.layers * a.parts), 256, 0, (hipStream_t)stream>>>(a);
+      const int rc = jit::check_launch("jit_kv_copy_pages_layers");
+      if (rc != JIT_OK) return rc;
+    }
   }
   return JIT_OK;
 }

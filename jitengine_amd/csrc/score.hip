@@ -588,8 +588,8 @@ extern "C" int jit_token_logprobs(const void *logits, int fp32, int B, int V, lo
                      kMaxTop, kMaxTokens, top, n_tokens);
   if (V > (1 << 30)) return jit::fail(JIT_EUNSUPPORTED, "token_logprobs covers rows of up to 2^30 values, got %d", V);
   const int ns = slices_of(B, V, top);
-  if ((long long)B * ns > 0x7fffffffLL)
-    return jit::fail(JIT_EUNSUPPORTED, "token_logprobs covers up to 2^31 - 1 workgroups, got %d rows", B);
+  if ((long long)B * ns * kThreads > 0xffffffffLL)  // (a launch has fewer than 2^32 threads)
+    return jit::fail(JIT_EUNSUPPORTED, "token_logprobs covers up to 2^24 - 1 rows, got %d", B);
   if (B == 0) return JIT_OK;
   if (!logits || !entropy || (n_tokens && (!tokens || !logprob || !rank)) || (top && (!top_ids || !top_logprobs)))
     return jit::fail(JIT_EINVAL, "token_logprobs: null pointer");

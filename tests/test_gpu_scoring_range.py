@@ -1,4 +1,5 @@
-"""Rows of logits far from 0 against 64-bit ones: masks of large negative numbers that leave nothing, and what lies beside them."""
+"""Rows of logits far from 0 against 64-bit ones: masks of large negative numbers that leave nothing, and what lies beside them;
+lists of very many pages."""
 
 from __future__ import annotations
 
@@ -66,3 +67,17 @@ def test_token_logprobs_are_never_above_zero(V, dtype):
     # (the sums hold one number of note: its exponential, up to a few joins, and the logarithm's argument are rounded)
     assert float(r.logprob.min()) >= -64 * U
     assert torch.equal(r.rank, torch.zeros_like(r.rank)) and torch.equal(r.top_ids[:, 0], tok.to(DEV))
+
+
+def test_copies_of_more_pages_than_a_launch_takes():
+    """140,000 entries in 128 layers, nearly all of them -1: a launch has 2^24 workgroups at most."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    pools = [torch.randn((12, 1, 2, 2048), generator=g, device=DEV).to(torch.bfloat16) for _ in range(128)]
+    want = [p.clone() for p in pools]
+    src, dst = (torch.full((140000,), -1, dtype=torch.int32) for _ in range(2))
+    for at, s, d in ((0, 0, 6), (131070, 1, 7), (131071, 2, 8), (139999, 3, 9)):
+        src[at], dst[at] = s, d
+        for w in want:
+            w[d] = w[s]
+    ops.kv_copy_pages_layers(ops.pool_layers(pools), src.to(DEV), dst.to(DEV))
+    assert all(torch.equal(p, w) for p, w in zip(pools, want))
