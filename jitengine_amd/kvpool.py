@@ -61,6 +61,7 @@ class KVPool:
             if allocate else []
         )
         self._layers: ops.PoolLayers | None = None
+        self._where: list = []  # the pools' memory that it was made of
 
     # ------------------------------------------------------------------ pages
     @property
@@ -103,11 +104,12 @@ class KVPool:
         ops.kv_copy_pages_layers(self.layers(), s, d)
 
     def layers(self) -> ops.PoolLayers:
-        """The layers' pools as one handle, for calls that work on every layer at once."""
-        h = self._layers
-        if h is None or len(h.pools) != len(self.pools) or any(a is not b for a, b in zip(h.pools, self.pools)):
-            h = self._layers = ops.pool_layers(self.pools)
-        return h
+        """The layers' pools as one handle, for calls that work on every layer at once: made anew where a pool has other
+        memory than before, whether it is another tensor or the same one."""
+        where = [(p.data_ptr(), p.shape) for p in self.pools]
+        if self._layers is None or where != self._where:
+            self._layers, self._where = ops.pool_layers(self.pools), where
+        return self._layers
 
     # -------------------------------------------------------------- sequences
     def open(self, seq_id, pages=(), length: int = 0) -> None:

@@ -1285,7 +1285,8 @@ class PoolLayers:
 
 
 def pool_layers(pools) -> PoolLayers:
-    """The pools of a model's layers (all bf16 or all 8-bit, of one shape and device) as one handle; made once."""
+    """The pools of a model's layers (all bf16 or all 8-bit, of one shape and device) as one handle, made once: it holds
+    their addresses, and a pool whose memory is exchanged (.data, set_, a storage resized) needs a new one."""
     pools = list(pools)
     if not pools:
         raise ValueError("pool_layers takes at least one pool")

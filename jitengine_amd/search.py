@@ -129,7 +129,7 @@ def _search(eng, prompts, sids, h, pages, n: int, max_tokens: int, eos: list, wi
     index = torch.arange(free.numel(), device=dev)
     ends = ops.upload(np.asarray(eos, np.int32), dev) if eos else None
     scores, done, rows = torch.zeros((G, 1), device=dev), None, 1
-    parents, tokens, statuses = [], [], []
+    parents, tokens, statuses, layers = [], [], [], pool.layers()
     for t in range(max_tokens):
         lp = ops.token_logprobs(lm.logits(h), top=n)
         b = ops.beam_select(scores, lp.top_logprobs.view(G, rows, n), lp.top_ids.view(G, rows, n), n, done, ends)
@@ -141,7 +141,7 @@ def _search(eng, prompts, sids, h, pages, n: int, max_tokens: int, eos: list, wi
         # (an ended beam, or one that is none, needs no pages any more)
         go = torch.where(done == 0, b.parents, -1).view(-1)
         f = ops.pages_fork(table, lens, go, refs, free, at)
-        ops.kv_copy_pages_layers(pool.layers(), f.src, f.dst)
+        ops.kv_copy_pages_layers(layers, f.src, f.dst)
         on = go >= 0
         s = ops.step_tables(f.lens, on.to(i32), f.page_table, G * n, free, f.status[1:2])
         pos = np.repeat(lens_host + t, n)
