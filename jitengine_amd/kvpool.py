@@ -105,10 +105,10 @@ class KVPool:
 
     def layers(self) -> ops.PoolLayers:
         """The layers' pools as one handle, for calls that work on every layer at once: made anew where a pool has other
-        memory than before, whether it is another tensor or the same one."""
+        memory than before, whether it is another tensor or the same one.  Layers that share a pool have it once."""
         where = [(p.data_ptr(), p.shape) for p in self.pools]
         if self._layers is None or where != self._where:
-            self._layers, self._where = ops.pool_layers(self.pools), where
+            self._layers, self._where = ops.pool_layers({p.data_ptr(): p for p in self.pools}.values()), where
         return self._layers
 
     # -------------------------------------------------------------- sequences

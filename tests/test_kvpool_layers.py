@@ -25,3 +25,11 @@ def test_the_layers_handle_follows_the_pools_memory(monkeypatch):
     pool.pools[0].data = torch.zeros((8, 1, 2, 2048), dtype=torch.bfloat16)
     pool.layers()
     assert pool.layers() == [p.data_ptr() for p in pool.pools] and len(made) == 5
+
+
+def test_layers_that_share_a_pool_have_it_once(monkeypatch):
+    """Their pages were copied layer by layer before, the shared one as often as it stood there."""
+    monkeypatch.setattr(ops, "pool_layers", list)
+    pool = KVPool(4, 4, 1, "cpu")
+    pool.pools[2] = pool.pools[0]
+    assert [any(p is q for q in pool.layers()) for p in pool.pools] == [True] * 4 and len(pool.layers()) == 3
