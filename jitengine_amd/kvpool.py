@@ -225,6 +225,13 @@ class PrefixStore:
         self.pool.decref(pages)
         return True
 
+    def held_alone(self) -> int:
+        """Pages that come free when every entry is evicted."""
+        held = np.zeros_like(self.pool.refs)
+        for pages in self.entries.values():
+            held[pages] += 1  # (a sequence's pages are distinct)
+        return int(np.count_nonzero((held > 0) & (held == self.pool.refs)))
+
     def make_room(self, n_pages: int) -> None:
         """Evict entries until n_pages are free or the store is empty."""
         while self.pool.free_pages < n_pages and self.evict_one():

@@ -39,11 +39,14 @@ class Beam:
 
 
 def _make_room(eng, pages: int) -> None:
-    """Evict stored prefixes until `pages` pages that no admitted request is owed are free (PoolExhausted)."""
+    """Evict stored prefixes until `pages` pages that no admitted request is owed are free; none where that many cannot
+    come free (PoolExhausted)."""
+    held = 0 if eng.store is None else eng.store.held_alone()
+    most = eng.pool.free_pages + held - eng.outstanding
+    if most < pages:
+        raise PoolExhausted(f"{pages} pages needed, {most} free or held by stored prefixes alone")
     if eng.store is not None:
         eng.store.make_room(pages + eng.outstanding)
-    if eng.pool.free_pages - eng.outstanding < pages:
-        raise PoolExhausted(f"{pages} pages needed, {eng.pool.free_pages - eng.outstanding} free")
 
 
 def _prompt(eng, tokens) -> list:
