@@ -1122,7 +1122,14 @@ def _workspace(workspace, need: int, device, name: str) -> torch.Tensor | None:
     return workspace
 
 
+def _past_32_bits(name: str, *sizes) -> None:
+    """Refuses sizes that the native calls' 32-bit arguments would cut."""
+    raise _lib.UnsupportedShape(f"{name} takes sizes in [0, 2^31), got {', '.join(str(int(s)) for s in sizes)}")
+
+
 def token_logprobs_workspace_bytes(B: int, V: int, n_tokens: int = 1, top: int = 0) -> int:
+    if max(B, V, n_tokens, top) >> 31:
+        _past_32_bits("token_logprobs", B, V, n_tokens, top)
     return int(_lib.lib().jit_token_logprobs_workspace_bytes(int(B), int(V), int(n_tokens), int(top)))
 
 
@@ -1136,10 +1143,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         raise ValueError(f"logits must be bf16 or fp32, got {logits.dtype}")
     if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError(f"logits must be [B, V] with adjacent values in a row, got {tuple(logits.shape)}")
+    (B, V), top, m, shape = logits.shape, int(top), 0, None
+    if (B | V | top) >> 31:
+        _past_32_bits("token_logprobs", B, V, top)
     dev = logits.get_device()
     if dev < 0:
         raise ValueError("logits must be a device tensor")
-    (B, V), top, m, shape = logits.shape, int(top), 0, None
     stride = logits.stride(0) if B > 1 else V
     if V < 1 or stride < V:
         raise ValueError(f"rows of {V} logits at a stride of {stride}")
@@ -1150,9 +1159,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         if tokens.dim() not in (1, 2) or shape[0] != B or (tokens.dim() == 2 and shape[1] < 1):
             raise ValueError(f"tokens must be [{B}] or [{B}, m], got {tuple(shape)}")
         m = 1 if tokens.dim() == 1 else shape[1]
-    need = lib.jit_token_logprobs_workspace_bytes(B, V, m, max(top, 0))
+        if m >> 31:
+            _past_32_bits("token_logprobs", m)
+    need = lib.jit_token_logprobs_workspace_bytes(B, V, m, top)
     ws = _workspace(workspace, need, logits.device, "token_logprobs")
-    n, k = B * m, B * max(top, 0)  # (two allocations: a row's launches are a few microseconds, and so is the host's side)
+    n, k = B * m, B * top  # (two allocations: a row's launches are a few microseconds, and so is the host's side)
     floats = torch.empty(B + n + k, dtype=f32, device=logits.device)
     ints = torch.empty(n + k, dtype=i32, device=logits.device)
     at, to = floats.data_ptr(), ints.data_ptr()
@@ -1178,6 +1189,8 @@ class HeadLogprobs:
 
 
 def head_logprobs_workspace_bytes(T: int, K: int, V: int) -> int:
+    if max(T, K, V) >> 31:
+        _past_32_bits("head_logprobs", T, K, V)
     return int(_lib.lib().jit_head_logprobs_workspace_bytes(int(T), int(K), int(V)))
 
 
@@ -1192,6 +1205,8 @@ def head_logprobs(x: torch.Tensor, head: PackedQ4, tokens: torch.Tensor,
     if x.dim() != 2 or x.shape[1] != head.K or tokens.shape != x.shape[:1]:
         raise ValueError(f"head_logprobs takes x [T, {head.K}] and tokens [T], got {tuple(x.shape)} and {tuple(tokens.shape)}")
     T, lib = x.shape[0], _lib.lib()
+    if (T | head.K | head.N) >> 31:
+        _past_32_bits("head_logprobs", T, head.K, head.N)
     ws = _workspace(workspace, lib.jit_head_logprobs_workspace_bytes(T, head.K, head.N), x.device, "head_logprobs")
     out = torch.empty((3, T), dtype=torch.float32, device=x.device)
     at = out.data_ptr()
@@ -1229,10 +1244,13 @@ def beam_select(scores: torch.Tensor, logprobs: torch.Tensor, ids: torch.Tensor,
     w = n if width is None else int(width)
     if w < 1:
         raise ValueError(f"width must be positive, got {w}")
+    e = 0 if eos is None else eos.numel()
+    if (G | n | m | w | e) >> 31:
+        _past_32_bits("beam_select", G, n, m, w, e)
     buf = torch.empty((4, G, w), dtype=i32, device=scores.device)
     at, step = buf.data_ptr(), 4 * G * w
     _launch(dev, _lib.lib().jit_beam_select, "beam_select", scores.data_ptr(), logprobs.data_ptr(), ids.data_ptr(), _ptr(done),
-            _ptr(eos), 0 if eos is None else eos.numel(), G, n, m, w, at, at + step, at + 2 * step, at + 3 * step)
+            _ptr(eos), e, G, n, m, w, at, at + step, at + 2 * step, at + 3 * step)
     p, t, s, d = buf.unbind(0)
     return Beams(p, t, s.view(f32), d)
 
@@ -1261,13 +1279,15 @@ def pages_fork(page_table: torch.Tensor, lens: torch.Tensor, parents: torch.Tens
             refs.dim() != 1 or refs.numel() < 1 or free.dim() != 1 or free_at.numel() != 1:
         raise ValueError(f"pages_fork takes page_table [S, W], lens [S], parents [N], refs [P], free [F], free_at [1], got "
                          f"{[tuple(t.shape) for t in (page_table, lens, parents, refs, free, free_at)]}")
-    (S, W), N, P, lib = page_table.shape, parents.numel(), refs.numel(), _lib.lib()
+    (S, W), N, P, F, lib = page_table.shape, parents.numel(), refs.numel(), free.numel(), _lib.lib()
+    if (S | W | N | P | F) >> 31:
+        _past_32_bits("pages_fork", S, W, N, P, F)
     ws = _workspace(workspace, lib.jit_pages_fork_workspace_bytes(S, N, P), refs.device, "pages_fork")
     buf = torch.empty(N * (W + 3) + 4, dtype=i32, device=refs.device)
     at = buf.data_ptr()
     p_len = at + 4 * N * W
     _launch(dev, lib.jit_pages_fork, "pages_fork", page_table.data_ptr(), lens.data_ptr(), S, W, parents.data_ptr(), N,
-            refs.data_ptr(), P, free.data_ptr(), free.numel(), free_at.data_ptr(), at, p_len, p_len + 4 * N, p_len + 8 * N,
+            refs.data_ptr(), P, free.data_ptr(), F, free_at.data_ptr(), at, p_len, p_len + 4 * N, p_len + 8 * N,
             p_len + 12 * N, ws.data_ptr(), ws.nbytes)
     table, *rest = buf.split_with_sizes([N * W, N, N, N, 4])
     return Fork(table.view(N, W), *rest)
@@ -1312,6 +1332,8 @@ def kv_copy_pages_layers(layers: PoolLayers, src: torch.Tensor, dst: torch.Tenso
         raise ValueError(f"src is on device {dev}, the pools on {layers.device}")
     if src.shape != dst.shape or src.dim() != 1:
         raise ValueError("src and dst must be equal-length 1-D page lists")
+    if src.numel() >> 31:
+        _past_32_bits("kv_copy_pages_layers", src.numel())
     _launch(dev, _lib.lib().jit_kv_copy_pages_layers, "kv_copy_pages_layers", layers.pointers, len(layers.pools),
             layers.num_pages, layers.page_bytes, src.data_ptr(), dst.data_ptr(), src.numel())
 
