@@ -511,7 +511,7 @@ int jit_kv_copy_pages(uint16_t *pool, int num_pages, int Hkv, const int32_t *src
  * elements after row b - 1, at any address that its type allows).  No counterpart in the reference, whose sampler keeps
  * whole rows of bf16 log-probabilities (Q36/sampler.py:295-297); here everything is fp32 or more from the logits on.
  * With any reference m near the largest logit of a row, l = sum e^(x - m), t = sum (x - m) e^(x - m):
- *   logprob [B, n_tokens]  (x_v - m) - ln l of the tokens v = tokens [B, n_tokens]; 0 for a v outside [0, V);
+ *   logprob [B, n_tokens]  (x_v - m) - ln l, never above 0, of the tokens v = tokens [B, n_tokens]; 0 for a v outside [0, V);
  *   rank    [B, n_tokens]  logits before x_v in the order (value descending, index ascending); -1 outside [0, V);
  *   entropy [B]            ln l - t / l, in nats;
  *   top_ids, top_logprobs [B, top]  the first `top` of that order.

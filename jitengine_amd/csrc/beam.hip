@@ -125,8 +125,11 @@ __global__ __launch_bounds__(64) void beam_select_kernel(const BeamArgs a) {
 // that came free (one workgroup); one launch for small tables.  Latency and the order among the parts bound it: 8 tables of 272
 // pages 12 us (13 as three launches, each of which costs the host some 3 more), 512 of 544 pages 5 + 8 + 11.
 constexpr int kForkThreads = 1024, kPage = JIT_PAGE_TOKENS;
-constexpr int kSmallFork = 4096;  // entries of the tables that one workgroup takes (2,176: 10.0 us in a graph, 10.7 as three
-                                  // launches; 8,160: 17.5 and 11.2)
+// Entries of the tables that one workgroup takes.  8 tables over a pool of 65,536 pages, in a graph with a copy of its counts,
+// as one launch and as three: 2,096 entries 15.7 and 16.6 us, 2,752 17.1 and 16.5, 3,952 18.6 and 16.6, 6,048 20.4 and 16.4.
+// As calls of their own, which the host bounds, one launch takes 21.4 us at all of them, three 25 to 28; of more tables 4,032
+// entries take 24.4 and 27.5, 5,120 26.7 and 27.4.  The rule stands between the two uses.
+constexpr int kSmallFork = 4096;
 
 struct ForkArgs {
   const int32_t *table, *lens, *parents, *free_at;

@@ -17,8 +17,11 @@
 // (32 rows, 20 alternatives: 67 + 19 us).
 //
 // What bounds it: many rows, the vector ALU (a value takes 5 1/2 instructions of 4 cycles and an exponential of 16, one
-// instruction more for the rank: 2,048 rows of 151,936 bf16 values, 622 MB, in 138 us, 4.5 TB/s; a large copy reaches 4.8);
-// few rows, latency: 1 row of 151,936 in 6.4 + 5.3 us of two launches, 32 rows of 248,320 under a mask in 17.0 + 5.7.
+// instruction more for the rank: 2,048 rows of 151,936 bf16 values, 622 MB, in 131 to 138 us, 4.5 to 4.7 TB/s; a large copy
+// reaches 4.8); few rows, latency: 1 row of 151,936 in 6.6 + 5.4 us of two launches, 32 rows of 248,320 under a mask in 17.5
+// + 5.8.  fp32 rows: 2,048 in 239 us, 5.2 TB/s; 1 in 13.7 (bf16 11.3, both calls in a graph).  Several tokens a row cost a
+// ballot and a count for each value of a lane and token: 2,048 rows take 124 us with 1 token and no alternatives, 141 with 2,
+// 340 with 8, 2,250 with 64; 1 row 7.0, 8.0, 11.0 and 41.
 #include "common.hpp"
 
 namespace {
@@ -258,8 +261,8 @@ __device__ __forceinline__ void write_rest(const ScoreArgs &a, int b, const Stat
 }
 
 // ------------------------------------------------------------------ a slice of a row
-constexpr int U = 2;  // 16-byte words a thread takes of a step (at an earlier state of this kernel, 2,048 rows took 209 us,
-                      // 251 with 1 and 239 with 4; 1 x 131,072 takes 11.5 us, 10.9 with 1)
+constexpr int U = 2;  // 16-byte words a thread takes of a step (5 alternatives, calls in a graph, with 2, 1 and 4 words: 1 row
+                      // of 151,936 11.7, 12.9, 12.4 us; 300 rows 41, 45, 46; 2,048 rows 149, 152, 161; 64 x 32,000 13, 12, 17)
 template <typename T>
 __global__ __launch_bounds__(kThreads) void score_rows_kernel(const ScoreArgs a) {
   constexpr int N = Elems<T>::N, kStep = kThreads * U, kBits = sizeof(T) * 8;  // values of a word, words of a step

@@ -107,8 +107,11 @@ struct Lds {
 // is the line of (token tile, unit of 32 or 16 blocks) pairs, tiles first to last, cut into equal runs, one a workgroup (the 8
 // waves do a unit at a time, so that no run has a part of one but at a tile's end).  What bounds
 // it: the issue slots that products (11 of their 32 cycles), scaling and unpacking share, at a clock that power holds near
-// 1.7 GHz: 2,048 rows of 248,320 x 2,048 take 2.05 to 2.16 ms, 1 PFLOP/s (a bare bf16 product of the library 1.68 ms).  Of a
-// tile's cycles 65% are its steps, 15% their barriers, 10% the biases and 10% the softmax.
+// 1.7 GHz: 2,048 rows of 248,320 x 2,048 take 2.04 to 2.22 ms, 1 PFLOP/s (a bare bf16 product of the library 1.68 ms).  Of a
+// tile's cycles 65% are its steps with what they wait for, 15% their barriers, 10% the biases and 10% the softmax.  Registers
+// spill: 139 of three token tiles, mostly around biases and softmax, and 65 of four, where an offset of load_x and one of the
+// rows' LDS addresses come back from memory behind a step's barrier, with a wait for every load before them: what the step
+// has just asked for ahead (x(p + 1), w(p + 2)) then has to land at its beginning.
 template <int TT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void head_tile_kernel(const HeadArgs a) {
   using L = Lds<TT>;
@@ -663,7 +666,9 @@ __global__ __launch_bounds__(64) void head_merge_kernel(const HeadArgs a, int NT
 // Token tiles of a launch: 32 TT tokens each, TT as even as they come, so many that the last workgroup ends first.
 // (Always the largest tiles, runs of any number of blocks: 500 rows x 2,000 x 512 58 us, x 20,000 x 1,024 66, x 40,000 x
 // 2,048 135, 200 rows x 40,000 x 2,048 95, 129 x 151,936 x 2,048 176; so 17, 49, 128, 74, 167.)
-constexpr int kHalfCost[kMaxTT] = {43, 63, 95, 103};  // of 16 blocks of a tile of 1 .. 4 (3: more of it in spilled registers)
+// What 16 blocks of a tile of 1 .. 4 cost, relative to each other, as first measured.  Now 16 blocks of a workgroup take 13.5,
+// 20.6, 28.2 and 38.9 us (384 rows x 262,144 x 2,048 in tiles of each kind: 647, 494, 452, 467 us), as 43 : 66 : 90 : 124.
+constexpr int kHalfCost[kMaxTT] = {43, 63, 95, 103};
 struct Shape {
   bool few, mid;  // up to 16 rows that fit LDS; one tile of up to 96
   int tt, tile, tiles, parts, segs, T16, G32, unit = kUnit;

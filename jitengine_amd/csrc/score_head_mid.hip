@@ -6,7 +6,8 @@
 // a lane's scale is its own row's), so biases, softmax and the meeting of lanes and waves come once a pass.  What bounds
 // it: the head's bytes below some 50 rows, past that the issue of products and the sums behind them (a 16 x 16 x 32
 // product holds the issue port for some 11 of its 16 cycles).  77 rows x 151,936 x 2,048 take 83 to 90 us (head_tile_kernel:
-// 127), 17 rows x 4,096 86 us (122), 96 rows x 4,096 190 us (222), 32 rows x 2,048 49 us.
+// 127), 17 rows x 4,096 86 us (122), 96 rows x 4,096 190 us (222), 32 rows x 2,048 49 us.  From 33 rows on 5 blocks a wave
+// spill registers (7, 47, 93, 138 of them for 48, 64, 80, 96 rows), of 96 rows weights that were asked for ahead too.
 #include "score_head.hpp"
 
 namespace {
